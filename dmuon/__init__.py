@@ -18,7 +18,7 @@ from dmuon_amd import __all__  # noqa: F401
 _SUBMODULES = (
     "api", "utils", "fast_clip", "grad_clip", "optim", "optim.muon", "optim.newton_schulz",
     "optim.syrk_dispatch", "optim.adamw", "_backends", "_backends.local",
-    "_backends.local.param",
+    "_backends.local.param", "vocab_loss", "norms",
 )
 for _name in _SUBMODULES:
     sys.modules[f"{__name__}.{_name}"] = importlib.import_module(f"dmuon_amd.{_name}")
@@ -27,4 +27,6 @@ utils = dmuon_amd.utils
 fast_clip = dmuon_amd.fast_clip
 grad_clip = dmuon_amd.grad_clip
 optim = dmuon_amd.optim
+vocab_loss = dmuon_amd.vocab_loss
+norms = dmuon_amd.norms
 del _name

@@ -27,7 +27,7 @@ NS_GRAM = 1
 # DMUON_ABI_VERSION of include/dmuon_amd.h: the argument lists below are those of this
 # version, and a library that reports another one is refused (its entry points would be
 # called with the wrong arguments).
-ABI_VERSION = 109
+ABI_VERSION = 110
 
 MAX_GROUPS = 8         # DMUON_MAX_GROUPS
 
@@ -41,6 +41,36 @@ class MuonGroup(ctypes.Structure):
 
 
 c_gp = ctypes.POINTER(MuonGroup)
+
+LOSS_ROWS, LOSS_MEAN, LOSS_SUM = 0, 1, 2      # DMUON_LOSS_*
+
+
+class HeadLossArgs(ctypes.Structure):
+    """``dmuon_head_loss_args``: one call of a vocabulary loss."""
+
+    _fields_ = [(k, c_vp) for k in ("hidden", "weight", "targets", "teacher_ids",
+                                    "teacher_logits", "teacher_lse", "row_grad", "loss",
+                                    "reduced", "d_hidden", "d_weight")] + \
+        [(k, c_i64) for k in ("ld_hidden", "ld_weight", "tokens", "vocab", "dim", "k_list",
+                              "chunk_tokens", "ignore_index")] + \
+        [("z_loss", c_f), ("temperature", c_f), ("dtype", c_int),
+         ("grad_dtype", c_int), ("reduction", c_int)]
+
+
+c_hp = ctypes.POINTER(HeadLossArgs)
+
+
+class ResidualNormArgs(ctypes.Structure):
+    """``dmuon_residual_norm_args``: one call of the norms around a block."""
+
+    _fields_ = [(k, c_vp) for k in ("x", "y", "w_pre", "w_post", "gate", "stats", "x_new", "h",
+                                    "dx_new", "dh", "dx", "dy", "d_pre", "d_post", "d_gate")] + \
+        [(k, c_i64) for k in ("rows", "dim", "gates", "ld_x", "ld_y", "ld_dx_new", "ld_dh")] + \
+        [("scale", c_f), ("eps", c_f)] + \
+        [(k, c_int) for k in ("dtype", "pre_dtype", "post_dtype", "gate_dtype")]
+
+
+c_np = ctypes.POINTER(ResidualNormArgs)
 
 # name -> (restype, argtypes); mirrors include/dmuon_amd.h
 _SIGNATURES = {
@@ -115,6 +145,12 @@ _SIGNATURES = {
     "dmuon_clip_workspace_size": (c_int, [c_i64, c_i64, c_int, ctypes.POINTER(c_i64)]),
     "dmuon_clip_norms": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int,
                                  c_int, c_d, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "dmuon_head_loss_workspace_size": (c_int, [c_hp, ctypes.POINTER(c_i64)]),
+    "dmuon_head_loss": (c_int, [c_hp, c_vp, c_i64, c_vp]),
+    "dmuon_scale_by": (c_int, [c_vp, c_int, c_vp, c_int, c_i64, c_vp, c_vp]),
+    "dmuon_residual_norm": (c_int, [c_np, c_vp]),
+    "dmuon_residual_norm_grad_workspace_size": (c_int, [c_np, ctypes.POINTER(c_i64)]),
+    "dmuon_residual_norm_grad": (c_int, [c_np, c_vp, c_i64, c_vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -2,7 +2,8 @@
 world_size=1 (``import dmuon_amd as dmuon``).
 
 Exports the names of X-Square-Robot/dmuon's ``dmuon/__init__.py:80-122`` that concern the
-owner-rank update path. The compute runs in ``dmuon_amd/csrc/libdmuon_amd.so`` (HIP, gfx950);
+owner-rank update path, and operators of the step that leads up to it: the losses over a large
+vocabulary with their gradients and the norms around a block. The compute runs in ``dmuon_amd/csrc/libdmuon_amd.so`` (HIP, gfx950);
 there is no CPU fallback.
 """
 from .api import dedicate_params, replicate
@@ -14,6 +15,7 @@ from .fast_clip import (
     try_clip_optimizer_grad_norm_buckets_,
 )
 from .grad_clip import MuonGradClipStats, clip_grad_norm_, register_muon_grad_clip_strategy
+from .norms import residual_norm
 from .optim import (
     KELLER_COEFFICIENTS,
     POLAR_EXPRESS_COEFFICIENTS,
@@ -39,6 +41,7 @@ from .utils import (
     wait_all_reduces,
     wait_all_replicate_broadcasts,
 )
+from .vocab_loss import linear_cross_entropy, linear_distillation
 
 __all__ = [
     "dedicate_params", "replicate", "Muon", "NewtonSchulz", "newton_schulz",
@@ -51,4 +54,5 @@ __all__ = [
     "clip_grad_norm_", "clip_grad_norm_buckets_", "try_clip_optimizer_grad_norm_buckets_",
     "register_muon_grad_clip_strategy", "MuonGradClipStats", "GradClipBucket",
     "GradClipBucketStats", "SegmentedGradClipResult",
+    "linear_cross_entropy", "linear_distillation", "residual_norm",
 ]

@@ -24,11 +24,10 @@ using namespace dmuon;
 static __device__ __align__(256) char scratch[DMUON_NOALLOC_SCRATCH_BYTES];
 
 namespace {
-
 thread_local std::string g_last_error;
+}
 
-int fail(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
-int fail(const char* fmt, ...) {
+int dmuon::fail(const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -38,10 +37,12 @@ int fail(const char* fmt, ...) {
   return 1;
 }
 
-int check_launch(hipError_t e, const char* what) {
+int dmuon::check_launch(hipError_t e, const char* what) {
   if (e != hipSuccess) return fail("%s: launch failed: %s", what, hipGetErrorString(e));
   return 0;
 }
+
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool ld_ok(int64_t ld) { return ld > 0 && (ld % 8) == 0; }

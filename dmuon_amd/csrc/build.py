@@ -14,7 +14,8 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent.parent
-SOURCES = ["ns_gemm.hip", "gram_small.hip", "ew_kernels.hip", "adamw.hip", "clip.hip", "abi.hip"]
+SOURCES = ["ns_gemm.hip", "gram_small.hip", "ew_kernels.hip", "adamw.hip", "clip.hip",
+           "head_gemm.hip", "head_rows.hip", "head_loss.hip", "residual_norm.hip", "abi.hip"]
 LIB_NAME = "libdmuon_amd.so"
 ARCH = "gfx950"
 

@@ -7,6 +7,11 @@
 
 namespace dmuon {
 
+// Records the text of an entry point's error (dmuon_last_error) and returns 1.
+int fail(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
+// 0, or fail() with the launch's error.
+int check_launch(hipError_t e, const char* what);
+
 // dtype codes used across the C-ABI (mirrors DMUON_DTYPE_* in dmuon_amd.h); DT_F16 only names
 // 16-bit product operands (SYRK / NS-GEMM entry points).
 enum DType : int { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };

@@ -1,0 +1,77 @@
+// Internal declarations of the vocabulary losses: the products of hidden states with a head's
+// weight and the row kernels between them. Not part of the public C ABI.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace dmuon {
+
+// Columns of one softmax statistic: every row keeps a (maximum, sum of exponentials) pair per
+// kStatCols columns of the logits.
+constexpr int kStatCols = 64;
+// The logit gradient is stored as 2^kGradShift times its row's value over the largest row weight:
+// fp16 then holds probabilities down to 2^-24 with all their bits and 2^-34 with some, and
+// 2^6 = 64 times the unit mass does not overflow.
+constexpr int kGradShift = 10;
+
+// What a product writes.
+//   HG_LOGITS  Z = scale * acc (fp32, pitch ldz, optional) and the statistics of its columns
+//   HG_GRAD    out = alpha[0] * (acc + part) rounded to out_dtype, or part (+)= acc in fp32
+enum HeadGemmMode : int { HG_LOGITS = 0, HG_GRAD = 1 };
+
+// acc[i][j] = sum_k A(i, k) * B(j, k): operand X's element (r, k) is X[r * ld + k], or
+// X[k * ld + r] with x_kmajor.
+struct HeadGemm {
+  const uint16_t* A; long long lda; int a_kmajor;
+  const uint16_t* B; long long ldb; int b_kmajor;
+  int M, N, K;
+  int mode, elt;
+  float scale;
+  float* Z; long long ldz;
+  float2* stats;                          // HG_LOGITS: [ceil(N / kStatCols)][M]
+  const float* alpha;
+  void* out; long long ldo; int out_dtype;   // HG_GRAD: result (DT_F32 or the operands'), or NULL
+  float* part; long long ldp;             // HG_GRAD: fp32 sums [M][ldp], or NULL
+  int add_part;                           // part holds earlier sums to add to
+};
+hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream);
+
+// One call's rows as the kernels see them. Entry k of row n is the class ids[n * k_list + k] with
+// the target probability probs[..] (0 for padding, whose id is -1).
+struct HeadRows {
+  int n;                                  // tokens of the call
+  int vocab, k_list;
+  const int64_t* targets;                 // hard targets [n] (k_list 1), or
+  const int64_t* teacher_ids;             // [n][k_list]
+  const float* teacher_logits;            // [n][k_list]
+  const float* teacher_lse;               // [n] or NULL
+  long long ignore_index;
+  float z_loss, temperature;
+  int reduction;                          // DMUON_LOSS_*
+  const float* row_grad;                  // DMUON_LOSS_ROWS: dL / d loss[n], or NULL
+  int* ids; float* probs;                 // [n][k_list]
+  float* mass;                            // [n]: sum of the row's probs, < 0: not counted
+  float* lse;                             // [n]
+  float* loss;                            // [n]
+  float* row_weight;                      // [n]: 2^kGradShift * row gradient / largest, or NULL
+  float* alpha;                           // [1]: what turns a stored gradient into the real one
+  float* mean;                            // [1] or NULL: the reduced loss
+};
+// ids, probs and mass of every row; row weights and alpha with `grads`.
+hipError_t launch_head_targets(const HeadRows& r, bool grads, hipStream_t stream);
+// lse and loss of rows first .. first + rows - 1 from their logits and statistics.
+hipError_t launch_head_loss(const HeadRows& r, int first, int rows, const float* Z, long long ldz,
+                            const float2* stats, hipStream_t stream);
+// G[row][v] = row_weight (mass softmax - target probability) for v < vocab, 0 for the columns up
+// to ldg.
+hipError_t launch_head_grad(const HeadRows& r, int first, int rows, const float* Z, long long ldz,
+                            uint16_t* G, long long ldg, int elt, hipStream_t stream);
+// mean[0] = sum of the losses, divided by the number of counted rows for DMUON_LOSS_MEAN.
+hipError_t launch_head_reduce(const HeadRows& r, hipStream_t stream);
+
+// dst = factor[0] * src for n values of the DT_* types; in place, nothing moves where it is 1.
+hipError_t launch_scale_by(const void* src, int src_dtype, void* dst, int dst_dtype, long long n,
+                           const float* factor, hipStream_t stream);
+
+}  // namespace dmuon

@@ -1,0 +1,214 @@
+// dmuon_head_loss: argument checks, workspace layout and launch sequence of the vocabulary losses.
+//
+// The rows go through in chunks of tokens. Per chunk: the logits with the softmax statistics of
+// every 64 columns, each row's log-sum-exp and loss, the logit gradient, and its two products with
+// the weight and the hidden states. The weight's gradient sums over the chunks in fp32.
+#include "../../include/dmuon_amd.h"
+#include "dmuon_amd_internal.h"
+#include "head_loss.h"
+
+using namespace dmuon;
+
+namespace {
+
+int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+// Workspace of a chunk's logits and logit gradient; a call of more tokens takes several chunks.
+constexpr int64_t kChunkBytes = int64_t(2) << 30;
+
+struct Layout {
+  int64_t chunk, ld;                      // tokens of a chunk, pitch of its logits
+  int64_t ids, probs, mass, lse, row_weight, alpha, Z, stats, G, part, bytes;
+};
+
+int elt_of(int dtype, int* elt) {
+  if (dtype == DMUON_DTYPE_BF16) *elt = ELT_BF16;
+  else if (dtype == DMUON_DTYPE_F16) *elt = ELT_F16;
+  else return 1;
+  return 0;
+}
+
+int check(const char* who, const dmuon_head_loss_args* a) {
+  int elt;
+  if (!a) return fail("%s: NULL arguments", who);
+  if (elt_of(a->dtype, &elt))
+    return fail("%s: dtype code %d is not a 16-bit type (bf16 %d, fp16 %d)", who, a->dtype,
+                DMUON_DTYPE_BF16, DMUON_DTYPE_F16);
+  if (a->grad_dtype != a->dtype && a->grad_dtype != DMUON_DTYPE_F32)
+    return fail("%s: gradients are fp32 or of the operands' dtype, got code %d", who,
+                a->grad_dtype);
+  if (a->tokens < 0 || a->tokens > (1 << 24))
+    return fail("%s: tokens must be 0 .. 2^24, got %lld", who, (long long)a->tokens);
+  if (a->vocab < 1 || a->vocab > (1LL << 30) || a->dim < 1 || a->dim > (1 << 20))
+    return fail("%s: vocab must be 1 .. 2^30 and dim 1 .. 2^20, got %lld and %lld", who,
+                (long long)a->vocab, (long long)a->dim);
+  if (a->ld_hidden < a->dim || a->ld_weight < a->dim)
+    return fail("%s: the pitches of hidden and weight must be at least dim", who);
+  if (a->chunk_tokens < 0) return fail("%s: chunk_tokens must not be negative", who);
+  if (a->reduction != DMUON_LOSS_ROWS && a->reduction != DMUON_LOSS_MEAN &&
+      a->reduction != DMUON_LOSS_SUM)
+    return fail("%s: unknown reduction %d", who, a->reduction);
+  if ((a->targets != nullptr) == (a->teacher_ids != nullptr) && a->tokens > 0)
+    return fail("%s: needs either targets or a teacher's lists", who);
+  if (a->teacher_ids) {
+    if (a->k_list < 1 || a->k_list > 4096)
+      return fail("%s: k_list must be 1 .. 4096, got %lld", who, (long long)a->k_list);
+    if (!a->teacher_logits) return fail("%s: teacher_logits is NULL", who);
+    if (!(a->temperature > 0.f)) return fail("%s: temperature must be positive", who);
+    if (a->z_loss != 0.f) return fail("%s: z_loss goes with hard targets", who);
+  }
+  return 0;
+}
+
+Layout lay_out(const dmuon_head_loss_args& a) {
+  const bool grads = a.d_hidden || a.d_weight;
+  Layout l{};
+  const int64_t k = a.teacher_ids ? a.k_list : 1, tiles = round_up(a.vocab, kStatCols) / kStatCols;
+  l.ld = round_up(a.vocab, 256);
+  const int64_t row = l.ld * (grads ? 6 : 4) + tiles * 8;
+  l.chunk = a.chunk_tokens > 0 ? a.chunk_tokens : kChunkBytes / row;
+  if (l.chunk < 1) l.chunk = 1;
+  if (l.chunk > 256) l.chunk = l.chunk / 256 * 256;
+  if (l.chunk > a.tokens) l.chunk = a.tokens;
+  auto take = [&](int64_t bytes) {
+    const int64_t at = l.bytes;
+    l.bytes += round_up(bytes, 256);
+    return at;
+  };
+  l.ids = take(a.tokens * k * 4);
+  l.probs = take(a.tokens * k * 4);
+  l.mass = take(a.tokens * 4);
+  l.lse = take(a.tokens * 4);
+  l.row_weight = take(a.tokens * 4);
+  l.alpha = take(4);
+  l.Z = take(l.chunk * l.ld * 4);
+  l.stats = take(l.chunk * tiles * 8);
+  l.G = take(grads ? l.chunk * l.ld * 2 : 0);
+  l.part = take(a.d_weight && a.grad_dtype != DMUON_DTYPE_F32 && l.chunk < a.tokens
+                    ? a.vocab * a.dim * 4 : 0);
+  return l;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dmuon_head_loss_workspace_size(const dmuon_head_loss_args* args, int64_t* workspace_bytes) {
+  const char* who = "dmuon_head_loss_workspace_size";
+  if (!workspace_bytes) return fail("%s: NULL output", who);
+  if (check(who, args)) return 1;
+  *workspace_bytes = lay_out(*args).bytes;
+  return 0;
+}
+
+int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t workspace_bytes,
+                    void* stream_) {
+  const char* who = "dmuon_head_loss";
+  if (check(who, args)) return 1;
+  const dmuon_head_loss_args& a = *args;
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  const bool grads = a.d_hidden || a.d_weight;
+  if (!a.weight || (a.tokens > 0 && (!a.hidden || !a.loss)))
+    return fail("%s: NULL hidden, weight or loss", who);
+  if (a.reduction != DMUON_LOSS_ROWS && !a.reduced) return fail("%s: reduced is NULL", who);
+  if (a.reduction == DMUON_LOSS_ROWS && grads && a.tokens > 0 && !a.row_grad)
+    return fail("%s: the gradients of unreduced losses need row_grad", who);
+  const Layout l = lay_out(a);
+  if (workspace_bytes < l.bytes || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return fail("%s: needs a 256-byte aligned workspace of %lld bytes, got %lld", who,
+                (long long)l.bytes, (long long)workspace_bytes);
+  int elt = 0;
+  elt_of(a.dtype, &elt);
+  const int64_t grad_size = a.grad_dtype == DMUON_DTYPE_F32 ? 4 : 2;
+  char* ws = static_cast<char*>(workspace);
+  auto floats = [&](int64_t at) { return reinterpret_cast<float*>(ws + at); };
+
+  HeadRows r{};
+  r.n = (int)a.tokens;
+  r.vocab = (int)a.vocab;
+  r.k_list = a.teacher_ids ? (int)a.k_list : 1;
+  r.targets = a.targets;
+  r.teacher_ids = a.teacher_ids;
+  r.teacher_logits = a.teacher_logits;
+  r.teacher_lse = a.teacher_lse;
+  r.ignore_index = a.ignore_index;
+  r.z_loss = a.teacher_ids ? 0.f : a.z_loss;
+  r.temperature = a.teacher_ids ? a.temperature : 1.f;
+  r.reduction = a.reduction;
+  r.row_grad = a.reduction == DMUON_LOSS_ROWS ? a.row_grad : nullptr;
+  r.ids = reinterpret_cast<int*>(ws + l.ids);
+  r.probs = floats(l.probs);
+  r.mass = floats(l.mass);
+  r.lse = floats(l.lse);
+  r.loss = a.loss;
+  r.row_weight = floats(l.row_weight);
+  r.alpha = floats(l.alpha);
+  r.mean = a.reduced;
+  float* Z = floats(l.Z);
+  float2* stats = reinterpret_cast<float2*>(ws + l.stats);
+  uint16_t* G = reinterpret_cast<uint16_t*>(ws + l.G);
+  const uint16_t* H = static_cast<const uint16_t*>(a.hidden);
+  const uint16_t* W = static_cast<const uint16_t*>(a.weight);
+
+  if (check_launch(launch_head_targets(r, grads, stream), who)) return 1;
+  for (int64_t first = 0; first < a.tokens || first == 0; first += l.chunk) {
+    const int rows = (int)(a.tokens - first < l.chunk ? a.tokens - first : l.chunk);
+    HeadGemm g{};
+    g.elt = elt;
+    g.mode = HG_LOGITS;
+    g.A = H + first * a.ld_hidden; g.lda = a.ld_hidden;
+    g.B = W; g.ldb = a.ld_weight;
+    g.M = rows; g.N = (int)a.vocab; g.K = (int)a.dim;
+    g.scale = 1.f / r.temperature;
+    g.Z = Z; g.ldz = l.ld;
+    g.stats = stats;
+    if (check_launch(launch_head_gemm(g, stream), who)) return 1;
+    if (check_launch(launch_head_loss(r, (int)first, rows, Z, l.ld, stats, stream), who)) return 1;
+    if (grads) {
+      if (check_launch(launch_head_grad(r, (int)first, rows, Z, l.ld, G, l.ld, elt, stream), who))
+        return 1;
+      g = HeadGemm{};
+      g.elt = elt;
+      g.mode = HG_GRAD;
+      g.alpha = r.alpha;
+      g.out_dtype = a.grad_dtype;
+      if (a.d_hidden) {
+        g.A = G; g.lda = l.ld;
+        g.B = W; g.ldb = a.ld_weight; g.b_kmajor = 1;
+        g.M = rows; g.N = (int)a.dim; g.K = (int)a.vocab;
+        g.out = static_cast<char*>(a.d_hidden) + first * a.dim * grad_size; g.ldo = a.dim;
+        if (check_launch(launch_head_gemm(g, stream), who)) return 1;
+      }
+      if (a.d_weight) {
+        const bool last = first + rows >= a.tokens;
+        g.A = G; g.lda = l.ld; g.a_kmajor = 1;
+        g.B = H + first * a.ld_hidden; g.ldb = a.ld_hidden; g.b_kmajor = 1;
+        g.M = (int)a.vocab; g.N = (int)a.dim; g.K = rows;
+        g.out = last ? a.d_weight : nullptr; g.ldo = a.dim;
+        // fp32 results gather in place
+        g.part = grad_size == 4 ? static_cast<float*>(a.d_weight) : floats(l.part); g.ldp = a.dim;
+        g.add_part = first > 0;
+        if (check_launch(launch_head_gemm(g, stream), who)) return 1;
+      }
+    }
+    if (l.chunk <= 0) break;
+  }
+  if (a.reduction != DMUON_LOSS_ROWS && check_launch(launch_head_reduce(r, stream), who)) return 1;
+  return 0;
+}
+
+int dmuon_scale_by(const void* src, int src_dtype, void* dst, int dst_dtype, int64_t n,
+                   const float* factor, void* stream) {
+  const char* who = "dmuon_scale_by";
+  for (int t : {src_dtype, dst_dtype})
+    if (t != DMUON_DTYPE_F32 && t != DMUON_DTYPE_BF16 && t != DMUON_DTYPE_F16)
+      return fail("%s: unknown dtype code %d", who, t);
+  if (n < 0) return fail("%s: negative size", who);
+  if (n == 0) return 0;
+  if (!src || !dst || !factor) return fail("%s: NULL argument", who);
+  if (src == dst && src_dtype != dst_dtype) return fail("%s: in place needs one dtype", who);
+  return check_launch(launch_scale_by(src, src_dtype, dst, dst_dtype, n, factor,
+                                      static_cast<hipStream_t>(stream)), who);
+}
+
+}  // extern "C"

@@ -72,7 +72,7 @@ extern "C" {
 const char* dmuon_last_error(void);
 
 /* ABI version (major*100 + minor): DMUON_ABI_VERSION of the header the library was built with. */
-#define DMUON_ABI_VERSION 109
+#define DMUON_ABI_VERSION 110
 int dmuon_abi_version(void);
 
 /*
@@ -444,6 +444,104 @@ int dmuon_clip_norms(const int64_t* ptrs, const int64_t* numels, const int32_t* 
                      int64_t chunk_size, int n_tensors, int n_segments, double max_norm,
                      float* norms, float* coefs, uint8_t* clipped, uint8_t* found_inf,
                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Loss of a head's logits over a vocabulary, with its gradients (no reference counterpart). For
+ * hidden states H [tokens][dim] and the head's weight W [vocab][dim], z = H W^T:
+ *   hard targets (targets != NULL): loss[n] = lse(z_n) - z[n][targets[n]] + z_loss * lse(z_n)^2;
+ *     a token whose target is ignore_index is not counted and has loss 0;
+ *   a teacher's lists (teacher_ids != NULL): with p = softmax(z_n / temperature) and the target
+ *     probabilities q of the k_list classes teacher_ids[n][..] -- the softmax of their
+ *     teacher_logits / temperature, or exp(teacher_logits / temperature - teacher_lse[n]) where
+ *     the teacher's own log-sum-exp (of logits / temperature) is given --
+ *     loss[n] = temperature^2 * sum_k q_k (log q_k - log p[id_k]). Negative ids are padding; a
+ *     token with padding only is not counted and has loss 0. A class that occurs twice counts
+ *     twice.
+ * Any other class outside [0, vocab) gives the token a NaN loss. The logits are never held: rows
+ * go through the workspace chunk by chunk.
+ *   reduction: DMUON_LOSS_MEAN (over the counted tokens; 0 where there are none) and _SUM write
+ *     reduced[0]; DMUON_LOSS_ROWS writes loss[] only, and its gradients weigh token n's loss with
+ *     row_grad[n] (fp32).
+ *   d_hidden [tokens][dim], d_weight [vocab][dim]: dense results or NULL, of `dtype` or, with
+ *     grad_dtype DMUON_DTYPE_F32, fp32 (gradients that a loss scale is still to multiply: a mean
+ *     over many tokens underflows fp16). Both NULL: values only.
+ * hidden and weight are 16-bit words of `dtype` (DMUON_DTYPE_BF16 or _F16), row by row with their
+ * pitches in elements, at any element alignment; products accumulate in fp32, and the logit
+ * gradient is rounded once to `dtype` between the products. loss [tokens] is always written. Results
+ * do not depend on anything but the arguments (no atomics). chunk_tokens: tokens worked on at a
+ * time (0: a size that keeps the workspace near 4 GiB); a workspace of
+ * dmuon_head_loss_workspace_size bytes (256-byte aligned) is the caller's.
+ */
+#define DMUON_LOSS_ROWS 0
+#define DMUON_LOSS_MEAN 1
+#define DMUON_LOSS_SUM 2
+typedef struct {
+  const void* hidden;
+  const void* weight;
+  const int64_t* targets;
+  const int64_t* teacher_ids;
+  const float* teacher_logits;
+  const float* teacher_lse;
+  const float* row_grad;
+  float* loss;
+  float* reduced;
+  void* d_hidden;
+  void* d_weight;
+  int64_t ld_hidden, ld_weight;
+  int64_t tokens, vocab, dim, k_list, chunk_tokens, ignore_index;
+  float z_loss, temperature;
+  int dtype, grad_dtype, reduction;
+} dmuon_head_loss_args;
+int dmuon_head_loss_workspace_size(const dmuon_head_loss_args* args, int64_t* workspace_bytes);
+int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
+/* dst = factor[0] * src (factor fp32, on the device) for n dense values, src of src_dtype and dst
+ * of dst_dtype, both fp32, bf16 or fp16; dst may be src itself, and then nothing is read or written
+ * where the factor is 1. */
+int dmuon_scale_by(const void* src, int src_dtype, void* dst, int dst_dtype, int64_t n,
+                   const float* factor, void* stream);
+
+/*
+ * The norms around a block with its gate and residual scale (no reference counterpart):
+ *   u = y * rsqrt(mean(y^2) + eps) * w_post  (w_post NULL: u = y)
+ *   x_new = scale * x + gate * u             (gate NULL: 1; y NULL: x_new = scale * x)
+ *   h = x_new * rsqrt(mean(x_new^2) + eps) * w_pre
+ * for `rows` rows of dim (1 .. 32768) values. x, y, x_new, h and their gradients are of `dtype`
+ * (DMUON_DTYPE_F32, _BF16 or _F16), x, y and the incoming gradients with a row pitch, the results
+ * dense; w_pre, w_post [dim] and gate [gates][dim] each have a dtype of their own. Gate row g
+ * belongs to the rows / gates consecutive rows from g * rows / gates on. Any element alignment.
+ * Arithmetic and sums are fp32, every result is rounded once. stats [rows][2] (fp32, or NULL
+ * where no gradient follows) keeps what dmuon_residual_norm_grad needs of the rows.
+ * dmuon_residual_norm_grad: from dx_new and dh (either may be NULL: zero) the gradients dx, dy,
+ * d_pre, d_post and d_gate, in the dtypes of what they belong to; any may be NULL. The sums over
+ * rows have a fixed order. Both entry points read what they need of one descriptor.
+ */
+typedef struct {
+  const void* x;
+  const void* y;
+  const void* w_pre;
+  const void* w_post;
+  const void* gate;
+  float* stats;
+  void* x_new;
+  void* h;
+  const void* dx_new;
+  const void* dh;
+  void* dx;
+  void* dy;
+  void* d_pre;
+  void* d_post;
+  void* d_gate;
+  int64_t rows, dim, gates, ld_x, ld_y, ld_dx_new, ld_dh;
+  float scale, eps;
+  int dtype, pre_dtype, post_dtype, gate_dtype;
+} dmuon_residual_norm_args;
+int dmuon_residual_norm(const dmuon_residual_norm_args* args, void* stream);
+int dmuon_residual_norm_grad_workspace_size(const dmuon_residual_norm_args* args,
+                                            int64_t* workspace_bytes);
+int dmuon_residual_norm_grad(const dmuon_residual_norm_args* args, void* workspace,
+                             int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
