@@ -3,73 +3,112 @@
 //   hidden gradient dH = G W        (W k-major)
 //   weight gradient dW = G^T H      (both operands k-major)
 // with the softmax statistics of the logits' columns taken in the first one's epilogue.
+//
+// 256 x 256 tiles, 8 waves of 128 x 64 in two groups that run one phase apart: while one wave of a
+// SIMD issues the MFMAs of a 64-wide K slice from registers, its partner reads its next fragments
+// from LDS and moves operands (buffer loads straight into a two-slot LDS ring), so the matrix pipe
+// waits for neither. Both operands may be stored row by row (K contiguous) or k-major; a k-major
+// slice lies in LDS as four blocks of 64 values by 64 k-rows and is read through transposing LDS
+// reads. Sizes need no padding: loads past an operand's rows give 0 by the buffer range, loads past
+// K by an offset outside it (row form) or by the range of the slice (k-major), and a wave whose
+// whole sub-tile lies outside the result does no MFMA work.
 #include "dmuon_amd_internal.h"
 #include "head_loss.h"
+#include "mfma_tile.h"
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
+#include <type_traits>
 
 namespace dmuon {
 namespace {
 
-template <int E>
-__device__ __forceinline__ uint16_t to_elt(float f) {
-  if constexpr (E == ELT_F16) return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
-  else return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f));
-}
-template <int E>
-__device__ __forceinline__ f32x4_t mfma_16x16x32(bf16x8_t b, bf16x8_t a, f32x4_t c) {
-  if constexpr (E == ELT_F16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, b),
-                                                  __builtin_bit_cast(f16x8_t, a), c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a, c, 0, 0, 0);
-}
+constexpr int kTile = 256, kSlice = 64;
+constexpr float kInf = __builtin_inff();
+// rows of any pitch and bases of any element alignment
+typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
+typedef f32x4_t f32x4_any_t __attribute__((aligned(4)));
 
-// 64 x 64 tile, four waves of 16 rows; operands pass through registers one value at a time, so
-// any stride, alignment and size is right.
-template <int E, int MODE>
-__global__ __launch_bounds__(256) void head_gemm_kernel(HeadGemm a) {
-  constexpr int T = 64, BK = 32, PITCH = BK + 8;
-  __shared__ __attribute__((aligned(16))) uint16_t sa[T * PITCH], sb[T * PITCH];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int j0 = blockIdx.x * T, i0 = blockIdx.y * T;
-  f32x4_t acc[4] = {};
-  auto fill = [&](uint16_t* s, const uint16_t* X, long long ld, int kmajor, int r0, int rows,
-                  int k0) {
-    for (int e = tid; e < T * BK; e += 256) {
-      const int r = kmajor ? e % T : e / BK, k = kmajor ? e / T : e % BK;
-      uint16_t v = 0;
-      if (r0 + r < rows && k0 + k < a.K)
-        v = kmajor ? X[(long long)(k0 + k) * ld + r0 + r] : X[(long long)(r0 + r) * ld + k0 + k];
-      s[r * PITCH + k] = v;
+using T = Tile<256, 256, 64, 2, 2, 4>;
+
+// One operand's part of the LDS ring: what each wave v of a group moves of a slice, in instructions
+// of 8 rows (k-major: k-rows) of 128 bytes. A lane's place in instruction q + 2 is 16 rows further,
+// and the swizzle moves its chunk of 8 values by an xor of 4 chunks between even and odd q, so one
+// byte offset and one chunk a lane describe them all.
+template <bool KM>
+struct Mover {
+  const uint16_t* base;                   // the tile's first row (k-major: first value)
+  long long ld;
+  int rows, K, width;                     // rows of the tile inside the operand; k-major: values
+  unsigned off;                           // byte offset of this lane's row in instruction 0
+  int chunk;                              // first value of its chunk
+  char* lds;
+
+  // B: this wave's block of 64 rows (values); A in row form: rows v * 32 and 128 + v * 32
+  __device__ __forceinline__ void init(const uint16_t* X, long long ld_, int r0, int n, int k,
+                                       int v, int rows_of_wave, int lane, char* lds_) {
+    ld = ld_;
+    K = k;
+    rows = min(kTile, n - r0);
+    width = (n + 7) / 8 * 8 - r0;         // whole chunks: the rows are padded to them
+    static_assert(T::CPR == 8 && T::RPI == 8 && T::RPL == 2, "8 rows of 8 chunks an instruction");
+    if constexpr (KM) {
+      base = X + r0;
+      lds = lds_ + v * kSlice * 128;
+      chunk = 8 * ((lane & 7) ^ kswz64(lane >> 3));
+      off = (unsigned)((lane >> 3) * ld + v * 64) * 2u;
+    } else {
+      base = X + (long long)r0 * ld;
+      lds = lds_ + v * rows_of_wave * T::ROWB;
+      chunk = 8 * T::slot(lane & 7, lane >> 3);
+      off = (unsigned)((v * rows_of_wave + (lane >> 3)) * ld) * 2u;
     }
-  };
-  for (int k0 = 0; k0 < a.K; k0 += BK) {
-    fill(sa, a.A, a.lda, a.a_kmajor, i0, a.M, k0);
-    fill(sb, a.B, a.ldb, a.b_kmajor, j0, a.N, k0);
-    __syncthreads();
-    const int at = (lane & 15) * PITCH + 8 * (lane >> 4);
-    const bf16x8_t af = *reinterpret_cast<const bf16x8_t*>(sa + wave * 16 * PITCH + at);
-#pragma unroll
-    for (int y = 0; y < 4; ++y)
-      acc[y] = mfma_16x16x32<E>(*reinterpret_cast<const bf16x8_t*>(sb + y * 16 * PITCH + at), af,
-                                acc[y]);
-    __syncthreads();
   }
-  // a lane holds row lane % 16, columns 16 y + 4 (lane / 16) .. + 3
-  const int i = i0 + wave * 16 + (lane & 15), jl = j0 + 4 * (lane >> 4);
-  if constexpr (MODE == HG_LOGITS) {
-    float m = -__builtin_inff();
+  // N instructions of slice `s` into ring slot `slot`, starting `hi` rows further
+  template <int N>
+  __device__ __forceinline__ void issue(int s, int slot, int hi) const {
+    typedef __attribute__((address_space(3))) void* lds_ptr_t;
+    const int k0 = s * kSlice;
+    const uint16_t* p = base;
+    int bytes;
+    if constexpr (KM) {
+      p += (long long)k0 * ld;
+      bytes = (int)(((long long)(min(kSlice, K - k0) - 1) * ld + width) * 2);
+    } else {
+      bytes = (int)(((long long)(rows - 1) * ld + (K + 7) / 8 * 8) * 2);
+    }
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(p), (short)0, bytes, 0x00020000);
+    const unsigned step = 8u * (unsigned)ld * 2u;
 #pragma unroll
-    for (int y = 0; y < 4; ++y)
+    for (int q = 0; q < N; ++q) {
+      const int c = chunk ^ (32 * (q & 1));
+      unsigned o = off + (unsigned)c * 2u + (unsigned)hi * (unsigned)ld * 2u + (unsigned)q * step;
+      // a chunk past K in the last slice: an offset outside any range reads 0
+      if constexpr (!KM) o = c + k0 >= K ? 0x80000000u : o + (unsigned)k0 * 2u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (lds_ptr_t)(lds + slot * T::STAGE + hi * T::ROWB + q * 1024), 16, o, 0, 0, 0);
+    }
+  }
+};
+
+// Statistics and values of a wave's 128 x 64 logits.
+__device__ __forceinline__ void logits_epilogue(const HeadGemm& a, const f32x4_t (&acc)[8][4],
+                                                int iw, int jw, int lane) {
+  const int j = jw + 4 * (lane >> 4);
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    const int i = iw + 16 * x + (lane & 15);
+    f32x4_t z[4];
+    float m = -kInf;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int j = jl + 16 * y + e;
-        const float z = acc[y][e] * a.scale;
-        if (j < a.N) m = fmaxf(m, z);
-        if (a.Z && i < a.M && j < a.N) a.Z[(long long)i * a.ldz + j] = z;
+        z[y][e] = acc[x][y][e] * a.scale;
+        if (j + 16 * y + e < a.N) m = fmaxf(m, z[y][e]);
       }
+      if (a.Z && i < a.M)
+        *reinterpret_cast<f32x4_t*>(a.Z + (long long)i * a.ldz + j + 16 * y) = z[y];
+    }
     m = fmaxf(m, __shfl_xor(m, 16));
     m = fmaxf(m, __shfl_xor(m, 32));
     float s = 0.f;
@@ -77,46 +116,301 @@ __global__ __launch_bounds__(256) void head_gemm_kernel(HeadGemm a) {
     for (int y = 0; y < 4; ++y)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (jl + 16 * y + e < a.N) {
-          const float z = acc[y][e] * a.scale;
-          s += z == -__builtin_inff() ? 0.f : __expf(z - m);
-        }
+        if (j + 16 * y + e < a.N) s += z[y][e] == -kInf ? 0.f : __expf(z[y][e] - m);
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
-    if (lane < 16 && i < a.M) a.stats[(long long)blockIdx.x * a.M + i] = make_float2(m, s);
-  } else {
-    if (i >= a.M) return;
-    const float alpha = a.out ? a.alpha[0] : 1.f;
-#pragma unroll
-    for (int y = 0; y < 4; ++y)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = jl + 16 * y + e;
-        if (j >= a.N) continue;
-        float v = acc[y][e];
-        if (a.add_part) v += a.part[(long long)i * a.ldp + j];
-        const long long o = (long long)i * a.ldo + j;
-        if (!a.out) a.part[(long long)i * a.ldp + j] = v;
-        else if (a.out_dtype == DT_F32) static_cast<float*>(a.out)[o] = alpha * v;
-        else static_cast<uint16_t*>(a.out)[o] = to_elt<E>(alpha * v);
-      }
+    if (lane < 16 && i < a.M) a.stats[(long long)(jw / kStatCols) * a.M + i] = make_float2(m, s);
   }
+}
+
+// A wave's 128 x 64 values of a gradient: fp32 sums, or the scaled result. 16-bit results pass
+// through LDS slab by slab, so that the stores are whole 128-byte row segments.
+template <int E>
+__device__ __forceinline__ void grad_epilogue(const HeadGemm& a, f32x4_t (&acc)[8][4], int iw,
+                                              int jw, int lane, char* slab, int split) {
+  const int jl = 4 * (lane >> 4);
+  const bool whole = a.out && a.splits == 1;
+  const float alpha = whole ? a.alpha[0] : 1.f;
+  const bool f32 = !whole || a.out_dtype == DT_F32;
+  float* part = a.part + (a.splits > 1 ? (long long)split * a.M * a.ldp : 0);
+  float* dst = whole ? static_cast<float*>(a.out) : part;
+  const long long ldd = whole ? a.ldo : a.ldp;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    const int i = iw + 16 * x + (lane & 15);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int j = jw + jl + 16 * y;
+      f32x4_t v = acc[x][y];
+      if (a.add_part && i < a.M && j < a.N) {
+        const float* p = part + (long long)i * a.ldp + j;
+        if (j + 3 < a.N) v += *reinterpret_cast<const f32x4_any_t*>(p);
+        else
+          for (int e = 0; e < 4; ++e)
+            if (j + e < a.N) v[e] += p[e];
+      }
+      v *= alpha;
+      if (f32) {
+        if (i >= a.M || j >= a.N) continue;
+        float* p = dst + (long long)i * ldd + j;
+        if (j + 3 < a.N) *reinterpret_cast<f32x4_any_t*>(p) = v;
+        else
+          for (int e = 0; e < 4; ++e)
+            if (j + e < a.N) p[e] = v[e];
+      } else {
+        const u32x2_t o = {pack2_elt<E>(v[0], v[1]), pack2_elt<E>(v[2], v[3])};
+        *reinterpret_cast<u32x2_t*>(slab + (16 * (x & 1) + (lane & 15)) * T::EPN +
+                                    (jl + 16 * y) * 2) = o;
+      }
+    }
+    if (!f32 && (x & 1)) {
+      const int cr = lane >> 3, cc = lane & 7;
+      u32x4_t d[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        d[k] = *reinterpret_cast<const u32x4_t*>(slab + (8 * k + cr) * T::EPN + 16 * cc);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = iw + 16 * (x - 1) + 8 * k + cr, c = jw + 8 * cc;
+        if (r >= a.M || c >= a.N) continue;
+        uint16_t* p = static_cast<uint16_t*>(a.out) + (long long)r * a.ldo + c;
+        if (c + 7 < a.N) {
+          __builtin_nontemporal_store(d[k], reinterpret_cast<u32x4_any_t*>(p));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c + e < a.N) p[e] = (uint16_t)(d[k][e >> 1] >> (16 * (e & 1)));
+        }
+      }
+    }
+  }
+}
+
+// One tile. Group 0 (waves 0-3) owns tile rows 0-127, group 1 rows 128-255:
+//   group 0:  |0 M0 |1 C0 |2 M1 |3 C1 |4 ...         |2KT-1 C(KT-1) |2KT epilogue
+//   group 1:  |0    |1 M0 |2 C0 |3 M1 |4 ... M(KT-1) |2KT C(KT-1), epilogue
+// M(k): fragments of slice k into registers; C(k): its MFMAs. The refill DMA is issued in memory
+// phases: group 0's M(k) starts A of slice k + 1 (its slot's last readers ended at the barrier that
+// opened the phase) and waits for it at the end of C(k); group 1's M(k) refills each wave's own B
+// block with slice k + 2 after its own reads of it (group 0 read it in the phase before) and waits
+// for slice k + 1's B. LIVE false: the wave's sub-tile lies outside the result; it moves operands
+// and passes the barriers only.
+template <int E, int MODE, bool AKM, bool BKM, bool LIVE>
+__device__ __forceinline__ void head_tile(const HeadGemm& a, char* smem, int bi, int bj, int split) {
+  constexpr int KS = kSlice / 32;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int grp = wave >> 2, v = wave & 3;
+  const int wj = grp == 0 ? 3 - v : v;    // group 1's wave v reads the B block it moves
+  const int i0 = bi * kTile, j0 = bj * kTile;
+
+  Mover<AKM> ma;
+  Mover<BKM> mb;
+  ma.init(a.A, a.lda, i0, a.M, a.K, v, 32, lane, smem);
+  mb.init(a.B, a.ldb, j0, a.N, a.K, v, 64, lane, smem + T::A_BYTES);
+  auto issue_a = [&](int s, int slot) {
+    if constexpr (AKM) {
+      ma.template issue<8>(s, slot, 0);
+    } else {
+      ma.template issue<4>(s, slot, 0);
+      ma.template issue<4>(s, slot, 128);
+    }
+  };
+
+  f32x4_t acc[8][4];
+#pragma unroll
+  for (int x = 0; x < 8; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) acc[x][y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  const int arow0 = grp * 128 + (lane & 15), brow0 = wj * 64 + (lane & 15), kq = lane >> 4;
+  int kaoff[4], kboff[4];
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    kaoff[y] = AKM ? grp * 2 * kSlice * 128 + kmajor64_lane_off(lane, 16 * y) : 0;
+    kboff[y] = BKM ? wj * kSlice * 128 + kmajor64_lane_off(lane, 16 * y) : 0;
+  }
+  bf16x8_t af[KS][8], bfr[KS][4];
+  auto mem_phase = [&](int slot) {
+    if constexpr (!LIVE) return;
+    const char* sa = smem + slot * T::STAGE;
+    const char* sb = sa + T::A_BYTES;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int kc = ks * 4 + kq;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int row = arow0 + x * 16;
+        if constexpr (AKM)
+          af[ks][x] = read_kmajor(sa + kaoff[x & 3] + (x >> 2) * kSlice * 128 + ks * 32 * 128, 128);
+        else
+          af[ks][x] = *reinterpret_cast<const bf16x8_t*>(sa + row * T::ROWB + (T::slot(kc, row) << 4));
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int row = brow0 + y * 16;
+        if constexpr (BKM)
+          bfr[ks][y] = read_kmajor(sb + kboff[y] + ks * 32 * 128, 128);
+        else
+          bfr[ks][y] = *reinterpret_cast<const bf16x8_t*>(sb + row * T::ROWB + (T::slot(kc, row) << 4));
+      }
+    }
+  };
+  auto compute_phase = [&]() {
+    if constexpr (!LIVE) return;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[x][y] = mfma_16x16x32<E>(bfr[ks][y], af[ks][x], acc[x][y]);
+  };
+
+  // slices of this split
+  const int all = (a.K + kSlice - 1) / kSlice, per = (all + a.splits - 1) / a.splits;
+  const int s0 = split * per, KT = min(per, all - s0);
+  if (KT > 0) {
+    if (grp == 1) {
+      // slices 0 and 1 (past the end: the last slice again, into a slot never read)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        issue_a(s0 + min(s, KT - 1), s);
+        mb.template issue<8>(s0 + min(s, KT - 1), s, 0);
+      }
+      wait_vmcnt<16>();                   // slice 0 has landed
+    }
+    phase_barrier();
+    if (grp == 1) phase_barrier();        // group 1 starts one phase behind
+    auto iteration = [&](int kt, auto ra_c, auto rb_c, auto last_c) {
+      constexpr bool RA = decltype(ra_c)::value, RB = decltype(rb_c)::value;
+      constexpr bool LAST = decltype(last_c)::value;
+      mem_phase(kt & 1);
+      if (RA && grp == 0) issue_a(s0 + kt + 1, (kt + 1) & 1);
+      __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): this wave's fragments are in registers
+      if (grp == 1) {
+        if (RB) {
+          mb.template issue<8>(s0 + kt + 2, kt & 1, 0);
+          wait_vmcnt<8>();                // all of slice kt + 1 has landed
+        } else {
+          wait_vmcnt<0>();
+        }
+      }
+      phase_barrier();
+      compute_phase();
+      if (RA && grp == 0) wait_vmcnt<0>();  // slice kt + 1's A has landed
+      // the last slice: group 1 stops at the barrier before its MFMAs, which is also the one after
+      // group 0's; no wave reads the ring after it
+      if (!(LAST && grp == 1)) phase_barrier();
+    };
+    const std::false_type no{};
+    const std::true_type yes{};
+    if (KT >= 3) {
+      iteration(0, no, yes, no);
+      int kt = 1;
+      for (; kt + 2 < KT; ++kt) iteration(kt, yes, yes, no);
+      iteration(kt, yes, no, no);
+      iteration(kt + 1, no, no, yes);
+    } else {
+      for (int kt = 0; kt + 1 < KT; ++kt) iteration(kt, no, no, no);
+      iteration(KT - 1, no, no, yes);
+    }
+    wait_vmcnt<0>();
+  }
+  if constexpr (LIVE) {
+    const int iw = i0 + grp * 128, jw = j0 + wj * 64;
+    if constexpr (MODE == HG_LOGITS) logits_epilogue(a, acc, iw, jw, lane);
+    else grad_epilogue<E>(a, acc, iw, jw, lane, smem + wave * T::EPI_REGION, split);
+  }
+}
+
+template <int E, int MODE, bool AKM, bool BKM>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void head_gemm_kernel(const HeadGemm a) {
+  __shared__ __attribute__((aligned(16))) char smem[T::LDS_BYTES];
+  // groups of 8 tile rows walked column by column, so that the tiles an XCD holds share panels
+  const int mt = (a.M + kTile - 1) / kTile, nt = (a.N + kTile - 1) / kTile;
+  int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = t / (mt * nt);
+  t -= split * mt * nt;
+  const int g = t / (8 * nt), rows = min(mt - 8 * g, 8), r = t - g * 8 * nt;
+  const int bi = __builtin_amdgcn_readfirstlane(8 * g + r % rows);
+  const int bj = __builtin_amdgcn_readfirstlane(r / rows);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int grp = wave >> 2, v = wave & 3;
+  const bool live = bi * kTile + 128 * grp < a.M && bj * kTile + 64 * (grp == 0 ? 3 - v : v) < a.N;
+  const int sp = __builtin_amdgcn_readfirstlane(split);
+  if (live) head_tile<E, MODE, AKM, BKM, true>(a, smem, bi, bj, sp);
+  else head_tile<E, MODE, AKM, BKM, false>(a, smem, bi, bj, sp);
+}
+
+// out = alpha * sum over the splits
+template <int D>
+__global__ __launch_bounds__(256) void join_splits_kernel(const HeadGemm a) {
+  const long long n = (long long)a.M * a.N;
+  const float alpha = a.alpha[0];
+  for (long long k = blockIdx.x * 256LL + threadIdx.x; k < n; k += 256LL * gridDim.x) {
+    const long long i = k / a.N, j = k - i * a.N;
+    float s = 0.f;
+    for (int p = 0; p < a.splits; ++p) s += a.part[((long long)p * a.M + i) * a.ldp + j];
+    s *= alpha;
+    if constexpr (D == DT_F32) static_cast<float*>(a.out)[i * a.ldo + j] = s;
+    else static_cast<uint16_t*>(a.out)[i * a.ldo + j] = to_elt<D == DT_F16 ? ELT_F16 : ELT_BF16>(s);
+  }
+}
+
+long long tiles_of(int M, int N) {
+  return ((long long)M + kTile - 1) / kTile * ((N + kTile - 1) / kTile);
 }
 
 }  // namespace
 
+int head_gemm_splits(int M, int N, int K) {
+  constexpr int kCus = 256, kLeast = 8;
+  const long long tiles = tiles_of(M, N);
+  const int slices = (K + kSlice - 1) / kSlice;
+  if (tiles <= 0 || tiles > kCus / 2) return 1;
+  long long s = kCus / tiles;
+  if (s > slices / kLeast) s = slices / kLeast;
+  if (s <= 1) return 1;
+  const int per = (int)((slices + s - 1) / s);
+  return (slices + per - 1) / per;        // no empty split
+}
+
 hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
-  const long long nb = (a.N + 63) / 64, mb = (a.M + 63) / 64;
-  if (mb > 65535) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)nb, (unsigned)mb);
-#define DMUON_HG(E, MODE) hipLaunchKernelGGL((head_gemm_kernel<E, MODE>), grid, dim3(256), 0, stream, a)
-  if (a.elt == ELT_F16) {
-    if (a.mode == HG_LOGITS) DMUON_HG(ELT_F16, HG_LOGITS); else DMUON_HG(ELT_F16, HG_GRAD);
-  } else {
-    if (a.mode == HG_LOGITS) DMUON_HG(ELT_BF16, HG_LOGITS); else DMUON_HG(ELT_BF16, HG_GRAD);
-  }
+  const long long nb = tiles_of(a.M, a.N) * a.splits;
+  // 32-bit offsets inside a tile's 256 rows (or a slice's 64), whole 16-byte chunks
+  const auto fits = [](const void* p, long long ld, long long width) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && ld >= width && ld < (1 << 22);
+  };
+  if (a.splits < 1 || nb > 0x7fffffffLL || a.K < 0 ||
+      (a.K > 0 && (!fits(a.A, a.lda, a.a_kmajor ? a.M : a.K) ||
+                   !fits(a.B, a.ldb, a.b_kmajor ? a.N : a.K))))
+    return hipErrorInvalidValue;
+  if (a.splits > 1 && (a.mode != HG_GRAD || !a.out || !a.part || a.add_part))
+    return hipErrorInvalidValue;
+  const dim3 grid((unsigned)nb);
+#define DMUON_HG(E, MODE, AKM, BKM) \
+  hipLaunchKernelGGL((head_gemm_kernel<E, MODE, AKM, BKM>), grid, dim3(512), 0, stream, a)
+#define DMUON_HG_E(E)                                                     \
+  do {                                                                    \
+    if (a.mode == HG_LOGITS) DMUON_HG(E, HG_LOGITS, false, false);        \
+    else if (a.a_kmajor) DMUON_HG(E, HG_GRAD, true, true);                \
+    else DMUON_HG(E, HG_GRAD, false, true);                               \
+  } while (0)
+  if ((a.mode == HG_LOGITS) != (!a.a_kmajor && !a.b_kmajor) || (a.mode == HG_GRAD && !a.b_kmajor))
+    return hipErrorInvalidValue;
+  if (a.elt == ELT_F16) DMUON_HG_E(ELT_F16);
+  else DMUON_HG_E(ELT_BF16);
+#undef DMUON_HG_E
 #undef DMUON_HG
+  if (a.splits > 1) {
+    const long long n = ((long long)a.M * a.N + 255) / 256;
+    const dim3 jg((unsigned)(n < 4096 ? n : 4096));
+    if (a.out_dtype == DT_F32) hipLaunchKernelGGL(join_splits_kernel<DT_F32>, jg, dim3(256), 0, stream, a);
+    else if (a.out_dtype == DT_F16) hipLaunchKernelGGL(join_splits_kernel<DT_F16>, jg, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(join_splits_kernel<DT_BF16>, jg, dim3(256), 0, stream, a);
+  }
   return hipGetLastError();
 }
 

@@ -34,7 +34,12 @@ struct HeadGemm {
   void* out; long long ldo; int out_dtype;   // HG_GRAD: result (DT_F32 or the operands'), or NULL
   float* part; long long ldp;             // HG_GRAD: fp32 sums [M][ldp], or NULL
   int add_part;                           // part holds earlier sums to add to
+  int splits;                             // HG_GRAD: K in so many parts, part [splits][M][ldp]
 };
+// K splits that fill the chip where a gradient has few tiles (1: none).
+int head_gemm_splits(int M, int N, int K);
+// Operands at 16-byte alignment with pitches of whole 16-byte chunks. Rows that end inside a chunk
+// are readable to its end, and hold zeros there in row form (past K).
 hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream);
 
 // One call's rows as the kernels see them. Entry k of row n is the class ids[n * k_list + k] with

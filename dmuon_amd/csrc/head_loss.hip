@@ -16,10 +16,20 @@ int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 // Workspace of a chunk's logits and logit gradient; a call of more tokens takes several chunks.
 constexpr int64_t kChunkBytes = int64_t(2) << 30;
 
+// The pitch of the logits stays inside the products' 32-bit tile offsets.
+constexpr int64_t kMaxVocab = (int64_t(1) << 22) - 256;
+
 struct Layout {
   int64_t chunk, ld;                      // tokens of a chunk, pitch of its logits
-  int64_t ids, probs, mass, lse, row_weight, alpha, Z, stats, G, part, bytes;
+  int64_t ids, probs, mass, lse, row_weight, alpha, Z, stats, G, part, H, W, bytes;
+  int64_t pad;                            // pitch of the copies of hidden and weight
+  bool copy_h, copy_w;
 };
+
+// The products read whole 16-byte chunks of aligned rows; anything else runs on zero-padded copies.
+bool in_place(const void* p, int64_t ld, int64_t dim) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && dim % 8 == 0 && ld < (1 << 22);
+}
 
 int elt_of(int dtype, int* elt) {
   if (dtype == DMUON_DTYPE_BF16) *elt = ELT_BF16;
@@ -39,9 +49,9 @@ int check(const char* who, const dmuon_head_loss_args* a) {
                 a->grad_dtype);
   if (a->tokens < 0 || a->tokens > (1 << 24))
     return fail("%s: tokens must be 0 .. 2^24, got %lld", who, (long long)a->tokens);
-  if (a->vocab < 1 || a->vocab > (1LL << 30) || a->dim < 1 || a->dim > (1 << 20))
-    return fail("%s: vocab must be 1 .. 2^30 and dim 1 .. 2^20, got %lld and %lld", who,
-                (long long)a->vocab, (long long)a->dim);
+  if (a->vocab < 1 || a->vocab > kMaxVocab || a->dim < 1 || a->dim > (1 << 20))
+    return fail("%s: vocab must be 1 .. %lld and dim 1 .. 2^20, got %lld and %lld", who,
+                (long long)kMaxVocab, (long long)a->vocab, (long long)a->dim);
   if (a->ld_hidden < a->dim || a->ld_weight < a->dim)
     return fail("%s: the pitches of hidden and weight must be at least dim", who);
   if (a->chunk_tokens < 0) return fail("%s: chunk_tokens must not be negative", who);
@@ -84,8 +94,25 @@ Layout lay_out(const dmuon_head_loss_args& a) {
   l.Z = take(l.chunk * l.ld * 4);
   l.stats = take(l.chunk * tiles * 8);
   l.G = take(grads ? l.chunk * l.ld * 2 : 0);
-  l.part = take(a.d_weight && a.grad_dtype != DMUON_DTYPE_F32 && l.chunk < a.tokens
-                    ? a.vocab * a.dim * 4 : 0);
+  // fp32 sums: the weight's gradient over several chunks, or of split products
+  int64_t part = 0;
+  if (a.d_weight && l.chunk < a.tokens) {
+    if (a.grad_dtype != DMUON_DTYPE_F32) part = a.vocab * a.dim * 4;
+  } else if (a.d_weight) {
+    const int s = head_gemm_splits((int)a.vocab, (int)a.dim, (int)a.tokens);
+    if (s > 1) part = s * a.vocab * a.dim * 4;
+  }
+  if (a.d_hidden)
+    for (int64_t rows : {l.chunk, l.chunk > 0 ? a.tokens % l.chunk : 0}) {
+      const int s = head_gemm_splits((int)rows, (int)a.dim, (int)a.vocab);
+      if (s > 1 && s * rows * a.dim * 4 > part) part = s * rows * a.dim * 4;
+    }
+  l.part = take(part);
+  l.pad = round_up(a.dim, 64);
+  l.copy_h = !in_place(a.hidden, a.ld_hidden, a.dim);
+  l.copy_w = !in_place(a.weight, a.ld_weight, a.dim);
+  l.H = take(l.copy_h ? l.chunk * l.pad * 2 : 0);
+  l.W = take(l.copy_w ? a.vocab * l.pad * 2 : 0);
   return l;
 }
 
@@ -150,14 +177,34 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
   const uint16_t* H = static_cast<const uint16_t*>(a.hidden);
   const uint16_t* W = static_cast<const uint16_t*>(a.weight);
 
+  // the fp32 sums' place is free for split products where no weight gradient gathers in it
+  const bool gathers = a.d_weight && l.chunk < a.tokens, split_h = !gathers || grad_size == 4;
+  int64_t ldw = a.ld_weight;
+  if (l.copy_w) {
+    uint16_t* copy = reinterpret_cast<uint16_t*>(ws + l.W);
+    if (check_launch(launch_pad_copy(W, a.ld_weight, 0, copy, l.pad, 0, (int)a.vocab, (int)a.dim,
+                                     (int)a.vocab, (int)l.pad, 1, stream), who)) return 1;
+    W = copy;
+    ldw = l.pad;
+  }
   if (check_launch(launch_head_targets(r, grads, stream), who)) return 1;
   for (int64_t first = 0; first < a.tokens || first == 0; first += l.chunk) {
     const int rows = (int)(a.tokens - first < l.chunk ? a.tokens - first : l.chunk);
+    const uint16_t* Hc = H + first * a.ld_hidden;
+    int64_t ldh = a.ld_hidden;
+    if (l.copy_h) {
+      uint16_t* copy = reinterpret_cast<uint16_t*>(ws + l.H);
+      if (check_launch(launch_pad_copy(Hc, a.ld_hidden, 0, copy, l.pad, 0, rows, (int)a.dim, rows,
+                                       (int)l.pad, 1, stream), who)) return 1;
+      Hc = copy;
+      ldh = l.pad;
+    }
     HeadGemm g{};
     g.elt = elt;
     g.mode = HG_LOGITS;
-    g.A = H + first * a.ld_hidden; g.lda = a.ld_hidden;
-    g.B = W; g.ldb = a.ld_weight;
+    g.splits = 1;
+    g.A = Hc; g.lda = ldh;
+    g.B = W; g.ldb = ldw;
     g.M = rows; g.N = (int)a.vocab; g.K = (int)a.dim;
     g.scale = 1.f / r.temperature;
     g.Z = Z; g.ldz = l.ld;
@@ -174,19 +221,23 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
       g.out_dtype = a.grad_dtype;
       if (a.d_hidden) {
         g.A = G; g.lda = l.ld;
-        g.B = W; g.ldb = a.ld_weight; g.b_kmajor = 1;
+        g.B = W; g.ldb = ldw; g.b_kmajor = 1;
         g.M = rows; g.N = (int)a.dim; g.K = (int)a.vocab;
+        g.splits = split_h ? head_gemm_splits(rows, g.N, g.K) : 1;
+        g.part = floats(l.part); g.ldp = a.dim;
         g.out = static_cast<char*>(a.d_hidden) + first * a.dim * grad_size; g.ldo = a.dim;
         if (check_launch(launch_head_gemm(g, stream), who)) return 1;
       }
       if (a.d_weight) {
         const bool last = first + rows >= a.tokens;
         g.A = G; g.lda = l.ld; g.a_kmajor = 1;
-        g.B = H + first * a.ld_hidden; g.ldb = a.ld_hidden; g.b_kmajor = 1;
+        g.B = Hc; g.ldb = ldh; g.b_kmajor = 1;
         g.M = (int)a.vocab; g.N = (int)a.dim; g.K = rows;
+        g.splits = gathers ? 1 : head_gemm_splits(g.M, g.N, g.K);
         g.out = last ? a.d_weight : nullptr; g.ldo = a.dim;
         // fp32 results gather in place
-        g.part = grad_size == 4 ? static_cast<float*>(a.d_weight) : floats(l.part); g.ldp = a.dim;
+        g.part = gathers && grad_size == 4 ? static_cast<float*>(a.d_weight) : floats(l.part);
+        g.ldp = a.dim;
         g.add_part = first > 0;
         if (check_launch(launch_head_gemm(g, stream), who)) return 1;
       }
