@@ -90,10 +90,13 @@ struct Mover {
   }
 };
 
-// Statistics and values of a wave's 128 x 64 logits.
+// A wave's 128 x 64 logits: statistics, and the exponentials (through LDS slab by slab, so that the
+// stores are whole 128-byte row segments) or the logits themselves.
+template <int MODE>
 __device__ __forceinline__ void logits_epilogue(const HeadGemm& a, const f32x4_t (&acc)[8][4],
-                                                int iw, int jw, int lane) {
-  const int j = jw + 4 * (lane >> 4);
+                                                int iw, int jw, int lane, char* slab) {
+  const int jl = 4 * (lane >> 4);
+  const bool inside = jw + 64 <= a.N;
 #pragma unroll
   for (int x = 0; x < 8; ++x) {
     const int i = iw + 16 * x + (lane & 15);
@@ -104,22 +107,51 @@ __device__ __forceinline__ void logits_epilogue(const HeadGemm& a, const f32x4_t
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         z[y][e] = acc[x][y][e] * a.scale;
-        if (j + 16 * y + e < a.N) m = fmaxf(m, z[y][e]);
+        // columns past the vocabulary: no maximum, no share of the sum
+        if (!inside && jw + jl + 16 * y + e >= a.N) z[y][e] = -kInf;
+        m = fmaxf(m, z[y][e]);
       }
-      if (a.Z && i < a.M)
-        *reinterpret_cast<f32x4_t*>(a.Z + (long long)i * a.ldz + j + 16 * y) = z[y];
+      if (MODE == HG_LOGITS && i < a.M)
+        *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.Z) + (long long)i * a.ldz + jw + jl +
+                                    16 * y) = z[y];
     }
     m = fmaxf(m, __shfl_xor(m, 16));
     m = fmaxf(m, __shfl_xor(m, 32));
     float s = 0.f;
 #pragma unroll
-    for (int y = 0; y < 4; ++y)
+    for (int y = 0; y < 4; ++y) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (j + 16 * y + e < a.N) s += z[y][e] == -kInf ? 0.f : __expf(z[y][e] - m);
+      for (int e = 0; e < 4; ++e) {
+        z[y][e] = z[y][e] == -kInf ? 0.f : __expf(z[y][e] - m);
+        s += z[y][e];
+      }
+      if constexpr (MODE == HG_EXP) {
+        constexpr float up = (float)(1 << kExpShift);
+        const u32x2_t o = {pack2_elt<ELT_F16>(up * z[y][0], up * z[y][1]),
+                           pack2_elt<ELT_F16>(up * z[y][2], up * z[y][3])};
+        *reinterpret_cast<u32x2_t*>(slab + (16 * (x & 1) + (lane & 15)) * T::EPN +
+                                    (jl + 16 * y) * 2) = o;
+      }
+    }
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
-    if (lane < 16 && i < a.M) a.stats[(long long)(jw / kStatCols) * a.M + i] = make_float2(m, s);
+    if (lane < 16 && i < a.M)
+      a.stats[(long long)i * a.n_stats + jw / kStatCols] = make_float2(m, s);
+    if (MODE == HG_EXP && (x & 1)) {
+      const int cr = lane >> 3, cc = lane & 7;
+      u32x4_t d[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        d[k] = *reinterpret_cast<const u32x4_t*>(slab + (8 * k + cr) * T::EPN + 16 * cc);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = iw + 16 * (x - 1) + 8 * k + cr;
+        if (r < a.M)
+          __builtin_nontemporal_store(
+              d[k], reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.Z) + (long long)r * a.ldz +
+                                               jw + 8 * cc));
+      }
+    }
   }
 }
 
@@ -318,8 +350,9 @@ __device__ __forceinline__ void head_tile(const HeadGemm& a, char* smem, int bi,
   }
   if constexpr (LIVE) {
     const int iw = i0 + grp * 128, jw = j0 + wj * 64;
-    if constexpr (MODE == HG_LOGITS) logits_epilogue(a, acc, iw, jw, lane);
-    else grad_epilogue<E>(a, acc, iw, jw, lane, smem + wave * T::EPI_REGION, split);
+    char* slab = smem + wave * T::EPI_REGION;
+    if constexpr (MODE == HG_GRAD) grad_epilogue<E>(a, acc, iw, jw, lane, slab, split);
+    else logits_epilogue<MODE>(a, acc, iw, jw, lane, slab);
   }
 }
 
@@ -364,16 +397,23 @@ long long tiles_of(int M, int N) {
 
 }  // namespace
 
+// The least of: waves of tiles on 256 CUs times the slices of a tile, and the join of the parts. In
+// units of one slice's time (1.8 us): a tile costs 8 more for its first loads and its results, the
+// join 3 for its launch and 8 bytes a value and split at 4 TB/s.
 int head_gemm_splits(int M, int N, int K) {
-  constexpr int kCus = 256, kLeast = 8;
+  constexpr int kCus = 256, kMost = 16, kLeast = 4;
   const long long tiles = tiles_of(M, N);
   const int slices = (K + kSlice - 1) / kSlice;
-  if (tiles <= 0 || tiles > kCus / 2) return 1;
-  long long s = kCus / tiles;
-  if (s > slices / kLeast) s = slices / kLeast;
-  if (s <= 1) return 1;
-  const int per = (int)((slices + s - 1) / s);
-  return (slices + per - 1) / per;        // no empty split
+  int best = 1;
+  double least = 0.;
+  for (int s = 1; s <= kMost && s * kLeast <= slices + kLeast - 1; ++s) {
+    const int per = (slices + s - 1) / s;
+    if (s > 1 && (slices + per - 1) / per != s) continue;      // an empty part
+    const double waves = (double)((tiles * s + kCus - 1) / kCus);
+    const double cost = waves * (per + 8) + (s > 1 ? 3 + 1.1e-6 * s * M * N : 0.);
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  return best;
 }
 
 hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream) {
@@ -394,11 +434,15 @@ hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream) {
   hipLaunchKernelGGL((head_gemm_kernel<E, MODE, AKM, BKM>), grid, dim3(512), 0, stream, a)
 #define DMUON_HG_E(E)                                                     \
   do {                                                                    \
-    if (a.mode == HG_LOGITS) DMUON_HG(E, HG_LOGITS, false, false);        \
+    if (a.mode == HG_STATS) DMUON_HG(E, HG_STATS, false, false);          \
+    else if (a.mode == HG_EXP) DMUON_HG(E, HG_EXP, false, false);         \
+    else if (a.mode == HG_LOGITS) DMUON_HG(E, HG_LOGITS, false, false);   \
     else if (a.a_kmajor) DMUON_HG(E, HG_GRAD, true, true);                \
     else DMUON_HG(E, HG_GRAD, false, true);                               \
   } while (0)
-  if ((a.mode == HG_LOGITS) != (!a.a_kmajor && !a.b_kmajor) || (a.mode == HG_GRAD && !a.b_kmajor))
+  if (a.mode == HG_GRAD ? !a.b_kmajor
+                        : a.a_kmajor || a.b_kmajor || !a.stats ||
+                              (a.mode != HG_STATS && (!a.Z || a.ldz < (a.N + 63) / 64 * 64)))
     return hipErrorInvalidValue;
   if (a.elt == ELT_F16) DMUON_HG_E(ELT_F16);
   else DMUON_HG_E(ELT_BF16);

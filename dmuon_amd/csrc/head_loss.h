@@ -16,9 +16,14 @@ constexpr int kStatCols = 64;
 constexpr int kGradShift = 10;
 
 // What a product writes.
-//   HG_LOGITS  Z = scale * acc (fp32, pitch ldz, optional) and the statistics of its columns
+//   HG_STATS   the softmax statistics of scale * acc
+//   HG_EXP     those and X = fp16(2^kExpShift exp(z - m)), m the row's maximum in its statistic's
+//              columns; 0 in the columns past N
+//   HG_LOGITS  those and Z = z in fp32
 //   HG_GRAD    out = alpha[0] * (acc + part) rounded to out_dtype, or part (+)= acc in fp32
-enum HeadGemmMode : int { HG_LOGITS = 0, HG_GRAD = 1 };
+enum HeadGemmMode : int { HG_STATS = 0, HG_EXP = 1, HG_LOGITS = 2, HG_GRAD = 3 };
+// fp16 holds exponentials down to 2^-29 of their maximum with all its bits
+constexpr int kExpShift = 15;
 
 // acc[i][j] = sum_k A(i, k) * B(j, k): operand X's element (r, k) is X[r * ld + k], or
 // X[k * ld + r] with x_kmajor.
@@ -28,8 +33,8 @@ struct HeadGemm {
   int M, N, K;
   int mode, elt;
   float scale;
-  float* Z; long long ldz;
-  float2* stats;                          // HG_LOGITS: [ceil(N / kStatCols)][M]
+  void* Z; long long ldz;                 // HG_EXP, HG_LOGITS: [M][ldz], ldz a multiple of 64
+  float2* stats; int n_stats;             // [M][n_stats], n_stats = ceil(N / kStatCols)
   const float* alpha;
   void* out; long long ldo; int out_dtype;   // HG_GRAD: result (DT_F32 or the operands'), or NULL
   float* part; long long ldp;             // HG_GRAD: fp32 sums [M][ldp], or NULL
@@ -56,6 +61,7 @@ struct HeadRows {
   int reduction;                          // DMUON_LOSS_*
   const float* row_grad;                  // DMUON_LOSS_ROWS: dL / d loss[n], or NULL
   int* ids; float* probs;                 // [n][k_list]
+  float* logits;                          // [n][k_list]: the entries' logits (over temperature)
   float* mass;                            // [n]: sum of the row's probs, < 0: not counted
   float* lse;                             // [n]
   float* loss;                            // [n]
@@ -63,15 +69,17 @@ struct HeadRows {
   float* alpha;                           // [1]: what turns a stored gradient into the real one
   float* mean;                            // [1] or NULL: the reduced loss
 };
-// ids, probs and mass of every row; row weights and alpha with `grads`.
-hipError_t launch_head_targets(const HeadRows& r, bool grads, hipStream_t stream);
-// lse and loss of rows first .. first + rows - 1 from their logits and statistics.
-hipError_t launch_head_loss(const HeadRows& r, int first, int rows, const float* Z, long long ldz,
-                            const float2* stats, hipStream_t stream);
-// G[row][v] = row_weight (mass softmax - target probability) for v < vocab, 0 for the columns up
-// to ldg.
-hipError_t launch_head_grad(const HeadRows& r, int first, int rows, const float* Z, long long ldz,
-                            uint16_t* G, long long ldg, int elt, hipStream_t stream);
+// ids, probs, mass and logits of every row (H, W: the products' operands, any alignment); row weights
+// and alpha with `grads`.
+hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long ldh,
+                               const uint16_t* W, long long ldw, int dim, int elt, bool grads,
+                               hipStream_t stream);
+// lse and loss of rows first .. first + rows - 1 from their statistics, and with G their logit
+// gradients G[row][v] = row_weight (mass softmax - target probability), 0 from the vocabulary's end
+// up to ldg: in place of the exponentials (Z == G), or from the fp32 logits Z.
+hipError_t launch_head_rows(const HeadRows& r, int first, int rows, const float2* stats,
+                            const void* Z, uint16_t* G, long long ldg, int elt,
+                            hipStream_t stream);
 // mean[0] = sum of the losses, divided by the number of counted rows for DMUON_LOSS_MEAN.
 hipError_t launch_head_reduce(const HeadRows& r, hipStream_t stream);
 

@@ -1,8 +1,14 @@
 // dmuon_head_loss: argument checks, workspace layout and launch sequence of the vocabulary losses.
 //
-// The rows go through in chunks of tokens. Per chunk: the logits with the softmax statistics of
-// every 64 columns, each row's log-sum-exp and loss, the logit gradient, and its two products with
-// the weight and the hidden states. The weight's gradient sums over the chunks in fp32.
+// The rows go through in chunks of tokens. Per chunk: the logits' product with the softmax statistics
+// of every 64 columns, each row's log-sum-exp and loss, the logit gradient, and its two products
+// with the weight and the hidden states. The weight's gradient sums over the chunks in fp32.
+//
+// Between the first product and the others a logit takes two bytes where the operands are bf16:
+// exp(z - m) in fp16, m the maximum of the row's 64 columns, which the row kernel turns into the
+// bf16 gradient in place. Its 2^-12 is small against the 2^-9 of the gradient's own rounding. For
+// fp16 operands it is not: there the product writes fp32 logits and the gradient has its own place,
+// six bytes a logit.
 #include "../../include/dmuon_amd.h"
 #include "dmuon_amd_internal.h"
 #include "head_loss.h"
@@ -14,14 +20,14 @@ namespace {
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 // Workspace of a chunk's logits and logit gradient; a call of more tokens takes several chunks.
-constexpr int64_t kChunkBytes = int64_t(2) << 30;
+constexpr int64_t kChunkBytes = int64_t(4) << 30;
 
 // The pitch of the logits stays inside the products' 32-bit tile offsets.
 constexpr int64_t kMaxVocab = (int64_t(1) << 22) - 256;
 
 struct Layout {
   int64_t chunk, ld;                      // tokens of a chunk, pitch of its logits
-  int64_t ids, probs, mass, lse, row_weight, alpha, Z, stats, G, part, H, W, bytes;
+  int64_t ids, probs, logits, mass, lse, row_weight, alpha, Z, stats, G, part, H, W, bytes;
   int64_t pad;                            // pitch of the copies of hidden and weight
   bool copy_h, copy_w;
 };
@@ -74,11 +80,17 @@ Layout lay_out(const dmuon_head_loss_args& a) {
   const bool grads = a.d_hidden || a.d_weight;
   Layout l{};
   const int64_t k = a.teacher_ids ? a.k_list : 1, tiles = round_up(a.vocab, kStatCols) / kStatCols;
-  l.ld = round_up(a.vocab, 256);
-  const int64_t row = l.ld * (grads ? 6 : 4) + tiles * 8;
+  const bool f16 = a.dtype == DMUON_DTYPE_F16;
+  l.ld = round_up(a.vocab, 64);
+  const int64_t row = (grads ? l.ld * (f16 ? 6 : 2) : 0) + tiles * 8;
   l.chunk = a.chunk_tokens > 0 ? a.chunk_tokens : kChunkBytes / row;
-  if (l.chunk < 1) l.chunk = 1;
   if (l.chunk > 256) l.chunk = l.chunk / 256 * 256;
+  if (l.chunk < 1) l.chunk = 1;
+  if (l.chunk < a.tokens && a.chunk_tokens == 0) {
+    // chunks of one size, in whole tiles
+    const int64_t n = (a.tokens + l.chunk - 1) / l.chunk;
+    l.chunk = round_up((a.tokens + n - 1) / n, l.chunk < 256 ? 1 : 256);
+  }
   if (l.chunk > a.tokens) l.chunk = a.tokens;
   auto take = [&](int64_t bytes) {
     const int64_t at = l.bytes;
@@ -87,13 +99,14 @@ Layout lay_out(const dmuon_head_loss_args& a) {
   };
   l.ids = take(a.tokens * k * 4);
   l.probs = take(a.tokens * k * 4);
+  l.logits = take(a.tokens * k * 4);
   l.mass = take(a.tokens * 4);
   l.lse = take(a.tokens * 4);
   l.row_weight = take(a.tokens * 4);
   l.alpha = take(4);
-  l.Z = take(l.chunk * l.ld * 4);
   l.stats = take(l.chunk * tiles * 8);
   l.G = take(grads ? l.chunk * l.ld * 2 : 0);
+  l.Z = grads && f16 ? take(l.chunk * l.ld * 4) : l.G;
   // fp32 sums: the weight's gradient over several chunks, or of split products
   int64_t part = 0;
   if (a.d_weight && l.chunk < a.tokens) {
@@ -165,13 +178,14 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
   r.row_grad = a.reduction == DMUON_LOSS_ROWS ? a.row_grad : nullptr;
   r.ids = reinterpret_cast<int*>(ws + l.ids);
   r.probs = floats(l.probs);
+  r.logits = floats(l.logits);
   r.mass = floats(l.mass);
   r.lse = floats(l.lse);
   r.loss = a.loss;
   r.row_weight = floats(l.row_weight);
   r.alpha = floats(l.alpha);
   r.mean = a.reduced;
-  float* Z = floats(l.Z);
+  void* Z = ws + l.Z;
   float2* stats = reinterpret_cast<float2*>(ws + l.stats);
   uint16_t* G = reinterpret_cast<uint16_t*>(ws + l.G);
   const uint16_t* H = static_cast<const uint16_t*>(a.hidden);
@@ -187,7 +201,8 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
     W = copy;
     ldw = l.pad;
   }
-  if (check_launch(launch_head_targets(r, grads, stream), who)) return 1;
+  if (check_launch(launch_head_targets(r, H, a.ld_hidden, static_cast<const uint16_t*>(a.weight),
+                                       a.ld_weight, (int)a.dim, elt, grads, stream), who)) return 1;
   for (int64_t first = 0; first < a.tokens || first == 0; first += l.chunk) {
     const int rows = (int)(a.tokens - first < l.chunk ? a.tokens - first : l.chunk);
     const uint16_t* Hc = H + first * a.ld_hidden;
@@ -201,19 +216,18 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
     }
     HeadGemm g{};
     g.elt = elt;
-    g.mode = HG_LOGITS;
+    g.mode = !grads ? HG_STATS : elt == ELT_F16 ? HG_LOGITS : HG_EXP;
     g.splits = 1;
     g.A = Hc; g.lda = ldh;
     g.B = W; g.ldb = ldw;
     g.M = rows; g.N = (int)a.vocab; g.K = (int)a.dim;
     g.scale = 1.f / r.temperature;
     g.Z = Z; g.ldz = l.ld;
-    g.stats = stats;
+    g.stats = stats; g.n_stats = (int)(round_up(a.vocab, kStatCols) / kStatCols);
     if (check_launch(launch_head_gemm(g, stream), who)) return 1;
-    if (check_launch(launch_head_loss(r, (int)first, rows, Z, l.ld, stats, stream), who)) return 1;
+    if (check_launch(launch_head_rows(r, (int)first, rows, stats, Z, grads ? G : nullptr, l.ld, elt,
+                                      stream), who)) return 1;
     if (grads) {
-      if (check_launch(launch_head_grad(r, (int)first, rows, Z, l.ld, G, l.ld, elt, stream), who))
-        return 1;
       g = HeadGemm{};
       g.elt = elt;
       g.mode = HG_GRAD;

@@ -1,12 +1,14 @@
-// Row kernels of the vocabulary losses on gfx950: targets, log-sum-exp and loss, the logit
-// gradient between the products, and the reductions. All of them stream their rows once; sums and
-// exponentials are fp32.
+// Row kernels of the vocabulary losses on gfx950: targets and their logits, log-sum-exp, loss and
+// logit gradient between the products, and the reductions. Sums and exponentials are fp32.
 #include "../../include/dmuon_amd.h"
 #include "dmuon_amd_internal.h"
 #include "head_loss.h"
+#include "mfma_tile.h"
 
 namespace dmuon {
 namespace {
+
+typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
 
 constexpr float kInf = __builtin_inff();
 
@@ -31,24 +33,53 @@ __device__ __forceinline__ float block_join(float v, float* lds) {
   return r;
 }
 
-// The entries of a row. Hard targets: one, with probability 1. A teacher's list: softmax of the
-// live logits over the temperature, or their exponentials under the teacher's own log-sum-exp. A
-// class outside the vocabulary that is neither the ignored index nor padding makes the row's mass
-// NaN, so its loss and gradients show it. One wave per row.
-__global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r) {
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= r.n) return;
+// h . w over `dim` values from element-aligned rows, in every lane.
+template <int E>
+__device__ __forceinline__ float wave_dot(const uint16_t* h, const uint16_t* w, int dim, int lane) {
+  float s = 0.f;
+#pragma unroll 4
+  for (int c = lane * 8; c + 8 <= dim; c += 512) {
+    const u32x4_t x = *reinterpret_cast<const u32x4_any_t*>(h + c);
+    const u32x4_t y = *reinterpret_cast<const u32x4_any_t*>(w + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s = __builtin_fmaf(from_elt<E>(x[e] & 0xffff), from_elt<E>(y[e] & 0xffff), s);
+      s = __builtin_fmaf(from_elt<E>(x[e] >> 16), from_elt<E>(y[e] >> 16), s);
+    }
+  }
+  const int c = dim / 8 * 8 + lane;
+  if (c < dim) s = __builtin_fmaf(from_elt<E>(h[c]), from_elt<E>(w[c]), s);
+  return wave_sum(s);
+}
+
+// The entries of a row and their logits. Hard targets: one, with probability 1. A teacher's list:
+// softmax of the live logits over the temperature, or their exponentials under the teacher's own
+// log-sum-exp. A class outside the vocabulary that is neither the ignored index nor padding makes
+// the row's mass NaN, so its loss and gradients show it. The entries' logits are formed here, in
+// fp32 from the rows themselves: the products' epilogue would have to search every row's list in
+// each of its tiles. Hard targets take one wave a row, lists four.
+template <int E>
+__global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uint16_t* H,
+                                                           long long ldh, const uint16_t* W,
+                                                           long long ldw, int dim) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float it = 1.f / r.temperature;
   if (r.targets) {
-    if (lane) return;
+    const int row = blockIdx.x * 4 + wave;
+    if (row >= r.n) return;
     const long long t = r.targets[row];
     const bool counted = t != r.ignore_index, inside = t >= 0 && t < r.vocab;
-    r.ids[row] = counted && inside ? (int)t : -1;
-    r.probs[row] = counted && inside ? 1.f : 0.f;
+    const bool live = counted && inside;
+    const float z = live ? wave_dot<E>(H + row * ldh, W + t * ldw, dim, lane) : 0.f;
+    if (lane) return;
+    r.ids[row] = live ? (int)t : -1;
+    r.probs[row] = live ? 1.f : 0.f;
+    r.logits[row] = z;
     r.mass[row] = !counted ? -1.f : inside ? 1.f : __builtin_nanf("");
     return;
   }
+  const int row = blockIdx.x;
   const long long base = (long long)row * r.k_list;
-  const float it = 1.f / r.temperature;
   float top = -kInf;
   int live = 0, outside = 0;
   for (int k = lane; k < r.k_list; k += 64) {
@@ -70,20 +101,19 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r) {
     }
   sum = wave_sum(sum);
   const float norm = r.teacher_lse ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-  float mass = 0.f;
-  for (int k = lane; k < r.k_list; k += 64) {
+  if (wave == 0 && lane == 0)
+    r.mass[row] = !live ? -1.f : outside ? __builtin_nanf("") : r.teacher_lse ? sum : sum * norm;
+  for (int k = wave; k < r.k_list; k += 4) {
     const long long id = r.teacher_ids[base + k];
-    float q = 0.f;
-    if (id >= 0) {
-      const float v = r.teacher_logits[base + k] * it;
-      q = v == -kInf ? 0.f : expf(v - shift) * norm;
-    }
-    r.ids[base + k] = id >= 0 && id < r.vocab ? (int)id : -1;
+    const float v = r.teacher_logits[base + k] * it;
+    const bool in = id >= 0 && id < r.vocab;
+    const float q = id < 0 || v == -kInf ? 0.f : expf(v - shift) * norm;
+    const float z = in && q != 0.f ? wave_dot<E>(H + row * ldh, W + id * ldw, dim, lane) * it : 0.f;
+    if (lane) continue;
+    r.ids[base + k] = in && q != 0.f ? (int)id : -1;
     r.probs[base + k] = q;
-    mass += q;
+    r.logits[base + k] = z;
   }
-  mass = wave_sum(mass);
-  if (lane == 0) r.mass[row] = !live ? -1.f : outside ? __builtin_nanf("") : mass;
 }
 
 // Row weights and alpha: the gradient of row n is alpha * row_weight[n] * (...). The weights are
@@ -113,110 +143,115 @@ __global__ __launch_bounds__(1024) void head_weights_kernel(HeadRows r) {
   }
 }
 
-// log-sum-exp and loss of 16 rows a block, 16 threads a row.
-__global__ __launch_bounds__(256) void head_loss_kernel(HeadRows r, int first, int rows,
-                                                        const float* __restrict__ Z, long long ldz,
-                                                        const float2* __restrict__ stats) {
-  __shared__ float2 part[16][17];
-  const int rl = threadIdx.x & 15, strand = threadIdx.x >> 4;
-  const int row = blockIdx.x * 16 + rl;
-  const int tiles = (r.vocab + kStatCols - 1) / kStatCols;
+// (maximum, sum of exponentials) of two sets of logits as one
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  if (top == -kInf) s += s2;              // empty sets, or a NaN to keep
+  else s = s * __expf(m - top) + s2 * __expf(m2 - top);
+  m = top;
+}
+
+// What head_rows_kernel makes its gradient from.
+enum { FROM_NONE = 0, FROM_EXP = 1, FROM_LOGITS = 2 };
+
+// One row a block, or `parts` blocks a row where there are few rows: the row's statistics joined
+// (every block for itself), its loss (part 0), and this part's columns of the logit gradient
+//   row_weight (mass + 2 z_loss lse) softmax - row_weight q
+// in place of the exponentials, whose factor exp(m - lse) is one of 64 columns, or from the
+// logits. Both cross memory once: 2 + 2 bytes a logit, or 4 + 2. The entries' columns come last,
+// from their fp32 logits: mass p - q cancels where the student is sure. (Entries of one class in one
+// row write the same value.)
+template <int E, int FROM>
+__global__ __launch_bounds__(256) void head_rows_kernel(HeadRows r, int first,
+                                                        const float2* __restrict__ stats,
+                                                        int n_stats, const void* Z, uint16_t* G,
+                                                        long long ldg, int parts) {
+  __shared__ float lds[2][4];
+  const int row = blockIdx.x / parts, part = blockIdx.x % parts;
+  const long long n = first + row;
+  stats += (long long)row * n_stats;
   float m = -kInf, s = 0.f;
-  auto join = [&](float2 o) {
-    const float top = fmaxf(m, o.x);
-    if (top == -kInf) { s += o.y; return; }
-    s = s * expf(m - top) + o.y * expf(o.x - top);
-    m = top;
-  };
-  if (row < rows)
-    for (int t = strand; t < tiles; t += 16) join(stats[(long long)t * rows + row]);
-  part[strand][rl] = make_float2(m, s);
+  for (int t = threadIdx.x; t < n_stats; t += 256) {
+    const float2 o = stats[t];
+    join(m, s, o.x, o.y);
+  }
+  for (int o = 1; o < 64; o <<= 1) {
+    const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
+    join(m, s, m2, s2);
+  }
+  if ((threadIdx.x & 63) == 0) lds[0][threadIdx.x >> 6] = m, lds[1][threadIdx.x >> 6] = s;
   __syncthreads();
-  if (row >= rows) return;
-  m = -kInf;
-  s = 0.f;
-  for (int k = 0; k < 16; ++k) join(part[k][rl]);
+  m = lds[0][0], s = lds[1][0];
+  for (int w = 1; w < 4; ++w) join(m, s, lds[0][w], lds[1][w]);
   const float lse = logf(s) + m;
-  const long long n = first + row;
   const float mass = r.mass[n];
-  float loss = 0.f;
-  if (!(mass < 0.f)) {
-    for (int k = strand; k < r.k_list; k += 16) {
-      const int id = r.ids[n * r.k_list + k];
-      const float q = r.probs[n * r.k_list + k];
-      if (id < 0 || q == 0.f) continue;
-      const float z = Z[(long long)row * ldz + id];
-      loss += r.targets ? lse - z : q * (logf(q) - (z - lse));
-    }
-  }
-  __syncthreads();
-  part[strand][rl].x = loss;
-  __syncthreads();
-  if (strand) return;
-  loss = 0.f;
-  for (int k = 0; k < 16; ++k) loss += part[k][rl].x;
-  if (!(mass < 0.f)) {
-    loss = loss * r.temperature * r.temperature + r.z_loss * lse * lse;
-    if (mass != mass) loss = mass;
-  }
-  r.lse[n] = lse;
-  r.loss[n] = loss;
-}
-
-template <int E>
-__device__ __forceinline__ uint16_t to_elt(float f) {
-  if constexpr (E == ELT_F16) return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
-  else return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f));
-}
-template <int E>
-__device__ __forceinline__ float from_elt(uint16_t h) {
-  if constexpr (E == ELT_F16) return static_cast<float>(__builtin_bit_cast(_Float16, h));
-  else return __uint_as_float(static_cast<uint32_t>(h) << 16);
-}
-
-// row weight times mass, with the z-loss term: d(z_loss lse^2) = 2 z_loss lse softmax
-__device__ __forceinline__ float row_factor(const HeadRows& r, long long n) {
-  return r.row_weight[n] * (r.mass[n] + (r.targets ? 2.f * r.z_loss * r.lse[n] : 0.f));
-}
-
-template <int E>
-__global__ __launch_bounds__(256) void head_grad_kernel(HeadRows r, int first,
-                                                        const float* __restrict__ Z, long long ldz,
-                                                        uint16_t* __restrict__ G, long long ldg) {
-  const long long n = first + blockIdx.y;
-  const long long row = blockIdx.y;
-  const int c0 = (blockIdx.x * 256 + threadIdx.x) * 8;
-  if (c0 >= ldg) return;
-  const float w = r.row_weight[n], f = row_factor(r, n), lse = r.lse[n];
-  for (int e = 0; e < 8; ++e) {
-    const int c = c0 + e;
-    float g = 0.f;
-    if (c < r.vocab && w != 0.f) g = f * expf(Z[row * ldz + c] - lse);
-    if (c < ldg) G[row * ldg + c] = to_elt<E>(g);
-  }
-}
-// The entries' classes, from their fp32 logits: mass p - q cancels where the student is sure.
-// Entries of one class in one row write the same value. One wave per row.
-template <int E>
-__global__ __launch_bounds__(256) void head_grad_entries_kernel(HeadRows r, int first, int rows,
-                                                                const float* __restrict__ Z,
-                                                                long long ldz,
-                                                                uint16_t* __restrict__ G,
-                                                                long long ldg) {
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= rows) return;
-  const long long n = first + row;
-  const float w = r.row_weight[n], f = row_factor(r, n), lse = r.lse[n];
-  if (w == 0.f) return;
+  const bool counted = !(mass < 0.f);
   const int* ids = r.ids + n * r.k_list;
   const float* probs = r.probs + n * r.k_list;
-  for (int k = lane; k < r.k_list; k += 64) {
-    const int id = ids[k];
-    if (id < 0) continue;
-    float q = 0.f;
-    for (int j = 0; j < r.k_list; ++j)
-      if (ids[j] == id) q += probs[j];
-    G[row * ldg + id] = to_elt<E>(f * expf(Z[(long long)row * ldz + id] - lse) - w * q);
+  const float* logits = r.logits + n * r.k_list;
+  if (part == 0) {
+    float loss = 0.f;
+    if (counted)
+      for (int k = threadIdx.x; k < r.k_list; k += 256) {
+        const float q = probs[k];
+        if (ids[k] < 0) continue;
+        loss += r.targets ? lse - logits[k] : q * (logf(q) - (logits[k] - lse));
+      }
+    loss = block_join<false>(loss, lds[0]);
+    if (threadIdx.x == 0) {
+      if (counted) {
+        loss = loss * r.temperature * r.temperature + r.z_loss * lse * lse;
+        if (mass != mass) loss = mass;
+      }
+      r.lse[n] = lse;
+      r.loss[n] = loss;
+    }
+  }
+  if constexpr (FROM != FROM_NONE) {
+    const float w = r.row_weight[n];
+    const float f = w == 0.f ? 0.f : w * (mass + 2.f * r.z_loss * lse);
+    const int chunks = (int)(ldg / 8), per = (chunks + parts - 1) / parts;
+    const int c0 = part * per, c1 = min(chunks, c0 + per);
+    uint16_t* g = G + (long long)row * ldg;
+    const float fe = f * (1.f / (float)(1 << kExpShift));
+#pragma unroll 4
+    for (int c = c0 + threadIdx.x; c < c1; c += 256) {
+      float v[8];
+      if (w == 0.f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      } else if constexpr (FROM == FROM_EXP) {
+        const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(g + 8 * c));
+        const float k = fe * __expf(stats[c / 8].x - lse);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[2 * e] = k * from_elt<ELT_F16>(x[e] & 0xffff);
+          v[2 * e + 1] = k * from_elt<ELT_F16>(x[e] >> 16);
+        }
+      } else {
+        const f32x4_t* z = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(Z) +
+                                                            (long long)row * ldg + 8 * c);
+        const f32x4_t lo = __builtin_nontemporal_load(z), hi = __builtin_nontemporal_load(z + 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = f * __expf(lo[e] - lse);
+          v[4 + e] = f * __expf(hi[e] - lse);
+        }
+      }
+      const u32x4_t o = {pack2_elt<E>(v[0], v[1]), pack2_elt<E>(v[2], v[3]),
+                         pack2_elt<E>(v[4], v[5]), pack2_elt<E>(v[6], v[7])};
+      *reinterpret_cast<u32x4_t*>(g + 8 * c) = o;
+    }
+    if (w == 0.f) return;
+    __syncthreads();
+    for (int k = threadIdx.x; k < r.k_list; k += 256) {
+      const int id = ids[k];
+      if (id < 8 * c0 || id >= 8 * c1) continue;
+      float q = 0.f;
+      for (int j = 0; j < r.k_list; ++j)
+        if (ids[j] == id) q += probs[j];
+      g[id] = to_elt<E>(f * __expf(logits[k] - lse) - w * q);
+    }
   }
 }
 
@@ -250,35 +285,37 @@ __global__ __launch_bounds__(256) void scale_by_kernel(const void* src, void* ds
 
 }  // namespace
 
-hipError_t launch_head_targets(const HeadRows& r, bool grads, hipStream_t stream) {
-  if (r.n > 0)
-    hipLaunchKernelGGL(head_targets_kernel, dim3((unsigned)((r.n + 3) / 4)), dim3(256), 0, stream, r);
+hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long ldh,
+                               const uint16_t* W, long long ldw, int dim, int elt, bool grads,
+                               hipStream_t stream) {
+  if (r.n > 0) {
+    const dim3 grid((unsigned)(r.targets ? (r.n + 3) / 4 : r.n));
+    if (elt == ELT_F16)
+      hipLaunchKernelGGL(head_targets_kernel<ELT_F16>, grid, dim3(256), 0, stream, r, H, ldh, W, ldw, dim);
+    else
+      hipLaunchKernelGGL(head_targets_kernel<ELT_BF16>, grid, dim3(256), 0, stream, r, H, ldh, W, ldw, dim);
+  }
   if (grads) hipLaunchKernelGGL(head_weights_kernel, dim3(1), dim3(1024), 0, stream, r);
   return hipGetLastError();
 }
 
-hipError_t launch_head_loss(const HeadRows& r, int first, int rows, const float* Z, long long ldz,
-                            const float2* stats, hipStream_t stream) {
+hipError_t launch_head_rows(const HeadRows& r, int first, int rows, const float2* stats,
+                            const void* Z, uint16_t* G, long long ldg, int elt,
+                            hipStream_t stream) {
   if (rows <= 0) return hipSuccess;
-  hipLaunchKernelGGL(head_loss_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, stream, r,
-                     first, rows, Z, ldz, stats);
-  return hipGetLastError();
-}
-
-hipError_t launch_head_grad(const HeadRows& r, int first, int rows, const float* Z, long long ldz,
-                            uint16_t* G, long long ldg, int elt, hipStream_t stream) {
-  if (rows <= 0) return hipSuccess;
-  const dim3 grid((unsigned)((ldg + 2047) / 2048), (unsigned)rows);
-  const dim3 rgrid((unsigned)((rows + 3) / 4));
-  if (elt == ELT_F16) {
-    hipLaunchKernelGGL(head_grad_kernel<ELT_F16>, grid, dim3(256), 0, stream, r, first, Z, ldz, G, ldg);
-    hipLaunchKernelGGL(head_grad_entries_kernel<ELT_F16>, rgrid, dim3(256), 0, stream, r, first,
-                       rows, Z, ldz, G, ldg);
-  } else {
-    hipLaunchKernelGGL(head_grad_kernel<ELT_BF16>, grid, dim3(256), 0, stream, r, first, Z, ldz, G, ldg);
-    hipLaunchKernelGGL(head_grad_entries_kernel<ELT_BF16>, rgrid, dim3(256), 0, stream, r, first,
-                       rows, Z, ldz, G, ldg);
-  }
+  const int n_stats = (r.vocab + kStatCols - 1) / kStatCols;
+  // few rows: as many blocks a row as give every CU two, of at least 2048 columns each
+  long long parts = G ? (512 + rows - 1) / rows : 1;
+  if (parts > ldg / 2048) parts = ldg / 2048 > 0 ? ldg / 2048 : 1;
+  const dim3 grid((unsigned)(rows * parts));
+#define DMUON_ROWS(E, FROM)                                                                   \
+  hipLaunchKernelGGL((head_rows_kernel<E, FROM>), grid, dim3(256), 0, stream, r, first, stats, \
+                     n_stats, Z, G, ldg, (int)parts)
+  if (!G) DMUON_ROWS(ELT_BF16, FROM_NONE);
+  else if (Z == G && elt == ELT_BF16) DMUON_ROWS(ELT_BF16, FROM_EXP);
+  else if (Z != G && elt == ELT_F16) DMUON_ROWS(ELT_F16, FROM_LOGITS);
+  else return hipErrorInvalidValue;
+#undef DMUON_ROWS
   return hipGetLastError();
 }
 
