@@ -204,6 +204,19 @@ def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args))
 
 
+def call_on(device, name: str, *args) -> None:
+    """``call`` with the device's current stream as last argument and the device current. (Entering
+    ``torch.cuda.device`` costs more than a small kernel's launch: only where it changes something.)"""
+    import torch
+
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        check(getattr(lib(), name)(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            check(getattr(lib(), name)(*args, stream))
+
+
 PROFILE_CLASSES = ("pre", "norm", "syrk", "poly", "gemm", "final", "adamw", "clip")
 
 

@@ -22,9 +22,10 @@ struct ResidualNorm {
   float* pre_part; float* post_part; float* gate_part;           // [blocks][dim]
   long long rows_per_block, blocks;
   int parts;                              // blocks of one gate group; 1: a block takes whole groups
+  int lanes;                              // backward: rows side by side in a block
 };
 hipError_t launch_residual_norm(ResidualNorm a, hipStream_t stream);
-// Sets rows_per_block, blocks and parts of the backward pass.
+// Sets rows_per_block, blocks, parts and lanes of the backward pass.
 void residual_norm_split(ResidualNorm* a);
 hipError_t launch_residual_norm_grad(const ResidualNorm& a, hipStream_t stream);
 

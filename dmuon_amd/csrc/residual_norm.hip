@@ -13,18 +13,22 @@
 //   dx = a d,  dy = r (c d - yhat (sum c yhat d) / D)
 // instead of a second reduction that waits for d.
 //
-// A block keeps its columns in registers -- NV chunks of 8 columns a thread -- and walks a
-// contiguous range of rows, so the weights are read once a block (the gate once a group) and the
-// gradients of the weights add up in registers; each block then writes one partial row, which a
-// second kernel sums in a fixed order.
+// A row is spread over blockDim.x threads, 8 columns each (16 past 8192 columns), blockDim.y rows
+// side by side. A block keeps its columns' weights in registers and walks a contiguous range of
+// rows, the next row's loads in flight under the sums of this one; the weights' gradients add up in
+// registers too, and each block writes one partial row, which a second kernel sums in a fixed order.
 #include "../../include/dmuon_amd.h"
 #include "dmuon_amd_internal.h"
+#include "mfma_tile.h"
 #include "residual_norm.h"
+
+// a * b + c in one instruction: the backward pass has some twenty operations a value, which would
+// otherwise cost as much as its memory traffic
+#pragma clang fp contract(fast)
 
 namespace dmuon {
 namespace {
 
-typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 // rows of any pitch and bases of any element alignment: the vectors state the element's alignment
 typedef u32x4_t v16_t __attribute__((aligned(2)));
 typedef u32x4_t v32_t __attribute__((aligned(4)));
@@ -38,32 +42,48 @@ __device__ __forceinline__ unsigned f_to_half(float f, int t) {
   return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f));
 }
 
-// n (at most 8) values from element `at` on; the rest are 0
-__device__ __forceinline__ void load8(const void* p, int t, long long at, int n, float* v) {
-  if (t == DT_F32) {
+// 8 values as they lie in memory
+template <int T>
+struct Raw {
+  u32x4_t v[T == DT_F32 ? 2 : 1];
+};
+// n (at most 8) values from element `at` on; the rest are 0. ONCE: past the caches
+template <int T, bool ONCE = false>
+__device__ __forceinline__ Raw<T> load_raw(const void* p, long long at, int n) {
+  Raw<T> r;
+  if constexpr (T == DT_F32) {
     const float* q = static_cast<const float*>(p) + at;
     if (n >= 8) {
-      const u32x4_t a = *(const v32_t*)q, b = *(const v32_t*)(q + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(a[i]), v[i + 4] = __uint_as_float(b[i]);
+      r.v[0] = ONCE ? __builtin_nontemporal_load((const v32_t*)q) : *(const v32_t*)q;
+      r.v[1] = ONCE ? __builtin_nontemporal_load((const v32_t*)(q + 4)) : *(const v32_t*)(q + 4);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < n ? q[i] : 0.f;
+      for (int i = 0; i < 8; ++i) r.v[i / 4][i % 4] = i < n ? __float_as_uint(q[i]) : 0u;
     }
   } else {
     const uint16_t* q = static_cast<const uint16_t*>(p) + at;
     if (n >= 8) {
-      const u32x4_t a = *(const v16_t*)q;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = half_to_f(a[i] & 0xffff, t);
-        v[2 * i + 1] = half_to_f(a[i] >> 16, t);
-      }
+      r.v[0] = ONCE ? __builtin_nontemporal_load((const v16_t*)q) : *(const v16_t*)q;
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < n ? half_to_f(q[i], t) : 0.f;
+      for (int i = 0; i < 4; ++i)
+        r.v[0][i] = (2 * i < n ? q[2 * i] : 0u) | ((2 * i + 1 < n ? q[2 * i + 1] : 0u) << 16);
     }
   }
+  return r;
+}
+template <int T>
+__device__ __forceinline__ void unpack(const Raw<T>& r, float* v) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (T == DT_F32) v[i] = __uint_as_float(r.v[i / 4][i % 4]);
+    else v[i] = half_to_f((i & 1) ? r.v[0][i / 2] >> 16 : r.v[0][i / 2] & 0xffff, T);
+  }
+}
+__device__ __forceinline__ void load8(const void* p, int t, long long at, int n, float* v) {
+  if (t == DT_F32) unpack<DT_F32>(load_raw<DT_F32>(p, at, n), v);
+  else if (t == DT_F16) unpack<DT_F16>(load_raw<DT_F16>(p, at, n), v);
+  else unpack<DT_BF16>(load_raw<DT_BF16>(p, at, n), v);
 }
 __device__ __forceinline__ void store8(void* p, int t, long long at, int n, const float* v) {
   if (t == DT_F32) {
@@ -72,8 +92,8 @@ __device__ __forceinline__ void store8(void* p, int t, long long at, int n, cons
       u32x4_t a, b;
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[i] = __float_as_uint(v[i]), b[i] = __float_as_uint(v[i + 4]);
-      *(v32_t*)q = a;
-      *(v32_t*)(q + 4) = b;
+      __builtin_nontemporal_store(a, (v32_t*)q);
+      __builtin_nontemporal_store(b, (v32_t*)(q + 4));
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -84,8 +104,10 @@ __device__ __forceinline__ void store8(void* p, int t, long long at, int n, cons
     if (n >= 8) {
       u32x4_t a;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = f_to_half(v[2 * i], t) | (f_to_half(v[2 * i + 1], t) << 16);
-      *(v16_t*)q = a;
+      for (int i = 0; i < 4; ++i)
+        a[i] = t == DT_F16 ? pack2_elt<ELT_F16>(v[2 * i], v[2 * i + 1])
+                           : pack2_elt<ELT_BF16>(v[2 * i], v[2 * i + 1]);
+      __builtin_nontemporal_store(a, (v16_t*)q);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -95,10 +117,10 @@ __device__ __forceinline__ void store8(void* p, int t, long long at, int n, cons
 }
 
 // Sums of `C` values over the threads of a row (blockDim.x of them): shuffles in a wave, then one
-// LDS exchange where the row has several waves. `flip` alternates so that a row's values are not
-// overwritten while the row before is still being read.
+// LDS exchange where the row has several waves. The caller passes another area than in its call
+// before, so that no area is written while it may still be read. The barrier leaves loads in flight.
 template <int C>
-__device__ __forceinline__ void row_sums(float* v, float (*lds)[4][16][C], int flip) {
+__device__ __forceinline__ void row_sums(float* v, float (*lds)[16][C], int ty) {
 #pragma unroll
   for (int c = 0; c < C; ++c)
     for (int o = 1; o < 64; o <<= 1) v[c] += __shfl_xor(v[c], o);
@@ -107,60 +129,87 @@ __device__ __forceinline__ void row_sums(float* v, float (*lds)[4][16][C], int f
   const int w = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0)
 #pragma unroll
-    for (int c = 0; c < C; ++c) lds[flip][threadIdx.y][w][c] = v[c];
-  __syncthreads();
+    for (int c = 0; c < C; ++c) lds[ty][w][c] = v[c];
+  __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 #pragma unroll
-  for (int c = 0; c < C; ++c) v[c] = lds[flip][threadIdx.y][0][c];
+  for (int c = 0; c < C; ++c) v[c] = lds[ty][0][c];
   for (int k = 1; k < waves; ++k)
 #pragma unroll
-    for (int c = 0; c < C; ++c) v[c] += lds[flip][threadIdx.y][k][c];
+    for (int c = 0; c < C; ++c) v[c] += lds[ty][k][c];
 }
 
-template <int T, int NV>
-__global__ __launch_bounds__(NV == 1 ? 256 : NV == 2 ? 512 : 1024) void residual_norm_kernel(ResidualNorm a) {
-  __shared__ float lds[2][4][16][1];
+// c = gate w_post of this thread's columns for gate row `group`
+template <int NV>
+__device__ __forceinline__ void load_factors(const ResidualNorm& a, long long group, const int* col,
+                                             const int* cnt, float (*c)[8]) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    float g[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[v][i] = g[i] = 1.f;
+    if (a.w_post) load8(a.w_post, a.post_dtype, col[v], cnt[v], c[v]);
+    if (a.gate) load8(a.gate, a.gate_dtype, group * a.dim + col[v], cnt[v], g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[v][i] *= g[i];
+  }
+}
+
+// NV chunks of 8 columns a thread. MANY: several rows side by side in 256 threads; otherwise the row
+// is the same for the block and its addresses stay scalar.
+template <int T, int NV, bool MANY>
+__global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_kernel(ResidualNorm a) {
+  __shared__ float lds[4][4][16][1];
+  const int ty = MANY ? threadIdx.y : 0, rows_at_once = MANY ? blockDim.y : 1;
   const float inv = 1.f / (float)a.dim;
   const long long first = (long long)blockIdx.x * a.rows_per_block;
   const long long end = first + a.rows_per_block < a.rows ? first + a.rows_per_block : a.rows;
-  int cnt[NV];
-  float pre[NV][8], post[NV][8], gate[NV][8];
+  int cnt[NV], col[NV];
+  float pre[NV][8], c[NV][8];
+  Raw<T> xr[NV], yr[NV];
+  auto fetch = [&](long long row) {
+    if (row >= end) row = end - 1;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      xr[v] = load_raw<T>(a.x, row * a.ld_x + col[v], cnt[v]);
+      if (a.y) yr[v] = load_raw<T>(a.y, row * a.ld_y + col[v], cnt[v]);
+    }
+  };
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int c = (v * blockDim.x + threadIdx.x) * 8;
-    cnt[v] = a.dim - c;
-    if (cnt[v] <= 0) cnt[v] = 0;
-    load8(a.w_pre, a.pre_dtype, c, cnt[v], pre[v]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) post[v][i] = gate[v][i] = 1.f;
-    if (a.w_post) load8(a.w_post, a.post_dtype, c, cnt[v], post[v]);
+    col[v] = (v * blockDim.x + threadIdx.x) * 8;
+    cnt[v] = a.dim - col[v] > 0 ? a.dim - col[v] : 0;
   }
+  fetch(first + ty);
+#pragma unroll
+  for (int v = 0; v < NV; ++v) load8(a.w_pre, a.pre_dtype, col[v], cnt[v], pre[v]);
+  int flip = 0;
   long long group = -1;
-  for (long long base = first; base < end; base += blockDim.y) {
-    const long long row = base + threadIdx.y < end ? base + threadIdx.y : end - 1;
+  for (long long base = first; base < end; base += rows_at_once) {
+    // threads past the last row repeat it: the barriers need every wave
+    const long long row = base + ty < end ? base + ty : end - 1;
     float x[NV][8], y[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * 8;
-      load8(a.x, T, row * a.ld_x + c, cnt[v], x[v]);
-      if (a.y) load8(a.y, T, row * a.ld_y + c, cnt[v], y[v]);
+      unpack<T>(xr[v], x[v]);
+      if (a.y) unpack<T>(yr[v], y[v]);
     }
-    if (a.gate) {
-      const long long g = row / a.rows_per_group;
-      if (g != group) {
-        group = g;
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-          load8(a.gate, a.gate_dtype, g * a.dim + (v * blockDim.x + threadIdx.x) * 8, cnt[v], gate[v]);
-      }
+    fetch(row + rows_at_once);
+    const long long g = a.gate ? row / a.rows_per_group : 0;
+    if (g != group) {
+      group = g;
+      load_factors<NV>(a, g, col, cnt, c);
     }
     float r = 1.f;
-    if (a.y && a.w_post) {
+    if (a.w_post) {
       float sq[1] = {0.f};
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int i = 0; i < 8; ++i) sq[0] += y[v][i] * y[v][i];
-      row_sums<1>(sq, lds, 0);
+      row_sums<1>(sq, lds[flip], ty);
       r = 1.f / sqrtf(sq[0] * inv + a.eps);
     }
     float sq[1] = {0.f};
@@ -169,30 +218,33 @@ __global__ __launch_bounds__(NV == 1 ? 256 : NV == 2 ? 512 : 1024) void residual
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         x[v][i] *= a.scale;
-        if (a.y) x[v][i] += gate[v][i] * (y[v][i] * r * post[v][i]);
+        if (a.y) x[v][i] += c[v][i] * (y[v][i] * r);
         sq[0] += x[v][i] * x[v][i];
       }
-    row_sums<1>(sq, lds, 1);
+    row_sums<1>(sq, lds[2 + flip], ty);
+    flip ^= 1;
     const float s = 1.f / sqrtf(sq[0] * inv + a.eps);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const long long at = row * a.dim + (v * blockDim.x + threadIdx.x) * 8;
+      const long long at = row * a.dim + col[v];
       if (a.x_new) store8(a.x_new, T, at, cnt[v], x[v]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[v][i] = x[v][i] * s * pre[v][i];
       store8(a.h, T, at, cnt[v], x[v]);
     }
     if (a.stats && threadIdx.x == 0) a.stats[row] = make_float2(r, s);
-    // one more meeting before the first exchange's values are overwritten by the next row
-    if (blockDim.x > 64 && !(a.y && a.w_post)) __syncthreads();
   }
 }
 
-template <int T, int NV>
-__global__ __launch_bounds__(NV == 1 ? 256 : NV == 2 ? 512 : 1024) void residual_norm_grad_kernel(ResidualNorm a) {
+// The gradients of gate and w_post come from one sum a column and gate group, t = sum d yhat:
+// d_gate = w_post t, d_post = sum over the groups of gate t.
+template <int T, int NV, bool MANY>
+__global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_grad_kernel(ResidualNorm a) {
   __shared__ float lds[2][4][16][3];
+  __shared__ float acc[MANY ? 256 * 8 : 1];
+  const int ty = MANY ? threadIdx.y : 0, rows_at_once = MANY ? blockDim.y : 1;
   const float inv = 1.f / (float)a.dim;
-  // rows of this block: a part of one gate group, or several whole groups
+  // rows of this block: a part of one gate group, or several whole groups (then not MANY)
   long long first, end;
   if (a.parts > 1) {
     const long long g = blockIdx.x / a.parts, p = blockIdx.x % a.parts;
@@ -203,180 +255,240 @@ __global__ __launch_bounds__(NV == 1 ? 256 : NV == 2 ? 512 : 1024) void residual
     first = (long long)blockIdx.x * a.rows_per_block;
     end = first + a.rows_per_block < a.rows ? first + a.rows_per_block : a.rows;
   }
-  int cnt[NV];
-  float pre[NV][8], post[NV][8], gate[NV][8];
-  float d_pre[NV][8], d_post[NV][8], d_gate[NV][8];
+  int cnt[NV], col[NV];
+  float pre[NV][8], c[NV][8], d_pre[NV][8], d_post[NV][8], t[NV][8];
+  Raw<T> xr[NV], yr[NV], er[NV], gr[NV];
+  float2 rs;
+  auto fetch = [&](long long row) {
+    if (row >= end) row = end - 1;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      xr[v] = load_raw<T, true>(a.x, row * a.ld_x + col[v], cnt[v]);
+      if (a.y) yr[v] = load_raw<T, true>(a.y, row * a.ld_y + col[v], cnt[v]);
+      if (a.dx_new) er[v] = load_raw<T, true>(a.dx_new, row * a.ld_dx_new + col[v], cnt[v]);
+      if (a.dh) gr[v] = load_raw<T, true>(a.dh, row * a.ld_dh + col[v], cnt[v]);
+    }
+    rs = a.stats[row];
+  };
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int c = (v * blockDim.x + threadIdx.x) * 8;
-    cnt[v] = a.dim - c;
-    if (cnt[v] <= 0) cnt[v] = 0;
-    load8(a.w_pre, a.pre_dtype, c, cnt[v], pre[v]);
+    col[v] = (v * blockDim.x + threadIdx.x) * 8;
+    cnt[v] = a.dim - col[v] > 0 ? a.dim - col[v] : 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      post[v][i] = gate[v][i] = 1.f;
-      d_pre[v][i] = d_post[v][i] = d_gate[v][i] = 0.f;
-    }
-    if (a.w_post) load8(a.w_post, a.post_dtype, c, cnt[v], post[v]);
+    for (int i = 0; i < 8; ++i) d_pre[v][i] = d_post[v][i] = t[v][i] = 0.f;
   }
+  fetch(first + ty);
+#pragma unroll
+  for (int v = 0; v < NV; ++v) load8(a.w_pre, a.pre_dtype, col[v], cnt[v], pre[v]);
+  // a gate group's end in this block: its shares of the gradients, into `out` row `at`
+  auto flush = [&](long long group, void* out, int dtype, long long at) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = 1.f;
+      if (a.gate) load8(a.gate, a.gate_dtype, group * a.dim + col[v], cnt[v], w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        d_post[v][i] += w[i] * t[v][i];
+        w[i] = 1.f;
+      }
+      if (out) {
+        if (a.w_post) load8(a.w_post, a.post_dtype, col[v], cnt[v], w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] *= t[v][i];
+        store8(out, dtype, at * a.dim + col[v], cnt[v], w);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[v][i] = 0.f;
+    }
+  };
   int flip = 0;
   long long group = -1;
-  for (long long row = first; row < end; ++row) {
+  for (long long base = first; base < end; base += rows_at_once) {
+    // threads past the last row repeat it without a share of the sums
+    const bool live = base + ty < end;
+    const long long row = live ? base + ty : end - 1;
+    const long long q = a.gate ? row / a.rows_per_group : 0;
+    if (q != group) {
+      if (!MANY && group >= 0) flush(group, a.d_gate, a.gate_dtype, group);
+      group = q;
+      load_factors<NV>(a, q, col, cnt, c);
+    }
     float x[NV][8], y[NV][8], e[NV][8], g[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * blockDim.x + threadIdx.x) * 8;
-      load8(a.x, T, row * a.ld_x + c, cnt[v], x[v]);
+      unpack<T>(xr[v], x[v]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[v][i] = e[v][i] = g[v][i] = 0.f;
-      if (a.y) load8(a.y, T, row * a.ld_y + c, cnt[v], y[v]);
-      if (a.dx_new) load8(a.dx_new, T, row * a.ld_dx_new + c, cnt[v], e[v]);
-      if (a.dh) load8(a.dh, T, row * a.ld_dh + c, cnt[v], g[v]);
+      if (a.y) unpack<T>(yr[v], y[v]);
+      if (a.dx_new) unpack<T>(er[v], e[v]);
+      if (a.dh) unpack<T>(gr[v], g[v]);
     }
-    if (a.gate) {
-      const long long q = row / a.rows_per_group;
-      if (q != group) {
-        group = q;
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-          load8(a.gate, a.gate_dtype, q * a.dim + (v * blockDim.x + threadIdx.x) * 8, cnt[v], gate[v]);
-      }
-    }
-    const float2 rs = a.stats[row];
     const float r = rs.x, s = rs.y;
+    fetch(row + rows_at_once);
     float sums[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         y[v][i] *= r;                                   // yhat
+        const float cy = c[v][i] * y[v][i];
         x[v][i] = a.scale * x[v][i];
-        if (a.y) x[v][i] += gate[v][i] * (y[v][i] * post[v][i]);
+        if (a.y) x[v][i] += cy;
         x[v][i] *= s;                                   // xhat
-        d_pre[v][i] += g[v][i] * x[v][i];
+        if (live) d_pre[v][i] += g[v][i] * x[v][i];
         g[v][i] *= pre[v][i];
-        const float cy = gate[v][i] * post[v][i] * y[v][i];
         e[v][i] += s * g[v][i];
         sums[0] += g[v][i] * x[v][i];
         sums[1] += cy * e[v][i];
         sums[2] += cy * x[v][i];
       }
-    row_sums<3>(sums, lds, flip);
+    row_sums<3>(sums, lds[flip], ty);
     flip ^= 1;
     const float ka = s * sums[0] * inv;
     const float kb = a.w_post ? (sums[1] - ka * sums[2]) * inv : 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const long long at = row * a.dim + (v * blockDim.x + threadIdx.x) * 8;
+      const long long at = row * a.dim + col[v];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float d = e[v][i] - ka * x[v][i];
-        const float du = gate[v][i] * d;
-        d_gate[v][i] += d * (y[v][i] * post[v][i]);
-        d_post[v][i] += du * y[v][i];
+        if (live) t[v][i] += d * y[v][i];
         x[v][i] = a.scale * d;
-        y[v][i] = r * (post[v][i] * du - y[v][i] * kb);
+        y[v][i] = r * (c[v][i] * d - y[v][i] * kb);
       }
       if (a.dx) store8(a.dx, T, at, cnt[v], x[v]);
       if (a.dy) store8(a.dy, T, at, cnt[v], y[v]);
     }
-    // the end of a gate group (parts == 1: its gradient is whole), or of this block's part
-    if (a.d_gate && (row + 1 == end || (row + 1) % a.rows_per_group == 0)) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int c = (v * blockDim.x + threadIdx.x) * 8;
-        if (a.parts > 1)
-          store8(a.gate_part, DT_F32, (long long)blockIdx.x * a.dim + c, cnt[v], d_gate[v]);
-        else
-          store8(a.d_gate, a.gate_dtype, row / a.rows_per_group * a.dim + c, cnt[v], d_gate[v]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d_gate[v][i] = 0.f;
-      }
-    }
   }
+  // rows side by side join through LDS in their order, into row 0's threads
+  auto gather = [&](float (&d)[NV][8]) {
+    if constexpr (MANY) {
+      float* mine = acc + (ty * blockDim.x + threadIdx.x) * 8;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine[i] = d[0][i];
+      __syncthreads();
+      if (ty == 0)
+        for (int k = 1; k < rows_at_once; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[0][i] += mine[k * blockDim.x * 8 + i];
+    }
+  };
+  gather(t);
+  gather(d_pre);
+  if (ty) return;
+  if (a.parts > 1) flush(group, a.d_gate ? a.gate_part : nullptr, DT_F32, blockIdx.x);
+  else flush(group, a.d_gate, a.gate_dtype, group);
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const long long at = (long long)blockIdx.x * a.dim + (v * blockDim.x + threadIdx.x) * 8;
+    const long long at = (long long)blockIdx.x * a.dim + col[v];
     if (a.d_pre) store8(a.pre_part, DT_F32, at, cnt[v], d_pre[v]);
     if (a.d_post) store8(a.post_part, DT_F32, at, cnt[v], d_post[v]);
   }
 }
 
-// out[g][c] = sum of rows g * n .. g * n + n - 1 of part [..][dim], 64 columns a block, 16 strands.
-__global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict__ part, long long n,
-                                                        int dim, void* out, int dtype) {
-  __shared__ float lds[16][64];
-  const int lane = threadIdx.x & 63, strand = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
-  const long long g = blockIdx.y;
+// Column sums of partial rows, 32 columns by 32 strands a block: blockIdx.y 0 and 1 are the two
+// weights' rows, the rest the gate groups' (`parts` rows each).
+__global__ __launch_bounds__(1024) void sum_partials_kernel(ResidualNorm a) {
+  __shared__ float lds[32][33];
+  const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  const int job = blockIdx.y;
+  const float* part = job == 0 ? a.pre_part : job == 1 ? a.post_part : a.gate_part;
+  void* out = job == 0 ? a.d_pre : job == 1 ? a.d_post : a.d_gate;
+  const int dtype = job == 0 ? a.pre_dtype : job == 1 ? a.post_dtype : a.gate_dtype;
+  if (!out) return;
+  const long long n = job < 2 ? a.blocks : a.parts, g = job < 2 ? 0 : job - 2;
   float s = 0.f;
-  if (c < dim)
-    for (long long k = strand; k < n; k += 16) s += part[(g * n + k) * dim + c];
+  if (c < a.dim) {
+#pragma unroll 4
+    for (long long k = strand; k < n; k += 32) s += part[(g * n + k) * a.dim + c];
+  }
   lds[strand][lane] = s;
   __syncthreads();
-  if (strand || c >= dim) return;
-  for (int k = 1; k < 16; ++k) s += lds[k][lane];
-  if (dtype == DT_F32) static_cast<float*>(out)[g * dim + c] = s;
-  else static_cast<uint16_t*>(out)[g * dim + c] = (uint16_t)f_to_half(s, dtype);
+  // a wave sums two columns: strands pairwise, always in the same order
+  const int cc = threadIdx.x >> 5;
+  s = lds[lane][cc];
+  for (int o = 16; o; o >>= 1) s += __shfl_xor(s, o);
+  const int oc = blockIdx.x * 32 + cc;
+  if (lane || oc >= a.dim) return;
+  if (dtype == DT_F32) static_cast<float*>(out)[g * a.dim + oc] = s;
+  else static_cast<uint16_t*>(out)[g * a.dim + oc] = (uint16_t)f_to_half(s, dtype);
 }
 
-// Threads of a row and chunks of 8 columns a thread: as few waves as hold the row with one chunk,
-// then two (whose gradients fit the registers of 512 threads), then four.
-bool row_shape(int dim, int* threads, int* nv) {
+// Threads of a row and chunks of 8 columns a thread: two for rows longer than `one`.
+bool row_shape(int dim, int one, int* threads, int* nv) {
   const int chunks = (dim + 7) / 8;
-  for (int t = 64; t <= 1024; t *= 2)
-    for (int v = 1; v <= 4; v *= 2)
-      if (t * v >= chunks && (v == 1 ? t <= 256 : v == 2 ? t <= 512 : t == 1024)) {
-        *threads = t;
-        *nv = v;
-        return true;
-      }
-  return false;
+  if (chunks > 2048) return false;
+  *nv = dim > one ? 2 : 1;
+  *threads = 64;
+  while (*threads * *nv < chunks) *threads *= 2;
+  return true;
 }
 
-constexpr long long kGradBlocks = 1024;
+constexpr long long kCus = 256;
+// Forward, two chunks a thread measured 98 against 106 us (16384 x 4096) and 105 against 129 (8192 x
+// 8192); the backward pass has no registers for them in less than 1024 threads.
+constexpr int kOneForward = 2048, kOneBackward = 8192;
 
 }  // namespace
 
 void residual_norm_split(ResidualNorm* a) {
+  int threads = 64, nv = 1;
+  row_shape(a->dim, kOneBackward, &threads, &nv);
   const long long groups = a->gate ? a->rows / a->rows_per_group : 1;
-  const long long per = a->gate ? a->rows_per_group : a->rows;
   if (!a->gate) a->rows_per_group = a->rows > 0 ? a->rows : 1;
-  if (groups >= kGradBlocks || per <= 1) {
-    const long long gpb = (groups + kGradBlocks - 1) / kGradBlocks;
+  const long long per = a->rows_per_group;
+  // as many blocks as their registers let run at once: 16 waves a CU, or three blocks of 256 threads
+  // (four took 196 us where three take 176: 65536 x 1024)
+  auto want = [&](int lanes) { return lanes > 1 ? kCus * 3 : kCus * 1024 / threads; };
+  a->lanes = threads < 256 ? 256 / threads : 1;
+  if (a->rows <= 0) {
     a->parts = 1;
-    a->rows_per_block = gpb * (per > 0 ? per : 1);
-    a->blocks = groups > 0 ? (groups + gpb - 1) / gpb : 0;
-    if (a->rows == 0) a->blocks = 0;
-    return;
+    a->blocks = 0;
+    a->rows_per_block = 1;
+  } else if (groups > want(a->lanes) / 2 && groups > 1) {
+    // whole groups: one row at a time, since a block's rows may lie in several of them
+    a->lanes = 1;
+    const long long each = (groups + want(1) - 1) / want(1);
+    a->parts = 1;
+    a->rows_per_block = each * per;
+    a->blocks = (groups + each - 1) / each;
+  } else {
+    long long parts = want(a->lanes) / groups, most = (per + a->lanes - 1) / a->lanes;
+    if (parts > most) parts = most;
+    a->rows_per_block = (per + parts - 1) / parts;
+    a->rows_per_block = (a->rows_per_block + a->lanes - 1) / a->lanes * a->lanes;
+    a->parts = (int)((per + a->rows_per_block - 1) / a->rows_per_block);
+    a->blocks = groups * a->parts;
+    if (a->parts == 1) a->rows_per_block = per;
   }
-  long long parts = kGradBlocks / groups;
-  if (parts > per) parts = per;
-  a->rows_per_block = (per + parts - 1) / parts;
-  a->parts = (int)((per + a->rows_per_block - 1) / a->rows_per_block);
-  a->blocks = groups * a->parts;
 }
 
 hipError_t launch_residual_norm(ResidualNorm a, hipStream_t stream) {
   int threads, nv;
-  if (!row_shape(a.dim, &threads, &nv)) return hipErrorInvalidValue;
+  if (!row_shape(a.dim, kOneForward, &threads, &nv)) return hipErrorInvalidValue;
   if (a.rows <= 0) return hipSuccess;
-  const int ry = threads < 256 ? 256 / threads : 1;
-  // a few rows a block once every CU has eight blocks
-  a.rows_per_block = (a.rows + 2047) / 2048;
-  a.rows_per_block = (a.rows_per_block + ry - 1) / ry * ry;
+  const int lanes = threads < 256 ? 256 / threads : 1;
+  const long long want = kCus * 4096 / (threads * lanes);
+  a.rows_per_block = (a.rows + want - 1) / want;
+  a.rows_per_block = (a.rows_per_block + lanes - 1) / lanes * lanes;
   const dim3 grid((unsigned)((a.rows + a.rows_per_block - 1) / a.rows_per_block));
-#define DMUON_RN(T, NV) \
-  hipLaunchKernelGGL((residual_norm_kernel<T, NV>), grid, dim3(threads, ry), 0, stream, a)
-#define DMUON_RN_T(NV)                              \
-  do {                                              \
-    if (a.dtype == DT_F32) DMUON_RN(DT_F32, NV);    \
-    else if (a.dtype == DT_F16) DMUON_RN(DT_F16, NV); \
-    else DMUON_RN(DT_BF16, NV);                     \
+  const dim3 block(threads, lanes);
+#define DMUON_RN(T, NV, MANY) \
+  hipLaunchKernelGGL((residual_norm_kernel<T, NV, MANY>), grid, block, 0, stream, a)
+#define DMUON_RN_T(T)                                  \
+  do {                                                 \
+    if (nv == 1 && lanes > 1) DMUON_RN(T, 1, true);    \
+    else if (lanes > 1) DMUON_RN(T, 2, true);          \
+    else if (nv == 1) DMUON_RN(T, 1, false);           \
+    else DMUON_RN(T, 2, false);                        \
   } while (0)
-  if (nv == 1) DMUON_RN_T(1);
-    else if (nv == 2) DMUON_RN_T(2);
-    else DMUON_RN_T(4);
+  if (a.dtype == DT_F32) DMUON_RN_T(DT_F32);
+  else if (a.dtype == DT_F16) DMUON_RN_T(DT_F16);
+  else DMUON_RN_T(DT_BF16);
 #undef DMUON_RN_T
 #undef DMUON_RN
   return hipGetLastError();
@@ -384,32 +496,29 @@ hipError_t launch_residual_norm(ResidualNorm a, hipStream_t stream) {
 
 hipError_t launch_residual_norm_grad(const ResidualNorm& a, hipStream_t stream) {
   int threads, nv;
-  if (!row_shape(a.dim, &threads, &nv) || a.blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (!row_shape(a.dim, kOneBackward, &threads, &nv) || a.blocks > 0x7fffffffLL) return hipErrorInvalidValue;
   if (a.blocks > 0) {
-    const dim3 grid((unsigned)a.blocks);
-#define DMUON_RN(T, NV) \
-  hipLaunchKernelGGL((residual_norm_grad_kernel<T, NV>), grid, dim3(threads), 0, stream, a)
-#define DMUON_RN_T(NV)                              \
-  do {                                              \
-    if (a.dtype == DT_F32) DMUON_RN(DT_F32, NV);    \
-    else if (a.dtype == DT_F16) DMUON_RN(DT_F16, NV); \
-    else DMUON_RN(DT_BF16, NV);                     \
+    const dim3 grid((unsigned)a.blocks), block(threads, a.lanes);
+#define DMUON_RN(T, NV, MANY) \
+  hipLaunchKernelGGL((residual_norm_grad_kernel<T, NV, MANY>), grid, block, 0, stream, a)
+#define DMUON_RN_T(T)                                  \
+  do {                                                 \
+    if (nv == 2) DMUON_RN(T, 2, false);                \
+    else if (a.lanes > 1) DMUON_RN(T, 1, true);        \
+    else DMUON_RN(T, 1, false);                        \
   } while (0)
-    if (nv == 1) DMUON_RN_T(1);
-    else if (nv == 2) DMUON_RN_T(2);
-    else DMUON_RN_T(4);
+    if (a.dtype == DT_F32) DMUON_RN_T(DT_F32);
+    else if (a.dtype == DT_F16) DMUON_RN_T(DT_F16);
+    else DMUON_RN_T(DT_BF16);
 #undef DMUON_RN_T
 #undef DMUON_RN
   }
-  const unsigned cols = (unsigned)((a.dim + 63) / 64);
-  auto sum = [&](const float* part, long long groups, long long n, void* out, int dtype) {
-    hipLaunchKernelGGL(sum_rows_kernel, dim3(cols, (unsigned)groups), dim3(1024), 0, stream, part,
-                       n, a.dim, out, dtype);
-  };
-  if (a.d_pre) sum(a.pre_part, 1, a.blocks, a.d_pre, a.pre_dtype);
-  if (a.d_post) sum(a.post_part, 1, a.blocks, a.d_post, a.post_dtype);
-  if (a.d_gate && a.parts > 1)
-    sum(a.gate_part, a.rows / a.rows_per_group, a.parts, a.d_gate, a.gate_dtype);
+  const bool gates = a.d_gate && a.parts > 1;
+  if (a.d_pre || a.d_post || gates) {
+    const dim3 grid((unsigned)((a.dim + 31) / 32),
+                    (unsigned)(gates ? 2 + a.rows / a.rows_per_group : a.d_post ? 2 : 1));
+    hipLaunchKernelGGL(sum_partials_kernel, grid, dim3(1024), 0, stream, a);
+  }
   return hipGetLastError();
 }
 
@@ -419,7 +528,7 @@ using namespace dmuon;
 
 namespace {
 
-constexpr int64_t kMaxDim = 32768;
+constexpr int64_t kMaxDim = 16384;
 
 int check(const char* who, const dmuon_residual_norm_args* a) {
   if (!a) return fail("%s: NULL arguments", who);

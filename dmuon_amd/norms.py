@@ -18,7 +18,7 @@ from . import _C
 from .vocab_loss import _dense_rows, _pitch
 
 _CODES = {torch.float32: _C.DTYPE_F32, torch.bfloat16: _C.DTYPE_BF16, torch.float16: _C.DTYPE_F16}
-_MAX_DIM = 32768
+_MAX_DIM = 16384
 
 
 def _describe(x, y, pre, post, gate, scale, eps):
@@ -50,7 +50,9 @@ def _gate_rows(who: str, gate: Tensor, x: Tensor) -> Tensor:
     if not fits:
         raise ValueError(f"{who}: a gate of {tuple(gate.shape)} has no row for each of equal runs "
                          f"of the rows of x {tuple(x.shape)}")
-    return gate.reshape(-1, dim) if gate.numel() else gate.new_zeros(1, dim)
+    if not gate.numel():
+        return gate.new_zeros(1, dim)
+    return gate if gate.dim() == 2 else gate.reshape(-1, dim)
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -58,7 +60,7 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, x, y, pre, post, gate, scale, eps, grads):
         ctx.scalars = scale, eps
         a = _describe(x, y, pre, post, gate, scale, eps)
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
         x_new = torch.empty_like(h) if y is not None or scale != 1.0 else None
         stats = None
         if grads:
@@ -67,9 +69,7 @@ class _ResidualNorm(torch.autograd.Function):
         a.h = h.data_ptr()
         if x_new is not None:
             a.x_new = x_new.data_ptr()
-        with torch.cuda.device(x.device):
-            _C.call("dmuon_residual_norm", ctypes.byref(a),
-                    torch.cuda.current_stream(x.device).cuda_stream)
+        _C.call_on(x.device, "dmuon_residual_norm", ctypes.byref(a))
         ctx.save_for_backward(x, y, pre, post, gate, stats)
         ctx.set_materialize_grads(False)
         return x_new, h
@@ -92,15 +92,13 @@ class _ResidualNorm(torch.autograd.Function):
                                  (x, y, pre, post, gate), ctx.needs_input_grad):
             g = None
             if t is not None and need:
-                g = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+                g = torch.empty_like(t, memory_format=torch.contiguous_format)
                 setattr(a, name, g.data_ptr())
             out.append(g)
         need = _C.c_i64()
-        with torch.cuda.device(x.device):
-            _C.call("dmuon_residual_norm_grad_workspace_size", ctypes.byref(a), ctypes.byref(need))
-            ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
-            _C.call("dmuon_residual_norm_grad", ctypes.byref(a), ws.data_ptr(), need.value,
-                    torch.cuda.current_stream(x.device).cuda_stream)
+        _C.call("dmuon_residual_norm_grad_workspace_size", ctypes.byref(a), ctypes.byref(need))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+        _C.call_on(x.device, "dmuon_residual_norm_grad", ctypes.byref(a), ws.data_ptr(), need.value)
         return (*out, None, None, None)
 
 
@@ -138,7 +136,9 @@ def residual_norm(x: Tensor, y: Optional[Tensor], pre_weight: Tensor, *,
     for name, t in (("pre_weight", pre_weight), ("post_weight", post_weight)):
         if t is not None and tuple(t.shape) != (dim,):
             raise ValueError(f"{who}: {name} must be [{dim}], got {tuple(t.shape)}")
-    rows = x.reshape(-1, dim)
+    # a two-dimensional x takes no views: each would be a node of the gradient's graph
+    flat = x.dim() == 2
+    rows = x if flat else x.reshape(-1, dim)
     if gate is not None:
         gate = _gate_rows(who, gate, x)
     for name, t in (("pre_weight", pre_weight), ("post_weight", post_weight), ("gate", gate)):
@@ -149,7 +149,9 @@ def residual_norm(x: Tensor, y: Optional[Tensor], pre_weight: Tensor, *,
             raise RuntimeError(f"{who}: tensors must live on one GPU (HIP kernel only)")
     contiguous = (None if t is None else t.contiguous() for t in (pre_weight, post_weight, gate))
     x_new, h = _ResidualNorm.apply(_dense_rows(rows),
-                                   None if y is None else _dense_rows(y.reshape(-1, dim)),
+                                   None if y is None else _dense_rows(y if flat else y.reshape(-1, dim)),
                                    *contiguous, float(residual_scale), float(eps),
                                    torch.is_grad_enabled())
-    return (x if x_new is None else x_new.view(x.shape)), h.view(x.shape)
+    if x_new is None:
+        x_new = x
+    return (x_new, h) if flat else (x_new.view(x.shape), h.view(x.shape))

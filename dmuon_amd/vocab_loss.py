@@ -64,12 +64,10 @@ class _Targets:
             if t is not None:
                 setattr(a, name, t.data_ptr())
         need = _C.c_i64()
-        with torch.cuda.device(dev):
-            _C.call("dmuon_head_loss_workspace_size", ctypes.byref(a), ctypes.byref(need))
-            # from the caching allocator: reused in this stream's order, nothing is kept
-            ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-            _C.call("dmuon_head_loss", ctypes.byref(a), ws.data_ptr(), need.value,
-                    torch.cuda.current_stream(dev).cuda_stream)
+        _C.call("dmuon_head_loss_workspace_size", ctypes.byref(a), ctypes.byref(need))
+        # from the caching allocator: reused in this stream's order, nothing is kept
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        _C.call_on(dev, "dmuon_head_loss", ctypes.byref(a), ws.data_ptr(), need.value)
         return loss, reduced, dh, dw
 
 
@@ -78,10 +76,8 @@ def _scaled(g: Optional[Tensor], dtype: torch.dtype, factor: Tensor) -> Optional
     if g is None:
         return None
     out = g if g.dtype == dtype else torch.empty_like(g, dtype=dtype)
-    code = {torch.float32: _C.DTYPE_F32, **_CODES}
-    with torch.cuda.device(g.device):
-        _C.call("dmuon_scale_by", g.data_ptr(), code[g.dtype], out.data_ptr(), code[dtype],
-                g.numel(), factor.data_ptr(), torch.cuda.current_stream(g.device).cuda_stream)
+    _C.call_on(g.device, "dmuon_scale_by", g.data_ptr(), _CODES.get(g.dtype, _C.DTYPE_F32),
+               out.data_ptr(), _CODES.get(dtype, _C.DTYPE_F32), g.numel(), factor.data_ptr())
     return out
 
 
@@ -145,10 +141,11 @@ def _index(who: str, name: str, t: Tensor, shape, device) -> Tensor:
 
 def _run(targets: _Targets, hidden: Tensor, weight: Tensor, reduction: str) -> Tensor:
     shape = hidden.shape[:-1]
-    rows = _dense_rows(hidden.reshape(-1, hidden.shape[-1]))
+    # a two-dimensional hidden takes no view: it would be a node of the gradient's graph
+    rows = _dense_rows(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1]))
     out = _HeadLoss.apply(rows, _dense_rows(weight), targets, _REDUCTIONS[reduction],
                           torch.is_grad_enabled())
-    return out if reduction != "none" else out.view(shape)
+    return out.view(shape) if reduction == "none" and len(shape) != 1 else out
 
 
 def linear_cross_entropy(hidden: Tensor, weight: Tensor, target: Tensor, *,

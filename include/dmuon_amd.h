@@ -507,7 +507,7 @@ int dmuon_scale_by(const void* src, int src_dtype, void* dst, int dst_dtype, int
  *   u = y * rsqrt(mean(y^2) + eps) * w_post  (w_post NULL: u = y)
  *   x_new = scale * x + gate * u             (gate NULL: 1; y NULL: x_new = scale * x)
  *   h = x_new * rsqrt(mean(x_new^2) + eps) * w_pre
- * for `rows` rows of dim (1 .. 32768) values. x, y, x_new, h and their gradients are of `dtype`
+ * for `rows` rows of dim (1 .. 16384) values. x, y, x_new, h and their gradients are of `dtype`
  * (DMUON_DTYPE_F32, _BF16 or _F16), x, y and the incoming gradients with a row pitch, the results
  * dense; w_pre, w_post [dim] and gate [gates][dim] each have a dtype of their own. Gate row g
  * belongs to the rows / gates consecutive rows from g * rows / gates on. Any element alignment.

@@ -205,7 +205,7 @@ def test_no_counted_token_gives_zeros(gpu):
         a, b = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
         loss = call(a, b)
         loss.backward()
-        assert float(loss) == 0.0 and not bool(a.grad.any()) and not bool(b.grad.any())
+        assert float(loss.detach()) == 0.0 and not bool(a.grad.any()) and not bool(b.grad.any())
 
 
 @pytest.mark.gpu
@@ -214,7 +214,7 @@ def test_no_token_at_all(gpu):
     a, b = h.requires_grad_(True), w.requires_grad_(True)
     loss = dmuon.linear_cross_entropy(a, b, t)
     loss.backward()
-    assert float(loss) == 0.0 and a.grad.shape == (0, 64) and not bool(b.grad.any())
+    assert float(loss.detach()) == 0.0 and a.grad.shape == (0, 64) and not bool(b.grad.any())
     assert dmuon.linear_cross_entropy(a, b, t, reduction="none").shape == (0,)
 
 
@@ -456,7 +456,7 @@ def test_c_entry_refusals_without_gpu():
     def says(rc, text):
         assert rc != 0 and text in lib.dmuon_last_error().decode()
 
-    assert size() == 0 and need.value > 4 * 256 * 4
+    assert size() == 0 and need.value >= 4 * 128 * 2      # two bytes a logit, rows of whole 64
     says(size(dtype=0), "16-bit")
     says(size(grad_dtype=2), "gradients")
     says(size(tokens=-1), "tokens")
