@@ -147,7 +147,7 @@ _SIGNATURES = {
                                  c_int, c_d, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
     "dmuon_head_loss_workspace_size": (c_int, [c_hp, ctypes.POINTER(c_i64)]),
     "dmuon_head_loss": (c_int, [c_hp, c_vp, c_i64, c_vp]),
-    "dmuon_scale_by": (c_int, [c_vp, c_int, c_vp, c_int, c_i64, c_vp, c_vp]),
+    "dmuon_scale_by": (c_int, [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_int, c_int, c_vp, c_vp]),
     "dmuon_residual_norm": (c_int, [c_np, c_vp]),
     "dmuon_residual_norm_grad_workspace_size": (c_int, [c_np, ctypes.POINTER(c_i64)]),
     "dmuon_residual_norm_grad": (c_int, [c_np, c_vp, c_i64, c_vp]),
@@ -204,17 +204,24 @@ def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args))
 
 
+def current_stream(device) -> int:
+    """Handle of the device's current stream."""
+    import torch
+
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # without a Stream object: 2 us less
+    return raw(device.index) if raw else torch.cuda.current_stream(device).cuda_stream
+
+
 def call_on(device, name: str, *args) -> None:
     """``call`` with the device's current stream as last argument and the device current. (Entering
     ``torch.cuda.device`` costs more than a small kernel's launch: only where it changes something.)"""
     import torch
 
-    stream = torch.cuda.current_stream(device).cuda_stream
     if torch.cuda.current_device() == device.index:
-        check(getattr(lib(), name)(*args, stream))
+        call(name, *args, current_stream(device))
     else:
         with torch.cuda.device(device):
-            check(getattr(lib(), name)(*args, stream))
+            call(name, *args, current_stream(device))
 
 
 PROFILE_CLASSES = ("pre", "norm", "syrk", "poly", "gemm", "final", "adamw", "clip")

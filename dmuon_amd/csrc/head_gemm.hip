@@ -21,7 +21,7 @@
 namespace dmuon {
 namespace {
 
-constexpr int kTile = 256, kSlice = 64;
+constexpr int kTile = 256, kSlice = 64, kCus = 256;
 constexpr float kInf = __builtin_inff();
 // rows of any pitch and bases of any element alignment
 typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
@@ -90,75 +90,70 @@ struct Mover {
   }
 };
 
-// A wave's 128 x 64 logits: statistics, and the exponentials (through LDS slab by slab, so that the
-// stores are whole 128-byte row segments) or the logits themselves.
+// 16 x 64 logits of a wave: statistics, and the exponentials (through LDS, so that the stores are
+// whole 128-byte row segments) or the logits themselves. acc[y]: columns 16 y ..
 template <int MODE>
-__device__ __forceinline__ void logits_epilogue(const HeadGemm& a, const f32x4_t (&acc)[8][4],
-                                                int iw, int jw, int lane, char* slab) {
-  const int jl = 4 * (lane >> 4);
+__device__ __forceinline__ void logits_epilogue(const HeadGemm& a, const f32x4_t (&acc)[4], int i0,
+                                                int jw, int lane, char* slab) {
+  const int jl = 4 * (lane >> 4), i = i0 + (lane & 15);
   const bool inside = jw + 64 <= a.N;
+  f32x4_t z[4];
+  float m = -kInf;
 #pragma unroll
-  for (int x = 0; x < 8; ++x) {
-    const int i = iw + 16 * x + (lane & 15);
-    f32x4_t z[4];
-    float m = -kInf;
+  for (int y = 0; y < 4; ++y) {
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        z[y][e] = acc[x][y][e] * a.scale;
-        // columns past the vocabulary: no maximum, no share of the sum
-        if (!inside && jw + jl + 16 * y + e >= a.N) z[y][e] = -kInf;
-        m = fmaxf(m, z[y][e]);
-      }
-      if (MODE == HG_LOGITS && i < a.M)
-        *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.Z) + (long long)i * a.ldz + jw + jl +
-                                    16 * y) = z[y];
+    for (int e = 0; e < 4; ++e) {
+      z[y][e] = acc[y][e] * a.scale;
+      // columns past the vocabulary: no maximum, no share of the sum
+      if (!inside && jw + jl + 16 * y + e >= a.N) z[y][e] = -kInf;
+      m = fmaxf(m, z[y][e]);
     }
-    m = fmaxf(m, __shfl_xor(m, 16));
-    m = fmaxf(m, __shfl_xor(m, 32));
-    float s = 0.f;
+    if (MODE == HG_LOGITS && i < a.M)
+      *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.Z) + (long long)i * a.ldz + jw + jl +
+                                  16 * y) = z[y];
+  }
+  m = fmaxf(m, __shfl_xor(m, 16));
+  m = fmaxf(m, __shfl_xor(m, 32));
+  float s = 0.f;
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
+  for (int y = 0; y < 4; ++y) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        z[y][e] = z[y][e] == -kInf ? 0.f : __expf(z[y][e] - m);
-        s += z[y][e];
-      }
-      if constexpr (MODE == HG_EXP) {
-        constexpr float up = (float)(1 << kExpShift);
-        const u32x2_t o = {pack2_elt<ELT_F16>(up * z[y][0], up * z[y][1]),
-                           pack2_elt<ELT_F16>(up * z[y][2], up * z[y][3])};
-        *reinterpret_cast<u32x2_t*>(slab + (16 * (x & 1) + (lane & 15)) * T::EPN +
-                                    (jl + 16 * y) * 2) = o;
-      }
+    for (int e = 0; e < 4; ++e) {
+      z[y][e] = z[y][e] == -kInf ? 0.f : __expf(z[y][e] - m);
+      s += z[y][e];
     }
-    s += __shfl_xor(s, 16);
-    s += __shfl_xor(s, 32);
-    if (lane < 16 && i < a.M)
-      a.stats[(long long)i * a.n_stats + jw / kStatCols] = make_float2(m, s);
-    if (MODE == HG_EXP && (x & 1)) {
-      const int cr = lane >> 3, cc = lane & 7;
-      u32x4_t d[4];
+    if constexpr (MODE == HG_EXP) {
+      constexpr float up = (float)(1 << kExpShift);
+      const u32x2_t o = {pack2_elt<ELT_F16>(up * z[y][0], up * z[y][1]),
+                         pack2_elt<ELT_F16>(up * z[y][2], up * z[y][3])};
+      *reinterpret_cast<u32x2_t*>(slab + (lane & 15) * T::EPN + (jl + 16 * y) * 2) = o;
+    }
+  }
+  s += __shfl_xor(s, 16);
+  s += __shfl_xor(s, 32);
+  if (lane < 16 && i < a.M)
+    a.stats[(long long)i * a.n_stats + jw / kStatCols] = make_float2(m, s);
+  if constexpr (MODE == HG_EXP) {
+    const int cr = lane >> 3, cc = lane & 7;
+    u32x4_t d[2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        d[k] = *reinterpret_cast<const u32x4_t*>(slab + (8 * k + cr) * T::EPN + 16 * cc);
+    for (int k = 0; k < 2; ++k)
+      d[k] = *reinterpret_cast<const u32x4_t*>(slab + (8 * k + cr) * T::EPN + 16 * cc);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = iw + 16 * (x - 1) + 8 * k + cr;
-        if (r < a.M)
-          __builtin_nontemporal_store(
-              d[k], reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.Z) + (long long)r * a.ldz +
-                                               jw + 8 * cc));
-      }
+    for (int k = 0; k < 2; ++k) {
+      const int r = i0 + 8 * k + cr;
+      if (r < a.M)
+        __builtin_nontemporal_store(
+            d[k], reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.Z) + (long long)r * a.ldz +
+                                             jw + 8 * cc));
     }
   }
 }
 
-// A wave's 128 x 64 values of a gradient: fp32 sums, or the scaled result. 16-bit results pass
+// A wave's 16 XB x 64 values of a gradient: fp32 sums, or the scaled result. 16-bit results pass
 // through LDS slab by slab, so that the stores are whole 128-byte row segments.
-template <int E>
-__device__ __forceinline__ void grad_epilogue(const HeadGemm& a, f32x4_t (&acc)[8][4], int iw,
+template <int E, int XB>
+__device__ __forceinline__ void grad_epilogue(const HeadGemm& a, f32x4_t (&acc)[XB][4], int iw,
                                               int jw, int lane, char* slab, int split) {
   const int jl = 4 * (lane >> 4);
   const bool whole = a.out && a.splits == 1;
@@ -168,7 +163,7 @@ __device__ __forceinline__ void grad_epilogue(const HeadGemm& a, f32x4_t (&acc)[
   float* dst = whole ? static_cast<float*>(a.out) : part;
   const long long ldd = whole ? a.ldo : a.ldp;
 #pragma unroll
-  for (int x = 0; x < 8; ++x) {
+  for (int x = 0; x < XB; ++x) {
     const int i = iw + 16 * x + (lane & 15);
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
@@ -301,13 +296,18 @@ __device__ __forceinline__ void head_tile(const HeadGemm& a, char* smem, int bi,
   // slices of this split
   const int all = (a.K + kSlice - 1) / kSlice, per = (all + a.splits - 1) / a.splits;
   const int s0 = split * per, KT = min(per, all - s0);
+  // Few rows: every tile has rows of B to itself, and starts elsewhere in K. (Rows of a power of two
+  // bytes begin on the same memory channel; together the tiles would ask a few channels at a time: 64
+  // rows against 128256 columns of 4096 take 185 us, 234 with every tile from 0 on.)
+  const int first = a.few && KT > 0 ? (int)(blockIdx.x >> 3) * 5 % KT : 0;
+  auto slice = [&](int k) { return s0 + k + first - (k + first >= KT ? KT : 0); };
   if (KT > 0) {
     if (grp == 1) {
       // slices 0 and 1 (past the end: the last slice again, into a slot never read)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        issue_a(s0 + min(s, KT - 1), s);
-        mb.template issue<8>(s0 + min(s, KT - 1), s, 0);
+        issue_a(slice(min(s, KT - 1)), s);
+        mb.template issue<8>(slice(min(s, KT - 1)), s, 0);
       }
       wait_vmcnt<16>();                   // slice 0 has landed
     }
@@ -317,11 +317,11 @@ __device__ __forceinline__ void head_tile(const HeadGemm& a, char* smem, int bi,
       constexpr bool RA = decltype(ra_c)::value, RB = decltype(rb_c)::value;
       constexpr bool LAST = decltype(last_c)::value;
       mem_phase(kt & 1);
-      if (RA && grp == 0) issue_a(s0 + kt + 1, (kt + 1) & 1);
+      if (RA && grp == 0) issue_a(slice(kt + 1), (kt + 1) & 1);
       __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): this wave's fragments are in registers
       if (grp == 1) {
         if (RB) {
-          mb.template issue<8>(s0 + kt + 2, kt & 1, 0);
+          mb.template issue<8>(slice(kt + 2), kt & 1, 0);
           wait_vmcnt<8>();                // all of slice kt + 1 has landed
         } else {
           wait_vmcnt<0>();
@@ -351,8 +351,10 @@ __device__ __forceinline__ void head_tile(const HeadGemm& a, char* smem, int bi,
   if constexpr (LIVE) {
     const int iw = i0 + grp * 128, jw = j0 + wj * 64;
     char* slab = smem + wave * T::EPI_REGION;
-    if constexpr (MODE == HG_GRAD) grad_epilogue<E>(a, acc, iw, jw, lane, slab, split);
-    else logits_epilogue<MODE>(a, acc, iw, jw, lane, slab);
+    if constexpr (MODE == HG_GRAD) grad_epilogue<E, 8>(a, acc, iw, jw, lane, slab, split);
+    else
+#pragma unroll
+      for (int x = 0; x < 8; ++x) logits_epilogue<MODE>(a, acc[x], iw + 16 * x, jw, lane, slab);
   }
 }
 
@@ -376,6 +378,127 @@ void head_gemm_kernel(const HeadGemm a) {
   else head_tile<E, MODE, AKM, BKM, false>(a, smem, bi, bj, sp);
 }
 
+// A weight gradient over few tokens: bound by writing it. 128 x 128 tiles, four waves of 64 x 64, one
+// K slice in LDS at a time; four blocks a CU hide each other's waits, where a 256-tile of a slice or
+// two waits alone for its first loads and its stores (see weight_is_short).
+template <int E>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 4)))
+void head_short_kernel(const HeadGemm a) {
+  constexpr int kSide = 128, kBlock = kSlice * 128;    // LDS bytes of 64 values of a slice
+  constexpr int kSlab = 32 * T::EPN;
+  static_assert(4 * kSlab <= 4 * kBlock, "results pass through the slices' place");
+  __shared__ __attribute__((aligned(16))) char smem[4 * kBlock];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int mt = (a.M + kSide - 1) / kSide, nt = (a.N + kSide - 1) / kSide;
+  const int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int g = t / (8 * nt), rows = min(mt - 8 * g, 8), r = t - g * 8 * nt;
+  const int i0 = __builtin_amdgcn_readfirstlane((8 * g + r % rows) * kSide);
+  const int j0 = __builtin_amdgcn_readfirstlane(r / rows * kSide);
+  // waves 0 and 1 move the slice's 64-value blocks of A, 2 and 3 those of B
+  Mover<true> mv;
+  if (wave < 2) mv.init(a.A, a.lda, i0, a.M, a.K, wave, 64, lane, smem);
+  else mv.init(a.B, a.ldb, j0, a.N, a.K, wave - 2, 64, lane, smem + 2 * kBlock);
+  const int wi = wave >> 1, wj = wave & 1;
+  f32x4_t acc[4][4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) acc[x][y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const int KT = (a.K + kSlice - 1) / kSlice;
+  for (int s = 0; s < KT; ++s) {
+    if (s > 0) __syncthreads();           // the slice before has been read
+    mv.issue<8>(s, 0, 0);
+    wait_vmcnt<0>();
+    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      bf16x8_t af[4], bfr[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int off = kmajor64_lane_off(lane, 16 * x) + ks * 32 * 128;
+        af[x] = read_kmajor(smem + wi * kBlock + off, 128);
+        bfr[x] = read_kmajor(smem + (2 + wj) * kBlock + off, 128);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[x][y] = mfma_16x16x32<E>(bfr[y], af[x], acc[x][y]);
+    }
+  }
+  __syncthreads();
+  const int iw = i0 + wi * 64, jw = j0 + wj * 64;
+  if (iw < a.M && jw < a.N) grad_epilogue<E, 4>(a, acc, iw, jw, lane, smem + wave * kSlab, 0);
+}
+
+// Logits of at most 16 rows over a vocabulary with less than a 256-tile for every CU. A block takes 64
+// columns, its four waves every fourth 64-wide K step each, straight from memory into MFMA operands
+// (a lane's 16 bytes are its operand); the partial sums join through LDS. One row of 2048 against
+// 32001 columns (126 tiles): 28 us, 41 on the 256-tiles; against 128256 columns of 4096 both take
+// 183 us, and 16 rows, which each block here reads for itself, 213 against 184.
+template <int E, int MODE>
+__global__ __launch_bounds__(256) void head_few_kernel(const HeadGemm a) {
+  __shared__ __attribute__((aligned(16))) f32x4_t part[4][4][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int jw = blockIdx.x * 64;
+  const int kl = 8 * (lane >> 4);
+  // rows past the operands repeat the last one: their results are not used
+  const uint16_t* hp = a.A + (long long)min(lane & 15, a.M - 1) * a.lda + kl;
+  const uint16_t* wp[4];
+  f32x4_t acc[4];
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    wp[y] = a.B + (long long)min(jw + 16 * y + (lane & 15), a.N - 1) * a.ldb + kl;
+    acc[y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  struct Step {
+    bf16x8_t h[2], w[2][4];
+  };
+  auto load = [&](Step& s, int k0) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int k = k0 + 32 * p;
+      const bool in = k + kl < a.K;
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        s.w[p][y] = in ? *reinterpret_cast<const bf16x8_t*>(wp[y] + k) : bf16x8_t{};
+      s.h[p] = in ? *reinterpret_cast<const bf16x8_t*>(hp + k) : bf16x8_t{};
+    }
+  };
+  auto multiply = [&](const Step& s) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) acc[y] = mfma_16x16x32<E>(s.w[p][y], s.h[p], acc[y]);
+  };
+  // the blocks start at different steps: see head_tile
+  const int n = (a.K + 4 * kSlice - 1) / (4 * kSlice), first = n > 0 ? (int)(blockIdx.x >> 3) % n : 0;
+  auto step = [&](int i) {
+    const int q = i + first - (i + first >= n ? n : 0);
+    return i < n ? (4 * q + wave) * kSlice : a.K;
+  };
+  Step s[2];
+  load(s[0], step(0));
+  for (int i = 0; i < n; i += 2) {
+    load(s[1], step(i + 1));
+    multiply(s[0]);
+    load(s[0], step(i + 2));
+    multiply(s[1]);
+  }
+#pragma unroll
+  for (int y = 0; y < 4; ++y) part[wave][y][lane] = acc[y];
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int y = 0; y < 4; ++y)
+#pragma unroll
+    for (int w = 1; w < 4; ++w) acc[y] += part[w][y][lane];
+  // the exponentials' way out lies over this wave's own part
+  static_assert(sizeof(part[0]) >= 16 * T::EPN, "exponentials of 16 rows");
+  logits_epilogue<MODE>(a, acc, 0, jw, lane, reinterpret_cast<char*>(part));
+}
+
 // out = alpha * sum over the splits
 template <int D>
 __global__ __launch_bounds__(256) void join_splits_kernel(const HeadGemm a) {
@@ -395,13 +518,22 @@ long long tiles_of(int M, int N) {
   return ((long long)M + kTile - 1) / kTile * ((N + kTile - 1) / kTile);
 }
 
+// Whether a weight gradient [M][N] over K tokens takes the 128-tiles. Measured against the 256-tiles:
+// 128256 x 4096 over 64 tokens 226 against 261 us, over 192 316 against 326, over 256 376 against
+// 372; 32000 x 2048 (1000 256-tiles) 29 against 38, over 512 73 against 76; 8192 x 512 (64) 5.1
+// against 9, over 512 9.7 against 17.
+bool weight_is_short(int M, int N, int K) {
+  return K <= 192 || (K <= 512 && tiles_of(M, N) <= 4 * kCus);
+}
+
 }  // namespace
 
 // The least of: waves of tiles on 256 CUs times the slices of a tile, and the join of the parts. In
 // units of one slice's time (1.8 us): a tile costs 8 more for its first loads and its results, the
 // join 3 for its launch and 8 bytes a value and split at 4 TB/s.
-int head_gemm_splits(int M, int N, int K) {
-  constexpr int kCus = 256, kMost = 16, kLeast = 4;
+int head_gemm_splits(int M, int N, int K, bool weight) {
+  if (weight && weight_is_short(M, N, K)) return 1;
+  constexpr int kMost = 16, kLeast = 4;
   const long long tiles = tiles_of(M, N);
   const int slices = (K + kSlice - 1) / kSlice;
   int best = 1;
@@ -429,21 +561,41 @@ hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream) {
     return hipErrorInvalidValue;
   if (a.splits > 1 && (a.mode != HG_GRAD || !a.out || !a.part || a.add_part))
     return hipErrorInvalidValue;
+  if (a.mode == HG_GRAD ? !a.b_kmajor
+                        : a.a_kmajor || a.b_kmajor || !a.stats ||
+                              (a.mode != HG_STATS && (!a.Z || a.ldz < (a.N + 63) / 64 * 64)))
+    return hipErrorInvalidValue;
+  if (a.few && a.mode != HG_GRAD && a.M <= 16 && nb < kCus) {
+    const dim3 few((unsigned)((a.N + 63) / 64));
+#define DMUON_FEW(E, MODE) hipLaunchKernelGGL((head_few_kernel<E, MODE>), few, dim3(256), 0, stream, a)
+    if (a.elt == ELT_F16 && a.mode == HG_STATS) DMUON_FEW(ELT_F16, HG_STATS);
+    else if (a.elt == ELT_F16 && a.mode == HG_LOGITS) DMUON_FEW(ELT_F16, HG_LOGITS);
+    else if (a.elt == ELT_BF16 && a.mode == HG_STATS) DMUON_FEW(ELT_BF16, HG_STATS);
+    else if (a.elt == ELT_BF16 && a.mode == HG_EXP) DMUON_FEW(ELT_BF16, HG_EXP);
+    else return hipErrorInvalidValue;
+#undef DMUON_FEW
+    return hipGetLastError();
+  }
+  if (a.mode == HG_GRAD && a.a_kmajor && a.splits == 1 && weight_is_short(a.M, a.N, a.K)) {
+    const long long tiles = ((long long)a.M + 127) / 128 * ((a.N + 127) / 128);
+    if (tiles > 0x7fffffffLL) return hipErrorInvalidValue;
+    const dim3 tg((unsigned)tiles);
+    if (a.elt == ELT_F16) hipLaunchKernelGGL(head_short_kernel<ELT_F16>, tg, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(head_short_kernel<ELT_BF16>, tg, dim3(256), 0, stream, a);
+    return hipGetLastError();
+  }
   const dim3 grid((unsigned)nb);
 #define DMUON_HG(E, MODE, AKM, BKM) \
   hipLaunchKernelGGL((head_gemm_kernel<E, MODE, AKM, BKM>), grid, dim3(512), 0, stream, a)
 #define DMUON_HG_E(E)                                                     \
   do {                                                                    \
     if (a.mode == HG_STATS) DMUON_HG(E, HG_STATS, false, false);          \
-    else if (a.mode == HG_EXP) DMUON_HG(E, HG_EXP, false, false);         \
-    else if (a.mode == HG_LOGITS) DMUON_HG(E, HG_LOGITS, false, false);   \
+    else if (a.mode == (E == ELT_F16 ? HG_LOGITS : HG_EXP))               \
+      DMUON_HG(E, (E == ELT_F16 ? HG_LOGITS : HG_EXP), false, false);     \
+    else if (a.mode != HG_GRAD) return hipErrorInvalidValue;              \
     else if (a.a_kmajor) DMUON_HG(E, HG_GRAD, true, true);                \
     else DMUON_HG(E, HG_GRAD, false, true);                               \
   } while (0)
-  if (a.mode == HG_GRAD ? !a.b_kmajor
-                        : a.a_kmajor || a.b_kmajor || !a.stats ||
-                              (a.mode != HG_STATS && (!a.Z || a.ldz < (a.N + 63) / 64 * 64)))
-    return hipErrorInvalidValue;
   if (a.elt == ELT_F16) DMUON_HG_E(ELT_F16);
   else DMUON_HG_E(ELT_BF16);
 #undef DMUON_HG_E

@@ -25,6 +25,9 @@ enum HeadGemmMode : int { HG_STATS = 0, HG_EXP = 1, HG_LOGITS = 2, HG_GRAD = 3 }
 // fp16 holds exponentials down to 2^-29 of their maximum with all its bits
 constexpr int kExpShift = 15;
 
+// Rows up to which the logits have one row of tiles, bound by reading the weight.
+constexpr int kFewRows = 256;
+
 // acc[i][j] = sum_k A(i, k) * B(j, k): operand X's element (r, k) is X[r * ld + k], or
 // X[k * ld + r] with x_kmajor.
 struct HeadGemm {
@@ -39,10 +42,11 @@ struct HeadGemm {
   void* out; long long ldo; int out_dtype;   // HG_GRAD: result (DT_F32 or the operands'), or NULL
   float* part; long long ldp;             // HG_GRAD: fp32 sums [M][ldp], or NULL
   int add_part;                           // part holds earlier sums to add to
+  int few;                                // logits of a call of at most kFewRows rows
   int splits;                             // HG_GRAD: K in so many parts, part [splits][M][ldp]
 };
-// K splits that fill the chip where a gradient has few tiles (1: none).
-int head_gemm_splits(int M, int N, int K);
+// K splits that fill the chip where a gradient has few tiles (1: none); weight: of the weight.
+int head_gemm_splits(int M, int N, int K, bool weight);
 // Operands at 16-byte alignment with pitches of whole 16-byte chunks. Rows that end inside a chunk
 // are readable to its end, and hold zeros there in row form (past K).
 hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream);
@@ -65,12 +69,12 @@ struct HeadRows {
   float* mass;                            // [n]: sum of the row's probs, < 0: not counted
   float* lse;                             // [n]
   float* loss;                            // [n]
-  float* row_weight;                      // [n]: 2^kGradShift * row gradient / largest, or NULL
+  float* row_weight;                      // [n]: 2^kGradShift * row gradient / largest
   float* alpha;                           // [1]: what turns a stored gradient into the real one
   float* mean;                            // [1] or NULL: the reduced loss
 };
-// ids, probs, mass and logits of every row (H, W: the products' operands, any alignment); row weights
-// and alpha with `grads`.
+// ids, probs, mass and logits of every row (H, W: the products' operands, any alignment); with
+// `grads` and row_grad the row weights and alpha.
 hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long ldh,
                                const uint16_t* W, long long ldw, int dim, int elt, bool grads,
                                hipStream_t stream);
@@ -80,11 +84,17 @@ hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long l
 hipError_t launch_head_rows(const HeadRows& r, int first, int rows, const float2* stats,
                             const void* Z, uint16_t* G, long long ldg, int elt,
                             hipStream_t stream);
-// mean[0] = sum of the losses, divided by the number of counted rows for DMUON_LOSS_MEAN.
+// mean[0] = sum of the losses, divided by the number of counted rows for DMUON_LOSS_MEAN, and alpha.
 hipError_t launch_head_reduce(const HeadRows& r, hipStream_t stream);
 
-// dst = factor[0] * src for n values of the DT_* types; in place, nothing moves where it is 1.
-hipError_t launch_scale_by(const void* src, int src_dtype, void* dst, int dst_dtype, long long n,
-                           const float* factor, hipStream_t stream);
+// dst[k] = factor[0] * src[k] for n[k] values, k = 0 and 1; in_place: every dst is its src, and
+// nothing moves where the factor is 1.
+struct ScaleBy {
+  const void* src[2]; void* dst[2];
+  long long n[2];
+  const float* factor;
+  int in_place;
+};
+hipError_t launch_scale_by(const ScaleBy& a, int src_dtype, int dst_dtype, hipStream_t stream);
 
 }  // namespace dmuon

@@ -27,7 +27,7 @@ constexpr int64_t kMaxVocab = (int64_t(1) << 22) - 256;
 
 struct Layout {
   int64_t chunk, ld;                      // tokens of a chunk, pitch of its logits
-  int64_t ids, probs, logits, mass, lse, row_weight, alpha, Z, stats, G, part, H, W, bytes;
+  int64_t ids, probs, logits, mass, lse, loss, row_weight, alpha, Z, stats, G, part, H, W, bytes;
   int64_t pad;                            // pitch of the copies of hidden and weight
   bool copy_h, copy_w;
 };
@@ -102,6 +102,7 @@ Layout lay_out(const dmuon_head_loss_args& a) {
   l.logits = take(a.tokens * k * 4);
   l.mass = take(a.tokens * 4);
   l.lse = take(a.tokens * 4);
+  l.loss = take(a.loss ? 0 : a.tokens * 4);
   l.row_weight = take(a.tokens * 4);
   l.alpha = take(4);
   l.stats = take(l.chunk * tiles * 8);
@@ -112,12 +113,12 @@ Layout lay_out(const dmuon_head_loss_args& a) {
   if (a.d_weight && l.chunk < a.tokens) {
     if (a.grad_dtype != DMUON_DTYPE_F32) part = a.vocab * a.dim * 4;
   } else if (a.d_weight) {
-    const int s = head_gemm_splits((int)a.vocab, (int)a.dim, (int)a.tokens);
+    const int s = head_gemm_splits((int)a.vocab, (int)a.dim, (int)a.tokens, true);
     if (s > 1) part = s * a.vocab * a.dim * 4;
   }
   if (a.d_hidden)
     for (int64_t rows : {l.chunk, l.chunk > 0 ? a.tokens % l.chunk : 0}) {
-      const int s = head_gemm_splits((int)rows, (int)a.dim, (int)a.vocab);
+      const int s = head_gemm_splits((int)rows, (int)a.dim, (int)a.vocab, false);
       if (s > 1 && s * rows * a.dim * 4 > part) part = s * rows * a.dim * 4;
     }
   l.part = take(part);
@@ -148,8 +149,8 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
   const dmuon_head_loss_args& a = *args;
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   const bool grads = a.d_hidden || a.d_weight;
-  if (!a.weight || (a.tokens > 0 && (!a.hidden || !a.loss)))
-    return fail("%s: NULL hidden, weight or loss", who);
+  if (!a.weight || (a.tokens > 0 && !a.hidden)) return fail("%s: NULL hidden or weight", who);
+  if (a.reduction == DMUON_LOSS_ROWS && a.tokens > 0 && !a.loss) return fail("%s: loss is NULL", who);
   if (a.reduction != DMUON_LOSS_ROWS && !a.reduced) return fail("%s: reduced is NULL", who);
   if (a.reduction == DMUON_LOSS_ROWS && grads && a.tokens > 0 && !a.row_grad)
     return fail("%s: the gradients of unreduced losses need row_grad", who);
@@ -181,7 +182,7 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
   r.logits = floats(l.logits);
   r.mass = floats(l.mass);
   r.lse = floats(l.lse);
-  r.loss = a.loss;
+  r.loss = a.loss ? a.loss : floats(l.loss);
   r.row_weight = floats(l.row_weight);
   r.alpha = floats(l.alpha);
   r.mean = a.reduced;
@@ -218,6 +219,7 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
     g.elt = elt;
     g.mode = !grads ? HG_STATS : elt == ELT_F16 ? HG_LOGITS : HG_EXP;
     g.splits = 1;
+    g.few = a.tokens <= kFewRows;         // of the call: its chunks do not change the bits
     g.A = Hc; g.lda = ldh;
     g.B = W; g.ldb = ldw;
     g.M = rows; g.N = (int)a.vocab; g.K = (int)a.dim;
@@ -227,6 +229,8 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
     if (check_launch(launch_head_gemm(g, stream), who)) return 1;
     if (check_launch(launch_head_rows(r, (int)first, rows, stats, Z, grads ? G : nullptr, l.ld, elt,
                                       stream), who)) return 1;
+    // before the gradients' products: they take its alpha. The last chunk's is the whole loss.
+    if (a.reduction != DMUON_LOSS_ROWS && check_launch(launch_head_reduce(r, stream), who)) return 1;
     if (grads) {
       g = HeadGemm{};
       g.elt = elt;
@@ -237,7 +241,7 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
         g.A = G; g.lda = l.ld;
         g.B = W; g.ldb = ldw; g.b_kmajor = 1;
         g.M = rows; g.N = (int)a.dim; g.K = (int)a.vocab;
-        g.splits = split_h ? head_gemm_splits(rows, g.N, g.K) : 1;
+        g.splits = split_h ? head_gemm_splits(rows, g.N, g.K, false) : 1;
         g.part = floats(l.part); g.ldp = a.dim;
         g.out = static_cast<char*>(a.d_hidden) + first * a.dim * grad_size; g.ldo = a.dim;
         if (check_launch(launch_head_gemm(g, stream), who)) return 1;
@@ -247,7 +251,7 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
         g.A = G; g.lda = l.ld; g.a_kmajor = 1;
         g.B = Hc; g.ldb = ldh; g.b_kmajor = 1;
         g.M = (int)a.vocab; g.N = (int)a.dim; g.K = rows;
-        g.splits = gathers ? 1 : head_gemm_splits(g.M, g.N, g.K);
+        g.splits = gathers ? 1 : head_gemm_splits(g.M, g.N, g.K, true);
         g.out = last ? a.d_weight : nullptr; g.ldo = a.dim;
         // fp32 results gather in place
         g.part = gathers && grad_size == 4 ? static_cast<float*>(a.d_weight) : floats(l.part);
@@ -258,22 +262,23 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
     }
     if (l.chunk <= 0) break;
   }
-  if (a.reduction != DMUON_LOSS_ROWS && check_launch(launch_head_reduce(r, stream), who)) return 1;
   return 0;
 }
 
-int dmuon_scale_by(const void* src, int src_dtype, void* dst, int dst_dtype, int64_t n,
-                   const float* factor, void* stream) {
+int dmuon_scale_by(const void* src, void* dst, int64_t n, const void* src2, void* dst2, int64_t n2,
+                   int src_dtype, int dst_dtype, const float* factor, void* stream) {
   const char* who = "dmuon_scale_by";
   for (int t : {src_dtype, dst_dtype})
     if (t != DMUON_DTYPE_F32 && t != DMUON_DTYPE_BF16 && t != DMUON_DTYPE_F16)
       return fail("%s: unknown dtype code %d", who, t);
-  if (n < 0) return fail("%s: negative size", who);
-  if (n == 0) return 0;
-  if (!src || !dst || !factor) return fail("%s: NULL argument", who);
-  if (src == dst && src_dtype != dst_dtype) return fail("%s: in place needs one dtype", who);
-  return check_launch(launch_scale_by(src, src_dtype, dst, dst_dtype, n, factor,
-                                      static_cast<hipStream_t>(stream)), who);
+  if (n < 0 || n2 < 0) return fail("%s: negative size", who);
+  if (n == 0 && n2 == 0) return 0;
+  if ((n > 0 && (!src || !dst)) || (n2 > 0 && (!src2 || !dst2)) || !factor)
+    return fail("%s: NULL argument", who);
+  const bool in1 = n > 0 && src == dst, in2 = n2 > 0 && src2 == dst2;
+  if (src_dtype != dst_dtype && (in1 || in2)) return fail("%s: in place needs one dtype", who);
+  ScaleBy a{{src, src2}, {dst, dst2}, {n, n2}, factor, (in1 || n == 0) && (in2 || n2 == 0)};
+  return check_launch(launch_scale_by(a, src_dtype, dst_dtype, static_cast<hipStream_t>(stream)), who);
 }
 
 }  // extern "C"

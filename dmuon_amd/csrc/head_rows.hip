@@ -116,31 +116,25 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uin
   }
 }
 
-// Row weights and alpha: the gradient of row n is alpha * row_weight[n] * (...). The weights are
-// relative to the largest, so that a 16-bit logit gradient neither over- nor underflows with the
-// size of the batch or a loss scale. One block.
+// What a row's stored logit gradient is multiplied with: 2^kGradShift, 0 for a row that is not
+// counted; with gradients of the rows' losses, times the row's share of the largest.
+constexpr float kUnit = (float)(1 << kGradShift);
+__device__ __forceinline__ float row_weight(const HeadRows& r, long long n) {
+  return r.mass[n] < 0.f ? 0.f : r.row_grad ? r.row_weight[n] : kUnit;
+}
+
+// Row weights and alpha from the rows' gradients: the gradient of row n is alpha * row_weight[n] *
+// (...). The weights are relative to the largest, so that a 16-bit logit gradient neither over- nor
+// underflows with the size of the batch or a loss scale. One block.
 __global__ __launch_bounds__(1024) void head_weights_kernel(HeadRows r) {
   __shared__ float lds[16];
-  const float unit = (float)(1 << kGradShift);
-  float count = 0.f, top = 0.f;
+  float top = 0.f;
   for (int n = threadIdx.x; n < r.n; n += 1024)
-    if (!(r.mass[n] < 0.f)) {
-      count += 1.f;                       // exact: at most 2^24 rows
-      if (r.row_grad) top = fmaxf(top, fabsf(r.row_grad[n]));
-    }
-  count = block_join<false>(count, lds);
+    if (!(r.mass[n] < 0.f)) top = fmaxf(top, fabsf(r.row_grad[n]));
   top = block_join<true>(top, lds);
-  const float t = r.temperature;
-  for (int n = threadIdx.x; n < r.n; n += 1024) {
-    const bool counted = !(r.mass[n] < 0.f);
-    float w = unit;
-    if (r.row_grad) w = r.row_grad[n] == 0.f ? 0.f : unit * (r.row_grad[n] / top);
-    r.row_weight[n] = counted ? w : 0.f;
-  }
-  if (threadIdx.x == 0) {
-    const float g = r.row_grad ? top : r.reduction == DMUON_LOSS_MEAN ? 1.f / fmaxf(count, 1.f) : 1.f;
-    r.alpha[0] = g * t / unit;
-  }
+  for (int n = threadIdx.x; n < r.n; n += 1024)
+    r.row_weight[n] = r.row_grad[n] == 0.f ? 0.f : kUnit * (r.row_grad[n] / top);
+  if (threadIdx.x == 0) r.alpha[0] = top * r.temperature / kUnit;
 }
 
 // (maximum, sum of exponentials) of two sets of logits as one
@@ -208,7 +202,7 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows r, int first,
     }
   }
   if constexpr (FROM != FROM_NONE) {
-    const float w = r.row_weight[n];
+    const float w = row_weight(r, n);
     const float f = w == 0.f ? 0.f : w * (mass + 2.f * r.z_loss * lse);
     const int chunks = (int)(ldg / 8), per = (chunks + parts - 1) / parts;
     const int c0 = part * per, c1 = min(chunks, c0 + per);
@@ -255,31 +249,82 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows r, int first,
   }
 }
 
+// The reduced loss, and alpha of its gradient.
 __global__ __launch_bounds__(1024) void head_reduce_kernel(HeadRows r) {
   __shared__ float lds[16];
-  float sum = 0.f, count = 0.f;
+  float sum = 0.f, count = 0.f;           // the count is exact: at most 2^24 rows
   for (int n = threadIdx.x; n < r.n; n += 1024) {
     sum += r.loss[n];
     count += r.mass[n] < 0.f ? 0.f : 1.f;
   }
   sum = block_join<false>(sum, lds);
   count = block_join<false>(count, lds);
-  if (threadIdx.x == 0)
+  if (threadIdx.x == 0) {
+    const float g = r.reduction == DMUON_LOSS_MEAN ? 1.f / fmaxf(count, 1.f) : 1.f;
     r.mean[0] = r.reduction == DMUON_LOSS_MEAN ? sum / fmaxf(count, 1.f) : sum;
+    r.alpha[0] = g * r.temperature / kUnit;
+  }
 }
 
+// dst = factor * src for two dense arrays, 8 values a thread and step.
 template <int S, int D>
-__global__ __launch_bounds__(256) void scale_by_kernel(const void* src, void* dst, long long n,
-                                                       const float* factor) {
-  const float f = factor[0];
-  if (S == D && src == dst && f == 1.f) return;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += 256LL * gridDim.x) {
-    float v;
-    if constexpr (S == DT_F32) v = static_cast<const float*>(src)[i];
-    else v = from_elt<S == DT_F16 ? ELT_F16 : ELT_BF16>(static_cast<const uint16_t*>(src)[i]);
-    v *= f;
-    if constexpr (D == DT_F32) static_cast<float*>(dst)[i] = v;
-    else static_cast<uint16_t*>(dst)[i] = to_elt<D == DT_F16 ? ELT_F16 : ELT_BF16>(v);
+__global__ __launch_bounds__(256) void scale_by_kernel(ScaleBy a) {
+  typedef f32x4_t f32x4_any_t __attribute__((aligned(4)));
+  const float f = a.factor[0];
+  if (S == D && f == 1.f && a.in_place) return;
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    const long long n = a.n[k];
+    for (long long i = (blockIdx.x * 256LL + threadIdx.x) * 8; i < n; i += 256LL * 8 * gridDim.x) {
+      float v[8];
+      const bool whole = i + 8 <= n;
+      if constexpr (S == DT_F32) {
+        const float* p = static_cast<const float*>(a.src[k]) + i;
+        if (whole) {
+          const f32x4_t x = *reinterpret_cast<const f32x4_any_t*>(p);
+          const f32x4_t y = *reinterpret_cast<const f32x4_any_t*>(p + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = x[e], v[e + 4] = y[e];
+        } else {
+          for (int e = 0; e < 8; ++e) v[e] = i + e < n ? p[e] : 0.f;
+        }
+      } else {
+        constexpr int E = S == DT_F16 ? ELT_F16 : ELT_BF16;
+        const uint16_t* p = static_cast<const uint16_t*>(a.src[k]) + i;
+        if (whole) {
+          const u32x4_t x = *reinterpret_cast<const u32x4_any_t*>(p);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[2 * e] = from_elt<E>(x[e] & 0xffff);
+            v[2 * e + 1] = from_elt<E>(x[e] >> 16);
+          }
+        } else {
+          for (int e = 0; e < 8; ++e) v[e] = i + e < n ? from_elt<E>(p[e]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= f;
+      if constexpr (D == DT_F32) {
+        float* p = static_cast<float*>(a.dst[k]) + i;
+        if (whole) {
+          *reinterpret_cast<f32x4_any_t*>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
+          *reinterpret_cast<f32x4_any_t*>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+        } else {
+          for (int e = 0; e < 8; ++e)
+            if (i + e < n) p[e] = v[e];
+        }
+      } else {
+        constexpr int E = D == DT_F16 ? ELT_F16 : ELT_BF16;
+        uint16_t* p = static_cast<uint16_t*>(a.dst[k]) + i;
+        if (whole) {
+          *reinterpret_cast<u32x4_any_t*>(p) = u32x4_t{pack2_elt<E>(v[0], v[1]), pack2_elt<E>(v[2], v[3]),
+                                                       pack2_elt<E>(v[4], v[5]), pack2_elt<E>(v[6], v[7])};
+        } else {
+          for (int e = 0; e < 8; ++e)
+            if (i + e < n) p[e] = to_elt<E>(v[e]);
+        }
+      }
+    }
   }
 }
 
@@ -295,7 +340,8 @@ hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long l
     else
       hipLaunchKernelGGL(head_targets_kernel<ELT_BF16>, grid, dim3(256), 0, stream, r, H, ldh, W, ldw, dim);
   }
-  if (grads) hipLaunchKernelGGL(head_weights_kernel, dim3(1), dim3(1024), 0, stream, r);
+  if (grads && r.row_grad)
+    hipLaunchKernelGGL(head_weights_kernel, dim3(1), dim3(1024), 0, stream, r);
   return hipGetLastError();
 }
 
@@ -325,24 +371,19 @@ hipError_t launch_head_reduce(const HeadRows& r, hipStream_t stream) {
 }
 
 template <int S>
-static void scale_from(const void* src, void* dst, int dst_dtype, long long n, const float* factor,
-                       dim3 grid, hipStream_t stream) {
-  if (dst_dtype == DT_F32)
-    hipLaunchKernelGGL((scale_by_kernel<S, DT_F32>), grid, dim3(256), 0, stream, src, dst, n, factor);
-  else if (dst_dtype == DT_F16)
-    hipLaunchKernelGGL((scale_by_kernel<S, DT_F16>), grid, dim3(256), 0, stream, src, dst, n, factor);
-  else
-    hipLaunchKernelGGL((scale_by_kernel<S, DT_BF16>), grid, dim3(256), 0, stream, src, dst, n, factor);
+static void scale_from(const ScaleBy& a, int dst_dtype, dim3 grid, hipStream_t stream) {
+  if (dst_dtype == DT_F32) hipLaunchKernelGGL((scale_by_kernel<S, DT_F32>), grid, dim3(256), 0, stream, a);
+  else if (dst_dtype == DT_F16) hipLaunchKernelGGL((scale_by_kernel<S, DT_F16>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((scale_by_kernel<S, DT_BF16>), grid, dim3(256), 0, stream, a);
 }
 
-hipError_t launch_scale_by(const void* src, int src_dtype, void* dst, int dst_dtype, long long n,
-                           const float* factor, hipStream_t stream) {
-  if (n <= 0) return hipSuccess;
-  const long long want = (n + 2047) / 2048;
-  const dim3 grid((unsigned)(want < 8192 ? want : 8192));
-  if (src_dtype == DT_F32) scale_from<DT_F32>(src, dst, dst_dtype, n, factor, grid, stream);
-  else if (src_dtype == DT_F16) scale_from<DT_F16>(src, dst, dst_dtype, n, factor, grid, stream);
-  else scale_from<DT_BF16>(src, dst, dst_dtype, n, factor, grid, stream);
+hipError_t launch_scale_by(const ScaleBy& a, int src_dtype, int dst_dtype, hipStream_t stream) {
+  const long long n = a.n[0] > a.n[1] ? a.n[0] : a.n[1], want = (n + 2047) / 2048;
+  if (want <= 0) return hipSuccess;
+  const dim3 grid((unsigned)(want < 2048 ? want : 2048));
+  if (src_dtype == DT_F32) scale_from<DT_F32>(a, dst_dtype, grid, stream);
+  else if (src_dtype == DT_F16) scale_from<DT_F16>(a, dst_dtype, grid, stream);
+  else scale_from<DT_BF16>(a, dst_dtype, grid, stream);
   return hipGetLastError();
 }
 

@@ -34,50 +34,60 @@ def _pitch(t: Tensor) -> int:
     return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
 
 
+def _dense_float(t: Tensor) -> Tensor:
+    if t.dtype is torch.float32 and t.is_contiguous() and not t.requires_grad:
+        return t                           # each no-op of torch costs a microsecond of the host
+    return t.detach().to(torch.float32).contiguous()
+
+
 class _Targets:
     """What a call is measured against, and the launches on it."""
 
-    def __init__(self, who: str, **tensors: Optional[Tensor]) -> None:
-        self.who, self.tensors = who, tensors
-        self.ignore_index, self.z_loss, self.temperature, self.k_list = -100, 0.0, 1.0, 1
-        self.chunk = 0
+    def __init__(self, targets: Optional[Tensor] = None, ids: Optional[Tensor] = None,
+                 logits: Optional[Tensor] = None, lse: Optional[Tensor] = None, *,
+                 ignore_index: int = -100, z_loss: float = 0.0, temperature: float = 1.0,
+                 k_list: int = 1, chunk: int = 0) -> None:
+        self.tensors = targets, ids, logits, lse
+        self.pointers = tuple(None if t is None else t.data_ptr() for t in self.tensors)
+        self.k_list, self.chunk, self.ignore_index = k_list, chunk, ignore_index
+        self.z_loss, self.temperature = z_loss, temperature
 
-    def launch(self, hidden: Tensor, weight: Tensor, reduction: int, want, *,
-               row_grad: Optional[Tensor] = None, grad_dtype: Optional[torch.dtype] = None):
-        """(loss of each token, reduced loss, d_hidden, d_weight); ``want`` says which gradients."""
-        dev, dt = hidden.device, hidden.dtype
+    def launch(self, hidden: Tensor, weight: Tensor, reduction: int, want, grad_dtype: torch.dtype,
+               row_grad: Optional[Tensor] = None):
+        """(the loss, of each token or reduced, d_hidden, d_weight); ``want`` says which gradients."""
+        dev = hidden.device
         n, dim = hidden.shape
         vocab = weight.shape[0]
-        grad_dtype = grad_dtype or dt
-        loss = torch.empty(n, dtype=torch.float32, device=dev)
-        reduced = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
-        dh = torch.empty(n, dim, dtype=grad_dtype, device=dev) if want[0] else None
-        dw = torch.empty(vocab, dim, dtype=grad_dtype, device=dev) if want[1] else None
+        loss = torch.empty(() if reduction else n, dtype=torch.float32, device=dev)
+        dh = torch.empty((n, dim), dtype=grad_dtype, device=dev) if want[0] else None
+        dw = torch.empty((vocab, dim), dtype=grad_dtype, device=dev) if want[1] else None
         a = _C.HeadLossArgs(
-            dtype=_CODES[dt], grad_dtype=_CODES.get(grad_dtype, _C.DTYPE_F32), reduction=reduction,
-            tokens=n, vocab=vocab, dim=dim, k_list=self.k_list, chunk_tokens=self.chunk,
-            ld_hidden=_pitch(hidden), ld_weight=_pitch(weight), ignore_index=self.ignore_index,
-            z_loss=self.z_loss, temperature=self.temperature)
-        for name, t in (("hidden", hidden), ("weight", weight), ("row_grad", row_grad),
-                        ("loss", loss), ("reduced", reduced), ("d_hidden", dh), ("d_weight", dw),
-                        *self.tensors.items()):
-            if t is not None:
-                setattr(a, name, t.data_ptr())
+            hidden.data_ptr(), weight.data_ptr(), *self.pointers,
+            None if row_grad is None else row_grad.data_ptr(),
+            None if reduction else loss.data_ptr(), loss.data_ptr() if reduction else None,
+            None if dh is None else dh.data_ptr(), None if dw is None else dw.data_ptr(),
+            _pitch(hidden), _pitch(weight), n, vocab, dim, self.k_list, self.chunk,
+            self.ignore_index, self.z_loss, self.temperature, _CODES[hidden.dtype],
+            _CODES.get(grad_dtype, _C.DTYPE_F32), reduction)
         need = _C.c_i64()
         _C.call("dmuon_head_loss_workspace_size", ctypes.byref(a), ctypes.byref(need))
         # from the caching allocator: reused in this stream's order, nothing is kept
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
         _C.call_on(dev, "dmuon_head_loss", ctypes.byref(a), ws.data_ptr(), need.value)
-        return loss, reduced, dh, dw
+        return loss, dh, dw
 
 
-def _scaled(g: Optional[Tensor], dtype: torch.dtype, factor: Tensor) -> Optional[Tensor]:
-    """``g * factor`` in ``dtype``, in place where ``g`` has it."""
-    if g is None:
-        return None
-    out = g if g.dtype == dtype else torch.empty_like(g, dtype=dtype)
-    _C.call_on(g.device, "dmuon_scale_by", g.data_ptr(), _CODES.get(g.dtype, _C.DTYPE_F32),
-               out.data_ptr(), _CODES.get(dtype, _C.DTYPE_F32), g.numel(), factor.data_ptr())
+def _scaled(grads, dtype: torch.dtype, factor: Tensor):
+    """The gradients (two, each may be None) times ``factor`` in ``dtype``, in place where they have
+    it."""
+    factor = _dense_float(factor)
+    out = [g if g is None or g.dtype == dtype else torch.empty_like(g, dtype=dtype) for g in grads]
+    args = []
+    for g, o in zip(grads, out):
+        args += (None, None, 0) if g is None else (g.data_ptr(), o.data_ptr(), g.numel())
+    held = next(g.dtype for g in grads if g is not None)
+    _C.call_on(factor.device, "dmuon_scale_by", *args, _CODES.get(held, _C.DTYPE_F32),
+               _CODES[dtype], factor.data_ptr())
     return out
 
 
@@ -85,31 +95,28 @@ class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, reduction, grads):
         want = ctx.needs_input_grad[:2]
-        ctx.targets, ctx.reduction = targets, reduction
         # fp16: the mean's gradients may only fit the type once a loss scale has multiplied them
-        ctx.held_dtype = torch.float32 if hidden.dtype == torch.float16 else hidden.dtype
-        now = grads and reduction and any(want)
-        loss, reduced, dh, dw = targets.launch(hidden, weight, reduction, want if now else (0, 0),
-                                               grad_dtype=ctx.held_dtype)
-        ctx.grads = (dh, dw) if now else None
-        ctx.save_for_backward(hidden, weight)
-        return reduced if reduction else loss
+        held = torch.float32 if hidden.dtype == torch.float16 and reduction else hidden.dtype
+        now = grads and reduction and (want[0] or want[1])
+        loss, dh, dw = targets.launch(hidden, weight, reduction, want if now else (False, False),
+                                      held)
+        if grads:
+            ctx.call, ctx.dtype = (targets, reduction, want, held), hidden.dtype
+            ctx.grads = (dh, dw) if now else None
+            ctx.save_for_backward(hidden, weight)
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        hidden, weight = ctx.saved_tensors
-        want = ctx.needs_input_grad[:2]
-        if not ctx.reduction:
-            _, _, dh, dw = ctx.targets.launch(hidden, weight, ctx.reduction, want,
-                                              row_grad=grad.float().contiguous())
-            return dh, dw, None, None, None
         grads, ctx.grads = ctx.grads, None
-        if grads is None:                  # a second pass over a retained graph
-            grads = ctx.targets.launch(hidden, weight, ctx.reduction, want,
-                                       grad_dtype=ctx.held_dtype)[2:]
-        factor = grad.float().contiguous()
-        return (*(_scaled(g, hidden.dtype, factor) for g in grads), None, None, None)
+        if grads is None:                  # unreduced losses, or a second pass over a kept graph
+            targets, reduction, want, held = ctx.call
+            row_grad = None if reduction else _dense_float(grad)
+            _, *grads = targets.launch(*ctx.saved_tensors, reduction, want, held, row_grad)
+            if not reduction:
+                return (*grads, None, None, None)
+        return (*_scaled(grads, ctx.dtype, grad), None, None, None)
 
 
 def _check(who: str, hidden: Tensor, weight: Tensor, reduction: str, chunk_tokens) -> None:
@@ -132,11 +139,20 @@ def _check(who: str, hidden: Tensor, weight: Tensor, reduction: str, chunk_token
 def _index(who: str, name: str, t: Tensor, shape, device) -> Tensor:
     if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
         raise ValueError(f"{who}: {name} must be integers, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{who}: {name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != device:
         raise RuntimeError(f"{who}: {name} must live on {device}")
-    return t.to(torch.int64).contiguous()
+    return t if t.dtype is torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
+
+
+def _floats(who: str, name: str, t: Tensor, shape, device) -> Tensor:
+    if not t.dtype.is_floating_point or t.shape != shape:
+        raise ValueError(f"{who}: {name} must be floating-point of the shape {tuple(shape)}, got "
+                         f"{t.dtype} {tuple(t.shape)}")
+    if t.device != device:
+        raise RuntimeError(f"{who}: {name} must live on {device}")
+    return _dense_float(t)
 
 
 def _run(targets: _Targets, hidden: Tensor, weight: Tensor, reduction: str) -> Tensor:
@@ -166,9 +182,9 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, target: Tensor, *,
     """
     who = "linear_cross_entropy"
     _check(who, hidden, weight, reduction, chunk_tokens)
-    t = _Targets(who, targets=_index(who, "target", target, hidden.shape[:-1], hidden.device))
-    t.ignore_index, t.z_loss, t.chunk = int(ignore_index), float(z_loss), int(chunk_tokens or 0)
-    return _run(t, hidden, weight, reduction)
+    t = _index(who, "target", target, hidden.shape[:-1], hidden.device)
+    return _run(_Targets(t, ignore_index=int(ignore_index), z_loss=float(z_loss),
+                         chunk=int(chunk_tokens or 0)), hidden, weight, reduction)
 
 
 def linear_distillation(hidden: Tensor, weight: Tensor, teacher_ids: Tensor,
@@ -197,17 +213,8 @@ def linear_distillation(hidden: Tensor, weight: Tensor, teacher_ids: Tensor,
                          f"{tuple(teacher_ids.shape)}")
     k = teacher_ids.shape[-1]
     ids = _index(who, "teacher_ids", teacher_ids, (*hidden.shape[:-1], k), hidden.device)
-    given = {"teacher_logits": (teacher_logits, ids.shape)}
-    if teacher_lse is not None:
-        given["teacher_lse"] = (teacher_lse, hidden.shape[:-1])
-    floats = {}
-    for name, (x, shape) in given.items():
-        if not x.dtype.is_floating_point or x.shape != shape:
-            raise ValueError(f"{who}: {name} must be floating-point of the shape {tuple(shape)}, "
-                             f"got {x.dtype} {tuple(x.shape)}")
-        if x.device != hidden.device:
-            raise RuntimeError(f"{who}: {name} must live on {hidden.device}")
-        floats[name] = x.detach().float().contiguous()
-    t = _Targets(who, teacher_ids=ids, **floats)
-    t.temperature, t.k_list, t.chunk = float(temperature), k, int(chunk_tokens or 0)
-    return _run(t, hidden, weight, reduction)
+    logits = _floats(who, "teacher_logits", teacher_logits, ids.shape, hidden.device)
+    lse = None if teacher_lse is None else \
+        _floats(who, "teacher_lse", teacher_lse, hidden.shape[:-1], hidden.device)
+    return _run(_Targets(None, ids, logits, lse, temperature=float(temperature), k_list=k,
+                         chunk=int(chunk_tokens or 0)), hidden, weight, reduction)

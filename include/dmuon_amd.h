@@ -467,8 +467,8 @@ int dmuon_clip_norms(const int64_t* ptrs, const int64_t* numels, const int32_t* 
  *     over many tokens underflows fp16). Both NULL: values only.
  * hidden and weight are 16-bit words of `dtype` (DMUON_DTYPE_BF16 or _F16), row by row with their
  * pitches in elements, at any element alignment; products accumulate in fp32, and the logit
- * gradient is rounded once to `dtype` between the products. loss [tokens] is always written. Results
- * do not depend on anything but the arguments (no atomics). chunk_tokens: tokens worked on at a
+ * gradient is rounded once to `dtype` between the products. loss [tokens] may be NULL with a
+ * reduction. Results do not depend on anything but the arguments (no atomics). chunk_tokens: tokens worked on at a
  * time (0: a size that keeps the workspace near 4 GiB); a workspace of
  * dmuon_head_loss_workspace_size bytes (256-byte aligned) is the caller's.
  */
@@ -496,11 +496,11 @@ int dmuon_head_loss_workspace_size(const dmuon_head_loss_args* args, int64_t* wo
 int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t workspace_bytes,
                     void* stream);
 
-/* dst = factor[0] * src (factor fp32, on the device) for n dense values, src of src_dtype and dst
- * of dst_dtype, both fp32, bf16 or fp16; dst may be src itself, and then nothing is read or written
- * where the factor is 1. */
-int dmuon_scale_by(const void* src, int src_dtype, void* dst, int dst_dtype, int64_t n,
-                   const float* factor, void* stream);
+/* dst = factor[0] * src (factor fp32, on the device) for one or two dense arrays of n and n2 values
+ * (0: none), src of src_dtype and dst of dst_dtype, each fp32, bf16 or fp16. A dst may be its src;
+ * where all are, nothing is read or written for a factor of 1. */
+int dmuon_scale_by(const void* src, void* dst, int64_t n, const void* src2, void* dst2, int64_t n2,
+                   int src_dtype, int dst_dtype, const float* factor, void* stream);
 
 /*
  * The norms around a block with its gate and residual scale (no reference counterpart):

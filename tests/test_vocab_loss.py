@@ -482,6 +482,9 @@ def test_c_entry_refusals_without_gpu():
     says(run(reduced=None), "reduced")
     says(run(reduction=0), "row_grad")
     says(lib.dmuon_head_loss_workspace_size(None, ctypes.byref(need)), "NULL")
-    says(lib.dmuon_scale_by(4096, 7, 4096, 1, 4, 4096, None), "dtype")
-    says(lib.dmuon_scale_by(4096, 1, 4096, 2, 4, 4096, None), "in place")
-    says(lib.dmuon_scale_by(None, 1, None, 1, 4, 4096, None), "NULL")
+    says(run(reduction=0, d_hidden=None, d_weight=None, loss=None), "loss")
+    says(lib.dmuon_scale_by(4096, 4096, 4, None, None, 0, 7, 1, 4096, None), "dtype")
+    says(lib.dmuon_scale_by(4096, 4096, 4, None, None, 0, 1, 2, 4096, None), "in place")
+    says(lib.dmuon_scale_by(None, None, 4, None, None, 0, 1, 1, 4096, None), "NULL")
+    says(lib.dmuon_scale_by(4096, 4096, 4, None, 4096, 2, 1, 1, 4096, None), "NULL")
+    assert lib.dmuon_scale_by(None, None, 0, None, None, 0, 1, 1, None, None) == 0
