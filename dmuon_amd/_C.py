@@ -204,24 +204,30 @@ def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args))
 
 
-def current_stream(device) -> int:
-    """Handle of the device's current stream."""
-    import torch
-
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # without a Stream object: 2 us less
-    return raw(device.index) if raw else torch.cuda.current_stream(device).cuda_stream
+_torch_ops = None
 
 
-def call_on(device, name: str, *args) -> None:
-    """``call`` with the device's current stream as last argument and the device current. (Entering
-    ``torch.cuda.device`` costs more than a small kernel's launch: only where it changes something.)"""
-    import torch
+def torch_ops():
+    """The module of native autograd operators (``csrc/torch_binding.cpp``), loaded once; raises if
+    it is missing or was built against another ABI version of the library."""
+    global _torch_ops
+    if _torch_ops is None:
+        import importlib
 
-    if torch.cuda.current_device() == device.index:
-        call(name, *args, current_stream(device))
-    else:
-        with torch.cuda.device(device):
-            call(name, *args, current_stream(device))
+        import torch  # noqa: F401  (its libraries come first)
+
+        lib()
+        try:
+            ops = importlib.import_module("dmuon_amd.csrc._dmuon_torch")
+        except ImportError as e:
+            raise RuntimeError(f"dmuon_amd.csrc._dmuon_torch does not load ({e}): build it first "
+                               "(python -m dmuon_amd.csrc.build)") from e
+        if ops.abi_version != ABI_VERSION:
+            raise RuntimeError(f"dmuon_amd.csrc._dmuon_torch was built for ABI version "
+                               f"{ops.abi_version}, this binding expects {ABI_VERSION}: rebuild it "
+                               "(python -m dmuon_amd.csrc.build)")
+        _torch_ops = ops
+    return _torch_ops
 
 
 PROFILE_CLASSES = ("pre", "norm", "syrk", "poly", "gemm", "final", "adamw", "clip")

@@ -1,4 +1,5 @@
-"""Builds libdmuon_amd.so (gfx950) in-tree with hipcc.
+"""Builds libdmuon_amd.so (gfx950) in-tree with hipcc, and the extension module of the autograd
+operators on it (_dmuon_torch.so, host code only).
 
     python -m dmuon_amd.csrc.build          # or: python dmuon_amd/csrc/build.py
 
@@ -10,6 +11,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -37,6 +40,10 @@ FLAGS = [
 ]
 
 
+BINDING = "torch_binding.cpp"
+BINDING_NAME = "_dmuon_torch.so"
+
+
 def hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
         if cand and os.path.exists(cand):
@@ -48,22 +55,68 @@ def lib_path() -> Path:
     return HERE / LIB_NAME
 
 
-def build(verbose: bool = False) -> Path:
-    out = lib_path()
-    tmp = out.with_suffix(".so.tmp")
-    cmd = [hipcc(), *FLAGS, "-I", str(ROOT / "include"), *[str(HERE / s) for s in SOURCES], "-o", str(tmp)]
+def _run(cmd, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
     err = "\n".join(l for l in (proc.stderr or "").splitlines() if noise not in l)
     if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{err}")
+        raise RuntimeError(f"{cmd[0]} failed ({proc.returncode}):\n{err}")
     if err.strip() and verbose:
         print(err, file=sys.stderr)
-    _check_launch_stubs(tmp)
-    os.replace(tmp, out)
+
+
+def build(verbose: bool = False) -> Path:
+    out = lib_path()
+    tmp = out.with_suffix(".so.tmp")
+    compile_flags = [f for f in FLAGS if f != "-shared"]
+    with tempfile.TemporaryDirectory() as d:
+        objects = [str(Path(d) / (s + ".o")) for s in [*SOURCES, BINDING]]
+        jobs = [[hipcc(), *compile_flags, "-I", str(ROOT / "include"), "-c", str(HERE / s), "-o", o]
+                for s, o in zip(SOURCES, objects)]
+        jobs.append(_binding_compile(objects[-1]))
+        # the files are independent code objects: one compiler each
+        with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 1, 8)) as pool:
+            list(pool.map(lambda cmd: _run(cmd, verbose), jobs))
+        _run([hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objects[:-1], "-o", str(tmp)],
+             verbose)
+        _check_launch_stubs(tmp)
+        os.replace(tmp, out)
+        binding = HERE / BINDING_NAME
+        tmp = binding.with_suffix(".so.tmp")
+        _run(_binding_link(objects[-1], str(tmp)), verbose)
+        os.replace(tmp, binding)
     return out
+
+
+def _cxx() -> str:
+    return shutil.which("g++") or hipcc()
+
+
+def _binding_compile(obj: str) -> list:
+    """The extension module is compiled against this interpreter's torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    return [_cxx(), "-O2", "-std=c++17", "-fPIC", "-Wall",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            *[x for d in cpp_extension.include_paths() for x in ("-isystem", d)],
+            "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"],
+            "-c", str(HERE / BINDING), "-o", obj]
+
+
+def _binding_link(obj: str, out: str) -> list:
+    """It finds the library beside itself."""
+    from torch.utils import cpp_extension
+
+    return [_cxx(), "-shared", obj, "-o", out,
+            *[f"-L{d}" for d in cpp_extension.library_paths()],
+            "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip",
+            f"-L{HERE}", f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN"]
 
 
 def _check_launch_stubs(so: Path) -> None:

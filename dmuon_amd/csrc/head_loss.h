@@ -74,7 +74,7 @@ struct HeadRows {
   float* mean;                            // [1] or NULL: the reduced loss
 };
 // ids, probs, mass and logits of every row (H, W: the products' operands, any alignment); with
-// `grads` and row_grad the row weights and alpha.
+// `grads` of unreduced losses the row weights and alpha.
 hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long ldh,
                                const uint16_t* W, long long ldw, int dim, int elt, bool grads,
                                hipStream_t stream);

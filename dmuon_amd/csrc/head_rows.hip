@@ -340,7 +340,7 @@ hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long l
     else
       hipLaunchKernelGGL(head_targets_kernel<ELT_BF16>, grid, dim3(256), 0, stream, r, H, ldh, W, ldw, dim);
   }
-  if (grads && r.row_grad)
+  if (grads && r.reduction == DMUON_LOSS_ROWS)
     hipLaunchKernelGGL(head_weights_kernel, dim3(1), dim3(1024), 0, stream, r);
   return hipGetLastError();
 }

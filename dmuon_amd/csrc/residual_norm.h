@@ -11,7 +11,7 @@ struct ResidualNorm {
   long long ld_x, ld_y;
   const void* w_pre; const void* w_post; const void* gate;   // [dim], [dim] or NULL, [groups][dim] or NULL
   int dtype, pre_dtype, post_dtype, gate_dtype;
-  long long rows, rows_per_group;
+  long long rows, rows_per_group, gates;
   int dim;
   float scale, eps;
   float2* stats;                          // [rows]: (r, s); forward: may be NULL
@@ -21,7 +21,8 @@ struct ResidualNorm {
   void* dx; void* dy; void* d_pre; void* d_post; void* d_gate;   // each may be NULL
   float* pre_part; float* post_part; float* gate_part;           // [blocks][dim]
   long long rows_per_block, blocks;
-  int parts;                              // blocks of one gate group; 1: a block takes whole groups
+  int parts;                              // blocks of one gate group; 1: a block takes whole groups;
+                                          // 0: no rows
   int lanes;                              // backward: rows side by side in a block
 };
 hipError_t launch_residual_norm(ResidualNorm a, hipStream_t stream);

@@ -446,7 +446,7 @@ void residual_norm_split(ResidualNorm* a) {
   auto want = [&](int lanes) { return lanes > 1 ? kCus * 3 : kCus * 1024 / threads; };
   a->lanes = threads < 256 ? 256 / threads : 1;
   if (a->rows <= 0) {
-    a->parts = 1;
+    a->parts = 0;                         // the gate's gradient is a sum of none
     a->blocks = 0;
     a->rows_per_block = 1;
   } else if (groups > want(a->lanes) / 2 && groups > 1) {
@@ -513,10 +513,10 @@ hipError_t launch_residual_norm_grad(const ResidualNorm& a, hipStream_t stream) 
 #undef DMUON_RN_T
 #undef DMUON_RN
   }
-  const bool gates = a.d_gate && a.parts > 1;
+  const bool gates = a.d_gate && a.parts != 1;
   if (a.d_pre || a.d_post || gates) {
     const dim3 grid((unsigned)((a.dim + 31) / 32),
-                    (unsigned)(gates ? 2 + a.rows / a.rows_per_group : a.d_post ? 2 : 1));
+                    (unsigned)(gates ? 2 + a.gates : a.d_post ? 2 : 1));
     hipLaunchKernelGGL(sum_partials_kernel, grid, dim3(1024), 0, stream, a);
   }
   return hipGetLastError();
@@ -558,6 +558,7 @@ ResidualNorm describe(const dmuon_residual_norm_args& a) {
   r.w_pre = a.w_pre; r.w_post = a.w_post; r.gate = a.gate;
   r.pre_dtype = a.pre_dtype; r.post_dtype = a.post_dtype; r.gate_dtype = a.gate_dtype;
   r.rows = a.rows; r.dim = (int)a.dim;
+  r.gates = a.gate ? a.gates : 0;
   r.rows_per_group = a.gate && a.rows > 0 ? a.rows / a.gates : 1;
   r.scale = a.scale; r.eps = a.eps;
   r.stats = reinterpret_cast<float2*>(a.stats);

@@ -194,6 +194,9 @@ def test_zero_rows_large_values_and_no_numbers(gpu):
 @pytest.mark.gpu
 def test_no_rows(gpu):
     v, outs = _inputs(gpu, (0, 96), torch.bfloat16, torch.float32, True, (96,), seed=6)
+    # memory that was used before: every result has to be written
+    held = [torch.full((96,), 7.0, device=gpu) for _ in range(8)]
+    del held
     leaves = {k: t.clone().requires_grad_(True) for k, t in v.items()}
     got = torch.autograd.grad(_call(leaves, 1.0), list(leaves.values()), outs)
     for a, t in zip(got, leaves.values()):

@@ -120,7 +120,11 @@ def _check(exact, call, h, w, reduction):
 SIZES = [  # tokens, vocabulary, dim: single ones, tile edges on both sides, odd pitches
     (1, 1, 1), (1, 1000, 64), (2, 63, 8), (3, 65, 100), (63, 257, 72), (64, 256, 64),
     (65, 1003, 300), (255, 511, 129), (256, 512, 256), (257, 2049, 320), (513, 700, 1001),
-    (5, 5000, 2048), (1100, 129, 96)]
+    (5, 5000, 2048), (1100, 129, 96),
+    # both sides of the sizes at which a call takes other kernels: rows of one tile and few rows,
+    # tokens of a short weight gradient, split sums
+    (16, 3000, 520), (17, 3000, 520), (192, 1500, 264), (193, 1500, 264), (512, 1000, 72),
+    (520, 1000, 72), (30, 20000, 256), (300, 12000, 64)]
 
 
 @pytest.mark.gpu
@@ -215,7 +219,10 @@ def test_no_token_at_all(gpu):
     loss = dmuon.linear_cross_entropy(a, b, t)
     loss.backward()
     assert float(loss.detach()) == 0.0 and a.grad.shape == (0, 64) and not bool(b.grad.any())
-    assert dmuon.linear_cross_entropy(a, b, t, reduction="none").shape == (0,)
+    rows = dmuon.linear_cross_entropy(a, b, t, reduction="none")
+    b.grad = None
+    rows.sum().backward()
+    assert rows.shape == (0,) and not bool(b.grad.any())
 
 
 @pytest.mark.gpu
@@ -402,6 +409,37 @@ def test_the_workspace_does_not_grow_with_the_tokens(gpu):
     torch.cuda.reset_peak_memory_stats()
     dmuon.linear_cross_entropy(a, b, t).backward()
     assert torch.cuda.max_memory_allocated() - before < 4.5e9
+
+
+@pytest.mark.gpu
+def test_weights_past_32_bit_offsets(gpu):
+    """A weight of more than 2^31 values: losses and gradients at its end and beginning."""
+    n, v, d = 8, (1 << 20) + 37, 2056
+    gen = torch.Generator(device=gpu).manual_seed(0)
+    w = torch.empty(v, d, dtype=torch.bfloat16, device=gpu).normal_(0, 0.02, generator=gen)
+    assert w.numel() > 1 << 31
+    h = torch.randn(n, d, device=gpu, generator=gen).bfloat16()
+    t = torch.tensor([0, 1, 70000, v // 2, v - 70000, v - 3, v - 2, v - 1], device=gpu)
+    a, b = h.requires_grad_(True), w.requires_grad_(True)
+    loss = dmuon.linear_cross_entropy(a, b, t)
+    loss.backward()
+    hd, wd = h.detach(), w.detach()
+    z = torch.cat([hd.double() @ part.double().t() for part in wd.split(1 << 17)], 1)
+    lse = torch.logsumexp(z, 1)
+    want = float((lse - z.gather(1, t[:, None])[:, 0]).mean())
+    assert abs(float(loss.detach()) - want) <= 2.0 ** -20 * (1 + abs(want)) * 4
+    dz = (z - lse[:, None]).exp()
+    dz[torch.arange(n, device=gpu), t] -= 1
+    dz /= n
+    for rows in (slice(0, 300), slice(v // 2 - 100, v // 2 + 100), slice(v - 300, v)):
+        want = dz[:, rows].t() @ hd.double()
+        slack = (U[hd.dtype] + 2.0 ** -11 + 1e-4) * (dz[:, rows].abs().t() @ hd.double().abs())
+        _within(b.grad[rows], want, slack + U[hd.dtype] * want.abs() + 1e-30)
+    want = sum(dz[:, i:i + (1 << 17)] @ part.double()
+               for i, part in zip(range(0, v, 1 << 17), wd.split(1 << 17)))
+    size = sum(dz[:, i:i + (1 << 17)].abs() @ part.double().abs()
+               for i, part in zip(range(0, v, 1 << 17), wd.split(1 << 17)))
+    _within(a.grad, want, (U[hd.dtype] + 2.0 ** -11 + 1e-4) * size + U[hd.dtype] * want.abs())
 
 
 def _refuse(match, call, kind=ValueError):
