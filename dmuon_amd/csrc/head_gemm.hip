@@ -29,20 +29,29 @@ typedef f32x4_t f32x4_any_t __attribute__((aligned(4)));
 
 using T = Tile<256, 256, 64, 2, 2, 4>;
 
+// How an operand of R rows by K lies in memory.
+//   ROWS      [R][ld], K contiguous
+//   KMAJOR    [K][ld], R contiguous
+//   G_ROWS    rows of the logit gradient (R tokens, K classes): blocks of 64 classes, [K / 64][ld][64]
+//   G_KMAJOR  its columns (R classes, K tokens) in the same blocks, [R / 64][ld][64]
+enum Form { ROWS, KMAJOR, G_ROWS, G_KMAJOR };
+
 // One operand's part of the LDS ring: what each wave v of a group moves of a slice, in instructions
 // of 8 rows (k-major: k-rows) of 128 bytes. A lane's place in instruction q + 2 is 16 rows further,
 // and the swizzle moves its chunk of 8 values by an xor of 4 chunks between even and odd q, so one
 // byte offset and one chunk a lane describe them all.
-template <bool KM>
+template <Form F>
 struct Mover {
-  const uint16_t* base;                   // the tile's first row (k-major: first value)
+  static constexpr bool kKMajor = F == KMAJOR || F == G_KMAJOR;
+  const uint16_t* base;                   // what the wave moves of slice 0 starts here, or before it
   long long ld;
-  int rows, K, width;                     // rows of the tile inside the operand; k-major: values
+  int rows, K, width;                     // rows of the tile inside the operand; KMAJOR: values
   unsigned off;                           // byte offset of this lane's row in instruction 0
   int chunk;                              // first value of its chunk
   char* lds;
 
-  // B: this wave's block of 64 rows (values); A in row form: rows v * 32 and 128 + v * 32
+  // k-major: this wave's block of 64 values; in row form B's block of 64 rows, or A's rows v * 32 and
+  // 128 + v * 32
   __device__ __forceinline__ void init(const uint16_t* X, long long ld_, int r0, int n, int k,
                                        int v, int rows_of_wave, int lane, char* lds_) {
     ld = ld_;
@@ -50,16 +59,29 @@ struct Mover {
     rows = min(kTile, n - r0);
     width = (n + 7) / 8 * 8 - r0;         // whole chunks: the rows are padded to them
     static_assert(T::CPR == 8 && T::RPI == 8 && T::RPL == 2, "8 rows of 8 chunks an instruction");
-    if constexpr (KM) {
-      base = X + r0;
+    if constexpr (kKMajor) {
       lds = lds_ + v * kSlice * 128;
       chunk = 8 * ((lane & 7) ^ kswz64(lane >> 3));
-      off = (unsigned)((lane >> 3) * ld + v * 64) * 2u;
+      if constexpr (F == KMAJOR) {
+        base = X + r0;
+        off = (unsigned)((lane >> 3) * ld + v * 64) * 2u;
+      } else {
+        // a block of classes past the last one holds nothing to move
+        rows = r0 + 64 * v < n ? 1 : 0;
+        base = X + (long long)(r0 / 64 + v) * ld * 64;
+        off = (unsigned)(lane >> 3) * 128u;
+      }
     } else {
-      base = X + (long long)r0 * ld;
       lds = lds_ + v * rows_of_wave * T::ROWB;
       chunk = 8 * T::slot(lane & 7, lane >> 3);
-      off = (unsigned)((v * rows_of_wave + (lane >> 3)) * ld) * 2u;
+      const int r = v * rows_of_wave + (lane >> 3);
+      if constexpr (F == ROWS) {
+        base = X + (long long)r0 * ld;
+        off = (unsigned)(r * ld) * 2u;
+      } else {
+        base = X + (long long)r0 * 64;
+        off = (unsigned)r * 128u;
+      }
     }
   }
   // N instructions of slice `s` into ring slot `slot`, starting `hi` rows further
@@ -69,70 +91,78 @@ struct Mover {
     const int k0 = s * kSlice;
     const uint16_t* p = base;
     int bytes;
-    if constexpr (KM) {
+    unsigned step = 1024u;                // 8 rows of a block of 64
+    if constexpr (F == KMAJOR) {
       p += (long long)k0 * ld;
       bytes = (int)(((long long)(min(kSlice, K - k0) - 1) * ld + width) * 2);
+      step = 8u * (unsigned)ld * 2u;
+    } else if constexpr (F == G_KMAJOR) {
+      p += (long long)k0 * 64;
+      bytes = rows * min(kSlice, K - k0) * 128;
+    } else if constexpr (F == G_ROWS) {
+      p += (long long)s * ld * 64;
+      bytes = rows * 128;
     } else {
       bytes = (int)(((long long)(rows - 1) * ld + (K + 7) / 8 * 8) * 2);
+      step = 8u * (unsigned)ld * 2u;
     }
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint16_t*>(p), (short)0, bytes, 0x00020000);
-    const unsigned step = 8u * (unsigned)ld * 2u;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       const int c = chunk ^ (32 * (q & 1));
-      unsigned o = off + (unsigned)c * 2u + (unsigned)hi * (unsigned)ld * 2u + (unsigned)q * step;
+      unsigned o = off + (unsigned)c * 2u + (unsigned)(hi / 8) * step + (unsigned)q * step;
       // a chunk past K in the last slice: an offset outside any range reads 0
-      if constexpr (!KM) o = c + k0 >= K ? 0x80000000u : o + (unsigned)k0 * 2u;
+      if constexpr (F == ROWS) o = c + k0 >= K ? 0x80000000u : o + (unsigned)k0 * 2u;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rs, (lds_ptr_t)(lds + slot * T::STAGE + hi * T::ROWB + q * 1024), 16, o, 0, 0, 0);
     }
   }
 };
 
-// 16 x 64 logits of a wave: statistics, and the exponentials (through LDS, so that the stores are
-// whole 128-byte row segments) or the logits themselves. acc[y]: columns 16 y ..
+// 16 x 64 logits of a wave: statistics, and the exponentials (through LDS, so that a store writes
+// whole rows of their block of 64 columns) or the logits themselves. acc[y]: columns 16 y ..
 template <int MODE>
 __device__ __forceinline__ void logits_epilogue(const HeadGemm& a, const f32x4_t (&acc)[4], int i0,
                                                 int jw, int lane, char* slab) {
   const int jl = 4 * (lane >> 4), i = i0 + (lane & 15);
   const bool inside = jw + 64 <= a.N;
+  const long long block = (long long)(jw / 64) * a.M;    // first row of these columns' block
+  const float k = a.scale * kLog2e;       // positive: the largest sum is the largest logit
   f32x4_t z[4];
-  float m = -kInf;
+  float top = -kInf;
 #pragma unroll
   for (int y = 0; y < 4; ++y) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      z[y][e] = acc[y][e] * a.scale;
       // columns past the vocabulary: no maximum, no share of the sum
-      if (!inside && jw + jl + 16 * y + e >= a.N) z[y][e] = -kInf;
-      m = fmaxf(m, z[y][e]);
+      z[y][e] = inside || jw + jl + 16 * y + e < a.N ? acc[y][e] : -kInf;
+      top = fmaxf(top, z[y][e]);
     }
     if (MODE == HG_LOGITS && i < a.M)
-      *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.Z) + (long long)i * a.ldz + jw + jl +
-                                  16 * y) = z[y];
+      *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.Z) + (block + i) * 64 + jl + 16 * y) = z[y] * k;
   }
-  m = fmaxf(m, __shfl_xor(m, 16));
-  m = fmaxf(m, __shfl_xor(m, 32));
+  top = fmaxf(top, __shfl_xor(top, 16));
+  top = fmaxf(top, __shfl_xor(top, 32));
+  // 2^kExpShift exp(z - m) as one multiply-add and v_exp_f32; a row of -inf throughout sums to 0
+  const float m = top * k, from = (top == -kInf ? 0.f : m) - (float)kExpShift;
   float s = 0.f;
 #pragma unroll
   for (int y = 0; y < 4; ++y) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      z[y][e] = z[y][e] == -kInf ? 0.f : __expf(z[y][e] - m);
+      z[y][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[y][e], k, -from));
       s += z[y][e];
     }
     if constexpr (MODE == HG_EXP) {
-      constexpr float up = (float)(1 << kExpShift);
-      const u32x2_t o = {pack2_elt<ELT_F16>(up * z[y][0], up * z[y][1]),
-                         pack2_elt<ELT_F16>(up * z[y][2], up * z[y][3])};
+      const u32x2_t o = {pack2_elt<ELT_F16>(z[y][0], z[y][1]), pack2_elt<ELT_F16>(z[y][2], z[y][3])};
       *reinterpret_cast<u32x2_t*>(slab + (lane & 15) * T::EPN + (jl + 16 * y) * 2) = o;
     }
   }
   s += __shfl_xor(s, 16);
   s += __shfl_xor(s, 32);
   if (lane < 16 && i < a.M)
-    a.stats[(long long)i * a.n_stats + jw / kStatCols] = make_float2(m, s);
+    a.stats[block + i] = make_float2(m, s * (1.f / (float)(1 << kExpShift)));
   if constexpr (MODE == HG_EXP) {
     const int cr = lane >> 3, cc = lane & 7;
     u32x4_t d[2];
@@ -144,8 +174,7 @@ __device__ __forceinline__ void logits_epilogue(const HeadGemm& a, const f32x4_t
       const int r = i0 + 8 * k + cr;
       if (r < a.M)
         __builtin_nontemporal_store(
-            d[k], reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.Z) + (long long)r * a.ldz +
-                                             jw + 8 * cc));
+            d[k], reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.Z) + (block + r) * 64 + 8 * cc));
     }
   }
 }
@@ -222,17 +251,18 @@ __device__ __forceinline__ void grad_epilogue(const HeadGemm& a, f32x4_t (&acc)[
 // block with slice k + 2 after its own reads of it (group 0 read it in the phase before) and waits
 // for slice k + 1's B. LIVE false: the wave's sub-tile lies outside the result; it moves operands
 // and passes the barriers only.
-template <int E, int MODE, bool AKM, bool BKM, bool LIVE>
+template <int E, int MODE, Form FA, Form FB, bool LIVE>
 __device__ __forceinline__ void head_tile(const HeadGemm& a, char* smem, int bi, int bj, int split) {
   constexpr int KS = kSlice / 32;
+  constexpr bool AKM = Mover<FA>::kKMajor, BKM = Mover<FB>::kKMajor;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int grp = wave >> 2, v = wave & 3;
   const int wj = grp == 0 ? 3 - v : v;    // group 1's wave v reads the B block it moves
   const int i0 = bi * kTile, j0 = bj * kTile;
 
-  Mover<AKM> ma;
-  Mover<BKM> mb;
+  Mover<FA> ma;
+  Mover<FB> mb;
   ma.init(a.A, a.lda, i0, a.M, a.K, v, 32, lane, smem);
   mb.init(a.B, a.ldb, j0, a.N, a.K, v, 64, lane, smem + T::A_BYTES);
   auto issue_a = [&](int s, int slot) {
@@ -358,7 +388,7 @@ __device__ __forceinline__ void head_tile(const HeadGemm& a, char* smem, int bi,
   }
 }
 
-template <int E, int MODE, bool AKM, bool BKM>
+template <int E, int MODE, Form FA, Form FB>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void head_gemm_kernel(const HeadGemm a) {
   __shared__ __attribute__((aligned(16))) char smem[T::LDS_BYTES];
@@ -374,8 +404,8 @@ void head_gemm_kernel(const HeadGemm a) {
   const int grp = wave >> 2, v = wave & 3;
   const bool live = bi * kTile + 128 * grp < a.M && bj * kTile + 64 * (grp == 0 ? 3 - v : v) < a.N;
   const int sp = __builtin_amdgcn_readfirstlane(split);
-  if (live) head_tile<E, MODE, AKM, BKM, true>(a, smem, bi, bj, sp);
-  else head_tile<E, MODE, AKM, BKM, false>(a, smem, bi, bj, sp);
+  if (live) head_tile<E, MODE, FA, FB, true>(a, smem, bi, bj, sp);
+  else head_tile<E, MODE, FA, FB, false>(a, smem, bi, bj, sp);
 }
 
 // A weight gradient over few tokens: bound by writing it. 128 x 128 tiles, four waves of 64 x 64, one
@@ -396,9 +426,10 @@ void head_short_kernel(const HeadGemm a) {
   const int i0 = __builtin_amdgcn_readfirstlane((8 * g + r % rows) * kSide);
   const int j0 = __builtin_amdgcn_readfirstlane(r / rows * kSide);
   // waves 0 and 1 move the slice's 64-value blocks of A, 2 and 3 those of B
-  Mover<true> mv;
-  if (wave < 2) mv.init(a.A, a.lda, i0, a.M, a.K, wave, 64, lane, smem);
-  else mv.init(a.B, a.ldb, j0, a.N, a.K, wave - 2, 64, lane, smem + 2 * kBlock);
+  Mover<G_KMAJOR> ma;
+  Mover<KMAJOR> mb;
+  ma.init(a.A, a.lda, i0, a.M, a.K, wave & 1, 64, lane, smem);
+  mb.init(a.B, a.ldb, j0, a.N, a.K, wave & 1, 64, lane, smem + 2 * kBlock);
   const int wi = wave >> 1, wj = wave & 1;
   f32x4_t acc[4][4];
 #pragma unroll
@@ -408,7 +439,8 @@ void head_short_kernel(const HeadGemm a) {
   const int KT = (a.K + kSlice - 1) / kSlice;
   for (int s = 0; s < KT; ++s) {
     if (s > 0) __syncthreads();           // the slice before has been read
-    mv.issue<8>(s, 0, 0);
+    if (wave < 2) ma.issue<8>(s, 0, 0);
+    else mb.issue<8>(s, 0, 0);
     wait_vmcnt<0>();
     __syncthreads();
 #pragma unroll
@@ -555,15 +587,16 @@ hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream) {
   const auto fits = [](const void* p, long long ld, long long width) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && ld >= width && ld < (1 << 22);
   };
+  const bool grad = a.mode == HG_GRAD;
   if (a.splits < 1 || nb > 0x7fffffffLL || a.K < 0 ||
-      (a.K > 0 && (!fits(a.A, a.lda, a.a_kmajor ? a.M : a.K) ||
-                   !fits(a.B, a.ldb, a.b_kmajor ? a.N : a.K))))
+      (a.K > 0 && !fits(a.B, a.ldb, a.b_kmajor ? a.N : a.K)) ||
+      (a.K > 0 && !grad && !fits(a.A, a.lda, a.K)) ||
+      (a.K > 0 && grad && ((reinterpret_cast<uintptr_t>(a.A) & 15) || a.lda < (a.a_kmajor ? a.K : a.M))))
     return hipErrorInvalidValue;
   if (a.splits > 1 && (a.mode != HG_GRAD || !a.out || !a.part || a.add_part))
     return hipErrorInvalidValue;
   if (a.mode == HG_GRAD ? !a.b_kmajor
-                        : a.a_kmajor || a.b_kmajor || !a.stats ||
-                              (a.mode != HG_STATS && (!a.Z || a.ldz < (a.N + 63) / 64 * 64)))
+                        : a.a_kmajor || a.b_kmajor || !a.stats || (a.mode != HG_STATS && !a.Z))
     return hipErrorInvalidValue;
   if (a.few && a.mode != HG_GRAD && a.M <= 16 && nb < kCus) {
     const dim3 few((unsigned)((a.N + 63) / 64));
@@ -585,16 +618,16 @@ hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream) {
     return hipGetLastError();
   }
   const dim3 grid((unsigned)nb);
-#define DMUON_HG(E, MODE, AKM, BKM) \
-  hipLaunchKernelGGL((head_gemm_kernel<E, MODE, AKM, BKM>), grid, dim3(512), 0, stream, a)
+#define DMUON_HG(E, MODE, FA, FB) \
+  hipLaunchKernelGGL((head_gemm_kernel<E, MODE, FA, FB>), grid, dim3(512), 0, stream, a)
 #define DMUON_HG_E(E)                                                     \
   do {                                                                    \
-    if (a.mode == HG_STATS) DMUON_HG(E, HG_STATS, false, false);          \
+    if (a.mode == HG_STATS) DMUON_HG(E, HG_STATS, ROWS, ROWS);          \
     else if (a.mode == (E == ELT_F16 ? HG_LOGITS : HG_EXP))               \
-      DMUON_HG(E, (E == ELT_F16 ? HG_LOGITS : HG_EXP), false, false);     \
+      DMUON_HG(E, (E == ELT_F16 ? HG_LOGITS : HG_EXP), ROWS, ROWS);       \
     else if (a.mode != HG_GRAD) return hipErrorInvalidValue;              \
-    else if (a.a_kmajor) DMUON_HG(E, HG_GRAD, true, true);                \
-    else DMUON_HG(E, HG_GRAD, false, true);                               \
+    else if (a.a_kmajor) DMUON_HG(E, HG_GRAD, G_KMAJOR, KMAJOR);          \
+    else DMUON_HG(E, HG_GRAD, G_ROWS, KMAJOR);                            \
   } while (0)
   if (a.elt == ELT_F16) DMUON_HG_E(ELT_F16);
   else DMUON_HG_E(ELT_BF16);

@@ -15,29 +15,36 @@ constexpr int kStatCols = 64;
 // 2^6 = 64 times the unit mass does not overflow.
 constexpr int kGradShift = 10;
 
-// What a product writes.
-//   HG_STATS   the softmax statistics of scale * acc
-//   HG_EXP     those and X = fp16(2^kExpShift exp(z - m)), m the row's maximum in its statistic's
+// What a product writes. Logits z = scale * acc and their statistics are in units of log 2.
+//   HG_STATS   the softmax statistics of z
+//   HG_EXP     those and Z = fp16(2^kExpShift 2^(z - m)), m the row's maximum in its statistic's
 //              columns; 0 in the columns past N
 //   HG_LOGITS  those and Z = z in fp32
 //   HG_GRAD    out = alpha[0] * (acc + part) rounded to out_dtype, or part (+)= acc in fp32
 enum HeadGemmMode : int { HG_STATS = 0, HG_EXP = 1, HG_LOGITS = 2, HG_GRAD = 3 };
 // fp16 holds exponentials down to 2^-29 of their maximum with all its bits
 constexpr int kExpShift = 15;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 // Rows up to which the logits have one row of tiles, bound by reading the weight.
 constexpr int kFewRows = 256;
 
-// acc[i][j] = sum_k A(i, k) * B(j, k): operand X's element (r, k) is X[r * ld + k], or
-// X[k * ld + r] with x_kmajor.
+// The logits and their gradient lie in blocks of kStatCols classes, [ceil(vocab / 64)][rows][64]: a
+// tile of any of the three products reads and writes them in runs of 8 to 32 KiB, where rows of the
+// whole vocabulary would be 128 bytes at a time (hidden gradient of 8192 x 128256 x 4096: 6.08 ms
+// that way, 5.73 in blocks).
+//
+// acc[i][j] = sum_k A(i, k) * B(j, k). HG_GRAD: A is the logit gradient in its blocks, lda its rows
+// (a_kmajor: i is the class, k the token). Otherwise A's element (i, k) is A[i * lda + k]. B's is
+// B[j * ldb + k], or B[k * ldb + j] with b_kmajor.
 struct HeadGemm {
   const uint16_t* A; long long lda; int a_kmajor;
   const uint16_t* B; long long ldb; int b_kmajor;
   int M, N, K;
   int mode, elt;
   float scale;
-  void* Z; long long ldz;                 // HG_EXP, HG_LOGITS: [M][ldz], ldz a multiple of 64
-  float2* stats; int n_stats;             // [M][n_stats], n_stats = ceil(N / kStatCols)
+  void* Z;                                // HG_EXP, HG_LOGITS: [ceil(N / 64)][M][64]
+  float2* stats;                          // [ceil(N / 64)][M]
   const float* alpha;
   void* out; long long ldo; int out_dtype;   // HG_GRAD: result (DT_F32 or the operands'), or NULL
   float* part; long long ldp;             // HG_GRAD: fp32 sums [M][ldp], or NULL
@@ -67,9 +74,10 @@ struct HeadRows {
   int* ids; float* probs;                 // [n][k_list]
   float* logits;                          // [n][k_list]: the entries' logits (over temperature)
   float* mass;                            // [n]: sum of the row's probs, < 0: not counted
-  float* lse;                             // [n]
+  float* top;                             // [n]: the largest logit, in units of log 2
   float* loss;                            // [n]
-  float* row_weight;                      // [n]: 2^kGradShift * row gradient / largest
+  float* row_weight;                      // [n]: 2^kGradShift * row gradient / largest, 0: not counted
+  float* factor;                          // [n]: of 2^(z - top) in the logit gradient
   float* alpha;                           // [1]: what turns a stored gradient into the real one
   float* mean;                            // [1] or NULL: the reduced loss
 };
@@ -78,12 +86,11 @@ struct HeadRows {
 hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long ldh,
                                const uint16_t* W, long long ldw, int dim, int elt, bool grads,
                                hipStream_t stream);
-// lse and loss of rows first .. first + rows - 1 from their statistics, and with G their logit
-// gradients G[row][v] = row_weight (mass softmax - target probability), 0 from the vocabulary's end
-// up to ldg: in place of the exponentials (Z == G), or from the fp32 logits Z.
+// Top, loss, row weight and factor of rows first .. first + rows - 1 from their statistics, and with G
+// their logit gradients row_weight (mass softmax - target probability), 0 past the vocabulary's end:
+// in place of the exponentials (Z == G), or from the fp32 logits Z.
 hipError_t launch_head_rows(const HeadRows& r, int first, int rows, const float2* stats,
-                            const void* Z, uint16_t* G, long long ldg, int elt,
-                            hipStream_t stream);
+                            const void* Z, uint16_t* G, int elt, hipStream_t stream);
 // mean[0] = sum of the losses, divided by the number of counted rows for DMUON_LOSS_MEAN, and alpha.
 hipError_t launch_head_reduce(const HeadRows& r, hipStream_t stream);
 

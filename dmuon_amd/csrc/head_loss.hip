@@ -22,12 +22,12 @@ int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 // Workspace of a chunk's logits and logit gradient; a call of more tokens takes several chunks.
 constexpr int64_t kChunkBytes = int64_t(4) << 30;
 
-// The pitch of the logits stays inside the products' 32-bit tile offsets.
-constexpr int64_t kMaxVocab = (int64_t(1) << 22) - 256;
+// Blocks of 64 classes are a grid's second dimension.
+constexpr int64_t kMaxVocab = int64_t(65535) * 64;
 
 struct Layout {
-  int64_t chunk, ld;                      // tokens of a chunk, pitch of its logits
-  int64_t ids, probs, logits, mass, lse, loss, row_weight, alpha, Z, stats, G, part, H, W, bytes;
+  int64_t chunk, ld;                      // tokens of a chunk, classes in whole blocks
+  int64_t ids, probs, logits, mass, top, loss, row_weight, factor, alpha, Z, stats, G, part, H, W, bytes;
   int64_t pad;                            // pitch of the copies of hidden and weight
   bool copy_h, copy_w;
 };
@@ -101,9 +101,10 @@ Layout lay_out(const dmuon_head_loss_args& a) {
   l.probs = take(a.tokens * k * 4);
   l.logits = take(a.tokens * k * 4);
   l.mass = take(a.tokens * 4);
-  l.lse = take(a.tokens * 4);
+  l.top = take(a.tokens * 4);
   l.loss = take(a.loss ? 0 : a.tokens * 4);
   l.row_weight = take(a.tokens * 4);
+  l.factor = take(a.tokens * 4);
   l.alpha = take(4);
   l.stats = take(l.chunk * tiles * 8);
   l.G = take(grads ? l.chunk * l.ld * 2 : 0);
@@ -181,9 +182,10 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
   r.probs = floats(l.probs);
   r.logits = floats(l.logits);
   r.mass = floats(l.mass);
-  r.lse = floats(l.lse);
+  r.top = floats(l.top);
   r.loss = a.loss ? a.loss : floats(l.loss);
   r.row_weight = floats(l.row_weight);
+  r.factor = floats(l.factor);
   r.alpha = floats(l.alpha);
   r.mean = a.reduced;
   void* Z = ws + l.Z;
@@ -224,11 +226,11 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
     g.B = W; g.ldb = ldw;
     g.M = rows; g.N = (int)a.vocab; g.K = (int)a.dim;
     g.scale = 1.f / r.temperature;
-    g.Z = Z; g.ldz = l.ld;
-    g.stats = stats; g.n_stats = (int)(round_up(a.vocab, kStatCols) / kStatCols);
+    g.Z = Z;
+    g.stats = stats;
     if (check_launch(launch_head_gemm(g, stream), who)) return 1;
-    if (check_launch(launch_head_rows(r, (int)first, rows, stats, Z, grads ? G : nullptr, l.ld, elt,
-                                      stream), who)) return 1;
+    if (check_launch(launch_head_rows(r, (int)first, rows, stats, Z, grads ? G : nullptr, elt, stream),
+                     who)) return 1;
     // before the gradients' products: they take its alpha. The last chunk's is the whole loss.
     if (a.reduction != DMUON_LOSS_ROWS && check_launch(launch_head_reduce(r, stream), who)) return 1;
     if (grads) {
@@ -238,7 +240,7 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
       g.alpha = r.alpha;
       g.out_dtype = a.grad_dtype;
       if (a.d_hidden) {
-        g.A = G; g.lda = l.ld;
+        g.A = G; g.lda = rows;
         g.B = W; g.ldb = ldw; g.b_kmajor = 1;
         g.M = rows; g.N = (int)a.dim; g.K = (int)a.vocab;
         g.splits = split_h ? head_gemm_splits(rows, g.N, g.K, false) : 1;
@@ -248,7 +250,7 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
       }
       if (a.d_weight) {
         const bool last = first + rows >= a.tokens;
-        g.A = G; g.lda = l.ld; g.a_kmajor = 1;
+        g.A = G; g.lda = rows; g.a_kmajor = 1;
         g.B = Hc; g.ldb = ldh; g.b_kmajor = 1;
         g.M = (int)a.vocab; g.N = (int)a.dim; g.K = rows;
         g.splits = gathers ? 1 : head_gemm_splits(g.M, g.N, g.K, true);

@@ -137,115 +137,142 @@ __global__ __launch_bounds__(1024) void head_weights_kernel(HeadRows r) {
   if (threadIdx.x == 0) r.alpha[0] = top * r.temperature / kUnit;
 }
 
-// (maximum, sum of exponentials) of two sets of logits as one
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// (maximum, sum of exponentials) of two sets of logits as one, in units of log 2
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2);
   if (top == -kInf) s += s2;              // empty sets, or a NaN to keep
-  else s = s * __expf(m - top) + s2 * __expf(m2 - top);
+  else s = s * exp2_fast(m - top) + s2 * exp2_fast(m2 - top);
   m = top;
 }
 
-// What head_rows_kernel makes its gradient from.
-enum { FROM_NONE = 0, FROM_EXP = 1, FROM_LOGITS = 2 };
-
-// One row a block, or `parts` blocks a row where there are few rows: the row's statistics joined
-// (every block for itself), its loss (part 0), and this part's columns of the logit gradient
-//   row_weight (mass + 2 z_loss lse) softmax - row_weight q
-// in place of the exponentials, whose factor exp(m - lse) is one of 64 columns, or from the
-// logits. Both cross memory once: 2 + 2 bytes a logit, or 4 + 2. The entries' columns come last,
-// from their fp32 logits: mass p - q cancels where the student is sure. (Entries of one class in one
-// row write the same value.)
-template <int E, int FROM>
-__global__ __launch_bounds__(256) void head_rows_kernel(HeadRows r, int first,
-                                                        const float2* __restrict__ stats,
-                                                        int n_stats, const void* Z, uint16_t* G,
-                                                        long long ldg, int parts) {
-  __shared__ float lds[2][4];
-  const int row = blockIdx.x / parts, part = blockIdx.x % parts;
-  const long long n = first + row;
-  stats += (long long)row * n_stats;
+// log-sum-exp, loss, row weight and factor of `side` rows a block (a power of two, at most 16): 1024
+// threads, thread t for row t % side, every 1024 / side-th statistic and entry.
+__global__ __launch_bounds__(1024) void head_lse_kernel(HeadRows r, int first, int rows,
+                                                        const float2* __restrict__ stats, int side,
+                                                        bool grads) {
+  __shared__ float lds[3][16][16];
+  const int rl = threadIdx.x & (side - 1), strand = threadIdx.x / side, strands = 1024 / side;
+  const int row = blockIdx.x * side + rl, wave = threadIdx.x >> 6;
+  const bool in = row < rows;
+  const long long n = first + (in ? row : 0);
+  const int tiles = (r.vocab + kStatCols - 1) / kStatCols;
   float m = -kInf, s = 0.f;
-  for (int t = threadIdx.x; t < n_stats; t += 256) {
-    const float2 o = stats[t];
-    join(m, s, o.x, o.y);
+  if (in) {
+#pragma unroll 4
+    for (int t = strand; t < tiles; t += strands) {
+      const float2 o = stats[(long long)t * rows + row];
+      join(m, s, o.x, o.y);
+    }
   }
-  for (int o = 1; o < 64; o <<= 1) {
+  for (int o = side; o < 64; o <<= 1) {
     const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
     join(m, s, m2, s2);
   }
-  if ((threadIdx.x & 63) == 0) lds[0][threadIdx.x >> 6] = m, lds[1][threadIdx.x >> 6] = s;
+  if ((threadIdx.x & 63) < side) lds[0][wave][rl] = m, lds[1][wave][rl] = s;
   __syncthreads();
-  m = lds[0][0], s = lds[1][0];
-  for (int w = 1; w < 4; ++w) join(m, s, lds[0][w], lds[1][w]);
-  const float lse = logf(s) + m;
+  m = lds[0][0][rl], s = lds[1][0][rl];
+  for (int w = 1; w < 16; ++w) join(m, s, lds[0][w][rl], lds[1][w][rl]);
+  const float lse = (log2f(s) + m) * kLn2;
   const float mass = r.mass[n];
   const bool counted = !(mass < 0.f);
+  float loss = 0.f;
+  if (in && counted)
+    for (int k = strand; k < r.k_list; k += strands) {
+      const long long at = n * r.k_list + k;
+      if (r.ids[at] < 0) continue;
+      const float q = r.probs[at], z = r.logits[at];
+      loss += r.targets ? lse - z : q * (logf(q) - (z - lse));
+    }
+  for (int o = side; o < 64; o <<= 1) loss += __shfl_xor(loss, o);
+  if ((threadIdx.x & 63) < side) lds[2][wave][rl] = loss;
+  __syncthreads();
+  if (!in || strand) return;
+  loss = 0.f;
+  for (int w = 0; w < 16; ++w) loss += lds[2][w][rl];
+  if (counted) {
+    loss = loss * r.temperature * r.temperature + r.z_loss * lse * lse;
+    if (mass != mass) loss = mass;
+  }
+  r.top[n] = m;
+  r.loss[n] = loss;
+  if (grads) {
+    const float w = row_weight(r, n);
+    r.row_weight[n] = w;
+    r.factor[n] = w == 0.f ? 0.f : w * (mass + 2.f * r.z_loss * lse) / s;
+  }
+}
+
+// The logit gradient: factor * 2^(z - top) - row_weight * q, in place of the exponentials (whose share
+// 2^(m - top) is one of a block's row) or from the logits (LOGITS). Crosses memory once, 2 + 2 bytes
+// a logit or 4 + 2: 4 x 32 rows of one block of 64 classes a workgroup, 16 bytes a thread and step.
+// A hard target's own class comes from its fp32 logit: softmax - 1 cancels where the student is sure. (So the
+// row's maximum and 1 / sum go in apart: their log-sum-exp would lose what 1 - p is made of.)
+template <int E, bool LOGITS>
+__global__ __launch_bounds__(256) void head_grad_kernel(HeadRows r, int first, int rows,
+                                                        const float2* __restrict__ stats,
+                                                        const float* __restrict__ Z, uint16_t* G) {
+  const int tile = blockIdx.y, c = threadIdx.x & 7;
+  const int row0 = blockIdx.x * 128 + (threadIdx.x >> 3);
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int row = row0 + 32 * p;
+    if (row >= rows) return;
+    const long long n = first + row, at = ((long long)tile * rows + row) * 64 + 8 * c;
+    const float f = r.factor[n], top = r.top[n];
+    const int id = r.targets ? r.ids[n] : -1;
+    float v[8];
+    if (f == 0.f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    } else if constexpr (!LOGITS) {
+      const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(G + at));
+      const float k = f * (1.f / (float)(1 << kExpShift)) *
+                      exp2_fast(stats[(long long)tile * rows + row].x - top);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[2 * e] = k * from_elt<ELT_F16>(x[e] & 0xffff);
+        v[2 * e + 1] = k * from_elt<ELT_F16>(x[e] >> 16);
+      }
+    } else {
+      const f32x4_t* z = reinterpret_cast<const f32x4_t*>(Z + at);
+      const f32x4_t lo = __builtin_nontemporal_load(z), hi = __builtin_nontemporal_load(z + 1);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = f * exp2_fast(lo[e] - top);
+        v[4 + e] = f * exp2_fast(hi[e] - top);
+      }
+    }
+    if (id >> 3 == 8 * tile + c) {
+      const float g = f * exp2_fast(__builtin_fmaf(r.logits[n], kLog2e, -top)) - r.row_weight[n];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (id & 7) == e ? g : v[e];
+    }
+    *reinterpret_cast<u32x4_t*>(G + at) = u32x4_t{pack2_elt<E>(v[0], v[1]), pack2_elt<E>(v[2], v[3]),
+                                                  pack2_elt<E>(v[4], v[5]), pack2_elt<E>(v[6], v[7])};
+  }
+}
+
+// The classes of the teachers' lists, from their fp32 logits: mass p - q cancels where the student
+// is sure. Entries of one class in one row write the same value. One wave a row.
+template <int E>
+__global__ __launch_bounds__(256) void head_entries_kernel(HeadRows r, int first, int rows,
+                                                           uint16_t* G) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  const long long n = first + row;
+  const float w = r.row_weight[n], f = r.factor[n], top = r.top[n];
+  if (w == 0.f) return;
   const int* ids = r.ids + n * r.k_list;
   const float* probs = r.probs + n * r.k_list;
-  const float* logits = r.logits + n * r.k_list;
-  if (part == 0) {
-    float loss = 0.f;
-    if (counted)
-      for (int k = threadIdx.x; k < r.k_list; k += 256) {
-        const float q = probs[k];
-        if (ids[k] < 0) continue;
-        loss += r.targets ? lse - logits[k] : q * (logf(q) - (logits[k] - lse));
-      }
-    loss = block_join<false>(loss, lds[0]);
-    if (threadIdx.x == 0) {
-      if (counted) {
-        loss = loss * r.temperature * r.temperature + r.z_loss * lse * lse;
-        if (mass != mass) loss = mass;
-      }
-      r.lse[n] = lse;
-      r.loss[n] = loss;
-    }
-  }
-  if constexpr (FROM != FROM_NONE) {
-    const float w = row_weight(r, n);
-    const float f = w == 0.f ? 0.f : w * (mass + 2.f * r.z_loss * lse);
-    const int chunks = (int)(ldg / 8), per = (chunks + parts - 1) / parts;
-    const int c0 = part * per, c1 = min(chunks, c0 + per);
-    uint16_t* g = G + (long long)row * ldg;
-    const float fe = f * (1.f / (float)(1 << kExpShift));
-#pragma unroll 4
-    for (int c = c0 + threadIdx.x; c < c1; c += 256) {
-      float v[8];
-      if (w == 0.f) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      } else if constexpr (FROM == FROM_EXP) {
-        const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(g + 8 * c));
-        const float k = fe * __expf(stats[c / 8].x - lse);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[2 * e] = k * from_elt<ELT_F16>(x[e] & 0xffff);
-          v[2 * e + 1] = k * from_elt<ELT_F16>(x[e] >> 16);
-        }
-      } else {
-        const f32x4_t* z = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(Z) +
-                                                            (long long)row * ldg + 8 * c);
-        const f32x4_t lo = __builtin_nontemporal_load(z), hi = __builtin_nontemporal_load(z + 1);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = f * __expf(lo[e] - lse);
-          v[4 + e] = f * __expf(hi[e] - lse);
-        }
-      }
-      const u32x4_t o = {pack2_elt<E>(v[0], v[1]), pack2_elt<E>(v[2], v[3]),
-                         pack2_elt<E>(v[4], v[5]), pack2_elt<E>(v[6], v[7])};
-      *reinterpret_cast<u32x4_t*>(g + 8 * c) = o;
-    }
-    if (w == 0.f) return;
-    __syncthreads();
-    for (int k = threadIdx.x; k < r.k_list; k += 256) {
-      const int id = ids[k];
-      if (id < 8 * c0 || id >= 8 * c1) continue;
-      float q = 0.f;
-      for (int j = 0; j < r.k_list; ++j)
-        if (ids[j] == id) q += probs[j];
-      g[id] = to_elt<E>(f * __expf(logits[k] - lse) - w * q);
-    }
+  for (int k = lane; k < r.k_list; k += 64) {
+    const int id = ids[k];
+    if (id < 0) continue;
+    float q = 0.f;
+    for (int j = 0; j < r.k_list; ++j)
+      if (ids[j] == id) q += probs[j];
+    const float p = f == 0.f ? 0.f : f * exp2_fast(__builtin_fmaf(r.logits[n * r.k_list + k], kLog2e, -top));
+    G[((long long)(id >> 6) * rows + row) * 64 + (id & 63)] = to_elt<E>(p - w * q);
   }
 }
 
@@ -346,22 +373,28 @@ hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long l
 }
 
 hipError_t launch_head_rows(const HeadRows& r, int first, int rows, const float2* stats,
-                            const void* Z, uint16_t* G, long long ldg, int elt,
-                            hipStream_t stream) {
+                            const void* Z, uint16_t* G, int elt, hipStream_t stream) {
   if (rows <= 0) return hipSuccess;
-  const int n_stats = (r.vocab + kStatCols - 1) / kStatCols;
-  // few rows: as many blocks a row as give every CU two, of at least 2048 columns each
-  long long parts = G ? (512 + rows - 1) / rows : 1;
-  if (parts > ldg / 2048) parts = ldg / 2048 > 0 ? ldg / 2048 : 1;
-  const dim3 grid((unsigned)(rows * parts));
-#define DMUON_ROWS(E, FROM)                                                                   \
-  hipLaunchKernelGGL((head_rows_kernel<E, FROM>), grid, dim3(256), 0, stream, r, first, stats, \
-                     n_stats, Z, G, ldg, (int)parts)
-  if (!G) DMUON_ROWS(ELT_BF16, FROM_NONE);
-  else if (Z == G && elt == ELT_BF16) DMUON_ROWS(ELT_BF16, FROM_EXP);
-  else if (Z != G && elt == ELT_F16) DMUON_ROWS(ELT_F16, FROM_LOGITS);
-  else return hipErrorInvalidValue;
-#undef DMUON_ROWS
+  const int tiles = (r.vocab + kStatCols - 1) / kStatCols;
+  // neighbouring rows share the lines of a statistic; few rows take more threads each
+  const int side = rows >= 1024 ? 16 : rows >= 128 ? 4 : 1;
+  hipLaunchKernelGGL(head_lse_kernel, dim3((unsigned)((rows + side - 1) / side)), dim3(1024), 0,
+                     stream, r, first, rows, stats, side, G != nullptr);
+  if (!G) return hipGetLastError();
+  if (tiles > 65535 || (Z == G) != (elt == ELT_BF16)) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)((rows + 127) / 128), (unsigned)tiles), lists((unsigned)((rows + 3) / 4));
+  const float* logits = static_cast<const float*>(Z);
+  if (elt == ELT_F16) {
+    hipLaunchKernelGGL((head_grad_kernel<ELT_F16, true>), grid, dim3(256), 0, stream, r, first, rows,
+                       stats, logits, G);
+    if (!r.targets)
+      hipLaunchKernelGGL(head_entries_kernel<ELT_F16>, lists, dim3(256), 0, stream, r, first, rows, G);
+  } else {
+    hipLaunchKernelGGL((head_grad_kernel<ELT_BF16, false>), grid, dim3(256), 0, stream, r, first, rows,
+                       stats, nullptr, G);
+    if (!r.targets)
+      hipLaunchKernelGGL(head_entries_kernel<ELT_BF16>, lists, dim3(256), 0, stream, r, first, rows, G);
+  }
   return hipGetLastError();
 }
 
