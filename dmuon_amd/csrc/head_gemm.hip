@@ -463,29 +463,31 @@ void head_short_kernel(const HeadGemm a) {
   if (iw < a.M && jw < a.N) grad_epilogue<E, 4>(a, acc, iw, jw, lane, smem + wave * kSlab, 0);
 }
 
-// Logits of at most 16 rows over a vocabulary with less than a 256-tile for every CU. A block takes 64
-// columns, its four waves every fourth 64-wide K step each, straight from memory into MFMA operands
-// (a lane's 16 bytes are its operand); the partial sums join through LDS. One row of 2048 against
-// 32001 columns (126 tiles): 28 us, 41 on the 256-tiles; against 128256 columns of 4096 both take
-// 183 us, and 16 rows, which each block here reads for itself, 213 against 184.
-template <int E, int MODE>
-__global__ __launch_bounds__(256) void head_few_kernel(const HeadGemm a) {
-  __shared__ __attribute__((aligned(16))) f32x4_t part[4][4][64];
+// Logits of a small call, whose 256-tiles would leave most CUs idle and wait alone on theirs. A block
+// takes 16 MB rows by 64 columns, its four waves every fourth 64-wide K step each, straight from
+// memory into MFMA operands (a lane's 16 bytes are its operand); the partial sums join through LDS,
+// and wave x finishes rows 16 x .. (see head_logits_small).
+template <int E, int MODE, int MB>
+__global__ __launch_bounds__(256) void head_small_kernel(const HeadGemm a) {
+  __shared__ __attribute__((aligned(16))) f32x4_t part[4][MB * 4][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int jw = blockIdx.x * 64;
+  const int i0 = blockIdx.y * 16 * MB, jw = blockIdx.x * 64;
   const int kl = 8 * (lane >> 4);
   // rows past the operands repeat the last one: their results are not used
-  const uint16_t* hp = a.A + (long long)min(lane & 15, a.M - 1) * a.lda + kl;
-  const uint16_t* wp[4];
-  f32x4_t acc[4];
+  const uint16_t *hp[MB], *wp[4];
+  f32x4_t acc[MB][4];
+#pragma unroll
+  for (int x = 0; x < MB; ++x)
+    hp[x] = a.A + (long long)min(i0 + 16 * x + (lane & 15), a.M - 1) * a.lda + kl;
 #pragma unroll
   for (int y = 0; y < 4; ++y) {
     wp[y] = a.B + (long long)min(jw + 16 * y + (lane & 15), a.N - 1) * a.ldb + kl;
-    acc[y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < MB; ++x) acc[x][y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   struct Step {
-    bf16x8_t h[2], w[2][4];
+    bf16x8_t h[2][MB], w[2][4];
   };
   auto load = [&](Step& s, int k0) {
 #pragma unroll
@@ -495,14 +497,18 @@ __global__ __launch_bounds__(256) void head_few_kernel(const HeadGemm a) {
 #pragma unroll
       for (int y = 0; y < 4; ++y)
         s.w[p][y] = in ? *reinterpret_cast<const bf16x8_t*>(wp[y] + k) : bf16x8_t{};
-      s.h[p] = in ? *reinterpret_cast<const bf16x8_t*>(hp + k) : bf16x8_t{};
+#pragma unroll
+      for (int x = 0; x < MB; ++x)
+        s.h[p][x] = in ? *reinterpret_cast<const bf16x8_t*>(hp[x] + k) : bf16x8_t{};
     }
   };
   auto multiply = [&](const Step& s) {
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int y = 0; y < 4; ++y) acc[y] = mfma_16x16x32<E>(s.w[p][y], s.h[p], acc[y]);
+      for (int x = 0; x < MB; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[x][y] = mfma_16x16x32<E>(s.w[p][y], s.h[p][x], acc[x][y]);
   };
   // the blocks start at different steps: see head_tile
   const int n = (a.K + 4 * kSlice - 1) / (4 * kSlice), first = n > 0 ? (int)(blockIdx.x >> 3) % n : 0;
@@ -519,16 +525,22 @@ __global__ __launch_bounds__(256) void head_few_kernel(const HeadGemm a) {
     multiply(s[1]);
   }
 #pragma unroll
-  for (int y = 0; y < 4; ++y) part[wave][y][lane] = acc[y];
+  for (int x = 0; x < MB; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) part[wave][4 * x + y][lane] = acc[x][y];
   __syncthreads();
-  if (wave) return;
+  f32x4_t sum[4];
 #pragma unroll
-  for (int y = 0; y < 4; ++y)
+  for (int y = 0; y < 4; ++y) {
+    sum[y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (wave < MB)
 #pragma unroll
-    for (int w = 1; w < 4; ++w) acc[y] += part[w][y][lane];
-  // the exponentials' way out lies over this wave's own part
-  static_assert(sizeof(part[0]) >= 16 * T::EPN, "exponentials of 16 rows");
-  logits_epilogue<MODE>(a, acc, 0, jw, lane, reinterpret_cast<char*>(part));
+      for (int w = 0; w < 4; ++w) sum[y] += part[w][4 * wave + y][lane];
+  }
+  __syncthreads();                        // the exponentials' way out lies over the sums
+  if (wave < MB && i0 + 16 * wave < a.M)
+    logits_epilogue<MODE>(a, sum, i0 + 16 * wave, jw, lane,
+                          reinterpret_cast<char*>(part) + wave * 16 * T::EPN);
 }
 
 // out = alpha * sum over the splits
@@ -539,6 +551,7 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const HeadGemm a) {
   for (long long k = blockIdx.x * 256LL + threadIdx.x; k < n; k += 256LL * gridDim.x) {
     const long long i = k / a.N, j = k - i * a.N;
     float s = 0.f;
+#pragma unroll 8
     for (int p = 0; p < a.splits; ++p) s += a.part[((long long)p * a.M + i) * a.ldp + j];
     s *= alpha;
     if constexpr (D == DT_F32) static_cast<float*>(a.out)[i * a.ldo + j] = s;
@@ -560,12 +573,22 @@ bool weight_is_short(int M, int N, int K) {
 
 }  // namespace
 
+// Measured against the 256-tiles, in us (K 1024 / 4096): 16 rows 7.5 / 22 against 20 / 63 (4096
+// columns), 14 / 56 against 21 / 71 (32768), 213 against 184 (128256 x 4096); 64 rows 10.9 / 32 against
+// 20 / 64 (4096), 12 / 42 against 21 / 70 (16384), 21 / 79 against 21 / 72 (32768).
+int head_logits_small(int tokens, int vocab) {
+  const long long cols = (vocab + 63) / 64;
+  if (tokens <= 16) return cols < 4 * kCus ? 1 : 0;
+  return (tokens + 63) / 64 * cols <= kCus * 3 / 2 ? 2 : 0;
+}
+
 // The least of: waves of tiles on 256 CUs times the slices of a tile, and the join of the parts. In
-// units of one slice's time (1.8 us): a tile costs 8 more for its first loads and its results, the
-// join 3 for its launch and 8 bytes a value and split at 4 TB/s.
+// units of one slice's time (1.5 us): a tile costs 4 more for its first loads and its results, the
+// join 3 for its launch, 0.05 a part and 8 bytes a value and part at 4 TB/s. Within 5% of the best of
+// 1 .. 64 parts for 1 .. 2047 tokens of 1000 x 256 .. 128256 x 4096 but for a few of 20 us.
 int head_gemm_splits(int M, int N, int K, bool weight) {
   if (weight && weight_is_short(M, N, K)) return 1;
-  constexpr int kMost = 16, kLeast = 4;
+  constexpr int kMost = 64, kLeast = 2;
   const long long tiles = tiles_of(M, N);
   const int slices = (K + kSlice - 1) / kSlice;
   int best = 1;
@@ -574,7 +597,7 @@ int head_gemm_splits(int M, int N, int K, bool weight) {
     const int per = (slices + s - 1) / s;
     if (s > 1 && (slices + per - 1) / per != s) continue;      // an empty part
     const double waves = (double)((tiles * s + kCus - 1) / kCus);
-    const double cost = waves * (per + 8) + (s > 1 ? 3 + 1.1e-6 * s * M * N : 0.);
+    const double cost = waves * (per + 4) + (s > 1 ? 3 + 0.05 * s + 1.3e-6 * s * M * N : 0.);
     if (s == 1 || cost < least) best = s, least = cost;
   }
   return best;
@@ -598,15 +621,20 @@ hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream) {
   if (a.mode == HG_GRAD ? !a.b_kmajor
                         : a.a_kmajor || a.b_kmajor || !a.stats || (a.mode != HG_STATS && !a.Z))
     return hipErrorInvalidValue;
-  if (a.few && a.mode != HG_GRAD && a.M <= 16 && nb < kCus) {
-    const dim3 few((unsigned)((a.N + 63) / 64));
-#define DMUON_FEW(E, MODE) hipLaunchKernelGGL((head_few_kernel<E, MODE>), few, dim3(256), 0, stream, a)
-    if (a.elt == ELT_F16 && a.mode == HG_STATS) DMUON_FEW(ELT_F16, HG_STATS);
-    else if (a.elt == ELT_F16 && a.mode == HG_LOGITS) DMUON_FEW(ELT_F16, HG_LOGITS);
-    else if (a.elt == ELT_BF16 && a.mode == HG_STATS) DMUON_FEW(ELT_BF16, HG_STATS);
-    else if (a.elt == ELT_BF16 && a.mode == HG_EXP) DMUON_FEW(ELT_BF16, HG_EXP);
+  if (a.small && !grad) {
+    const int mb = a.small == 1 ? 16 : 64;
+    const dim3 sg((unsigned)((a.N + 63) / 64), (unsigned)((a.M + mb - 1) / mb));
+#define DMUON_SMALL(E, MODE)                                                                     \
+  do {                                                                                           \
+    if (mb == 16) hipLaunchKernelGGL((head_small_kernel<E, MODE, 1>), sg, dim3(256), 0, stream, a); \
+    else hipLaunchKernelGGL((head_small_kernel<E, MODE, 4>), sg, dim3(256), 0, stream, a);       \
+  } while (0)
+    if (a.elt == ELT_F16 && a.mode == HG_STATS) DMUON_SMALL(ELT_F16, HG_STATS);
+    else if (a.elt == ELT_F16 && a.mode == HG_LOGITS) DMUON_SMALL(ELT_F16, HG_LOGITS);
+    else if (a.elt == ELT_BF16 && a.mode == HG_STATS) DMUON_SMALL(ELT_BF16, HG_STATS);
+    else if (a.elt == ELT_BF16 && a.mode == HG_EXP) DMUON_SMALL(ELT_BF16, HG_EXP);
     else return hipErrorInvalidValue;
-#undef DMUON_FEW
+#undef DMUON_SMALL
     return hipGetLastError();
   }
   if (a.mode == HG_GRAD && a.a_kmajor && a.splits == 1 && weight_is_short(a.M, a.N, a.K)) {

@@ -49,9 +49,13 @@ struct HeadGemm {
   void* out; long long ldo; int out_dtype;   // HG_GRAD: result (DT_F32 or the operands'), or NULL
   float* part; long long ldp;             // HG_GRAD: fp32 sums [M][ldp], or NULL
   int add_part;                           // part holds earlier sums to add to
-  int few;                                // logits of a call of at most kFewRows rows
+  int few, small;                         // logits: of a call of at most kFewRows rows; its
+                                          // head_logits_small
   int splits;                             // HG_GRAD: K in so many parts, part [splits][M][ldp]
 };
+// Whether a call's logits take the kernel for small ones (1: of at most 16 rows, 2: of more). By the
+// call's sizes, not a chunk's: chunks do not change its bits.
+int head_logits_small(int tokens, int vocab);
 // K splits that fill the chip where a gradient has few tiles (1: none); weight: of the weight.
 int head_gemm_splits(int M, int N, int K, bool weight);
 // Operands at 16-byte alignment with pitches of whole 16-byte chunks. Rows that end inside a chunk

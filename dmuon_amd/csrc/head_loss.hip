@@ -221,7 +221,8 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
     g.elt = elt;
     g.mode = !grads ? HG_STATS : elt == ELT_F16 ? HG_LOGITS : HG_EXP;
     g.splits = 1;
-    g.few = a.tokens <= kFewRows;         // of the call: its chunks do not change the bits
+    g.few = a.tokens <= kFewRows;
+    g.small = head_logits_small((int)a.tokens, (int)a.vocab);
     g.A = Hc; g.lda = ldh;
     g.B = W; g.ldb = ldw;
     g.M = rows; g.N = (int)a.vocab; g.K = (int)a.dim;
