@@ -116,16 +116,17 @@ __device__ __forceinline__ void store8(void* p, int t, long long at, int n, cons
   }
 }
 
-// Sums of `C` values over the threads of a row (blockDim.x of them): shuffles in a wave, then one
-// LDS exchange where the row has several waves. The caller passes another area than in its call
+// Sums of `C` values over the threads of a row (blockDim.x of them, a power of two): shuffles in a
+// wave, then one LDS exchange where the row has several waves. The caller passes another area than in its call
 // before, so that no area is written while it may still be read. The barrier leaves loads in flight.
 template <int C>
 __device__ __forceinline__ void row_sums(float* v, float (*lds)[16][C], int ty) {
+  const int lanes = blockDim.x < 64 ? blockDim.x : 64;
+  for (int o = 1; o < lanes; o <<= 1)
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-    for (int o = 1; o < 64; o <<= 1) v[c] += __shfl_xor(v[c], o);
+    for (int c = 0; c < C; ++c) v[c] += __shfl_xor(v[c], o);
   const int waves = blockDim.x >> 6;
-  if (waves == 1) return;
+  if (waves <= 1) return;
   const int w = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0)
 #pragma unroll
@@ -157,7 +158,8 @@ __device__ __forceinline__ void load_factors(const ResidualNorm& a, long long gr
   }
 }
 
-// NV chunks of 8 columns a thread. MANY: several rows side by side in 256 threads; otherwise the row
+// NV chunks of 8 columns a thread (two in 1024 threads spill registers in the backward pass: rows
+// past 8192 columns take 285 us for 2048 x 16384, a third of the rate of shorter ones). MANY: several rows side by side in 256 threads; otherwise the row
 // is the same for the block and its addresses stay scalar.
 template <int T, int NV, bool MANY>
 __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_kernel(ResidualNorm a) {
@@ -418,12 +420,13 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(ResidualNorm a) {
   else static_cast<uint16_t*>(out)[g * a.dim + oc] = (uint16_t)f_to_half(s, dtype);
 }
 
-// Threads of a row and chunks of 8 columns a thread: two for rows longer than `one`.
+// Threads of a row (8 .. 1024, a power of two) and chunks of 8 columns a thread: two for rows longer
+// than `one`.
 bool row_shape(int dim, int one, int* threads, int* nv) {
   const int chunks = (dim + 7) / 8;
   if (chunks > 2048) return false;
   *nv = dim > one ? 2 : 1;
-  *threads = 64;
+  *threads = 8;
   while (*threads * *nv < chunks) *threads *= 2;
   return true;
 }
