@@ -33,23 +33,33 @@ __device__ __forceinline__ float block_join(float v, float* lds) {
   return r;
 }
 
-// h . w over `dim` values from element-aligned rows, in every lane.
-template <int E>
-__device__ __forceinline__ float wave_dot(const uint16_t* h, const uint16_t* w, int dim, int lane) {
-  float s = 0.f;
-#pragma unroll 4
+// h . w[k] over `dim` values from element-aligned rows, in every lane, for N rows at once.
+template <int E, int N>
+__device__ __forceinline__ void wave_dots(const uint16_t* h, const uint16_t* const (&w)[N], int dim,
+                                          int lane, float (&s)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) s[k] = 0.f;
+#pragma unroll 2
   for (int c = lane * 8; c + 8 <= dim; c += 512) {
     const u32x4_t x = *reinterpret_cast<const u32x4_any_t*>(h + c);
-    const u32x4_t y = *reinterpret_cast<const u32x4_any_t*>(w + c);
+    u32x4_t y[N];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s = __builtin_fmaf(from_elt<E>(x[e] & 0xffff), from_elt<E>(y[e] & 0xffff), s);
-      s = __builtin_fmaf(from_elt<E>(x[e] >> 16), from_elt<E>(y[e] >> 16), s);
-    }
+    for (int k = 0; k < N; ++k) y[k] = *reinterpret_cast<const u32x4_any_t*>(w[k] + c);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[k] = __builtin_fmaf(from_elt<E>(x[e] & 0xffff), from_elt<E>(y[k][e] & 0xffff), s[k]);
+        s[k] = __builtin_fmaf(from_elt<E>(x[e] >> 16), from_elt<E>(y[k][e] >> 16), s[k]);
+      }
   }
   const int c = dim / 8 * 8 + lane;
-  if (c < dim) s = __builtin_fmaf(from_elt<E>(h[c]), from_elt<E>(w[c]), s);
-  return wave_sum(s);
+  if (c < dim)
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] = __builtin_fmaf(from_elt<E>(h[c]), from_elt<E>(w[k][c]), s[k]);
+  for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] += __shfl_xor(s[k], o);
 }
 
 // The entries of a row and their logits. Hard targets: one, with probability 1. A teacher's list:
@@ -70,11 +80,15 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uin
     const long long t = r.targets[row];
     const bool counted = t != r.ignore_index, inside = t >= 0 && t < r.vocab;
     const bool live = counted && inside;
-    const float z = live ? wave_dot<E>(H + row * ldh, W + t * ldw, dim, lane) : 0.f;
+    float z[1] = {0.f};
+    if (live) {
+      const uint16_t* const w[1] = {W + t * ldw};
+      wave_dots<E, 1>(H + row * ldh, w, dim, lane, z);
+    }
     if (lane) return;
     r.ids[row] = live ? (int)t : -1;
     r.probs[row] = live ? 1.f : 0.f;
-    r.logits[row] = z;
+    r.logits[row] = z[0];
     r.mass[row] = !counted ? -1.f : inside ? 1.f : __builtin_nanf("");
     return;
   }
@@ -103,16 +117,29 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uin
   const float norm = r.teacher_lse ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
   if (wave == 0 && lane == 0)
     r.mass[row] = !live ? -1.f : outside ? __builtin_nanf("") : r.teacher_lse ? sum : sum * norm;
-  for (int k = wave; k < r.k_list; k += 4) {
-    const long long id = r.teacher_ids[base + k];
-    const float v = r.teacher_logits[base + k] * it;
-    const bool in = id >= 0 && id < r.vocab;
-    const float q = id < 0 || v == -kInf ? 0.f : expf(v - shift) * norm;
-    const float z = in && q != 0.f ? wave_dot<E>(H + row * ldh, W + id * ldw, dim, lane) * it : 0.f;
+  // four entries a wave at a time: their loads and sums overlap
+  for (int k0 = 4 * wave; k0 < r.k_list; k0 += 16) {
+    const uint16_t* w[4];
+    float q[4], z[4];
+    int cls[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int k = k0 + e < r.k_list ? k0 + e : k0;
+      const long long id = r.teacher_ids[base + k];
+      const float v = r.teacher_logits[base + k] * it;
+      q[e] = id < 0 || v == -kInf ? 0.f : expf(v - shift) * norm;
+      cls[e] = id >= 0 && id < r.vocab && q[e] != 0.f ? (int)id : -1;
+      w[e] = W + (cls[e] < 0 ? 0 : cls[e]) * ldw;         // an entry without a class: any row
+    }
+    wave_dots<E, 4>(H + row * ldh, w, dim, lane, z);
     if (lane) continue;
-    r.ids[base + k] = in && q != 0.f ? (int)id : -1;
-    r.probs[base + k] = q;
-    r.logits[base + k] = z;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (k0 + e >= r.k_list) continue;
+      r.ids[base + k0 + e] = cls[e];
+      r.probs[base + k0 + e] = q[e];
+      r.logits[base + k0 + e] = z[e] * it;
+    }
   }
 }
 
@@ -254,24 +281,34 @@ __global__ __launch_bounds__(256) void head_grad_kernel(HeadRows r, int first, i
 }
 
 // The classes of the teachers' lists, from their fp32 logits: mass p - q cancels where the student
-// is sure. Entries of one class in one row write the same value. One wave a row.
+// is sure. Entries of one class in one row sum their probabilities and write the same value. One wave
+// a row, 64 entries against 64 from lane to lane.
 template <int E>
 __global__ __launch_bounds__(256) void head_entries_kernel(HeadRows r, int first, int rows,
                                                            uint16_t* G) {
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63;
+  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   if (row >= rows) return;
   const long long n = first + row;
   const float w = r.row_weight[n], f = r.factor[n], top = r.top[n];
   if (w == 0.f) return;
   const int* ids = r.ids + n * r.k_list;
   const float* probs = r.probs + n * r.k_list;
-  for (int k = lane; k < r.k_list; k += 64) {
-    const int id = ids[k];
-    if (id < 0) continue;
+  for (int k0 = 0; k0 < r.k_list; k0 += 64) {
+    const int id = k0 + lane < r.k_list ? ids[k0 + lane] : -1;
     float q = 0.f;
-    for (int j = 0; j < r.k_list; ++j)
-      if (ids[j] == id) q += probs[j];
-    const float p = f == 0.f ? 0.f : f * exp2_fast(__builtin_fmaf(r.logits[n * r.k_list + k], kLog2e, -top));
+    for (int j0 = 0; j0 < r.k_list; j0 += 64) {
+      const int jd = j0 + lane < r.k_list ? ids[j0 + lane] : -1;
+      const float jq = j0 + lane < r.k_list ? probs[j0 + lane] : 0.f;
+      const int m = min(64, r.k_list - j0);
+      for (int j = 0; j < m; ++j) {
+        const float p = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(jq), j));
+        q += __builtin_amdgcn_readlane(jd, j) == id ? p : 0.f;
+      }
+    }
+    if (id < 0) continue;
+    const float p = f == 0.f ? 0.f
+        : f * exp2_fast(__builtin_fmaf(r.logits[n * r.k_list + k0 + lane], kLog2e, -top));
     G[((long long)(id >> 6) * rows + row) * 64 + (id & 63)] = to_elt<E>(p - w * q);
   }
 }

@@ -47,13 +47,15 @@ template <int T>
 struct Raw {
   u32x4_t v[T == DT_F32 ? 2 : 1];
 };
-// n (at most 8) values from element `at` on; the rest are 0. ONCE: past the caches
+// 8 values from element `at` on, or, of a row of less, n of them and zeros. (`whole` is the same for
+// all threads: a vector load beside a per-element one in another lane would have to be waited for
+// before the other may write its registers.) ONCE: past the caches
 template <int T, bool ONCE = false>
-__device__ __forceinline__ Raw<T> load_raw(const void* p, long long at, int n) {
+__device__ __forceinline__ Raw<T> load_raw(const void* p, long long at, bool whole, int n) {
   Raw<T> r;
   if constexpr (T == DT_F32) {
     const float* q = static_cast<const float*>(p) + at;
-    if (n >= 8) {
+    if (whole) {
       r.v[0] = ONCE ? __builtin_nontemporal_load((const v32_t*)q) : *(const v32_t*)q;
       r.v[1] = ONCE ? __builtin_nontemporal_load((const v32_t*)(q + 4)) : *(const v32_t*)(q + 4);
     } else {
@@ -62,7 +64,7 @@ __device__ __forceinline__ Raw<T> load_raw(const void* p, long long at, int n) {
     }
   } else {
     const uint16_t* q = static_cast<const uint16_t*>(p) + at;
-    if (n >= 8) {
+    if (whole) {
       r.v[0] = ONCE ? __builtin_nontemporal_load((const v16_t*)q) : *(const v16_t*)q;
     } else {
 #pragma unroll
@@ -80,15 +82,44 @@ __device__ __forceinline__ void unpack(const Raw<T>& r, float* v) {
     else v[i] = half_to_f((i & 1) ? r.v[0][i / 2] >> 16 : r.v[0][i / 2] & 0xffff, T);
   }
 }
-__device__ __forceinline__ void load8(const void* p, int t, long long at, int n, float* v) {
-  if (t == DT_F32) unpack<DT_F32>(load_raw<DT_F32>(p, at, n), v);
-  else if (t == DT_F16) unpack<DT_F16>(load_raw<DT_F16>(p, at, n), v);
-  else unpack<DT_BF16>(load_raw<DT_BF16>(p, at, n), v);
+
+// A thread's chunk of 8 columns of a row. The last chunk of a row that is no multiple of 8 begins
+// earlier, over columns of the one before, and threads past the row's end repeat it: every thread
+// loads a whole vector. The first `lo` columns are not the thread's: they count as zeros and are not
+// stored. Rows of less than 8: n columns, none past the first thread.
+struct Cols {
+  int at, lo, dim;
+  __device__ __forceinline__ void init(int c, int dim_) {
+    dim = dim_;
+    at = dim >= 8 ? min(c, dim - 8) : c;
+    lo = c - at;
+  }
+  __device__ __forceinline__ bool whole() const { return dim >= 8; }
+  __device__ __forceinline__ int n() const { return whole() ? 8 : max(dim - at, 0); }
+};
+template <int T, bool ONCE = false>
+__device__ __forceinline__ Raw<T> load_raw(const void* p, long long row, const Cols& c) {
+  return load_raw<T, ONCE>(p, row + c.at, c.whole(), c.n());
 }
-__device__ __forceinline__ void store8(void* p, int t, long long at, int n, const float* v) {
+__device__ __forceinline__ void load8(const void* p, int t, long long row, const Cols& c, float* v) {
+  if (t == DT_F32) unpack<DT_F32>(load_raw<DT_F32>(p, row, c), v);
+  else if (t == DT_F16) unpack<DT_F16>(load_raw<DT_F16>(p, row, c), v);
+  else unpack<DT_BF16>(load_raw<DT_BF16>(p, row, c), v);
+}
+template <int T>
+__device__ __forceinline__ void unpack(const Raw<T>& r, const Cols& c, float* v) {
+  unpack<T>(r, v);
+  if (c.lo > 0)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < c.lo ? 0.f : v[i];
+}
+__device__ __forceinline__ void store8(void* p, int t, long long row, const Cols& c, const float* v) {
+  const long long at = row + c.at;
+  const int n = c.n();
+  const bool all = c.lo == 0 && c.whole();
   if (t == DT_F32) {
     float* q = static_cast<float*>(p) + at;
-    if (n >= 8) {
+    if (all) {
       u32x4_t a, b;
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[i] = __float_as_uint(v[i]), b[i] = __float_as_uint(v[i + 4]);
@@ -97,11 +128,11 @@ __device__ __forceinline__ void store8(void* p, int t, long long at, int n, cons
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i < n) q[i] = v[i];
+        if (i >= c.lo && i < n) q[i] = v[i];
     }
   } else {
     uint16_t* q = static_cast<uint16_t*>(p) + at;
-    if (n >= 8) {
+    if (all) {
       u32x4_t a;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -111,14 +142,15 @@ __device__ __forceinline__ void store8(void* p, int t, long long at, int n, cons
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i < n) q[i] = (uint16_t)f_to_half(v[i], t);
+        if (i >= c.lo && i < n) q[i] = (uint16_t)f_to_half(v[i], t);
     }
   }
 }
 
-// Sums of `C` values over the threads of a row (blockDim.x of them, a power of two): shuffles in a
-// wave, then one LDS exchange where the row has several waves. The caller passes another area than in its call
-// before, so that no area is written while it may still be read. The barrier leaves loads in flight.
+// Sums of `C` values over the threads of a row (blockDim.x of them: a power of two, or whole waves):
+// shuffles in a wave, then one LDS exchange where the row has several waves. The caller passes another
+// area than in its call before, so that no area is written while it may still be read. The barrier
+// leaves loads in flight.
 template <int C>
 __device__ __forceinline__ void row_sums(float* v, float (*lds)[16][C], int ty) {
   const int lanes = blockDim.x < 64 ? blockDim.x : 64;
@@ -144,15 +176,15 @@ __device__ __forceinline__ void row_sums(float* v, float (*lds)[16][C], int ty) 
 
 // c = gate w_post of this thread's columns for gate row `group`
 template <int NV>
-__device__ __forceinline__ void load_factors(const ResidualNorm& a, long long group, const int* col,
-                                             const int* cnt, float (*c)[8]) {
+__device__ __forceinline__ void load_factors(const ResidualNorm& a, long long group, const Cols* col,
+                                             float (*c)[8]) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     float g[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[v][i] = g[i] = 1.f;
-    if (a.w_post) load8(a.w_post, a.post_dtype, col[v], cnt[v], c[v]);
-    if (a.gate) load8(a.gate, a.gate_dtype, group * a.dim + col[v], cnt[v], g);
+    if (a.w_post) load8(a.w_post, a.post_dtype, 0, col[v], c[v]);
+    if (a.gate) load8(a.gate, a.gate_dtype, group * a.dim, col[v], g);
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[v][i] *= g[i];
   }
@@ -168,25 +200,24 @@ __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_kernel(Residu
   const float inv = 1.f / (float)a.dim;
   const long long first = (long long)blockIdx.x * a.rows_per_block;
   const long long end = first + a.rows_per_block < a.rows ? first + a.rows_per_block : a.rows;
-  int cnt[NV], col[NV];
+  Cols col[NV];
   float pre[NV][8], c[NV][8];
   Raw<T> xr[NV], yr[NV];
   auto fetch = [&](long long row) {
     if (row >= end) row = end - 1;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      xr[v] = load_raw<T>(a.x, row * a.ld_x + col[v], cnt[v]);
-      if (a.y) yr[v] = load_raw<T>(a.y, row * a.ld_y + col[v], cnt[v]);
+      xr[v] = load_raw<T>(a.x, row * a.ld_x, col[v]);
+      if (a.y) yr[v] = load_raw<T>(a.y, row * a.ld_y, col[v]);
     }
   };
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    col[v] = (v * blockDim.x + threadIdx.x) * 8;
-    cnt[v] = a.dim - col[v] > 0 ? a.dim - col[v] : 0;
+    col[v].init((v * blockDim.x + threadIdx.x) * 8, a.dim);
   }
   fetch(first + ty);
 #pragma unroll
-  for (int v = 0; v < NV; ++v) load8(a.w_pre, a.pre_dtype, col[v], cnt[v], pre[v]);
+  for (int v = 0; v < NV; ++v) load8(a.w_pre, a.pre_dtype, 0, col[v], pre[v]);
   int flip = 0;
   long long group = -1;
   for (long long base = first; base < end; base += rows_at_once) {
@@ -195,14 +226,14 @@ __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_kernel(Residu
     float x[NV][8], y[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      unpack<T>(xr[v], x[v]);
-      if (a.y) unpack<T>(yr[v], y[v]);
+      unpack<T>(xr[v], col[v], x[v]);
+      if (a.y) unpack<T>(yr[v], col[v], y[v]);
     }
     fetch(row + rows_at_once);
     const long long g = a.gate ? row / a.rows_per_group : 0;
     if (g != group) {
       group = g;
-      load_factors<NV>(a, g, col, cnt, c);
+      load_factors<NV>(a, g, col, c);
     }
     float r = 1.f;
     if (a.w_post) {
@@ -228,19 +259,19 @@ __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_kernel(Residu
     const float s = 1.f / sqrtf(sq[0] * inv + a.eps);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const long long at = row * a.dim + col[v];
-      if (a.x_new) store8(a.x_new, T, at, cnt[v], x[v]);
+      const long long at = row * a.dim;
+      if (a.x_new) store8(a.x_new, T, at, col[v], x[v]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[v][i] = x[v][i] * s * pre[v][i];
-      store8(a.h, T, at, cnt[v], x[v]);
+      store8(a.h, T, at, col[v], x[v]);
     }
     if (a.stats && threadIdx.x == 0) a.stats[row] = make_float2(r, s);
   }
 }
 
 // The gradients of gate and w_post come from one sum a column and gate group, t = sum d yhat:
-// d_gate = w_post t, d_post = sum over the groups of gate t.
-template <int T, int NV, bool MANY>
+// d_gate = w_post t, d_post = sum over the groups of gate t. GROUPS: a block has several gate groups.
+template <int T, int NV, bool MANY, bool GROUPS>
 __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_grad_kernel(ResidualNorm a) {
   __shared__ float lds[2][4][16][3];
   __shared__ float acc[MANY ? 256 * 8 : 1];
@@ -257,7 +288,7 @@ __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_grad_kernel(R
     first = (long long)blockIdx.x * a.rows_per_block;
     end = first + a.rows_per_block < a.rows ? first + a.rows_per_block : a.rows;
   }
-  int cnt[NV], col[NV];
+  Cols col[NV];
   float pre[NV][8], c[NV][8], d_pre[NV][8], d_post[NV][8], t[NV][8];
   Raw<T> xr[NV], yr[NV], er[NV], gr[NV];
   float2 rs;
@@ -265,23 +296,22 @@ __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_grad_kernel(R
     if (row >= end) row = end - 1;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      xr[v] = load_raw<T, true>(a.x, row * a.ld_x + col[v], cnt[v]);
-      if (a.y) yr[v] = load_raw<T, true>(a.y, row * a.ld_y + col[v], cnt[v]);
-      if (a.dx_new) er[v] = load_raw<T, true>(a.dx_new, row * a.ld_dx_new + col[v], cnt[v]);
-      if (a.dh) gr[v] = load_raw<T, true>(a.dh, row * a.ld_dh + col[v], cnt[v]);
+      xr[v] = load_raw<T, true>(a.x, row * a.ld_x, col[v]);
+      if (a.y) yr[v] = load_raw<T, true>(a.y, row * a.ld_y, col[v]);
+      if (a.dx_new) er[v] = load_raw<T, true>(a.dx_new, row * a.ld_dx_new, col[v]);
+      if (a.dh) gr[v] = load_raw<T, true>(a.dh, row * a.ld_dh, col[v]);
     }
     rs = a.stats[row];
   };
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    col[v] = (v * blockDim.x + threadIdx.x) * 8;
-    cnt[v] = a.dim - col[v] > 0 ? a.dim - col[v] : 0;
+    col[v].init((v * blockDim.x + threadIdx.x) * 8, a.dim);
 #pragma unroll
     for (int i = 0; i < 8; ++i) d_pre[v][i] = d_post[v][i] = t[v][i] = 0.f;
   }
   fetch(first + ty);
 #pragma unroll
-  for (int v = 0; v < NV; ++v) load8(a.w_pre, a.pre_dtype, col[v], cnt[v], pre[v]);
+  for (int v = 0; v < NV; ++v) load8(a.w_pre, a.pre_dtype, 0, col[v], pre[v]);
   // a gate group's end in this block: its shares of the gradients, into `out` row `at`
   auto flush = [&](long long group, void* out, int dtype, long long at) {
 #pragma unroll
@@ -289,17 +319,17 @@ __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_grad_kernel(R
       float w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = 1.f;
-      if (a.gate) load8(a.gate, a.gate_dtype, group * a.dim + col[v], cnt[v], w);
+      if (a.gate) load8(a.gate, a.gate_dtype, group * a.dim, col[v], w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         d_post[v][i] += w[i] * t[v][i];
         w[i] = 1.f;
       }
       if (out) {
-        if (a.w_post) load8(a.w_post, a.post_dtype, col[v], cnt[v], w);
+        if (a.w_post) load8(a.w_post, a.post_dtype, 0, col[v], w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] *= t[v][i];
-        store8(out, dtype, at * a.dim + col[v], cnt[v], w);
+        store8(out, dtype, at * a.dim, col[v], w);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) t[v][i] = 0.f;
@@ -313,19 +343,19 @@ __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_grad_kernel(R
     const long long row = live ? base + ty : end - 1;
     const long long q = a.gate ? row / a.rows_per_group : 0;
     if (q != group) {
-      if (!MANY && group >= 0) flush(group, a.d_gate, a.gate_dtype, group);
+      if (GROUPS && group >= 0) flush(group, a.d_gate, a.gate_dtype, group);
       group = q;
-      load_factors<NV>(a, q, col, cnt, c);
+      load_factors<NV>(a, q, col, c);
     }
     float x[NV][8], y[NV][8], e[NV][8], g[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      unpack<T>(xr[v], x[v]);
+      unpack<T>(xr[v], col[v], x[v]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[v][i] = e[v][i] = g[v][i] = 0.f;
-      if (a.y) unpack<T>(yr[v], y[v]);
-      if (a.dx_new) unpack<T>(er[v], e[v]);
-      if (a.dh) unpack<T>(gr[v], g[v]);
+      if (a.y) unpack<T>(yr[v], col[v], y[v]);
+      if (a.dx_new) unpack<T>(er[v], col[v], e[v]);
+      if (a.dh) unpack<T>(gr[v], col[v], g[v]);
     }
     const float r = rs.x, s = rs.y;
     fetch(row + rows_at_once);
@@ -352,7 +382,7 @@ __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_grad_kernel(R
     const float kb = a.w_post ? (sums[1] - ka * sums[2]) * inv : 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const long long at = row * a.dim + col[v];
+      const long long at = row * a.dim;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float d = e[v][i] - ka * x[v][i];
@@ -360,8 +390,8 @@ __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_grad_kernel(R
         x[v][i] = a.scale * d;
         y[v][i] = r * (c[v][i] * d - y[v][i] * kb);
       }
-      if (a.dx) store8(a.dx, T, at, cnt[v], x[v]);
-      if (a.dy) store8(a.dy, T, at, cnt[v], y[v]);
+      if (a.dx) store8(a.dx, T, at, col[v], x[v]);
+      if (a.dy) store8(a.dy, T, at, col[v], y[v]);
     }
   }
   // rows side by side join through LDS in their order, into row 0's threads
@@ -385,9 +415,9 @@ __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_grad_kernel(R
   else flush(group, a.d_gate, a.gate_dtype, group);
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const long long at = (long long)blockIdx.x * a.dim + col[v];
-    if (a.d_pre) store8(a.pre_part, DT_F32, at, cnt[v], d_pre[v]);
-    if (a.d_post) store8(a.post_part, DT_F32, at, cnt[v], d_post[v]);
+    const long long at = (long long)blockIdx.x * a.dim;
+    if (a.d_pre) store8(a.pre_part, DT_F32, at, col[v], d_pre[v]);
+    if (a.d_post) store8(a.post_part, DT_F32, at, col[v], d_post[v]);
   }
 }
 
@@ -420,14 +450,15 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(ResidualNorm a) {
   else static_cast<uint16_t*>(out)[g * a.dim + oc] = (uint16_t)f_to_half(s, dtype);
 }
 
-// Threads of a row (8 .. 1024, a power of two) and chunks of 8 columns a thread: two for rows longer
-// than `one`.
+// Threads of a row (a power of two up to 128, then whole waves up to 1024) and chunks of 8 columns a
+// thread: two for rows longer than `one`.
 bool row_shape(int dim, int one, int* threads, int* nv) {
   const int chunks = (dim + 7) / 8;
   if (chunks > 2048) return false;
   *nv = dim > one ? 2 : 1;
   *threads = 8;
-  while (*threads * *nv < chunks) *threads *= 2;
+  while (*threads * *nv < chunks && *threads < 128) *threads *= 2;
+  if (*threads * *nv < chunks) *threads = ((chunks + *nv - 1) / *nv + 63) / 64 * 64;
   return true;
 }
 
@@ -446,7 +477,7 @@ void residual_norm_split(ResidualNorm* a) {
   const long long per = a->rows_per_group;
   // as many blocks as their registers let run at once: 16 waves a CU, or three blocks of 256 threads
   // (four took 196 us where three take 176: 65536 x 1024)
-  auto want = [&](int lanes) { return lanes > 1 ? kCus * 3 : kCus * 1024 / threads; };
+  auto want = [&](int lanes) { return lanes > 1 ? kCus * 3 : kCus * (1024 / threads); };
   a->lanes = threads < 256 ? 256 / threads : 1;
   if (a->rows <= 0) {
     a->parts = 0;                         // the gate's gradient is a sum of none
@@ -502,14 +533,16 @@ hipError_t launch_residual_norm_grad(const ResidualNorm& a, hipStream_t stream) 
   if (!row_shape(a.dim, kOneBackward, &threads, &nv) || a.blocks > 0x7fffffffLL) return hipErrorInvalidValue;
   if (a.blocks > 0) {
     const dim3 grid((unsigned)a.blocks), block(threads, a.lanes);
-#define DMUON_RN(T, NV, MANY) \
-  hipLaunchKernelGGL((residual_norm_grad_kernel<T, NV, MANY>), grid, block, 0, stream, a)
+#define DMUON_RN(T, NV, MANY, GROUPS) \
+  hipLaunchKernelGGL((residual_norm_grad_kernel<T, NV, MANY, GROUPS>), grid, block, 0, stream, a)
 #define DMUON_RN_T(T)                                  \
   do {                                                 \
-    if (nv == 2) DMUON_RN(T, 2, false);                \
-    else if (a.lanes > 1) DMUON_RN(T, 1, true);        \
-    else DMUON_RN(T, 1, false);                        \
+    if (nv == 2) DMUON_RN(T, 2, false, true);          \
+    else if (a.lanes > 1) DMUON_RN(T, 1, true, false); \
+    else if (several) DMUON_RN(T, 1, false, true);     \
+    else DMUON_RN(T, 1, false, false);                 \
   } while (0)
+    const bool several = a.rows_per_block > a.rows_per_group;
     if (a.dtype == DT_F32) DMUON_RN_T(DT_F32);
     else if (a.dtype == DT_F16) DMUON_RN_T(DT_F16);
     else DMUON_RN_T(DT_BF16);
