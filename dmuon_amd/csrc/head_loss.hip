@@ -6,7 +6,7 @@
 //
 // Between the first product and the others a logit takes two bytes where the operands are bf16:
 // exp(z - m) in fp16, m the maximum of the row's 64 columns, which the row kernel turns into the
-// bf16 gradient in place. Its 2^-12 is small against the 2^-9 of the gradient's own rounding. For
+// bf16 gradient in place. Its 2^-11 is small against the 2^-8 of the gradient's own rounding. For
 // fp16 operands it is not: there the product writes fp32 logits and the gradient has its own place,
 // six bytes a logit.
 #include "../../include/dmuon_amd.h"

@@ -68,6 +68,8 @@ __device__ __forceinline__ void wave_dots(const uint16_t* h, const uint16_t* con
 // the row's mass NaN, so its loss and gradients show it. The entries' logits are formed here, in
 // fp32 from the rows themselves: the products' epilogue would have to search every row's list in
 // each of its tiles. Hard targets take one wave a row, lists four.
+// Memory bound by the gathered rows of W: 4096 rows of 64 entries x 4096 columns (2.1 GB, classes of
+// several rows from the caches) 258 us.
 template <int E>
 __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uint16_t* H,
                                                            long long ldh, const uint16_t* W,
@@ -174,7 +176,8 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 }
 
 // log-sum-exp, loss, row weight and factor of `side` rows a block (a power of two, at most 16): 1024
-// threads, thread t for row t % side, every 1024 / side-th statistic and entry.
+// threads, thread t for row t % side, every 1024 / side-th statistic and entry. 8192 rows of 2004 statistics
+// (131 MB) 30 us, 4.4 TB/s; a few rows cost their chain of dependent steps, 5 to 9 us.
 __global__ __launch_bounds__(1024) void head_lse_kernel(HeadRows r, int first, int rows,
                                                         const float2* __restrict__ stats, int side,
                                                         bool grads) {
@@ -233,8 +236,10 @@ __global__ __launch_bounds__(1024) void head_lse_kernel(HeadRows r, int first, i
 // The logit gradient: factor * 2^(z - top) - row_weight * q, in place of the exponentials (whose share
 // 2^(m - top) is one of a block's row) or from the logits (LOGITS). Crosses memory once, 2 + 2 bytes
 // a logit or 4 + 2: 4 x 32 rows of one block of 64 classes a workgroup, 16 bytes a thread and step.
-// A hard target's own class comes from its fp32 logit: softmax - 1 cancels where the student is sure. (So the
-// row's maximum and 1 / sum go in apart: their log-sum-exp would lose what 1 - p is made of.)
+// A hard target's own class comes from its fp32 logit: softmax - 1 cancels where the student is
+// sure. (So the row's maximum and 1 / sum go in apart: their log-sum-exp would lose what 1 - p is
+// made of.)
+// Memory bound: 8192 x 128256 in place (4.2 GB) 737 us, 5.7 TB/s.
 template <int E, bool LOGITS>
 __global__ __launch_bounds__(256) void head_grad_kernel(HeadRows r, int first, int rows,
                                                         const float2* __restrict__ stats,
@@ -282,7 +287,7 @@ __global__ __launch_bounds__(256) void head_grad_kernel(HeadRows r, int first, i
 
 // The classes of the teachers' lists, from their fp32 logits: mass p - q cancels where the student
 // is sure. Entries of one class in one row sum their probabilities and write the same value. One wave
-// a row, 64 entries against 64 from lane to lane.
+// a row, 64 entries against 64 from lane to lane: 4096 rows of 64 entries 16 us.
 template <int E>
 __global__ __launch_bounds__(256) void head_entries_kernel(HeadRows r, int first, int rows,
                                                            uint16_t* G) {
@@ -330,7 +335,8 @@ __global__ __launch_bounds__(1024) void head_reduce_kernel(HeadRows r) {
   }
 }
 
-// dst = factor * src for two dense arrays, 8 values a thread and step.
+// dst = factor * src for two dense arrays, 8 values a thread and step. Memory bound: 50001 x 1528 and
+// 1023 x 1528 values from fp32 to fp16 (468 MB) 98 us, 4.8 TB/s; in place at factor 1 2 to 5 us.
 template <int S, int D>
 __global__ __launch_bounds__(256) void scale_by_kernel(ScaleBy a) {
   typedef f32x4_t f32x4_any_t __attribute__((aligned(4)));
