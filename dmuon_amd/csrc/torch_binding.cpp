@@ -74,6 +74,13 @@ struct Loss : torch::CustomClassHolder {
   at::ScalarType held = at::kFloat;       // the type the gradients are formed in
   Tensor d_hidden, d_weight;              // until the first backward pass takes them
 
+  void against(const Tensor& t, const Tensor& i, const Tensor& l, const Tensor& e) {
+    targets = t;
+    ids = i;
+    logits = l;
+    lse = e;
+  }
+
   // The loss of each token or reduced; the gradients into d_hidden and d_weight.
   Tensor launch(const Tensor& hidden, const Tensor& weight, bool grads, const Tensor& row_grad) {
     const c10::DeviceGuard guard(hidden.device());
@@ -134,9 +141,12 @@ using LossPtr = c10::intrusive_ptr<Loss>;
 struct HeadLoss : torch::autograd::Function<HeadLoss> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
                         const LossPtr& s) {
+    const Tensor loss = s->launch(hidden, weight, s->reduction != DMUON_LOSS_ROWS, Tensor());
     ctx->saved_data["call"] = c10::IValue::make_capsule(s);
-    ctx->save_for_backward({hidden, weight});
-    return s->launch(hidden, weight, s->reduction != DMUON_LOSS_ROWS, Tensor());
+    // the targets too: a pass that forms the logits anew must not see others than the loss did
+    ctx->save_for_backward({hidden, weight, s->targets, s->ids, s->logits, s->lse});
+    s->against({}, {}, {}, {});
+    return loss;
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -144,6 +154,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
         c10::static_intrusive_pointer_cast<Loss>(ctx->saved_data["call"].toCapsule());
     once(s->who);
     const auto saved = ctx->get_saved_variables();
+    s->against(saved[2], saved[3], saved[4], saved[5]);
     if (s->reduction == DMUON_LOSS_ROWS) {
       s->launch(saved[0], saved[1], true, grads[0].to(at::kFloat).contiguous());
     } else {
@@ -151,6 +162,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
       if (!s->d_hidden.defined() && !s->d_weight.defined()) s->launch(saved[0], saved[1], true, Tensor());
       s->scale(grads[0], saved[0].scalar_type());
     }
+    s->against({}, {}, {}, {});
     Tensor dh = std::move(s->d_hidden), dw = std::move(s->d_weight);
     s->d_hidden = Tensor();
     s->d_weight = Tensor();

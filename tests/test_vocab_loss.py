@@ -347,6 +347,24 @@ def test_incoming_gradients_and_retained_graphs(gpu, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("what", ["target", "ids", "logits", "lse", "hidden", "weight"])
+def test_operands_that_change_before_the_gradient(gpu, what):
+    """A gradient that forms the logits anew refuses operands that were written to meanwhile."""
+    h, w, t, gen = _inputs(gpu, 20, 300, 64, torch.bfloat16, seed=10)
+    a, b = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    ids = t[:, None].clone()
+    logits, lse = torch.randn(20, 1, device=gpu, generator=gen), torch.full((20,), 3.0, device=gpu)
+    if what == "target":
+        loss = dmuon.linear_cross_entropy(a, b, t, reduction="none")
+    else:
+        loss = dmuon.linear_distillation(a, b, ids, logits, teacher_lse=lse, reduction="none")
+    with torch.no_grad():
+        dict(target=t, ids=ids, logits=logits, lse=lse, hidden=a, weight=b)[what].zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences(gpu):
     """Directional derivative of the mean loss by central differences of the exact losses."""
     h, w, t, gen = _inputs(gpu, 33, 190, 48, torch.bfloat16, seed=9)
