@@ -92,11 +92,12 @@ hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long l
                                hipStream_t stream);
 // Top, loss, row weight and factor of rows first .. first + rows - 1 from their statistics, and with G
 // their logit gradients row_weight (mass softmax - target probability), 0 past the vocabulary's end:
-// in place of the exponentials (Z == G), or from the fp32 logits Z.
+// in place of the exponentials (Z == G), or from the fp32 logits Z. Unless reduction is
+// DMUON_LOSS_ROWS, mean[0] = sum of the losses, divided by the number of counted rows for
+// DMUON_LOSS_MEAN, and alpha: with the last rows, with G after every chunk (mean is right after the
+// last; alpha, which the gradient's products take, after each).
 hipError_t launch_head_rows(const HeadRows& r, int first, int rows, const float2* stats,
                             const void* Z, uint16_t* G, int elt, hipStream_t stream);
-// mean[0] = sum of the losses, divided by the number of counted rows for DMUON_LOSS_MEAN, and alpha.
-hipError_t launch_head_reduce(const HeadRows& r, hipStream_t stream);
 
 // dst[k] = factor[0] * src[k] for n[k] values, k = 0 and 1; in_place: every dst is its src, and
 // nothing moves where the factor is 1.

@@ -232,8 +232,6 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
     if (check_launch(launch_head_gemm(g, stream), who)) return 1;
     if (check_launch(launch_head_rows(r, (int)first, rows, stats, Z, grads ? G : nullptr, elt, stream),
                      who)) return 1;
-    // before the gradients' products: they take its alpha. The last chunk's is the whole loss.
-    if (a.reduction != DMUON_LOSS_ROWS && check_launch(launch_head_reduce(r, stream), who)) return 1;
     if (grads) {
       g = HeadGemm{};
       g.elt = elt;

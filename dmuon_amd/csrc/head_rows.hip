@@ -233,18 +233,47 @@ __global__ __launch_bounds__(1024) void head_lse_kernel(HeadRows r, int first, i
   }
 }
 
+// The reduced loss and alpha of its gradient, by a block of 256 threads: four strands of rows each,
+// so that their loads are in flight together.
+__device__ __forceinline__ void reduce_losses(const HeadRows& r, float* lds) {
+  float sum[4] = {}, count[4] = {};       // the count is exact: at most 2^24 rows
+  for (int n = threadIdx.x; n < r.n; n += 1024)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool in = n + 256 * k < r.n;
+      const int m = in ? n + 256 * k : n;
+      const float loss = r.loss[m], mass = r.mass[m];
+      sum[k] += in ? loss : 0.f;
+      count[k] += in && !(mass < 0.f) ? 1.f : 0.f;
+    }
+  const float total = block_join<false>((sum[0] + sum[1]) + (sum[2] + sum[3]), lds);
+  const float rows = block_join<false>((count[0] + count[1]) + (count[2] + count[3]), lds);
+  if (threadIdx.x == 0) {
+    const float g = r.reduction == DMUON_LOSS_MEAN ? 1.f / fmaxf(rows, 1.f) : 1.f;
+    r.mean[0] = r.reduction == DMUON_LOSS_MEAN ? total / fmaxf(rows, 1.f) : total;
+    r.alpha[0] = g * r.temperature / kUnit;
+  }
+}
+
 // The logit gradient: factor * 2^(z - top) - row_weight * q, in place of the exponentials (whose share
 // 2^(m - top) is one of a block's row) or from the logits (LOGITS). Crosses memory once, 2 + 2 bytes
 // a logit or 4 + 2: 4 x 32 rows of one block of 64 classes a workgroup, 16 bytes a thread and step.
 // A hard target's own class comes from its fp32 logit: softmax - 1 cancels where the student is
 // sure. (So the row's maximum and 1 / sum go in apart: their log-sum-exp would lose what 1 - p is
 // made of.)
+// Blocks past the rows' are the reduction's, which the products after this kernel wait for and nothing
+// in it: a launch of its own cost small calls 4 us.
 // Memory bound: 8192 x 128256 in place (4.2 GB) 737 us, 5.7 TB/s.
 template <int E, bool LOGITS>
 __global__ __launch_bounds__(256) void head_grad_kernel(HeadRows r, int first, int rows,
                                                         const float2* __restrict__ stats,
                                                         const float* __restrict__ Z, uint16_t* G) {
+  __shared__ float lds[16];
   const int tile = blockIdx.y, c = threadIdx.x & 7;
+  if ((int)blockIdx.x * 128 >= rows) {
+    if (tile == 0) reduce_losses(r, lds);
+    return;
+  }
   const int row0 = blockIdx.x * 128 + (threadIdx.x >> 3);
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
@@ -318,21 +347,10 @@ __global__ __launch_bounds__(256) void head_entries_kernel(HeadRows r, int first
   }
 }
 
-// The reduced loss, and alpha of its gradient.
-__global__ __launch_bounds__(1024) void head_reduce_kernel(HeadRows r) {
+// The reduced loss alone, of calls without gradients.
+__global__ __launch_bounds__(256) void head_reduce_kernel(HeadRows r) {
   __shared__ float lds[16];
-  float sum = 0.f, count = 0.f;           // the count is exact: at most 2^24 rows
-  for (int n = threadIdx.x; n < r.n; n += 1024) {
-    sum += r.loss[n];
-    count += r.mass[n] < 0.f ? 0.f : 1.f;
-  }
-  sum = block_join<false>(sum, lds);
-  count = block_join<false>(count, lds);
-  if (threadIdx.x == 0) {
-    const float g = r.reduction == DMUON_LOSS_MEAN ? 1.f / fmaxf(count, 1.f) : 1.f;
-    r.mean[0] = r.reduction == DMUON_LOSS_MEAN ? sum / fmaxf(count, 1.f) : sum;
-    r.alpha[0] = g * r.temperature / kUnit;
-  }
+  reduce_losses(r, lds);
 }
 
 // dst = factor * src for two dense arrays, 8 values a thread and step. Memory bound: 50001 x 1528 and
@@ -415,17 +433,24 @@ hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long l
   return hipGetLastError();
 }
 
+static hipError_t reduce(const HeadRows& r, hipStream_t stream) {
+  if (r.reduction != DMUON_LOSS_ROWS)
+    hipLaunchKernelGGL(head_reduce_kernel, dim3(1), dim3(256), 0, stream, r);
+  return hipGetLastError();
+}
+
 hipError_t launch_head_rows(const HeadRows& r, int first, int rows, const float2* stats,
                             const void* Z, uint16_t* G, int elt, hipStream_t stream) {
-  if (rows <= 0) return hipSuccess;
+  if (rows <= 0) return reduce(r, stream);
   const int tiles = (r.vocab + kStatCols - 1) / kStatCols;
   // neighbouring rows share the lines of a statistic; few rows take more threads each
   const int side = rows >= 1024 ? 16 : rows >= 128 ? 4 : 1;
   hipLaunchKernelGGL(head_lse_kernel, dim3((unsigned)((rows + side - 1) / side)), dim3(1024), 0,
                      stream, r, first, rows, stats, side, G != nullptr);
-  if (!G) return hipGetLastError();
+  if (!G) return first + rows < r.n ? hipGetLastError() : reduce(r, stream);
   if (tiles > 65535 || (Z == G) != (elt == ELT_BF16)) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)((rows + 127) / 128), (unsigned)tiles), lists((unsigned)((rows + 3) / 4));
+  const dim3 grid((unsigned)((rows + 127) / 128 + (r.reduction != DMUON_LOSS_ROWS)), (unsigned)tiles);
+  const dim3 lists((unsigned)((rows + 3) / 4));
   const float* logits = static_cast<const float*>(Z);
   if (elt == ELT_F16) {
     hipLaunchKernelGGL((head_grad_kernel<ELT_F16, true>), grid, dim3(256), 0, stream, r, first, rows,
@@ -438,11 +463,6 @@ hipError_t launch_head_rows(const HeadRows& r, int first, int rows, const float2
     if (!r.targets)
       hipLaunchKernelGGL(head_entries_kernel<ELT_BF16>, lists, dim3(256), 0, stream, r, first, rows, G);
   }
-  return hipGetLastError();
-}
-
-hipError_t launch_head_reduce(const HeadRows& r, hipStream_t stream) {
-  hipLaunchKernelGGL(head_reduce_kernel, dim3(1), dim3(1024), 0, stream, r);
   return hipGetLastError();
 }
 
