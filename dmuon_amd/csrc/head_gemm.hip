@@ -418,13 +418,32 @@ void head_gemm_kernel(const HeadGemm a) {
   else head_tile<E, MODE, FA, FB, false>(a, smem, bi, bj, sp);
 }
 
+// out = alpha * sum over the splits, by block `block` of `blocks`. Memory bound: two parts of 2047 x
+// 2048 values (42 MB with the result, largely from the caches) 17 us.
+__device__ __forceinline__ void join_splits(const HeadGemm& a, int block, int blocks) {
+  const long long n = (long long)a.M * a.N;
+  const float alpha = a.alpha[0];
+  for (long long k = block * 256LL + threadIdx.x; k < n; k += 256LL * blocks) {
+    const long long i = k / a.N, j = k - i * a.N, at = i * a.ldo + j;
+    float s = 0.f;
+#pragma unroll 8
+    for (int p = 0; p < a.splits; ++p) s += a.part[((long long)p * a.M + i) * a.ldp + j];
+    s *= alpha;
+    if (a.out_dtype == DT_F32) static_cast<float*>(a.out)[at] = s;
+    else static_cast<uint16_t*>(a.out)[at] = a.out_dtype == DT_F16 ? to_elt<ELT_F16>(s)
+                                                                   : to_elt<ELT_BF16>(s);
+  }
+}
+
 // A weight gradient over few tokens: bound by writing it. 128 x 128 tiles, four waves of 64 x 64, one
 // K slice in LDS at a time; four blocks a CU hide each other's waits, where a 256-tile of a slice or
 // two waits alone for its first loads and its stores (see weight_is_short). 64 tokens x 128256 x
-// 4096: 226 us, 4.7 TB/s.
+// 4096: 226 us, 4.7 TB/s. The first `joins` blocks (whole eights, so that the others stay on their
+// XCDs) join the hidden gradient's parts, `h`.
 template <int E>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 4)))
-void head_short_kernel(const HeadGemm a) {
+void head_short_kernel(const HeadGemm a, const HeadGemm h, int joins) {
+  if ((int)blockIdx.x < joins) return join_splits(h, blockIdx.x, joins);
   constexpr int kSide = 128, kBlock = kSlice * 128;    // LDS bytes of 64 values of a slice
   constexpr int kSlab = 32 * T::EPN;
   static_assert(4 * kSlab <= 4 * kBlock, "results pass through the slices' place");
@@ -432,7 +451,7 @@ void head_short_kernel(const HeadGemm a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int mt = (a.M + kSide - 1) / kSide, nt = (a.N + kSide - 1) / kSide;
-  const int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int t = xcd_remap(blockIdx.x - joins, gridDim.x - joins);
   const int g = t / (8 * nt), rows = min(mt - 8 * g, 8), r = t - g * 8 * nt;
   const int i0 = __builtin_amdgcn_readfirstlane((8 * g + r % rows) * kSide);
   const int j0 = __builtin_amdgcn_readfirstlane(r / rows * kSide);
@@ -555,21 +574,8 @@ __global__ __launch_bounds__(256) void head_small_kernel(const HeadGemm a) {
                           reinterpret_cast<char*>(part) + wave * 16 * T::EPN);
 }
 
-// out = alpha * sum over the splits. Memory bound: two parts of 2047 x 2048 values (42 MB with the
-// result, largely from the caches) 17 us.
-template <int D>
 __global__ __launch_bounds__(256) void join_splits_kernel(const HeadGemm a) {
-  const long long n = (long long)a.M * a.N;
-  const float alpha = a.alpha[0];
-  for (long long k = blockIdx.x * 256LL + threadIdx.x; k < n; k += 256LL * gridDim.x) {
-    const long long i = k / a.N, j = k - i * a.N;
-    float s = 0.f;
-#pragma unroll 8
-    for (int p = 0; p < a.splits; ++p) s += a.part[((long long)p * a.M + i) * a.ldp + j];
-    s *= alpha;
-    if constexpr (D == DT_F32) static_cast<float*>(a.out)[i * a.ldo + j] = s;
-    else static_cast<uint16_t*>(a.out)[i * a.ldo + j] = to_elt<D == DT_F16 ? ELT_F16 : ELT_BF16>(s);
-  }
+  join_splits(a, blockIdx.x, gridDim.x);
 }
 
 long long tiles_of(int M, int N) {
@@ -584,7 +590,16 @@ bool weight_is_short(int M, int N, int K) {
   return K <= 192 || (K <= 512 && tiles_of(M, N) <= 4 * kCus);
 }
 
+unsigned join_blocks(const HeadGemm& a) {
+  const long long n = ((long long)a.M * a.N + 255) / 256;
+  return n < 4096 ? (unsigned)((n + 7) / 8 * 8) : 4096u;
+}
+
 }  // namespace
+
+bool head_joins_later(const HeadGemm& h, int vocab) {
+  return h.splits > 1 && weight_is_short(vocab, h.N, h.M);
+}
 
 // Measured against the 256-tiles, in us (K 1024 / 4096): 16 rows 7.5 / 22 against 20 / 63 (4096
 // columns), 14 / 56 against 21 / 71 (32768), 213 against 184 (128256 x 4096); 64 rows 10.9 / 32 against
@@ -652,12 +667,17 @@ hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream) {
   }
   if (a.mode == HG_GRAD && a.a_kmajor && a.splits == 1 && weight_is_short(a.M, a.N, a.K)) {
     const long long tiles = ((long long)a.M + 127) / 128 * ((a.N + 127) / 128);
-    if (tiles > 0x7fffffffLL) return hipErrorInvalidValue;
-    const dim3 tg((unsigned)tiles);
-    if (a.elt == ELT_F16) hipLaunchKernelGGL(head_short_kernel<ELT_F16>, tg, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(head_short_kernel<ELT_BF16>, tg, dim3(256), 0, stream, a);
+    const unsigned joins = a.join ? join_blocks(*a.join) : 0;
+    if (tiles > 0x7fffffffLL - joins) return hipErrorInvalidValue;
+    const HeadGemm& h = a.join ? *a.join : a;
+    const dim3 tg((unsigned)tiles + joins);
+    if (a.elt == ELT_F16)
+      hipLaunchKernelGGL(head_short_kernel<ELT_F16>, tg, dim3(256), 0, stream, a, h, (int)joins);
+    else
+      hipLaunchKernelGGL(head_short_kernel<ELT_BF16>, tg, dim3(256), 0, stream, a, h, (int)joins);
     return hipGetLastError();
   }
+  if (a.join) return hipErrorInvalidValue;
   const dim3 grid((unsigned)nb);
 #define DMUON_HG(E, MODE, FA, FB) \
   hipLaunchKernelGGL((head_gemm_kernel<E, MODE, FA, FB>), grid, dim3(512), 0, stream, a)
@@ -674,13 +694,8 @@ hipError_t launch_head_gemm(const HeadGemm& a, hipStream_t stream) {
   else DMUON_HG_E(ELT_BF16);
 #undef DMUON_HG_E
 #undef DMUON_HG
-  if (a.splits > 1) {
-    const long long n = ((long long)a.M * a.N + 255) / 256;
-    const dim3 jg((unsigned)(n < 4096 ? n : 4096));
-    if (a.out_dtype == DT_F32) hipLaunchKernelGGL(join_splits_kernel<DT_F32>, jg, dim3(256), 0, stream, a);
-    else if (a.out_dtype == DT_F16) hipLaunchKernelGGL(join_splits_kernel<DT_F16>, jg, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(join_splits_kernel<DT_BF16>, jg, dim3(256), 0, stream, a);
-  }
+  if (a.splits > 1 && !a.join_later)
+    hipLaunchKernelGGL(join_splits_kernel, dim3(join_blocks(a)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 

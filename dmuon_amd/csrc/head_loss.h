@@ -52,7 +52,13 @@ struct HeadGemm {
   int few, small;                         // logits: of a call of at most kFewRows rows; its
                                           // head_logits_small
   int splits;                             // HG_GRAD: K in so many parts, part [splits][M][ldp]
+  int join_later;                         // a hidden gradient whose parts a weight gradient's launch,
+  const HeadGemm* join;                   // with it in `join`, makes the result (see head_joins_later)
 };
+// Whether the parts of hidden gradient h (its sizes and splits) join in the launch of the weight
+// gradient of `vocab` classes: one of few tokens, whose kernel takes them beside its tiles. A launch of
+// their own costs a small call's step 4 us more.
+bool head_joins_later(const HeadGemm& h, int vocab);
 // Whether a call's logits take the kernel for small ones (1: of at most 16 rows, 2: of more). By the
 // call's sizes, not a chunk's: chunks do not change its bits.
 int head_logits_small(int tokens, int vocab);

@@ -245,9 +245,13 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
         g.splits = split_h ? head_gemm_splits(rows, g.N, g.K, false) : 1;
         g.part = floats(l.part); g.ldp = a.dim;
         g.out = static_cast<char*>(a.d_hidden) + first * a.dim * grad_size; g.ldo = a.dim;
+        g.join_later = a.d_weight && head_joins_later(g, (int)a.vocab);
         if (check_launch(launch_head_gemm(g, stream), who)) return 1;
       }
       if (a.d_weight) {
+        const HeadGemm h = g;
+        g.join_later = 0;
+        g.join = h.join_later ? &h : nullptr;
         const bool last = first + rows >= a.tokens;
         g.A = G; g.lda = rows; g.a_kmajor = 1;
         g.B = Hc; g.ldb = ldh; g.b_kmajor = 1;
