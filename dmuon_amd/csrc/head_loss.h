@@ -105,6 +105,22 @@ hipError_t launch_head_targets(const HeadRows& r, const uint16_t* H, long long l
 hipError_t launch_head_rows(const HeadRows& r, int first, int rows, const float2* stats,
                             const void* Z, uint16_t* G, int elt, hipStream_t stream);
 
+// Copies of up to two operands with rows of `pad` values (a multiple of 8) at 16-byte alignment, zeros
+// past `dim`: what the products read where an operand's own rows do not fit their loads.
+struct HeadPad {
+  const uint16_t* src[2]; long long ld[2];
+  uint16_t* dst[2];
+  int rows[2];
+  int n, dim, pad;
+  void add(const uint16_t* s, long long lds, int count, void* d) {
+    src[n] = s;
+    ld[n] = lds;
+    rows[n] = count;
+    dst[n++] = static_cast<uint16_t*>(d);
+  }
+};
+hipError_t launch_head_pad(const HeadPad& a, hipStream_t stream);
+
 // dst[k] = factor[0] * src[k] for n[k] values, k = 0 and 1; in_place: every dst is its src, and
 // nothing moves where the factor is 1.
 struct ScaleBy {

@@ -198,10 +198,7 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
   const bool gathers = a.d_weight && l.chunk < a.tokens, split_h = !gathers || grad_size == 4;
   int64_t ldw = a.ld_weight;
   if (l.copy_w) {
-    uint16_t* copy = reinterpret_cast<uint16_t*>(ws + l.W);
-    if (check_launch(launch_pad_copy(W, a.ld_weight, 0, copy, l.pad, 0, (int)a.vocab, (int)a.dim,
-                                     (int)a.vocab, (int)l.pad, 1, stream), who)) return 1;
-    W = copy;
+    W = reinterpret_cast<const uint16_t*>(ws + l.W);
     ldw = l.pad;
   }
   if (check_launch(launch_head_targets(r, H, a.ld_hidden, static_cast<const uint16_t*>(a.weight),
@@ -210,13 +207,17 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
     const int rows = (int)(a.tokens - first < l.chunk ? a.tokens - first : l.chunk);
     const uint16_t* Hc = H + first * a.ld_hidden;
     int64_t ldh = a.ld_hidden;
+    HeadPad pad{};
+    pad.dim = (int)a.dim;
+    pad.pad = (int)l.pad;
+    if (l.copy_w && first == 0)
+      pad.add(static_cast<const uint16_t*>(a.weight), a.ld_weight, (int)a.vocab, ws + l.W);
     if (l.copy_h) {
-      uint16_t* copy = reinterpret_cast<uint16_t*>(ws + l.H);
-      if (check_launch(launch_pad_copy(Hc, a.ld_hidden, 0, copy, l.pad, 0, rows, (int)a.dim, rows,
-                                       (int)l.pad, 1, stream), who)) return 1;
-      Hc = copy;
+      pad.add(Hc, ldh, rows, ws + l.H);
+      Hc = reinterpret_cast<const uint16_t*>(ws + l.H);
       ldh = l.pad;
     }
+    if (check_launch(launch_head_pad(pad, stream), who)) return 1;
     HeadGemm g{};
     g.elt = elt;
     g.mode = !grads ? HG_STATS : elt == ELT_F16 ? HG_LOGITS : HG_EXP;
