@@ -14,8 +14,8 @@
 // whole sub-tile lies outside the result does no MFMA work.
 //
 // Bound by the matrix pipe under the board's power limit. 8192 tokens x 128256 x 4096 in bf16: logits
-// with their statistics and exponentials 6.44 ms (1.34 PFLOP/s), hidden gradient 5.68 (1.52), weight
-// gradient 6.65 (1.29); a library's plain products of that size take 6.05, 6.23 and 7.26. Where K is
+// with their statistics and exponentials 6.35 ms (1.36 PFLOP/s), hidden gradient 5.61 (1.53), weight
+// gradient 6.54 (1.32); a library's plain products of that size take 6.05, 6.23 and 7.26. Where K is
 // short, a tile's first loads and results (5 to 6 us) show: 2047 x 32001 x 2048 0.22 ms (1.21) for the
 // logits. Up to 256 tokens it is reading the weight: 5.7 TB/s for one token of 128256 x 4096.
 #include "dmuon_amd_internal.h"
