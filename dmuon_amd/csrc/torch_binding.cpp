@@ -7,7 +7,9 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <optional>
 
@@ -59,6 +61,19 @@ Tensor workspace(int64_t bytes, const Tensor& like) {
 void once(const char* who) {
   TORCH_CHECK(!at::GradMode::is_enabled(), who,
               ": the gradient has no gradient of its own (create_graph=True)");
+}
+
+// The kernels write into memory that torch has only seen allocated. A recorder of its operators would
+// keep the allocation alone and replay it, and a tangent (forward-mode gradient) would be lost where no
+// operand asks for the other kind: both are refused.
+void untraced(const char* who) {
+  const bool graph = c10::impl::TorchDispatchModeTLS::get_mode(
+      c10::impl::TorchDispatchModeKey::PROXY).has_value();
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !graph, who,
+              ": cannot be recorded by a tracer (torch.jit.trace, make_fx)");
+}
+void no_tangent(const char* who, const Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), who, ": has no forward-mode gradient (dual tensors)");
 }
 
 // ---- losses over a vocabulary -------------------------------------------------------------------
@@ -171,6 +186,9 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
 };
 
 void check_head(const char* who, const Tensor& hidden, const Tensor& weight) {
+  untraced(who);
+  no_tangent(who, hidden);
+  no_tangent(who, weight);
   TORCH_CHECK_VALUE(hidden.dim() >= 1 && weight.dim() == 2 && hidden.size(-1) == weight.size(1), who,
                     ": hidden [..., dim] and weight [vocab, dim] do not fit: ", hidden.sizes(), ", ",
                     weight.sizes());
@@ -365,6 +383,11 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& y, co
                                          const OptTensor& post, const OptTensor& gate, double scale,
                                          double eps, int64_t most) {
   const char* who = "residual_norm";
+  untraced(who);
+  no_tangent(who, x);
+  no_tangent(who, pre);
+  for (const OptTensor* t : {&y, &post, &gate})
+    if (live(*t)) no_tangent(who, **t);
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= most, who,
                     ": x must be [..., dim] with 1 <= dim <= ", most, ", got ", x.sizes());
   TORCH_CHECK_VALUE(code(x.scalar_type()) >= 0, who, ": unsupported dtype ", x.scalar_type());

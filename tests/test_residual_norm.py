@@ -341,3 +341,26 @@ def test_c_entry_refusals_without_gpu():
     says(grad(args(stats=None), 4096, 1 << 30, None), "stats")
     says(grad(args(ld_dh=63), 4096, 1 << 30, None), "pitch")
     says(grad(args(w_post=None), 4096, 1 << 30, None), "not there")
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_tangents_and_tracers_are_refused(dev):
+    """A tangent would be lost and a recorded call would return memory that nothing has written."""
+    import torch.autograd.forward_ad as forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    v = [torch.ones(2, 8, device=dev), torch.ones(2, 8, device=dev), torch.ones(8, device=dev),
+         torch.ones(8, device=dev), torch.ones(8, device=dev)]
+
+    def call(x, y, pre, post, gate):
+        return dmuon.residual_norm(x, y, pre, post_weight=post, gate=gate)
+
+    for k in range(5):
+        with forward_ad.dual_level():
+            dual = [forward_ad.make_dual(t, t) if i == k else t for i, t in enumerate(v)]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(*dual)
+    with pytest.raises(RuntimeError, match="tracer"):
+        torch.jit.trace(call, tuple(v), check_trace=False)
+    with pytest.raises(RuntimeError, match="tracer"):
+        make_fx(call)(*v)

@@ -544,3 +544,23 @@ def test_c_entry_refusals_without_gpu():
     says(lib.dmuon_scale_by(None, None, 4, None, None, 0, 1, 1, 4096, None), "NULL")
     says(lib.dmuon_scale_by(4096, 4096, 4, None, 4096, 2, 1, 1, 4096, None), "NULL")
     assert lib.dmuon_scale_by(None, None, 0, None, None, 0, 1, 1, None, None) == 0
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_tangents_and_tracers_are_refused(dev):
+    """A tangent would be lost and a recorded call would return memory that nothing has written."""
+    import torch.autograd.forward_ad as forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    h = torch.zeros(4, 8, dtype=torch.bfloat16, device=dev)
+    w = torch.zeros(10, 8, dtype=torch.bfloat16, device=dev)
+    t = torch.zeros(4, dtype=torch.int64, device=dev)
+    ids, logits = t[:, None], torch.zeros(4, 1, device=dev)
+    calls = (lambda a, b: dmuon.linear_cross_entropy(a, b, t),
+             lambda a, b: dmuon.linear_distillation(a, b, ids, logits))
+    for call in calls:
+        with forward_ad.dual_level():
+            _refuse("forward-mode", lambda: call(forward_ad.make_dual(h, h), w), RuntimeError)
+            _refuse("forward-mode", lambda: call(h, forward_ad.make_dual(w, w)), RuntimeError)
+        _refuse("tracer", lambda: torch.jit.trace(call, (h, w), check_trace=False), RuntimeError)
+        _refuse("tracer", lambda: make_fx(call)(h, w), RuntimeError)
