@@ -564,3 +564,20 @@ def test_tangents_and_tracers_are_refused(dev):
             _refuse("forward-mode", lambda: call(h, forward_ad.make_dual(w, w)), RuntimeError)
         _refuse("tracer", lambda: torch.jit.trace(call, (h, w), check_trace=False), RuntimeError)
         _refuse("tracer", lambda: make_fx(call)(h, w), RuntimeError)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,chunks", [(200, (1, 100)), (1100, (256, 512, 1024))])
+@pytest.mark.parametrize("v", [1003, 5000, 32001])
+def test_chunks_do_not_change_a_losss_bits(gpu, n, chunks, v):
+    """Statistics of many classes join in one order whatever the chunk: calls on both sides of 128
+    and 1024 tokens, in chunks on the other side and with a shorter last one."""
+    h, w, t, gen = _inputs(gpu, n, v, 64, torch.bfloat16, seed=11)
+    ids = torch.randint(0, v, (n, 70), device=gpu, generator=gen)
+    logits = torch.randn(n, 70, device=gpu, generator=gen)
+    for call in (lambda c: dmuon.linear_cross_entropy(h, w, t, reduction="none", chunk_tokens=c),
+                 lambda c: dmuon.linear_distillation(h, w, ids, logits, reduction="none",
+                                                     chunk_tokens=c)):
+        whole = call(None)
+        for chunk in chunks:
+            assert torch.equal(call(chunk), whole)
