@@ -193,6 +193,9 @@ __device__ __forceinline__ void grad_epilogue(const HeadGemm& a, f32x4_t (&acc)[
   const int jl = 4 * (lane >> 4);
   const bool whole = a.out && a.splits == 1;
   const float alpha = whole ? a.alpha[0] : 1.f;
+  // parts and gathered sums hold the gradient's own scale, whatever shift its values were stored with
+  const float up = E == ELT_F16 && a.peak
+      ? __uint_as_float((unsigned)(127 + peak_shift(*a.peak)) << 23) : 1.f;
   const bool f32 = !whole || a.out_dtype == DT_F32;
   float* part = a.part + (a.splits > 1 ? (long long)split * a.M * a.ldp : 0);
   float* dst = whole ? static_cast<float*>(a.out) : part;
@@ -207,6 +210,7 @@ __device__ __forceinline__ void grad_epilogue(const HeadGemm& a, f32x4_t (&acc)[
     for (int y = 0; y < 4; ++y) {
       const int j = jw + jl + 16 * y;
       f32x4_t v = acc[x][y];
+      if constexpr (E == ELT_F16) v *= up;
       if (a.add_part && i < a.M && j < a.N) {
         const float* p = part + (long long)i * a.ldp + j;
         if (j + 3 < a.N) v += *reinterpret_cast<const f32x4_any_t*>(p);

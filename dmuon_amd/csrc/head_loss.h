@@ -11,9 +11,15 @@ namespace dmuon {
 // kStatCols columns of the logits.
 constexpr int kStatCols = 64;
 // The logit gradient is stored as 2^kGradShift times its row's value over the largest row weight:
-// fp16 then holds probabilities down to 2^-24 with all their bits and 2^-34 with some, and
-// 2^6 = 64 times the unit mass does not overflow.
-constexpr int kGradShift = 10;
+// fp16 then holds probabilities down to 2^-24 with all their bits and 2^-34 with some. A row's
+// largest value is its factor mass + 2 z_loss lse and its mass at most. Where they reach 2^kPeakBits
+// (an unusual z_loss or teacher), fp16 gradients shrink by the power of two that keeps them under it,
+// and the products' sums grow by it again: peak_shift of the largest so far.
+constexpr int kGradShift = 10, kPeakBits = 15;
+__host__ __device__ __forceinline__ int peak_shift(unsigned peak) {
+  const int shift = (int)(peak >> 23) - (127 + kPeakBits - 1);
+  return shift > 0 ? shift : 0;
+}
 
 // What a product writes. Logits z = scale * acc and their statistics are in units of log 2.
 //   HG_STATS   the softmax statistics of z
@@ -46,6 +52,7 @@ struct HeadGemm {
   void* Z;                                // HG_EXP, HG_LOGITS: [ceil(N / 64)][M][64]
   float2* stats;                          // [ceil(N / 64)][M]
   const float* alpha;
+  const unsigned* peak;                   // HG_GRAD in fp16: see HeadRows; NULL: no shift
   void* out; long long ldo; int out_dtype;   // HG_GRAD: result (DT_F32 or the operands'), or NULL
   float* part; long long ldp;             // HG_GRAD: fp32 sums [M][ldp], or NULL
   int add_part;                           // part holds earlier sums to add to
@@ -89,6 +96,8 @@ struct HeadRows {
   float* row_weight;                      // [n]: 2^kGradShift * row gradient / largest, 0: not counted
   float* factor;                          // [n]: of 2^(z - top) in the logit gradient
   float* alpha;                           // [1]: what turns a stored gradient into the real one
+  unsigned* peak;                         // [1], fp16 gradients: bits of the largest row value so far
+                                          // of 2^kPeakBits and more, or 0
   float* mean;                            // [1] or NULL: the reduced loss
 };
 // ids, probs, mass and logits of every row (H, W: the products' operands, any alignment); with

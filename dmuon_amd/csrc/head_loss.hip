@@ -27,7 +27,7 @@ constexpr int64_t kMaxVocab = int64_t(65535) * 64;
 
 struct Layout {
   int64_t chunk, ld;                      // tokens of a chunk, classes in whole blocks
-  int64_t ids, probs, logits, mass, top, loss, row_weight, factor, alpha, Z, stats, G, part, H, W, bytes;
+  int64_t ids, probs, logits, mass, top, loss, row_weight, factor, alpha, peak, Z, stats, G, part, H, W, bytes;
   int64_t pad;                            // pitch of the copies of hidden and weight
   bool copy_h, copy_w;
 };
@@ -106,6 +106,7 @@ Layout lay_out(const dmuon_head_loss_args& a) {
   l.row_weight = take(a.tokens * 4);
   l.factor = take(a.tokens * 4);
   l.alpha = take(4);
+  l.peak = take(grads && f16 ? 4 : 0);
   l.stats = take(l.chunk * tiles * 8);
   l.G = take(grads ? l.chunk * l.ld * 2 : 0);
   l.Z = grads && f16 ? take(l.chunk * l.ld * 4) : l.G;
@@ -187,6 +188,7 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
   r.row_weight = floats(l.row_weight);
   r.factor = floats(l.factor);
   r.alpha = floats(l.alpha);
+  r.peak = grads && elt == ELT_F16 ? reinterpret_cast<unsigned*>(ws + l.peak) : nullptr;
   r.mean = a.reduced;
   void* Z = ws + l.Z;
   float2* stats = reinterpret_cast<float2*>(ws + l.stats);
@@ -238,6 +240,7 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
       g.elt = elt;
       g.mode = HG_GRAD;
       g.alpha = r.alpha;
+      g.peak = rows > 0 ? r.peak : nullptr;
       g.out_dtype = a.grad_dtype;
       if (a.d_hidden) {
         g.A = G; g.lda = rows;

@@ -76,6 +76,7 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uin
                                                            long long ldw, int dim) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float it = 1.f / r.temperature;
+  if (r.peak && blockIdx.x == 0 && threadIdx.x == 0) *r.peak = 0u;
   if (r.targets) {
     const int row = blockIdx.x * 4 + wave;
     if (row >= r.n) return;
@@ -229,7 +230,11 @@ __global__ __launch_bounds__(1024) void head_lse_kernel(HeadRows r, int first, i
   if (grads) {
     const float w = row_weight(r, n);
     r.row_weight[n] = w;
-    r.factor[n] = w == 0.f ? 0.f : w * (mass + 2.f * r.z_loss * lse) / s;
+    const float c = mass + 2.f * r.z_loss * lse, top_value = fabsf(w) * (fabsf(c) + mass);
+    r.factor[n] = w == 0.f ? 0.f : w * c / s;
+    // the largest of the rows: an order of atomics does not show; infinities and NaN stay their row's
+    if (r.peak && top_value >= (float)(1 << kPeakBits) && top_value < kInf)
+      atomicMax(r.peak, __float_as_uint(top_value));
   }
 }
 
@@ -255,12 +260,16 @@ __device__ __forceinline__ void reduce_losses(const HeadRows& r, float* lds) {
   }
 }
 
+__device__ __forceinline__ float peak_down(const HeadRows& r) {
+  return __uint_as_float((unsigned)(127 - peak_shift(*r.peak)) << 23);
+}
+
 // The logit gradient: factor * 2^(z - top) - row_weight * q, in place of the exponentials (whose share
 // 2^(m - top) is one of a block's row) or from the logits (LOGITS). Crosses memory once, 2 + 2 bytes
 // a logit or 4 + 2: 4 x 32 rows of one block of 64 classes a workgroup, 16 bytes a thread and step.
 // A hard target's own class comes from its fp32 logit: softmax - 1 cancels where the student is
 // sure. (So the row's maximum and 1 / sum go in apart: their log-sum-exp would lose what 1 - p is
-// made of.)
+// made of.) LOGITS is fp16: its values shrink by peak_shift.
 // Blocks past the rows' are the reduction's, which the products after this kernel wait for and nothing
 // in it: a launch of its own cost small calls 4 us.
 // Memory bound: 8192 x 128256 in place (4.2 GB) 737 us, 5.7 TB/s.
@@ -275,12 +284,13 @@ __global__ __launch_bounds__(256) void head_grad_kernel(HeadRows r, int first, i
     return;
   }
   const int row0 = blockIdx.x * 128 + (threadIdx.x >> 3);
+  const float down = LOGITS ? peak_down(r) : 1.f;
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int row = row0 + 32 * p;
     if (row >= rows) return;
     const long long n = first + row, at = ((long long)tile * rows + row) * 64 + 8 * c;
-    const float f = r.factor[n], top = r.top[n];
+    const float f = r.factor[n] * down, top = r.top[n];
     const int id = r.targets ? r.ids[n] : -1;
     float v[8];
     if (f == 0.f) {
@@ -305,7 +315,7 @@ __global__ __launch_bounds__(256) void head_grad_kernel(HeadRows r, int first, i
       }
     }
     if (id >> 3 == 8 * tile + c) {
-      const float g = f * exp2_fast(__builtin_fmaf(r.logits[n], kLog2e, -top)) - r.row_weight[n];
+      const float g = f * exp2_fast(__builtin_fmaf(r.logits[n], kLog2e, -top)) - r.row_weight[n] * down;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = (id & 7) == e ? g : v[e];
     }
@@ -324,7 +334,8 @@ __global__ __launch_bounds__(256) void head_entries_kernel(HeadRows r, int first
   const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   if (row >= rows) return;
   const long long n = first + row;
-  const float w = r.row_weight[n], f = r.factor[n], top = r.top[n];
+  const float down = E == ELT_F16 ? peak_down(r) : 1.f;
+  const float w = r.row_weight[n] * down, f = r.factor[n] * down, top = r.top[n];
   if (w == 0.f) return;
   const int* ids = r.ids + n * r.k_list;
   const float* probs = r.probs + n * r.k_list;
@@ -468,7 +479,8 @@ hipError_t launch_head_rows(const HeadRows& r, int first, int rows, const float2
   hipLaunchKernelGGL(head_lse_kernel, dim3((unsigned)((rows + side - 1) / side)), dim3(1024), 0,
                      stream, r, first, rows, stats, side, G != nullptr);
   if (!G) return first + rows < r.n ? hipGetLastError() : reduce(r, stream);
-  if (tiles > 65535 || (Z == G) != (elt == ELT_BF16)) return hipErrorInvalidValue;
+  if (tiles > 65535 || (Z == G) != (elt == ELT_BF16) || (elt == ELT_F16) != (r.peak != nullptr))
+    return hipErrorInvalidValue;
   const dim3 grid((unsigned)((rows + 127) / 128 + (r.reduction != DMUON_LOSS_ROWS)), (unsigned)tiles);
   const dim3 lists((unsigned)((rows + 3) / 4));
   const float* logits = static_cast<const float*>(Z);

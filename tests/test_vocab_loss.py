@@ -581,3 +581,47 @@ def test_chunks_do_not_change_a_losss_bits(gpu, n, chunks, v):
         whole = call(None)
         for chunk in chunks:
             assert torch.equal(call(chunk), whole)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,chunk", [(150, None), (700, 256)])
+@pytest.mark.parametrize("what", ["z_loss", "negative z_loss", "teacher_lse"])
+def test_large_factors_of_the_probabilities(gpu, what, n, chunk, dt):
+    """A probability's factor in the gradient is c = mass + 2 z_loss lse, which a z_loss, or a teacher's
+    log-sum-exp under its own logits, makes large: 16-bit gradients stay finite and right.
+
+    Bounds, beside those above: c p is off relatively (c itself by z_err / lse at most, lse > 1); what
+    the type holds of the smallest values goes with the largest c, 2^-34 of it in fp16 and 2^-39 of
+    exponentials in bf16; the loss has c's size."""
+    v, d = 300, 64
+    h, w, t, gen = _inputs(gpu, n, v, d, dt, seed=12, lean=30.0)
+    t[::7] = -100
+    z = h.double() @ w.double().t()
+    top = z.abs().amax()
+    if what == "teacher_lse":
+        ids = torch.rand(n, v, device=gpu, generator=gen).argsort(1)[:, :6]
+        logits = torch.randn(n, 6, device=gpu, generator=gen)
+        lse = -3.0 * torch.rand(n, device=gpu, generator=gen)
+        lse[: n // 2] += 3.0                                       # the largest in a later chunk
+        exact = _kd(h, w, ids, logits, lse)
+        c = (logits.double() - lse.double()[:, None]).exp().sum(1)
+        exact.loss_tol = 8 * (1 + c.amax()) * exact.loss_tol
+        def call(a, b, r):
+            return dmuon.linear_distillation(a, b, ids, logits, teacher_lse=lse, reduction=r,
+                                             chunk_tokens=chunk)
+    else:
+        zl = 4.0 if what == "z_loss" else -4.0
+        exact = _ce(h, w, t, z_loss=zl)
+        c = 1 + 2 * abs(zl) * torch.logsumexp(z, 1)
+        exact.loss_tol = (1 + 2 * abs(zl) * top) * (2 * exact.z_err + 2.0 ** -20 * (1 + top))
+        def call(a, b, r):
+            return dmuon.linear_cross_entropy(a, b, t, z_loss=zl, reduction=r, chunk_tokens=chunk)
+    assert float(c.amax()) > 64
+    exact.p = exact.p * c[:, None]
+    least = float(c.amax()) * (2.0 ** -34 if dt == torch.float16 else 2.0 ** -39)
+    plain = exact.grads
+    exact.grads = lambda row: [(g, b + least * row.abs().amax() * other.abs().sum(0))
+                               for (g, b), other in zip(plain(row), (exact.w, exact.h))]
+    for reduction in ("mean", "none"):
+        _check(exact, call, h, w, reduction)
