@@ -155,13 +155,15 @@ __device__ __forceinline__ float row_weight(const HeadRows& r, long long n) {
 
 // Row weights and alpha from the rows' gradients: the gradient of row n is alpha * row_weight[n] *
 // (...). The weights are relative to the largest, so that a 16-bit logit gradient neither over- nor
-// underflows with the size of the batch or a loss scale. One block.
+// underflows with the size of the batch or a loss scale. The largest finite one: an infinite gradient
+// is its own row's. One block.
 __global__ __launch_bounds__(1024) void head_weights_kernel(HeadRows r) {
   __shared__ float lds[16];
   float top = 0.f;
   for (int n = threadIdx.x; n < r.n; n += 1024)
-    if (!(r.mass[n] < 0.f)) top = fmaxf(top, fabsf(r.row_grad[n]));
+    if (!(r.mass[n] < 0.f) && fabsf(r.row_grad[n]) < kInf) top = fmaxf(top, fabsf(r.row_grad[n]));
   top = block_join<true>(top, lds);
+  if (top == 0.f) top = 1.f;
   for (int n = threadIdx.x; n < r.n; n += 1024)
     r.row_weight[n] = r.row_grad[n] == 0.f ? 0.f : kUnit * (r.row_grad[n] / top);
   if (threadIdx.x == 0) r.alpha[0] = top * r.temperature / kUnit;

@@ -625,3 +625,26 @@ def test_large_factors_of_the_probabilities(gpu, what, n, chunk, dt):
                                for (g, b), other in zip(plain(row), (exact.w, exact.h))]
     for reduction in ("mean", "none"):
         _check(exact, call, h, w, reduction)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_a_row_gradient_that_is_no_number_stays_in_its_row(gpu, dt):
+    h, w, t, _ = _inputs(gpu, 40, 300, 64, dt, seed=13)
+    t[9] = -100
+    row = torch.linspace(-1.0, 2.0, 40, device=gpu)
+    exact = _ce(h, w, t)
+    want, bound = exact.grads(row)[0]
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        for others in (row, torch.zeros_like(row)):
+            a = h.clone().requires_grad_(True)
+            g = others.clone()
+            g[5] = bad
+            g[9] = bad                                       # of an ignored token: no share
+            dmuon.linear_cross_entropy(a, w, t, reduction="none").backward(g)
+            keep = [i for i in range(40) if i != 5]
+            assert not bool(a.grad[5].isfinite().all())
+            if others is row:
+                _within(a.grad[keep], want[keep], bound[keep])
+            else:
+                assert not bool(a.grad[keep].any())
