@@ -63,8 +63,8 @@ __device__ __forceinline__ void wave_dots(const uint16_t* h, const uint16_t* con
 }
 
 // The entries of a row and their logits. Hard targets: one, with probability 1. A teacher's list:
-// softmax of the live logits over the temperature, or their exponentials under the teacher's own
-// log-sum-exp. A class outside the vocabulary that is neither the ignored index nor padding makes
+// softmax of the live logits over the temperature (of their differences from the largest, which the
+// temperature cannot overflow), or their exponentials under the teacher's own log-sum-exp. A class outside the vocabulary that is neither the ignored index nor padding makes
 // the row's mass NaN, so its loss and gradients show it. The entries' logits are formed here, in
 // fp32 from the rows themselves: the products' epilogue would have to search every row's list in
 // each of its tiles. Hard targets take one wave a row, lists four.
@@ -104,18 +104,18 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uin
     if (id < 0) continue;
     live = 1;
     outside |= id >= r.vocab;
-    top = fmaxf(top, r.teacher_logits[base + k] * it);
+    top = fmaxf(top, r.teacher_logits[base + k]);
   }
   live = __any(live);
   outside = __any(outside);
   top = wave_max(top);
-  const float shift = r.teacher_lse ? r.teacher_lse[row] : top;
+  const float under = r.teacher_lse ? r.teacher_lse[row] : 0.f;
+  auto share = [&](float v) {
+    return v == -kInf ? 0.f : expf(r.teacher_lse ? v * it - under : (v - top) * it);
+  };
   float sum = 0.f;
   for (int k = lane; k < r.k_list; k += 64)
-    if (r.teacher_ids[base + k] >= 0) {
-      const float v = r.teacher_logits[base + k] * it;
-      sum += v == -kInf ? 0.f : expf(v - shift);
-    }
+    if (r.teacher_ids[base + k] >= 0) sum += share(r.teacher_logits[base + k]);
   sum = wave_sum(sum);
   const float norm = r.teacher_lse ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
   if (wave == 0 && lane == 0)
@@ -129,8 +129,7 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uin
     for (int e = 0; e < 4; ++e) {
       const int k = k0 + e < r.k_list ? k0 + e : k0;
       const long long id = r.teacher_ids[base + k];
-      const float v = r.teacher_logits[base + k] * it;
-      q[e] = id < 0 || v == -kInf ? 0.f : expf(v - shift) * norm;
+      q[e] = id < 0 ? 0.f : share(r.teacher_logits[base + k]) * norm;
       cls[e] = id >= 0 && id < r.vocab && q[e] != 0.f ? (int)id : -1;
       w[e] = W + (cls[e] < 0 ? 0 : cls[e]) * ldw;         // an entry without a class: any row
     }

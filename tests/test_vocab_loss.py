@@ -648,3 +648,23 @@ def test_a_row_gradient_that_is_no_number_stays_in_its_row(gpu, dt):
                 _within(a.grad[keep], want[keep], bound[keep])
             else:
                 assert not bool(a.grad[keep].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [0.25, 0.5, 1.0, 2.0])
+def test_lists_of_extreme_logits_at_any_temperature(gpu, temperature):
+    """Lists throughout of the type's lowest value, or with its highest, have finite logits: their
+    probabilities are those of the differences."""
+    h, w, t, _ = _inputs(gpu, 3, 300, 64, torch.bfloat16)
+    big = torch.finfo(torch.float32).max
+    ids = torch.arange(8, device=gpu).expand(3, 8).contiguous()
+    logits = torch.zeros(3, 8, device=gpu)
+    logits[0] = -big
+    logits[1, 3] = big
+    logits[2] = big
+    even = torch.zeros(3, 8, device=gpu)
+    even[1] = float("-inf")
+    even[1, 3] = 0.0
+    exact = _kd(h, w, ids, even, temperature=temperature)
+    _check(exact, lambda a, b, r: dmuon.linear_distillation(a, b, ids, logits, reduction=r,
+                                                            temperature=temperature), h, w, "none")
