@@ -375,7 +375,8 @@ Tensor gate_rows(const char* who, const Tensor& gate, const Tensor& x) {
   }
   TORCH_CHECK_VALUE(fits, who, ": a gate of ", gate.sizes(),
                     " has no row for each of equal runs of the rows of x ", x.sizes());
-  if (gate.numel() == 0) return gate.new_zeros({1, dim});
+  // no row at all: one that no row of x uses, behind the gate's own
+  if (gate.numel() == 0) return at::cat({gate.reshape({0, dim}), gate.new_zeros({1, dim})});
   return gate.dim() == 2 ? gate.contiguous() : gate.reshape({-1, dim}).contiguous();
 }
 

@@ -364,3 +364,14 @@ def test_tangents_and_tracers_are_refused(dev):
         torch.jit.trace(call, tuple(v), check_trace=False)
     with pytest.raises(RuntimeError, match="tracer"):
         make_fx(call)(*v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,gate", [((0, 5, 40), (0, 1, 40)), ((0, 5, 40), (0, 5, 40)),
+                                        ((3, 0, 40), (3, 1, 40)), ((0, 40), (7, 40))])
+def test_no_rows_give_every_gate_a_gradient(gpu, shape, gate):
+    v, outs = _inputs(gpu, shape, torch.bfloat16, torch.float32, True, gate, seed=10)
+    leaves = {k: t.clone().requires_grad_(True) for k, t in v.items()}
+    got = torch.autograd.grad(_call(leaves, 1.0), list(leaves.values()), outs)
+    for a, t in zip(got, leaves.values()):
+        assert a.shape == t.shape and not bool(a.any())
