@@ -13,6 +13,8 @@
 #include "dmuon_amd_internal.h"
 #include "head_loss.h"
 
+#include <cmath>
+
 using namespace dmuon;
 
 namespace {
@@ -70,7 +72,8 @@ int check(const char* who, const dmuon_head_loss_args* a) {
     if (a->k_list < 1 || a->k_list > 4096)
       return fail("%s: k_list must be 1 .. 4096, got %lld", who, (long long)a->k_list);
     if (!a->teacher_logits) return fail("%s: teacher_logits is NULL", who);
-    if (!(a->temperature > 0.f)) return fail("%s: temperature must be positive", who);
+    if (!(a->temperature > 0.f) || !std::isfinite(a->temperature) || !std::isfinite(1.f / a->temperature))
+      return fail("%s: temperature must be positive, and finite like its inverse", who);
     if (a->z_loss != 0.f) return fail("%s: z_loss goes with hard targets", who);
   }
   return 0;

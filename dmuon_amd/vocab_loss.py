@@ -65,8 +65,10 @@ def linear_distillation(hidden: Tensor, weight: Tensor, teacher_ids: Tensor,
     loss. Gradients go to ``hidden`` and ``weight``, not to the teacher. Types, ``reduction`` and
     ``chunk_tokens`` as in ``linear_cross_entropy``.
     """
-    if not 0.0 < float(temperature) < float("inf"):
-        raise ValueError(f"linear_distillation: temperature must be positive, got {temperature}")
+    # normal fp32 numbers: the kernels take its inverse too
+    if not 2.0 ** -126 <= float(temperature) < 2.0 ** 128:
+        raise ValueError("linear_distillation: temperature must be positive and within fp32, got "
+                         f"{temperature}")
     return _C.torch_ops().linear_distillation(
         hidden, weight, teacher_ids, teacher_logits, teacher_lse, float(temperature),
         *_options("linear_distillation", reduction, chunk_tokens))

@@ -668,3 +668,20 @@ def test_lists_of_extreme_logits_at_any_temperature(gpu, temperature):
     exact = _kd(h, w, ids, even, temperature=temperature)
     _check(exact, lambda a, b, r: dmuon.linear_distillation(a, b, ids, logits, reduction=r,
                                                             temperature=temperature), h, w, "none")
+
+
+def test_temperatures_past_fp32_are_refused():
+    import ctypes
+
+    from dmuon_amd import _C
+    h, w = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(10, 8, dtype=torch.bfloat16)
+    ids, logits = torch.zeros(4, 1, dtype=torch.int64), torch.zeros(4, 1)
+    for t in (1e-300, 1e-45, 1e-40, 1e39, float("inf"), -1.0):
+        _refuse("temperature", lambda: dmuon.linear_distillation(h, w, ids, logits, temperature=t))
+    lib, need = _C.lib(), ctypes.c_int64()
+    for t in (1e-40, float("inf"), float("nan")):
+        a = _C.HeadLossArgs(dtype=1, grad_dtype=1, reduction=1, tokens=4, vocab=100, dim=64,
+                            ld_hidden=64, ld_weight=64, teacher_ids=4096, teacher_logits=4096,
+                            k_list=1, temperature=t)
+        assert lib.dmuon_head_loss_workspace_size(ctypes.byref(a), ctypes.byref(need)) != 0
+        assert "temperature" in lib.dmuon_last_error().decode()
