@@ -1,5 +1,5 @@
 """Builds libdmuon_amd.so (gfx950) in-tree with hipcc, and the extension module of the autograd
-operators on it (_dmuon_torch.so, host code only).
+operators on it (_dmuon_torch.so, host code only; left out where there is no torch to build against).
 
     python -m dmuon_amd.csrc.build          # or: python dmuon_amd/csrc/build.py
 
@@ -55,6 +55,10 @@ def lib_path() -> Path:
     return HERE / LIB_NAME
 
 
+def binding_path() -> Path:
+    return HERE / BINDING_NAME
+
+
 def _run(cmd, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
@@ -72,21 +76,28 @@ def build(verbose: bool = False) -> Path:
     tmp = out.with_suffix(".so.tmp")
     compile_flags = [f for f in FLAGS if f != "-shared"]
     with tempfile.TemporaryDirectory() as d:
-        objects = [str(Path(d) / (s + ".o")) for s in [*SOURCES, BINDING]]
+        objects = [str(Path(d) / (s + ".o")) for s in SOURCES]
         jobs = [[hipcc(), *compile_flags, "-I", str(ROOT / "include"), "-c", str(HERE / s), "-o", o]
                 for s, o in zip(SOURCES, objects)]
-        jobs.append(_binding_compile(objects[-1]))
+        module = str(Path(d) / (BINDING + ".o"))
+        try:
+            module_job = _binding_compile(module)
+        except ImportError as e:
+            module_job = None
+            print(f"{BINDING_NAME} is not built: {e}", file=sys.stderr)
         # the files are independent code objects: one compiler each
-        with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 1, 8)) as pool:
+        with ThreadPoolExecutor(max_workers=min(len(jobs) + 1, os.cpu_count() or 1, 8)) as pool:
+            compiled = pool.submit(_run, module_job, verbose) if module_job else None
             list(pool.map(lambda cmd: _run(cmd, verbose), jobs))
-        _run([hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objects[:-1], "-o", str(tmp)],
-             verbose)
+        _run([hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objects, "-o", str(tmp)], verbose)
         _check_launch_stubs(tmp)
         os.replace(tmp, out)
-        binding = HERE / BINDING_NAME
-        tmp = binding.with_suffix(".so.tmp")
-        _run(_binding_link(objects[-1], str(tmp)), verbose)
-        os.replace(tmp, binding)
+        # the library needs no torch: the module's errors come after it
+        if compiled:
+            compiled.result()
+            tmp = binding_path().with_suffix(".so.tmp")
+            _run(_binding_link(module, str(tmp)), verbose)
+            os.replace(tmp, binding_path())
     return out
 
 
