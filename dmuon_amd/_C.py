@@ -209,12 +209,12 @@ _torch_ops = None
 
 def torch_ops():
     """The module of native autograd operators (``csrc/torch_binding.cpp``), loaded once; raises if
-    it is missing or was built against another ABI version of the library."""
+    it is missing or was built against another torch or another ABI version of the library."""
     global _torch_ops
     if _torch_ops is None:
         import importlib
 
-        import torch  # noqa: F401  (its libraries come first)
+        import torch  # its libraries come first
 
         lib()
         try:
@@ -226,6 +226,11 @@ def torch_ops():
             raise RuntimeError(f"dmuon_amd.csrc._dmuon_torch was built for ABI version "
                                f"{ops.abi_version}, this binding expects {ABI_VERSION}: rebuild it "
                                "(python -m dmuon_amd.csrc.build)")
+        # torch's C++ interface is that of one build
+        if ops.torch_version != str(torch.__version__):
+            raise RuntimeError(f"dmuon_amd.csrc._dmuon_torch was built for torch {ops.torch_version}, "
+                               f"this is {torch.__version__}: rebuild it (python -m "
+                               "dmuon_amd.csrc.build)")
         _torch_ops = ops
     return _torch_ops
 

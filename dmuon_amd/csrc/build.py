@@ -114,7 +114,7 @@ def _binding_compile(obj: str) -> list:
 
     return [_cxx(), "-O2", "-std=c++17", "-fPIC", "-Wall",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f'-DDMUON_TORCH="{torch.__version__}"',
             *[x for d in cpp_extension.include_paths() for x in ("-isystem", d)],
             "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"],
             "-c", str(HERE / BINDING), "-o", obj]

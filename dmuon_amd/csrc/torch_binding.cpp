@@ -433,6 +433,7 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& y, co
 
 PYBIND11_MODULE(_dmuon_torch, m) {
   m.attr("abi_version") = DMUON_ABI_VERSION;
+  m.attr("torch_version") = DMUON_TORCH;
   const auto free = py::call_guard<py::gil_scoped_release>();
   m.def("linear_cross_entropy", &linear_cross_entropy, free);
   m.def("linear_distillation", &linear_distillation, free);

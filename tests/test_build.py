@@ -47,3 +47,26 @@ def test_both_are_built(recorded, tmp_path):
     b.build()
     assert (tmp_path / b.LIB_NAME).exists() and (tmp_path / b.BINDING_NAME).exists()
     assert len(recorded) == len(b.SOURCES) + 3
+
+
+def test_a_module_of_another_torch_or_abi_is_refused(monkeypatch):
+    import types
+
+    import torch
+
+    from dmuon_amd import _C
+    ours = dict(abi_version=_C.ABI_VERSION, torch_version=str(torch.__version__))
+    for other, text in ((dict(torch_version="2.9.1"), "torch 2.9.1"), (dict(abi_version=1), "version 1")):
+        module = types.SimpleNamespace(**{**ours, **other})
+        monkeypatch.setattr(_C, "_torch_ops", None)
+        monkeypatch.setitem(sys.modules, "dmuon_amd.csrc._dmuon_torch", module)
+        with pytest.raises(RuntimeError, match=text):
+            _C.torch_ops()
+        assert _C._torch_ops is None
+
+
+def test_the_module_names_its_torch():
+    import torch
+
+    from dmuon_amd import _C
+    assert _C.torch_ops().torch_version == str(torch.__version__)
