@@ -511,6 +511,8 @@ hipError_t launch_residual_norm(ResidualNorm a, hipStream_t stream) {
   if (!row_shape(a.dim, kOneForward, &threads, &nv)) return hipErrorInvalidValue;
   if (a.rows <= 0) return hipSuccess;
   const int lanes = threads < 256 ? 256 / threads : 1;
+  // rows of two chunks a thread have 192 threads or more
+  if (nv == 2 && lanes > 1) return hipErrorInvalidValue;
   const long long want = kCus * 4096 / (threads * lanes);
   a.rows_per_block = (a.rows + want - 1) / want;
   a.rows_per_block = (a.rows_per_block + lanes - 1) / lanes * lanes;
@@ -520,8 +522,7 @@ hipError_t launch_residual_norm(ResidualNorm a, hipStream_t stream) {
   hipLaunchKernelGGL((residual_norm_kernel<T, NV, MANY>), grid, block, 0, stream, a)
 #define DMUON_RN_T(T)                                  \
   do {                                                 \
-    if (nv == 1 && lanes > 1) DMUON_RN(T, 1, true);    \
-    else if (lanes > 1) DMUON_RN(T, 2, true);          \
+    if (lanes > 1) DMUON_RN(T, 1, true);               \
     else if (nv == 1) DMUON_RN(T, 1, false);           \
     else DMUON_RN(T, 2, false);                        \
   } while (0)

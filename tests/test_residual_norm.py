@@ -375,3 +375,14 @@ def test_no_rows_give_every_gate_a_gradient(gpu, shape, gate):
     got = torch.autograd.grad(_call(leaves, 1.0), list(leaves.values()), outs)
     for a, t in zip(got, leaves.values()):
         assert a.shape == t.shape and not bool(a.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,gate", [((300, 8200), (300, 8200)), ((600, 8200), (300, 8200)),
+                                        ((2, 130, 16384), (2, 130, 16384)), ((130, 4096), (130, 4096)),
+                                        ((1100, 2056), (550, 2056))])
+def test_gates_of_wide_rows(gpu, shape, gate, dt):
+    """Several gate groups in a block, one and two chunks of columns a thread."""
+    v, outs = _inputs(gpu, shape, dt, torch.float32, True, gate, seed=11)
+    _check(v, outs, 0.5)
