@@ -685,3 +685,50 @@ def test_temperatures_past_fp32_are_refused():
                             k_list=1, temperature=t)
         assert lib.dmuon_head_loss_workspace_size(ctypes.byref(a), ctypes.byref(need)) != 0
         assert "temperature" in lib.dmuon_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,chunk", [(700, 256), (300, 100), (20, 7)])
+def test_unreduced_losses_in_chunks(gpu, n, chunk, dt):
+    h, w, t, gen = _inputs(gpu, n, 600, 72, dt, seed=14)
+    t[::6] = -100
+    _check(_ce(h, w, t), lambda a, b, r: dmuon.linear_cross_entropy(
+        a, b, t, reduction=r, chunk_tokens=chunk), h, w, "none")
+    ids = torch.rand(n, 600, device=gpu, generator=gen).argsort(1)[:, :9]
+    logits = torch.randn(n, 9, device=gpu, generator=gen)
+    _check(_kd(h, w, ids, logits, temperature=1.5), lambda a, b, r: dmuon.linear_distillation(
+        a, b, ids, logits, temperature=1.5, reduction=r, chunk_tokens=chunk), h, w, "none")
+
+
+@pytest.mark.gpu
+def test_the_default_chunks(gpu):
+    """More tokens than a default chunk holds: the memory stays the chunk's, and loss and gradients
+    are those of 64 bits."""
+    n, v, d = 90000, 50000, 64
+    h, w, t, _ = _inputs(gpu, n, v, d, torch.bfloat16)
+    t[::9] = -100
+    a, b = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    loss = dmuon.linear_cross_entropy(a, b, t)
+    loss.backward()
+    assert torch.cuda.max_memory_allocated() - before < 4.5e9      # two bytes a logit would be 9e9
+    count = int((t != -100).sum())
+    cols = torch.tensor([0, 1, 63, 64, 255, 256, 25000, v - 2, v - 1], device=gpu)
+    total, dw, bw = 0.0, 0.0, 0.0
+    for i in range(0, n, 3000):
+        exact = _ce(h[i:i + 3000], w, t[i:i + 3000])
+        total += float(exact.loss.sum())
+        row = torch.full((exact.loss.shape[0],), 1.0 / count, device=gpu)
+        dz = exact.dz[:, cols] / count
+        slack = U[h.dtype] * dz.abs() + (2.0 ** -11 + 3 * exact.z_err) / count * torch.maximum(
+            exact.p[:, cols], exact.dz[:, cols].abs())
+        dw = dw + dz.t() @ exact.h
+        bw = bw + slack.t() @ exact.h.abs()
+        if i in (0, 30000, 60000, 87000):                          # chunks begin and end here
+            (dh, bh), _ = exact.grads(row)
+            _within(a.grad[i:i + 3000], dh, bh)
+    assert abs(float(loss) - total / count) <= exact.loss_tol
+    _within(b.grad[cols], dw, bw + U[h.dtype] * dw.abs() + 1e-30)
