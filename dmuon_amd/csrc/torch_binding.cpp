@@ -38,8 +38,16 @@ void* stream_of(const Tensor& t) {
 }
 
 bool live(const OptTensor& t) { return t.has_value() && t->defined(); }
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-void* ptr(const OptTensor& t) { return live(t) ? t->data_ptr() : nullptr; }
+// NULL stands for an operand that is not there: a subclass that wraps other tensors (a distributed
+// one) must not pass for that.
+void* ptr(const Tensor& t) {
+  if (!t.defined()) return nullptr;
+  void* p = t.data_ptr();
+  TORCH_CHECK(p || t.numel() == 0, "dmuon_amd: a tensor without memory of its own (a wrapper subclass) "
+              "cannot be an operand");
+  return p;
+}
+void* ptr(const OptTensor& t) { return live(t) ? ptr(*t) : nullptr; }
 
 // The same matrix with its last dimension contiguous and rows that do not overlap.
 Tensor dense_rows(const Tensor& t) {
@@ -105,8 +113,8 @@ struct Loss : torch::CustomClassHolder {
     if (grads && want_hidden) d_hidden = at::empty({n, dim}, hidden.options().dtype(held));
     if (grads && want_weight) d_weight = at::empty({vocab, dim}, hidden.options().dtype(held));
     dmuon_head_loss_args a{};
-    a.hidden = hidden.data_ptr();
-    a.weight = weight.data_ptr();
+    a.hidden = ptr(hidden);
+    a.weight = ptr(weight);
     a.targets = static_cast<const int64_t*>(ptr(targets));
     a.teacher_ids = static_cast<const int64_t*>(ptr(ids));
     a.teacher_logits = static_cast<const float*>(ptr(logits));
@@ -146,7 +154,7 @@ struct Loss : torch::CustomClassHolder {
     const Tensor f = factor.to(at::kFloat).contiguous();
     call(dmuon_scale_by(ptr(d_hidden), ptr(out[0]), d_hidden.defined() ? d_hidden.numel() : 0,
                         ptr(d_weight), ptr(out[1]), d_weight.defined() ? d_weight.numel() : 0,
-                        code(held), code(dtype), f.data_ptr<float>(), stream_of(f)));
+                        code(held), code(dtype), static_cast<const float*>(ptr(f)), stream_of(f)));
     d_hidden = out[0];
     d_weight = out[1];
   }
@@ -270,14 +278,14 @@ dmuon_residual_norm_args describe(const Tensor& x, const OptTensor& y, const Ten
                                   const OptTensor& post, const OptTensor& gate, double scale,
                                   double eps) {
   dmuon_residual_norm_args a{};
-  a.x = x.data_ptr();
+  a.x = ptr(x);
   a.rows = x.size(0);
   a.dim = x.size(1);
   a.ld_x = pitch(x);
   a.dtype = code(x.scalar_type());
   a.y = ptr(y);
   if (live(y)) a.ld_y = pitch(*y);
-  a.w_pre = pre.data_ptr();
+  a.w_pre = ptr(pre);
   a.pre_dtype = code(pre.scalar_type());
   a.w_post = ptr(post);
   if (live(post)) a.post_dtype = code(post->scalar_type());
@@ -335,12 +343,12 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     Tensor dx_new = grads.size() == 2 ? grads[0] : Tensor(), dh = grads.back();
     if (dx_new.defined()) {
       dx_new = dense_rows(dx_new);
-      a.dx_new = dx_new.data_ptr();
+      a.dx_new = ptr(dx_new);
       a.ld_dx_new = pitch(dx_new);
     }
     if (dh.defined()) {
       dh = dense_rows(dh);
-      a.dh = dh.data_ptr();
+      a.dh = ptr(dh);
       a.ld_dh = pitch(dh);
     }
     variable_list out(7);

@@ -386,3 +386,30 @@ def test_gates_of_wide_rows(gpu, shape, gate, dt):
     """Several gate groups in a block, one and two chunks of columns a thread."""
     v, outs = _inputs(gpu, shape, dt, torch.float32, True, gate, seed=11)
     _check(v, outs, 0.5)
+
+
+class _Wrapped(torch.Tensor):
+    """A tensor that holds another and has no memory itself, as distributed tensors do."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype,
+                                                   device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        out = func(*(t.inner if isinstance(t, _Wrapped) else t for t in args), **(kwargs or {}))
+        return _Wrapped(out) if isinstance(out, torch.Tensor) else out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["x", "y", "pre", "post", "gate"])
+def test_tensors_without_memory_are_refused(gpu, which):
+    """An optional operand must not count as absent."""
+    v, _ = _inputs(gpu, (2, 8), torch.float32, torch.float32, True, (1, 8), seed=12)
+    v[which] = _Wrapped(v[which])
+    with pytest.raises(RuntimeError, match="memory"):
+        _call(v, 1.0)

@@ -730,5 +730,38 @@ def test_the_default_chunks(gpu):
         if i in (0, 30000, 60000, 87000):                          # chunks begin and end here
             (dh, bh), _ = exact.grads(row)
             _within(a.grad[i:i + 3000], dh, bh)
-    assert abs(float(loss) - total / count) <= exact.loss_tol
+    assert abs(float(loss.detach()) - total / count) <= exact.loss_tol
     _within(b.grad[cols], dw, bw + U[h.dtype] * dw.abs() + 1e-30)
+
+
+class _Wrapped(torch.Tensor):
+    """A tensor that holds another and has no memory itself, as distributed tensors do."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype,
+                                                   device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        out = func(*(t.inner if isinstance(t, _Wrapped) else t for t in args), **(kwargs or {}))
+        return _Wrapped(out) if isinstance(out, torch.Tensor) else out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["hidden", "weight", "target", "ids", "logits", "lse"])
+def test_tensors_without_memory_are_refused(gpu, which):
+    """An optional operand must not count as absent."""
+    h, w, t, _ = _inputs(gpu, 4, 10, 8, torch.bfloat16)
+    v = dict(hidden=h, weight=w, target=t, ids=t[:, None], logits=torch.zeros(4, 1, device=gpu),
+             lse=torch.ones(4, device=gpu))
+    v[which] = _Wrapped(v[which])
+    with pytest.raises(RuntimeError, match="memory"):
+        if which == "target":
+            dmuon.linear_cross_entropy(v["hidden"], v["weight"], v["target"])
+        else:
+            dmuon.linear_distillation(v["hidden"], v["weight"], v["ids"], v["logits"],
+                                      teacher_lse=v["lse"])
