@@ -49,8 +49,12 @@ void* ptr(const Tensor& t) {
 }
 void* ptr(const OptTensor& t) { return live(t) ? ptr(*t) : nullptr; }
 
+// Torch may put a view's negation off; the kernels read what lies in memory.
+Tensor dense(const Tensor& t) { return t.resolve_neg().contiguous(); }
+
 // The same matrix with its last dimension contiguous and rows that do not overlap.
 Tensor dense_rows(const Tensor& t) {
+  if (t.is_neg()) return dense(t);
   if ((t.stride(1) == 1 || t.size(1) == 1) && (t.stride(0) >= t.size(1) || t.size(0) <= 1)) return t;
   return t.contiguous();
 }
@@ -151,7 +155,7 @@ struct Loss : torch::CustomClassHolder {
     for (int i = 0; i < 2; ++i)
       if (g[i]->defined())
         out[i] = held == dtype ? *g[i] : at::empty(g[i]->sizes(), g[i]->options().dtype(dtype));
-    const Tensor f = factor.to(at::kFloat).contiguous();
+    const Tensor f = dense(factor.to(at::kFloat));
     call(dmuon_scale_by(ptr(d_hidden), ptr(out[0]), d_hidden.defined() ? d_hidden.numel() : 0,
                         ptr(d_weight), ptr(out[1]), d_weight.defined() ? d_weight.numel() : 0,
                         code(held), code(dtype), static_cast<const float*>(ptr(f)), stream_of(f)));
@@ -179,7 +183,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
     const auto saved = ctx->get_saved_variables();
     s->against(saved[2], saved[3], saved[4], saved[5]);
     if (s->reduction == DMUON_LOSS_ROWS) {
-      s->launch(saved[0], saved[1], true, grads[0].to(at::kFloat).contiguous());
+      s->launch(saved[0], saved[1], true, dense(grads[0].to(at::kFloat)));
     } else {
       // a second pass over a kept graph forms them anew
       if (!s->d_hidden.defined() && !s->d_weight.defined()) s->launch(saved[0], saved[1], true, Tensor());
@@ -222,7 +226,7 @@ Tensor of_tokens(const char* who, const char* name, const Tensor& t, const Tenso
   TORCH_CHECK_VALUE(t.sizes() == at::IntArrayRef(shape), who, ": ", name, " must have the shape ",
                     at::IntArrayRef(shape), ", got ", t.sizes());
   TORCH_CHECK(t.device() == hidden.device(), who, ": ", name, " must live on ", hidden.device());
-  return t.detach().to(integers ? at::kLong : at::kFloat).contiguous();
+  return dense(t.detach().to(integers ? at::kLong : at::kFloat));
 }
 
 Tensor run_loss(const LossPtr& s, const Tensor& hidden, const Tensor& weight) {
@@ -385,7 +389,7 @@ Tensor gate_rows(const char* who, const Tensor& gate, const Tensor& x) {
                     " has no row for each of equal runs of the rows of x ", x.sizes());
   // no row at all: one that no row of x uses, behind the gate's own
   if (gate.numel() == 0) return at::cat({gate.reshape({0, dim}), gate.new_zeros({1, dim})});
-  return gate.dim() == 2 ? gate.contiguous() : gate.reshape({-1, dim}).contiguous();
+  return dense(gate.dim() == 2 ? gate : gate.reshape({-1, dim}));
 }
 
 std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& y, const Tensor& pre,
@@ -423,10 +427,10 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& y, co
   auto here = [&](const OptTensor& t) { return !live(t) || t->device() == x.device(); };
   TORCH_CHECK(x.is_cuda() && here(y) && pre.device() == x.device() && here(post) && here(g), who,
               ": tensors must live on one GPU (HIP kernel only)");
-  const Tensor rows = rows_of(x), w = pre.contiguous();
+  const Tensor rows = rows_of(x), w = dense(pre);
   OptTensor yr, p;
   if (live(y)) yr = rows_of(*y);
-  if (live(post)) p = post->contiguous();
+  if (live(post)) p = dense(*post);
   bool grad = x.requires_grad() || w.requires_grad();
   for (const OptTensor* t : {&yr, &p, &g}) grad = grad || (live(*t) && (*t)->requires_grad());
   const variable_list out = at::GradMode::is_enabled() && grad

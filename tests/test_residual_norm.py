@@ -413,3 +413,18 @@ def test_tensors_without_memory_are_refused(gpu, which):
     v[which] = _Wrapped(v[which])
     with pytest.raises(RuntimeError, match="memory"):
         _call(v, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["x", "y", "pre", "post", "gate"])
+def test_lazily_negated_operands(gpu, which):
+    """A view whose negation torch has put off (as of a conjugate's imaginary part)."""
+    v, outs = _inputs(gpu, (6, 40), torch.float32, torch.float32, True, (2, 40), seed=13)
+    put_off = {**v, which: torch._neg_view(v[which])}
+    assert put_off[which].is_neg()
+    v[which] = -v[which]
+    for a, b in zip(_call(put_off, 0.5), _call(v, 0.5)):
+        assert torch.equal(a, b)
+    grads = [torch.autograd.grad(_call({**v, "x": x}, 0.5), x, [f(o) for o in outs])[0]
+             for f in (torch._neg_view, torch.neg) for x in [v["x"].clone().requires_grad_(True)]]
+    assert torch.equal(*grads)

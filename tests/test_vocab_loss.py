@@ -765,3 +765,29 @@ def test_tensors_without_memory_are_refused(gpu, which):
         else:
             dmuon.linear_distillation(v["hidden"], v["weight"], v["ids"], v["logits"],
                                       teacher_lse=v["lse"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["hidden", "weight", "target", "ids", "logits", "lse"])
+def test_lazily_negated_operands(gpu, which):
+    """A view whose negation torch has put off (as of a conjugate's imaginary part)."""
+    h, w, t, gen = _inputs(gpu, 6, 50, 40, torch.bfloat16, seed=15)
+    v = dict(hidden=h, weight=w, target=t, ids=t[:, None], lse=torch.ones(6, device=gpu),
+             logits=torch.randn(6, 1, device=gpu, generator=gen))
+
+    def call(v):
+        if which == "target":
+            return dmuon.linear_cross_entropy(v["hidden"], v["weight"], v["target"], reduction="none")
+        return dmuon.linear_distillation(v["hidden"], v["weight"], v["ids"], v["logits"],
+                                         teacher_lse=v["lse"], reduction="none")
+
+    put_off = {**v, which: torch._neg_view((-v[which]).contiguous())}
+    assert put_off[which].is_neg()
+    assert torch.equal(call(put_off), call(v))
+    for reduction in ("none", "sum"):
+        grads = []
+        for f in (torch._neg_view, torch.neg):
+            a = h.clone().requires_grad_(True)
+            loss = dmuon.linear_cross_entropy(a, w, t, reduction=reduction)
+            grads += torch.autograd.grad(loss, a, f(torch.ones_like(loss)))
+        assert torch.equal(*grads)
