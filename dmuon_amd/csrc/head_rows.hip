@@ -76,7 +76,6 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uin
                                                            long long ldw, int dim) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float it = 1.f / r.temperature;
-  if (r.peak && blockIdx.x == 0 && threadIdx.x == 0) *r.peak = 0u;
   if (r.targets) {
     const int row = blockIdx.x * 4 + wave;
     if (row >= r.n) return;
@@ -93,6 +92,7 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uin
     r.probs[row] = live ? 1.f : 0.f;
     r.logits[row] = z[0];
     r.mass[row] = !counted ? -1.f : inside ? 1.f : __builtin_nanf("");
+    if (row == 0 && r.peak) *r.peak = 0u;
     return;
   }
   const int row = blockIdx.x;
@@ -109,17 +109,20 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uin
   live = __any(live);
   outside = __any(outside);
   top = wave_max(top);
-  const float under = r.teacher_lse ? r.teacher_lse[row] : 0.f;
-  auto share = [&](float v) {
-    return v == -kInf ? 0.f : expf(r.teacher_lse ? v * it - under : (v - top) * it);
-  };
+  const float from = r.teacher_lse ? 0.f : top, under = r.teacher_lse ? r.teacher_lse[row] : 0.f;
+  auto share = [&](float v) { return expf((v - from) * it - under); };
   float sum = 0.f;
   for (int k = lane; k < r.k_list; k += 64)
-    if (r.teacher_ids[base + k] >= 0) sum += share(r.teacher_logits[base + k]);
+    if (r.teacher_ids[base + k] >= 0) {
+      const float v = r.teacher_logits[base + k];
+      sum += v == -kInf ? 0.f : share(v);
+    }
   sum = wave_sum(sum);
   const float norm = r.teacher_lse ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-  if (wave == 0 && lane == 0)
+  if (wave == 0 && lane == 0) {
     r.mass[row] = !live ? -1.f : outside ? __builtin_nanf("") : r.teacher_lse ? sum : sum * norm;
+    if (row == 0 && r.peak) *r.peak = 0u;
+  }
   // four entries a wave at a time: their loads and sums overlap
   for (int k0 = 4 * wave; k0 < r.k_list; k0 += 16) {
     const uint16_t* w[4];
@@ -129,7 +132,8 @@ __global__ __launch_bounds__(256) void head_targets_kernel(HeadRows r, const uin
     for (int e = 0; e < 4; ++e) {
       const int k = k0 + e < r.k_list ? k0 + e : k0;
       const long long id = r.teacher_ids[base + k];
-      q[e] = id < 0 ? 0.f : share(r.teacher_logits[base + k]) * norm;
+      const float v = r.teacher_logits[base + k];          // padding's too: four loads at a time
+      q[e] = id < 0 || v == -kInf ? 0.f : share(v) * norm;
       cls[e] = id >= 0 && id < r.vocab && q[e] != 0.f ? (int)id : -1;
       w[e] = W + (cls[e] < 0 ? 0 : cls[e]) * ldw;         // an entry without a class: any row
     }
