@@ -6,7 +6,9 @@
 //
 // Between the first product and the others a logit takes two bytes where the operands are bf16:
 // exp(z - m) in fp16, m the maximum of the row's 64 columns, which the row kernel turns into the
-// bf16 gradient in place. Its 2^-11 is small against the 2^-8 of the gradient's own rounding. For
+// bf16 gradient in place. Its 2^-11 is small against the 2^-8 of the gradient's own rounding down to
+// probabilities of 2^-29 of their block's largest; under that fp16 has fewer bits, and under 2^-40
+// none: such a class's share of the gradient, less than 1e-12 of its neighbour's, is left out. For
 // fp16 operands it is not: there the product writes fp32 logits and the gradient has its own place,
 // six bytes a logit.
 #include "../../include/dmuon_amd.h"
@@ -21,7 +23,10 @@ namespace {
 
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// Workspace of a chunk's logits and logit gradient; a call of more tokens takes several chunks.
+// Workspace of a chunk's logits, logit gradient and statistics; a call of more tokens takes several
+// chunks. (In bf16 the weight gradient's fp32 sums over them then take the place of the hidden
+// gradient's parts, whose K is not split: 8192 x 128256 x 4096 in one chunk 19.3 ms, in chunks of 4096
+// 20.2, 2048 24.8, 1024 37.9, 256 118; fp16, whose sums are the result, 22.7, -, 24.6, 28.6, 57.)
 constexpr int64_t kChunkBytes = int64_t(4) << 30;
 
 // Blocks of 64 classes are a grid's second dimension.
@@ -32,6 +37,8 @@ struct Layout {
   int64_t ids, probs, logits, mass, top, loss, row_weight, factor, alpha, peak, Z, stats, G, part, H, W, bytes;
   int64_t pad;                            // pitch of the copies of hidden and weight
   bool copy_h, copy_w;
+  bool gathers, split_h;                  // the weight gradient sums over chunks; the hidden one's K is
+                                          // split: not where those sums have the parts' place
 };
 
 // The products read whole 16-byte chunks of aligned rows; anything else runs on zero-padded copies.
@@ -115,13 +122,15 @@ Layout lay_out(const dmuon_head_loss_args& a) {
   l.Z = grads && f16 ? take(l.chunk * l.ld * 4) : l.G;
   // fp32 sums: the weight's gradient over several chunks, or of split products
   int64_t part = 0;
-  if (a.d_weight && l.chunk < a.tokens) {
-    if (a.grad_dtype != DMUON_DTYPE_F32) part = a.vocab * a.dim * 4;
+  l.gathers = a.d_weight && l.chunk < a.tokens;
+  l.split_h = !l.gathers || a.grad_dtype == DMUON_DTYPE_F32;
+  if (l.gathers) {
+    if (!l.split_h) part = a.vocab * a.dim * 4;
   } else if (a.d_weight) {
     const int s = head_gemm_splits((int)a.vocab, (int)a.dim, (int)a.tokens, true);
     if (s > 1) part = s * a.vocab * a.dim * 4;
   }
-  if (a.d_hidden)
+  if (a.d_hidden && l.split_h)
     for (int64_t rows : {l.chunk, l.chunk > 0 ? a.tokens % l.chunk : 0}) {
       const int s = head_gemm_splits((int)rows, (int)a.dim, (int)a.vocab, false);
       if (s > 1 && s * rows * a.dim * 4 > part) part = s * rows * a.dim * 4;
@@ -199,8 +208,6 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
   const uint16_t* H = static_cast<const uint16_t*>(a.hidden);
   const uint16_t* W = static_cast<const uint16_t*>(a.weight);
 
-  // the fp32 sums' place is free for split products where no weight gradient gathers in it
-  const bool gathers = a.d_weight && l.chunk < a.tokens, split_h = !gathers || grad_size == 4;
   int64_t ldw = a.ld_weight;
   if (l.copy_w) {
     W = reinterpret_cast<const uint16_t*>(ws + l.W);
@@ -249,7 +256,7 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
         g.A = G; g.lda = rows;
         g.B = W; g.ldb = ldw; g.b_kmajor = 1;
         g.M = rows; g.N = (int)a.dim; g.K = (int)a.vocab;
-        g.splits = split_h ? head_gemm_splits(rows, g.N, g.K, false) : 1;
+        g.splits = l.split_h ? head_gemm_splits(rows, g.N, g.K, false) : 1;
         g.part = floats(l.part); g.ldp = a.dim;
         g.out = static_cast<char*>(a.d_hidden) + first * a.dim * grad_size; g.ldo = a.dim;
         g.join_later = a.d_weight && head_joins_later(g, (int)a.vocab);
@@ -263,10 +270,10 @@ int dmuon_head_loss(const dmuon_head_loss_args* args, void* workspace, int64_t w
         g.A = G; g.lda = rows; g.a_kmajor = 1;
         g.B = Hc; g.ldb = ldh; g.b_kmajor = 1;
         g.M = (int)a.vocab; g.N = (int)a.dim; g.K = rows;
-        g.splits = gathers ? 1 : head_gemm_splits(g.M, g.N, g.K, true);
+        g.splits = l.gathers ? 1 : head_gemm_splits(g.M, g.N, g.K, true);
         g.out = last ? a.d_weight : nullptr; g.ldo = a.dim;
         // fp32 results gather in place
-        g.part = gathers && grad_size == 4 ? static_cast<float*>(a.d_weight) : floats(l.part);
+        g.part = l.gathers && grad_size == 4 ? static_cast<float*>(a.d_weight) : floats(l.part);
         g.ldp = a.dim;
         g.add_part = first > 0;
         if (check_launch(launch_head_gemm(g, stream), who)) return 1;

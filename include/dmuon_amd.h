@@ -454,7 +454,8 @@ int dmuon_clip_norms(const int64_t* ptrs, const int64_t* numels, const int32_t* 
  *     probabilities q of the k_list classes teacher_ids[n][..] -- the softmax of their
  *     teacher_logits / temperature, or exp(teacher_logits / temperature - teacher_lse[n]) where
  *     the teacher's own log-sum-exp (of logits / temperature) is given --
- *     loss[n] = temperature^2 * sum_k q_k (log q_k - log p[id_k]). Negative ids are padding; a
+ *     loss[n] = temperature^2 * sum_k q_k (log q_k - log p[id_k]); temperature and its inverse are
+ *     positive and finite. Negative ids are padding; a
  *     token with padding only is not counted and has loss 0. A class that occurs twice counts
  *     twice.
  * Any other class outside [0, vocab) gives the token a NaN loss. The logits are never held: rows
@@ -468,9 +469,16 @@ int dmuon_clip_norms(const int64_t* ptrs, const int64_t* numels, const int32_t* 
  * hidden and weight are 16-bit words of `dtype` (DMUON_DTYPE_BF16 or _F16), row by row with their
  * pitches in elements, at any element alignment; products accumulate in fp32, and the logit
  * gradient is rounded once to `dtype` between the products. loss [tokens] may be NULL with a
- * reduction. Results do not depend on anything but the arguments (no atomics). chunk_tokens: tokens worked on at a
- * time (0: a size that keeps the workspace near 4 GiB); a workspace of
- * dmuon_head_loss_workspace_size bytes (256-byte aligned) is the caller's.
+ * reduction. Results do not depend on anything but the arguments, and a loss's bits not on
+ * chunk_tokens. fp16 logit gradients share a smaller scale where a row's |mass + 2 z_loss lse| + mass,
+ * times its share of the largest row_grad, reaches 32.
+ * chunk_tokens: tokens worked on at a time, past 256 in whole 256 (0: as many as keep a chunk's logits,
+ * logit gradient and statistics within 4 GiB). The workspace, dmuon_head_loss_workspace_size bytes at
+ * 256-byte alignment, is the caller's: a chunk's 2 bytes a logit (bf16) or 6 (fp16; without gradients
+ * none) and 8 bytes per 64 logits; per token of the call 20 bytes and 12 for each entry of its list;
+ * and as far as the call has them the larger of the fp32 sums of a 16-bit weight gradient over several
+ * chunks and the fp32 parts of products split over K, and 2 bytes a value for copies of the weight and
+ * of a chunk's hidden states where their rows are not whole 16-byte chunks at 16-byte alignment.
  */
 #define DMUON_LOSS_ROWS 0
 #define DMUON_LOSS_MEAN 1

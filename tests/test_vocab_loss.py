@@ -791,3 +791,29 @@ def test_lazily_negated_operands(gpu, which):
             loss = dmuon.linear_cross_entropy(a, w, t, reduction=reduction)
             grads += torch.autograd.grad(loss, a, f(torch.ones_like(loss)))
         assert torch.equal(*grads)
+
+
+@pytest.mark.parametrize("n,v,d,k", [(8192, 128256, 4096, 0), (20000, 128256, 4096, 0),
+                                     (20000, 128256, 4100, 0), (65536, 128256, 4096, 4096),
+                                     (90000, 50000, 64, 0)])
+def test_the_workspace_is_what_is_documented(n, v, d, k):
+    """A chunk's logits, gradient and statistics within 4 GiB, and the terms beside them: the weight
+    gradient's fp32 sums over several chunks, padded copies, a few bytes a token and list entry."""
+    import ctypes
+
+    from dmuon_amd import _C
+    need = ctypes.c_int64()
+    what = dict(teacher_ids=4096, teacher_logits=4096, k_list=k) if k else dict(targets=4096)
+    a = _C.HeadLossArgs(dtype=1, grad_dtype=1, reduction=1, tokens=n, vocab=v, dim=d, ld_hidden=d,
+                        ld_weight=d, hidden=4096, weight=4096, reduced=4096, d_hidden=4096,
+                        d_weight=4096, temperature=1.0, **what)
+    assert _C.lib().dmuon_head_loss_workspace_size(ctypes.byref(a), ctypes.byref(need)) == 0
+    row = -(-v // 64) * (64 * 2 + 8)
+    most = (4 << 30) // row
+    chunks = -(-n // most)
+    chunk = min(n, -(-(-(-n // chunks)) // 256) * 256) if chunks > 1 else n
+    assert chunk * row <= 4 << 30
+    pad = -(-d // 64) * 64
+    total = chunk * row + n * (20 + 12 * max(k, 1)) + (4 * v * d if chunks > 1 else 0) + \
+        (2 * (v + chunk) * pad if d % 8 else 0)
+    assert total <= need.value <= total + 16 * 256
