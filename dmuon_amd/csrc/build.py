@@ -22,8 +22,8 @@ SOURCES = ["ns_gemm.hip", "gram_small.hip", "ew_kernels.hip", "adamw.hip", "clip
 LIB_NAME = "libdmuon_amd.so"
 ARCH = "gfx950"
 
-# -packed-fp32-ops: keep hipcc from emitting v_pk_{add,mul,fma}_f32 (unreliable on the target
-# pool); the host pass prints a harmless "not a recognized feature" warning for it.
+# -packed-fp32-ops: keep hipcc from emitting v_pk_{add,mul,fma}_f32 (some forms have given wrong
+# results on the target machines); the host pass prints a harmless "not a recognized feature" warning for it.
 FLAGS = [
     f"--offload-arch={ARCH}",
     "-O3",

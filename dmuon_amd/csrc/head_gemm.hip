@@ -440,7 +440,7 @@ __device__ __forceinline__ void join_splits(const HeadGemm& a, int block, int bl
 }
 
 // A weight gradient over few tokens: bound by writing it. 128 x 128 tiles, four waves of 64 x 64, one
-// K slice in LDS at a time; four blocks a CU hide each other's waits, where a 256-tile of a slice or
+// K slice in LDS at a time; three blocks a CU (148 registers) hide each other's waits, where a 256-tile of a slice or
 // two waits alone for its first loads and its stores (see weight_is_short). 64 tokens x 128256 x
 // 4096: 226 us, 4.7 TB/s. The first `joins` blocks (whole eights, so that the others stay on their
 // XCDs) join the hidden gradient's parts, `h`.

@@ -19,8 +19,18 @@
 // gradients add up in registers too, and each block writes one partial row, which a second kernel
 // sums in a fixed order.
 //
-// bf16, with the weights' gradients: 16384 x 4096 forward 104 us (5.2 TB/s), backward 156 + 8 (4.9);
-// 8192 x 8192 105 and 160; 13328 x 6030, of rows off the vectors' alignment, 168 and 255.
+// With the weights' gradients, forward and backward in TB/s: bf16 16384 x 4096 100 and 174 us (5.4 and
+// 4.6), 8192 x 8192 104 and 161 (5.2, 5.0), 32768 x 2048 5.2 and 4.4; fp32 16384 x 4096 228 and 446
+// (4.7, 3.6). Widths whose blocks of 64 to 768 threads leave a part of a CU's waves empty are slower,
+// whatever their rows' alignment: bf16 13328 x 6032 164 and 250 us (3.9, 3.9), x 6030 167 and 253,
+// 40000 x 1008 4.2 and 4.0, x 1002 4.1 and 3.9; 12288 x 5120 4.2 and 4.8. A gate per token 5.4 and 3.9
+// (16384 x 4096), without a block's output 5.4 and 5.0.
+//
+// Registers: 128 where a block may have 1024 threads. The forward kernel of two chunks spills 29 in
+// fp32 and none in 16 bits; the backward kernel of one row a block 24 in fp32 (70 with several gate
+// groups a block) and 5 (12) in 16 bits; of two chunks 385 to 597, which costs rows past 8192 columns
+// three quarters of the rate: 2048 x 16384 297 us in bf16 (1.4 TB/s), 493 in fp32. Several rows a block
+// spill none.
 #include "../../include/dmuon_amd.h"
 #include "dmuon_amd_internal.h"
 #include "mfma_tile.h"
@@ -194,10 +204,8 @@ __device__ __forceinline__ void load_factors(const ResidualNorm& a, long long gr
   }
 }
 
-// NV chunks of 8 columns a thread (two in 1024 threads spill registers in the backward pass: rows
-// past 8192 columns take 285 us for 2048 x 16384, a third of the rate of shorter ones). MANY: several
-// rows side by side in 256 threads; otherwise the row is the same for the block and its addresses
-// stay scalar.
+// NV chunks of 8 columns a thread. MANY: several rows side by side in 256 threads; otherwise the row is
+// the same for the block and its addresses stay scalar.
 template <int T, int NV, bool MANY>
 __global__ __launch_bounds__(MANY ? 256 : 1024) void residual_norm_kernel(ResidualNorm a) {
   __shared__ float lds[4][4][16][1];

@@ -147,7 +147,9 @@ struct Loss : torch::CustomClassHolder {
     return loss;
   }
 
-  // d_hidden and d_weight times `factor` in the operands' type, in place where they have it.
+  // d_hidden and d_weight times `factor` in the operands' type, in place where they have it: bf16
+  // gradients, rounded when they were formed, round a second time for a factor that is no power of two
+  // (2^-8 again; holding them in fp32 would take twice their memory from one pass to the other).
   void scale(const Tensor& factor, at::ScalarType dtype) {
     const c10::DeviceGuard guard(factor.device());
     Tensor* g[2] = {&d_hidden, &d_weight};

@@ -33,7 +33,8 @@ def residual_norm(x: Tensor, y: Optional[Tensor], pre_weight: Tensor, *,
     ``x.shape``: per token); for a two-dimensional ``x`` it may be ``[g, dim]``, one row for every
     ``rows / g`` consecutive rows. Arithmetic is fp32 and every result is rounded once; the
     gradients of the weights and of a shared gate sum in a fixed order, and have no gradients of their
-    own. Can be captured into a graph.
+    own. Dual tensors (forward-mode gradients), tracers and wrapper subclasses raise. Can be captured
+    into a graph.
     """
     return _C.torch_ops().residual_norm(x, y, pre_weight, post_weight, gate, float(residual_scale),
                                         float(eps), _MAX_DIM)
