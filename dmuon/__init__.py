@@ -18,7 +18,7 @@ from dmuon_amd import __all__  # noqa: F401
 _SUBMODULES = (
     "api", "utils", "fast_clip", "grad_clip", "optim", "optim.muon", "optim.newton_schulz",
     "optim.syrk_dispatch", "optim.adamw", "_backends", "_backends.local",
-    "_backends.local.param", "vocab_loss", "norms",
+    "_backends.local.param", "vocab_loss", "norms", "heads", "lookup",
 )
 for _name in _SUBMODULES:
     sys.modules[f"{__name__}.{_name}"] = importlib.import_module(f"dmuon_amd.{_name}")
@@ -29,4 +29,6 @@ grad_clip = dmuon_amd.grad_clip
 optim = dmuon_amd.optim
 vocab_loss = dmuon_amd.vocab_loss
 norms = dmuon_amd.norms
+heads = dmuon_amd.heads
+lookup = dmuon_amd.lookup
 del _name

@@ -27,7 +27,7 @@ NS_GRAM = 1
 # DMUON_ABI_VERSION of include/dmuon_amd.h: the argument lists below are those of this
 # version, and a library that reports another one is refused (its entry points would be
 # called with the wrong arguments).
-ABI_VERSION = 110
+ABI_VERSION = 111
 
 MAX_GROUPS = 8         # DMUON_MAX_GROUPS
 
@@ -71,6 +71,47 @@ class ResidualNormArgs(ctypes.Structure):
 
 
 c_np = ctypes.POINTER(ResidualNormArgs)
+
+class AttentionArgs(ctypes.Structure):
+    """``dmuon_attention_args``: one call of attention over heads."""
+
+    _fields_ = [(k, c_vp) for k in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv",
+                                    "kv_lengths", "q_starts", "kv_starts")] + \
+        [(k, c_i64) for k in ("batch", "q_len", "kv_len", "heads", "kv_heads", "dim", "window",
+                              "q_batch", "q_token", "q_head", "k_batch", "k_token", "k_head",
+                              "v_batch", "v_token", "v_head", "do_batch", "do_token", "do_head")] + \
+        [("scale", c_f), ("causal", c_int), ("dtype", c_int)]
+
+
+c_ap = ctypes.POINTER(AttentionArgs)
+
+
+class RotaryHeadsArgs(ctypes.Structure):
+    """``dmuon_rotary_heads_args``: one call of the heads' norms and rotation."""
+
+    _fields_ = [(k, c_vp) for k in ("q", "k", "positions", "inv_freq", "q_weight", "k_weight",
+                                    "q_out", "k_out", "dq_out", "dk_out", "dq", "dk", "d_q_weight",
+                                    "d_k_weight")] + \
+        [(k, c_i64) for k in ("tokens", "period", "heads", "kv_heads", "dim", "rotary_dim", "q_token",
+                              "q_head", "k_token", "k_head", "dq_out_token", "dq_out_head",
+                              "dk_out_token", "dk_out_head")] + \
+        [("eps", c_f)] + \
+        [(k, c_int) for k in ("interleaved", "inv_freq_double", "dtype", "q_weight_dtype",
+                              "k_weight_dtype")]
+
+
+c_rp = ctypes.POINTER(RotaryHeadsArgs)
+
+
+class EmbeddingArgs(ctypes.Structure):
+    """``dmuon_embedding_args``: one call of the token lookup."""
+
+    _fields_ = [(k, c_vp) for k in ("tokens", "weight", "out", "dy", "d_weight")] + \
+        [(k, c_i64) for k in ("tokens_n", "vocab", "dim", "ld_weight", "ld_dy", "padding_idx")] + \
+        [("scale", c_f), ("dtype", c_int)]
+
+
+c_ep = ctypes.POINTER(EmbeddingArgs)
 
 # name -> (restype, argtypes); mirrors include/dmuon_amd.h
 _SIGNATURES = {
@@ -151,6 +192,16 @@ _SIGNATURES = {
     "dmuon_residual_norm": (c_int, [c_np, c_vp]),
     "dmuon_residual_norm_grad_workspace_size": (c_int, [c_np, ctypes.POINTER(c_i64)]),
     "dmuon_residual_norm_grad": (c_int, [c_np, c_vp, c_i64, c_vp]),
+    "dmuon_attention_workspace_size": (c_int, [c_ap, ctypes.POINTER(c_i64)]),
+    "dmuon_attention": (c_int, [c_ap, c_vp, c_i64, c_vp]),
+    "dmuon_attention_grad_workspace_size": (c_int, [c_ap, ctypes.POINTER(c_i64)]),
+    "dmuon_attention_grad": (c_int, [c_ap, c_vp, c_i64, c_vp]),
+    "dmuon_rotary_heads": (c_int, [c_rp, c_vp]),
+    "dmuon_rotary_heads_grad_workspace_size": (c_int, [c_rp, ctypes.POINTER(c_i64)]),
+    "dmuon_rotary_heads_grad": (c_int, [c_rp, c_vp, c_i64, c_vp]),
+    "dmuon_embedding": (c_int, [c_ep, c_vp]),
+    "dmuon_embedding_grad_workspace_size": (c_int, [c_ep, ctypes.POINTER(c_i64)]),
+    "dmuon_embedding_grad": (c_int, [c_ep, c_vp, c_i64, c_vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -2,8 +2,9 @@
 world_size=1 (``import dmuon_amd as dmuon``).
 
 Exports the names of X-Square-Robot/dmuon's ``dmuon/__init__.py:80-122`` that concern the
-owner-rank update path, and operators of the step that leads up to it: the losses over a large
-vocabulary with their gradients and the norms around a block. The compute runs in ``dmuon_amd/csrc/libdmuon_amd.so`` (HIP, gfx950);
+owner-rank update path, and operators of the step that leads up to it: the token lookup, attention with
+its heads' norms and rotation, the norms around a block and the losses over a large vocabulary, each with
+its gradients. The compute runs in ``dmuon_amd/csrc/libdmuon_amd.so`` (HIP, gfx950);
 there is no CPU fallback.
 """
 from .api import dedicate_params, replicate
@@ -15,7 +16,9 @@ from .fast_clip import (
     try_clip_optimizer_grad_norm_buckets_,
 )
 from .grad_clip import MuonGradClipStats, clip_grad_norm_, register_muon_grad_clip_strategy
-from .norms import residual_norm
+from .heads import attention
+from .lookup import embedding
+from .norms import residual_norm, rotary_heads
 from .optim import (
     KELLER_COEFFICIENTS,
     POLAR_EXPRESS_COEFFICIENTS,
@@ -55,4 +58,5 @@ __all__ = [
     "register_muon_grad_clip_strategy", "MuonGradClipStats", "GradClipBucket",
     "GradClipBucketStats", "SegmentedGradClipResult",
     "linear_cross_entropy", "linear_distillation", "residual_norm",
+    "attention", "rotary_heads", "embedding",
 ]

@@ -1,0 +1,429 @@
+// The gradients of attention over heads on gfx950. With S = c q k^T, P = exp2(S log2(e) - lse) formed
+// anew and delta = sum of do o over a row:
+//   dv = P^T do,  dP = do v^T,  dS = P (dP - delta),  dq = scale dS k,  dk = scale dS^T q
+// Two kernels, one over keys (dk, dv) and one over queries (dq), each with its sums in registers: seven
+// products where one pass would do with five, but no sums over blocks, so no atomics and one order.
+//
+// P and dS are rounded to the operands' type between the products. In fp16 they are held times powers of
+// two: P times 2^10 (a long row's probabilities are under the type's normal range) and dS by a further one
+// that the largest rows of do and v set, so that it neither over- nor underflows with a loss scale or a
+// row's length.
+#include "attention.h"
+
+namespace dmuon {
+namespace {
+
+constexpr int kTile = 64;                 // rows or keys of a tile in LDS
+constexpr float kInf = __builtin_inff();
+
+template <int E>
+constexpr float kShift = E == ELT_F16 ? 10.f : 0.f;
+
+// The power of two of dS: |dS| 2^kShift <= 2 |do| |v| 2^10 P times it stays under 2^15.
+template <int E>
+__device__ __forceinline__ float ds_scale(const Attention& a) {
+  if constexpr (E != ELT_F16) return 1.f;
+  const float most = 2.f * sqrtf(__uint_as_float(a.peaks[0])) * sqrtf(__uint_as_float(a.peaks[1]));
+  if (!(most > 0.f)) return 1.f;
+  int e = 5 - __builtin_amdgcn_frexp_expf(most);           // most < 2^frexp
+  e = e > 60 ? 60 : e < -60 ? -60 : e;
+  return __uint_as_float((unsigned)(127 + e) << 23);
+}
+
+template <int E>
+__device__ __forceinline__ bf16x8_t pack8(const f32x16_t& v, int from) {
+  u32x4_t w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack2_elt<E>(v[from + 2 * i], v[from + 2 * i + 1]);
+  return __builtin_bit_cast(bf16x8_t, w);
+}
+
+// A row's share of a transposed result: values result_row(i, h) of each 32
+template <int E, int DB>
+__device__ __forceinline__ void store_turned(uint16_t* out, const f32x16_t* v, float f, int h, int dim) {
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = 32 * b + result_row(i, h);
+      if (d < dim)
+        *reinterpret_cast<u32x2_t*>(out + d) = u32x2_t{pack2_elt<E>(v[b][i] * f, v[b][i + 1] * f),
+                                                       pack2_elt<E>(v[b][i + 2] * f, v[b][i + 3] * f)};
+    }
+}
+
+// Moves 64 rows of queries (row r is query r / group of head r % group) into LDS, 4 waves together.
+template <int D>
+struct RowMover {
+  static constexpr int CPR = D / 8, RPI = 64 / CPR, N = kTile / RPI / 4;
+  int wave, row, chunk;
+  __device__ __forceinline__ void init(int wave_, int lane) {
+    wave = wave_;
+    row = wave * N * RPI + lane / CPR;    // of instruction 0
+    chunk = lane % CPR;
+  }
+  // rows r0 .. r0 + 63 of p (the key head's first head), of which those under `end` are there
+  __device__ __forceinline__ void issue(const uint16_t* p, long long token, long long head, int group,
+                                        unsigned magic, int dim, int r0, int end, char* lds) const {
+    typedef __attribute__((address_space(3))) void* lds_ptr_t;
+    const int q0 = r0 / group, rem = r0 - q0 * group;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(p + q0 * token), (short)0, 0x7fffffff, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = row + i * RPI, x = rem + r;
+      const int q = (int)(group == 1 ? (unsigned)x : __umulhi((unsigned)x, magic));
+      const int c = chunk ^ slot_mask<D>(r);
+      unsigned off = (unsigned)(q * (int)token + (x - q * group) * (int)head) * 2u + (unsigned)c * 16u;
+      if (r0 + r >= end || c * 8 >= dim) off = kNowhere;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (wave * N + i) * 1024), 16, off, 0,
+                                               0, 0);
+    }
+  }
+};
+
+// delta of every row, and in fp16 the largest row of do. 16 lanes a row, 8 values each.
+template <int E>
+__global__ __launch_bounds__(256) void attention_delta_kernel(const Attention a, unsigned* peaks) {
+  const long long rows = (long long)a.q_len * a.heads * (a.seqs ? 1 : a.batch);
+  const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int at = 8 * (threadIdx.x & 15);
+  float s = 0.f, n = 0.f;
+  if (row < rows && at < a.dim) {
+    const long long token = row / a.heads, b = a.seqs ? 0 : token / a.q_len;
+    const int head = (int)(row - token * a.heads);
+    const uint16_t* d = a.dout + b * a.do_batch + (token - b * a.q_len) * a.do_token + head * a.do_head + at;
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(d);
+    const u32x4_t y = *reinterpret_cast<const u32x4_t*>(a.out + row * a.dim + at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t u = (uint16_t)(i & 1 ? x[i / 2] >> 16 : x[i / 2]);
+      const uint16_t w = (uint16_t)(i & 1 ? y[i / 2] >> 16 : y[i / 2]);
+      const float f = from_elt<E>(u);
+      s += f * from_elt<E>(w);
+      n += f * f;
+    }
+  }
+  for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o), n += __shfl_xor(n, o);
+  const bool live = row < rows;
+  if (live && (threadIdx.x & 15) == 0) a.delta[row] = s;
+  if constexpr (E == ELT_F16) {
+    // a maximum, which no order shows in; rows that see nothing, or of no numbers, do not count
+    float most = live && a.lse[row] < kInf && n < kInf ? n : 0.f;
+    for (int o = 16; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+    if ((threadIdx.x & 63) == 0 && most > 0.f) atomicMax(peaks, __float_as_uint(most));
+  }
+}
+
+// fp16: the largest row of v among those that a query may see
+__global__ __launch_bounds__(256) void attention_value_peak_kernel(const Attention a, unsigned* peak) {
+  const int batch = a.seqs ? 1 : a.batch;
+  const long long rows = (long long)a.kv_len * a.kv_heads * batch;
+  const int at = 8 * (threadIdx.x & 15);
+  float most = 0.f;
+  for (long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); row < rows;
+       row += (long long)gridDim.x * 16) {
+    const long long token = row / a.kv_heads, b = token / a.kv_len, j = token - b * a.kv_len;
+    const int head = (int)(row - token * a.kv_heads);
+    bool live = true;
+    if (a.kv_lengths) live = j < a.kv_lengths[b];
+    if (a.seqs) live = j >= a.seqs[a.batch + 2].kn && j < a.seqs[a.batch + 3].k0;
+    float n = 0.f;
+    if (live && at < a.dim) {
+      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(
+          a.v + b * a.v_batch + j * a.v_token + head * a.v_head + at);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = from_elt<ELT_F16>((uint16_t)(i & 1 ? x[i / 2] >> 16 : x[i / 2]));
+        n += f * f;
+      }
+    }
+    for (int o = 1; o < 16; o <<= 1) n += __shfl_xor(n, o);
+    if (n < kInf) most = fmaxf(most, n);
+  }
+  for (int o = 16; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+  if ((threadIdx.x & 63) == 0 && most > 0.f) atomicMax(peak, __float_as_uint(most));
+}
+
+__global__ void attention_clear_kernel(unsigned* peaks) {
+  if (threadIdx.x < 2) peaks[threadIdx.x] = 0u;
+}
+
+// dk and dv of 128 keys, 32 a wave and one a lane: S = Q K^T and dP = dO V^T leave a lane 16 rows of every
+// 32 for its key, which go as they are into dV^T = dO^T P and dK^T = Q^T dS.
+template <int E, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void attention_keys_kernel(const Attention a) {
+  constexpr int KS = D / 16, DB = D / 32, TILE = kTile * D * 2, SLOT = 2 * TILE + 2 * kTile * 4;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * SLOT];
+  const Place p = place_of<true>(a, false);
+  if (!p.live) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int j0 = p.tile * kKeyRows, j = j0 + wave * 32 + (lane & 31);
+  const int rows = p.qn * a.group, before = p.kn - p.qn;
+
+  bf16x8_t kf[KS], vf[KS];
+  const bool key_live = j < p.kn;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int at = 16 * s + 8 * h;
+    kf[s] = vf[s] = bf16x8_t{};
+    if (key_live && at < a.dim) {
+      kf[s] = *reinterpret_cast<const bf16x8_t*>(a.k + p.k_off + j * a.k_token + at);
+      vf[s] = *reinterpret_cast<const bf16x8_t*>(a.v + p.v_off + j * a.v_token + at);
+    }
+  }
+  // rows that see a key: its own, and those of all keys of the block
+  auto rows_of = [&](int key, int* lo, int* hi) {
+    *lo = 0;
+    *hi = p.qn;
+    if (a.causal) {
+      if (key - before > 0) *lo = key - before;
+      if (a.window && key - before + a.window < p.qn) *hi = key - before + a.window;
+    }
+  };
+  const int last_key = j0 + kKeyRows < p.kn ? j0 + kKeyRows - 1 : p.kn - 1;
+  int lo, hi, first_lo, first_hi, last_lo, last_hi;
+  rows_of(j, &lo, &hi);
+  if (!key_live) hi = 0;
+  lo *= a.group;
+  hi = hi > 0 ? hi * a.group : 0;
+  rows_of(j0, &first_lo, &first_hi);
+  rows_of(last_key, &last_lo, &last_hi);
+  const int r_lo = first_lo * a.group, r_hi = last_hi > 0 ? last_hi * a.group : 0;
+  // rows that see every key of the block need no mask
+  const int full_lo = last_lo * a.group;
+  const int full_hi = last_key == j0 + kKeyRows - 1 ? first_hi * a.group : 0;
+  const int n = r_hi > r_lo && j0 < p.kn ? (r_hi - r_lo + kTile - 1) / kTile : 0;
+
+  RowMover<D> mover;
+  mover.init(wave, lane);
+  const unsigned magic = (unsigned)(0x100000000ULL / (unsigned)a.group + 1);
+  const long long row0 = p.q_row * a.heads + (long long)p.kvh * a.group;
+  auto fetch = [&](int t, char* to) __attribute__((always_inline)) {
+    typedef __attribute__((address_space(3))) void* lds_ptr_t;
+    const int r0 = r_lo + t * kTile;
+    mover.issue(a.q + p.q_off, a.q_token, a.q_head, a.group, magic, a.dim, r0, rows, to);
+    mover.issue(a.dout + p.do_off, a.do_token, a.do_head, a.group, magic, a.dim, r0, rows, to + TILE);
+    if (wave < 2) {
+      // lse (wave 0) and delta (wave 1) of the rows
+      const int q0 = r0 / a.group, x = r0 - q0 * a.group + lane;
+      const int q = (int)(a.group == 1 ? (unsigned)x : __umulhi((unsigned)x, magic));
+      const float* src = (wave == 0 ? a.lse : a.delta) + row0 + (long long)q0 * a.heads;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<float*>(src), (short)0, 0x7fffffff, 0x00020000);
+      unsigned off = (unsigned)(q * a.heads + (x - q * a.group)) * 4u;
+      if (r0 + lane >= rows) off = kNowhere;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(to + 2 * TILE + wave * kTile * 4), 4, off, 0,
+                                               0, 0);
+    }
+  };
+  const int row_at = row_form<D>(lane), turn_at = turned_form<D>(lane);
+  const float sigma = ds_scale<E>(a);
+  f32x16_t dk[DB], dv[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b) dk[b] = dv[b] = f32x16_t{};
+
+  auto step = [&](int t, const char* __restrict__ qt, char* __restrict__ next) __attribute__((always_inline)) {
+    const char* dt = qt + TILE;
+    const float* stats = reinterpret_cast<const float*>(qt + 2 * TILE);
+    if (t + 1 < n) fetch(t + 1, next);
+    const int r0 = r_lo + t * kTile;
+    const bool masked = r0 < full_lo || r0 + kTile > full_hi;
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      f32x16_t s = {}, dp = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int at = y * 64 * D + (row_at ^ (32 * k));
+        s = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(qt + at), kf[k], s);
+        dp = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(dt + at), vf[k], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int r = 32 * y + result_row(i, h);
+        const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(stats + r);
+        const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(stats + kTile + r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + e], a.c, kShift<E> - lse[e]));
+          dp[i + e] = s[i + e] * ((dp[i + e] - delta[e]) * sigma);
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = r0 + 32 * y + result_row(i, h);
+          const bool seen = r >= lo && r < hi;
+          s[i] = seen ? s[i] : 0.f;
+          dp[i] = seen ? dp[i] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bf16x8_t pf = pack8<E>(s, 8 * u), sf = pack8<E>(dp, 8 * u);
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          const int at = (2 * y + u) * 32 * D;
+          dv[b] = mfma_32x32x16<E>(read_turned<D>(dt + at, turn_at ^ (64 * b)), pf, dv[b]);
+          dk[b] = mfma_32x32x16<E>(read_turned<D>(qt + at, turn_at ^ (64 * b)), sf, dk[b]);
+        }
+      }
+    }
+  };
+  if (n > 0) fetch(0, lds);
+  for (int t = 0; t < n; ++t) {
+    wait_vmcnt<0>();
+    bare_barrier();
+    step(t, lds + (t & 1) * SLOT, lds + ((t & 1) ^ 1) * SLOT);
+  }
+  // keys past a sequence's own, up to the tensor's, have no gradient
+  const int most = a.seqs ? p.kn : a.kv_len;
+  if (j < most) {
+    const long long at = ((p.k_row + j) * a.kv_heads + p.kvh) * a.dim;
+    constexpr float down = E == ELT_F16 ? 1.f / 1024.f : 1.f;
+    if (a.dk) store_turned<E, DB>(a.dk + at, dk, a.scale * down / sigma, h, a.dim);
+    if (a.dv) store_turned<E, DB>(a.dv + at, dv, down, h, a.dim);
+  }
+}
+
+// dq of 128 rows, 32 a wave and one a lane: S^T = K Q^T and dP^T = V dO^T, dQ^T = K^T dS^T.
+template <int E, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void attention_queries_kernel(const Attention a) {
+  constexpr int KS = D / 16, DB = D / 32, TILE = kTile * D * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
+  const Place p = place_of<false>(a, a.causal);
+  if (!p.live) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int r0 = p.tile * kQueryRows, rows = p.qn * a.group;
+  const int r = r0 + wave * 32 + (lane & 31);
+  const bool live = r < rows;
+  const int query = r / a.group, head = r - query * a.group;
+  const long long row = (p.q_row + query) * a.heads + (long long)p.kvh * a.group + head;
+  bf16x8_t qf[KS], df[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int at = 16 * s + 8 * h;
+    qf[s] = df[s] = bf16x8_t{};
+    if (live && at < a.dim) {
+      qf[s] = *reinterpret_cast<const bf16x8_t*>(a.q + p.q_off + query * a.q_token + head * a.q_head + at);
+      df[s] = *reinterpret_cast<const bf16x8_t*>(a.dout + p.do_off + query * a.do_token + head * a.do_head + at);
+    }
+  }
+  const float lse = live ? a.lse[row] : kInf, delta = live ? a.delta[row] : 0.f;
+  const Sight see = live ? sight_of(a, p, query) : Sight{0, 0};
+  const int last_row = r0 + kQueryRows < rows ? r0 + kQueryRows - 1 : rows - 1;
+  const Sight first = sight_of(a, p, r0 / a.group), last = sight_of(a, p, last_row / a.group);
+  const int t0 = first.lo / kTile, t1 = (last.hi + kTile - 1) / kTile;
+  const int full_lo = last.lo, full_hi = last_row == r0 + kQueryRows - 1 ? first.hi : 0;
+
+  TileMover<D, kTile, 4> mk, mv;
+  mk.init(a.k_token, a.dim, wave, lane);
+  mv.init(a.v_token, a.dim, wave, lane);
+  auto fetch = [&](int t, char* to) __attribute__((always_inline)) {
+    const int j0 = t * kTile;
+    mk.issue(a.k + p.k_off + j0 * a.k_token, a.k_token, a.dim, p.kn - j0, to);
+    mv.issue(a.v + p.v_off + j0 * a.v_token, a.v_token, a.dim, p.kn - j0, to + TILE);
+  };
+  const int row_at = row_form<D>(lane), turn_at = turned_form<D>(lane);
+  const float sigma = ds_scale<E>(a);
+  f32x16_t dq[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b) dq[b] = f32x16_t{};
+  auto step = [&](int t, const char* __restrict__ kt, char* __restrict__ next) __attribute__((always_inline)) {
+    const char* vt = kt + TILE;
+    if (t + 1 < t1) fetch(t + 1, next);
+    const int j0 = t * kTile;
+    const bool masked = j0 < full_lo || j0 + kTile > full_hi;
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      f32x16_t s = {}, dp = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int at = y * 64 * D + (row_at ^ (32 * k));
+        s = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(kt + at), qf[k], s);
+        dp = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(vt + at), df[k], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        dp[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kShift<E> - lse)) *
+                ((dp[i] - delta) * sigma);
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = j0 + 32 * y + result_row(i, h);
+          dp[i] = j >= see.lo && j < see.hi ? dp[i] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bf16x8_t sf = pack8<E>(dp, 8 * u);
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+          dq[b] = mfma_32x32x16<E>(read_turned<D>(kt + (2 * y + u) * 32 * D, turn_at ^ (64 * b)), sf, dq[b]);
+      }
+    }
+  };
+  if (t0 < t1) fetch(t0, lds);
+  for (int t = t0; t < t1; ++t) {
+    wait_vmcnt<0>();
+    bare_barrier();
+    const int slot = (t - t0) & 1;
+    step(t, lds + slot * 2 * TILE, lds + (slot ^ 1) * 2 * TILE);
+  }
+  constexpr float down = E == ELT_F16 ? 1.f / 1024.f : 1.f;
+  if (live) store_turned<E, DB>(a.dq + row * a.dim, dq, a.scale * down / sigma, h, a.dim);
+}
+
+template <int E, int D>
+void launch_main(Attention a, unsigned* peaks, hipStream_t stream) {
+  const long long units = (long long)a.kv_heads * (a.seqs ? 1 : a.batch);
+  (void)peaks;
+  if (a.dk || a.dv) {
+    Attention k = a;
+    k.tiles = a.seqs ? a.kv_len / kKeyRows + a.batch + 4 : (a.kv_len + kKeyRows - 1) / kKeyRows;
+    if (units * k.tiles > 0)
+      hipLaunchKernelGGL((attention_keys_kernel<E, D>), dim3((unsigned)(units * k.tiles)), dim3(256), 0,
+                         stream, k);
+  }
+  if (a.dq && units * a.tiles > 0)
+    hipLaunchKernelGGL((attention_queries_kernel<E, D>), dim3((unsigned)(units * a.tiles)), dim3(256), 0,
+                       stream, a);
+}
+
+}  // namespace
+
+hipError_t launch_attention_grad(const Attention& a, hipStream_t stream) {
+  const long long batch = a.seqs ? 1 : a.batch;
+  const long long rows = (long long)a.q_len * a.heads * batch, keys = (long long)a.kv_len * a.kv_heads * batch;
+  const long long units = (long long)a.kv_heads * batch;
+  const long long most = units * ((long long)a.kv_len / kKeyRows + a.batch + 4);
+  if (rows / 16 > 0x7ffffff0LL || most > 0x7fffffffLL || units * a.tiles > 0x7fffffffLL)
+    return hipErrorInvalidValue;
+  unsigned* peaks = const_cast<unsigned*>(a.peaks);
+  const bool f16 = a.dtype == DT_F16;
+  if (f16) {
+    hipLaunchKernelGGL(attention_clear_kernel, dim3(1), dim3(64), 0, stream, peaks);
+    const long long blocks = (keys + 15) / 16 < 2048 ? (keys + 15) / 16 : 2048;
+    if (blocks > 0)
+      hipLaunchKernelGGL(attention_value_peak_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a,
+                         peaks + 1);
+  }
+  if (rows > 0) {
+    const dim3 grid((unsigned)((rows + 15) / 16));
+    if (f16) hipLaunchKernelGGL((attention_delta_kernel<ELT_F16>), grid, dim3(256), 0, stream, a, peaks);
+    else hipLaunchKernelGGL((attention_delta_kernel<ELT_BF16>), grid, dim3(256), 0, stream, a, peaks);
+  }
+  const bool wide = a.dim > 64;
+  if (f16) {
+    if (wide) launch_main<ELT_F16, 128>(a, peaks, stream);
+    else launch_main<ELT_F16, 64>(a, peaks, stream);
+  } else {
+    if (wide) launch_main<ELT_BF16, 128>(a, peaks, stream);
+    else launch_main<ELT_BF16, 64>(a, peaks, stream);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace dmuon

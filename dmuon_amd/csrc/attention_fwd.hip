@@ -1,0 +1,343 @@
+// Attention over heads on gfx950: o = softmax(c q k^T) v in one pass over the keys with the running
+// maximum and sum of each row.
+#include "attention.h"
+
+namespace dmuon {
+namespace {
+
+constexpr float kInf = __builtin_inff();
+constexpr int kKeys = 64;                 // keys of a tile
+
+// A wave has RT x 32 rows of queries, one a lane (l % 32): S^T = K Q^T leaves each lane 16 keys of
+// every 32 for its own row, the other half of the wave's lanes the rest, and goes as it is into
+// O^T = V^T P^T.
+template <int E, int D, int RT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1, RT == 1 ? 2 : 1)))
+void attention_kernel(const Attention a) {
+  constexpr int ROWS = 128 * RT, KS = D / 16, DB = D / 32, TILE = kKeys * D * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
+  const Place p = place_of<false>(a, a.causal);
+  if (!p.live) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int r0 = p.tile * ROWS, rows = p.qn * a.group;
+
+  // queries of this lane's rows; rows past the last one see nothing
+  bf16x8_t qf[RT][KS];
+  int query[RT], head[RT];
+  bool row_live[RT];
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    const int r = r0 + (wave * RT + x) * 32 + (lane & 31);
+    row_live[x] = r < rows;
+    query[x] = r / a.group;
+    head[x] = r - query[x] * a.group;
+    const uint16_t* src = a.q + p.q_off + query[x] * a.q_token + head[x] * a.q_head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int at = 16 * s + 8 * h;
+      qf[x][s] = bf16x8_t{};
+      if (row_live[x] && at < a.dim) qf[x][s] = *reinterpret_cast<const bf16x8_t*>(src + at);
+    }
+  }
+  Sight see[RT];
+#pragma unroll
+  for (int x = 0; x < RT; ++x) see[x] = row_live[x] ? sight_of(a, p, query[x]) : Sight{0, 0};
+  // the block's tiles: what its first and last row see
+  const int last_row = r0 + ROWS < rows ? r0 + ROWS - 1 : rows - 1;
+  const Sight first = sight_of(a, p, r0 / a.group), last = sight_of(a, p, last_row / a.group);
+  int t0 = first.lo / kKeys, t1 = (last.hi + kKeys - 1) / kKeys;
+  if (t1 < t0) t1 = t0;
+  if (a.splits > 1) {
+    const int each = (t1 - t0 + a.splits - 1) / a.splits;
+    t0 = t0 + p.split * each < t1 ? t0 + p.split * each : t1;
+    t1 = t0 + each < t1 ? t0 + each : t1;
+  }
+  // keys that every row sees need no mask
+  const int full_lo = last.lo, full_hi = last_row == r0 + ROWS - 1 ? first.hi : 0;
+
+  TileMover<D, kKeys, 4> mk, mv;
+  mk.init(a.k_token, a.dim, wave, lane);
+  mv.init(a.v_token, a.dim, wave, lane);
+  auto fetch = [&](int t, char* to) __attribute__((always_inline)) {
+    const int j0 = t * kKeys;
+    mk.issue(a.k + p.k_off + j0 * a.k_token, a.k_token, a.dim, p.kn - j0, to);
+    mv.issue(a.v + p.v_off + j0 * a.v_token, a.v_token, a.dim, p.kn - j0, to + TILE);
+  };
+  const int row_at = row_form<D>(lane), turn_at = turned_form<D>(lane);
+
+  f32x16_t o[RT][DB];
+  float ref[RT], sum[RT];
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+#pragma unroll
+    for (int b = 0; b < DB; ++b) o[x][b] = f32x16_t{};
+    ref[x] = -kInf;
+    sum[x] = 0.f;
+  }
+  // the slots' pointers are restrict: the compiler need not wait for loads into `next` before reads of `kt`
+  auto step = [&](int t, const char* __restrict__ kt, char* __restrict__ next) __attribute__((always_inline)) {
+    const char* vt = kt + TILE;
+    if (t + 1 < t1) fetch(t + 1, next);
+    f32x16_t s[RT][2];
+#pragma unroll
+    for (int x = 0; x < RT; ++x) s[x][0] = s[x][1] = f32x16_t{};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kt + b * 64 * D + (row_at ^ (32 * k)));
+#pragma unroll
+        for (int x = 0; x < RT; ++x) s[x][b] = mfma_32x32x16<E>(kf, qf[x][k], s[x][b]);
+      }
+    const int j0 = t * kKeys;
+    if (j0 < full_lo || j0 + kKeys > full_hi) {
+#pragma unroll
+      for (int x = 0; x < RT; ++x)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = j0 + 32 * b + result_row(i, h);
+            s[x][b][i] = j >= see[x].lo && j < see[x].hi ? s[x][b][i] : -kInf;
+          }
+    }
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+      float top = -kInf;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][b][i]);
+      top = half_max(top) * a.c;
+      // the reference follows the maximum only when that has grown by 2^8: any reference gives the same
+      // quotient, and sums and 16-bit probabilities have room for 256
+      if (__ballot(top > ref[x] + 8.f)) {
+        const float now = fmaxf(ref[x], top), from = now == -kInf ? 0.f : now;
+        const float f = __builtin_amdgcn_exp2f(ref[x] - from);
+        ref[x] = now;
+        sum[x] *= f;
+#pragma unroll
+        for (int b = 0; b < DB; ++b) o[x][b] *= f;
+      }
+      const float from = ref[x] == -kInf ? 0.f : ref[x];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[x][b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][b][i], a.c, -from));
+          sum[x] += s[x][b][i];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      bf16x8_t pf[RT];
+#pragma unroll
+      for (int x = 0; x < RT; ++x) {
+        u32x4_t w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = pack2_elt<E>(s[x][u / 2][8 * (u & 1) + 2 * i], s[x][u / 2][8 * (u & 1) + 2 * i + 1]);
+        pf[x] = __builtin_bit_cast(bf16x8_t, w);
+      }
+#pragma unroll
+      for (int b = 0; b < DB; ++b) {
+        const bf16x8_t vf = read_turned<D>(vt + u * 32 * D, turn_at ^ (64 * b));
+#pragma unroll
+        for (int x = 0; x < RT; ++x) o[x][b] = mfma_32x32x16<E>(vf, pf[x], o[x][b]);
+      }
+    }
+  };
+  if (t0 < t1) fetch(t0, lds);
+  for (int t = t0; t < t1; ++t) {
+    wait_vmcnt<0>();
+    bare_barrier();
+    const int slot = (t - t0) & 1;
+    step(t, lds + slot * 2 * TILE, lds + (slot ^ 1) * 2 * TILE);
+  }
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    const float total = half_sum(sum[x]);
+    if (!row_live[x]) continue;
+    const long long token = p.q_row + query[x];
+    const long long row = token * a.heads + (long long)p.kvh * a.group + head[x];
+    if (a.splits > 1) {
+      const long long at = (long long)p.split * a.q_len * a.heads * (a.seqs ? 1 : a.batch) + row;
+      float* part = a.part + at * a.dim;
+      if (h == 0) a.part_stats[at] = make_float2(ref[x], total);
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int d = 32 * b + result_row(i, h);
+          if (d < a.dim)
+            *reinterpret_cast<f32x4_t*>(part + d) =
+                f32x4_t{o[x][b][i], o[x][b][i + 1], o[x][b][i + 2], o[x][b][i + 3]};
+        }
+      continue;
+    }
+    // a row that sees nothing is 0
+    const float f = total == 0.f ? 0.f : 1.f / total;
+    uint16_t* out = a.out + row * a.dim;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int d = 32 * b + result_row(i, h);
+        if (d < a.dim)
+          *reinterpret_cast<u32x2_t*>(out + d) = u32x2_t{pack2_elt<E>(o[x][b][i] * f, o[x][b][i + 1] * f),
+                                                         pack2_elt<E>(o[x][b][i + 2] * f, o[x][b][i + 3] * f)};
+      }
+    if (a.lse && h == 0) a.lse[row] = total == 0.f ? kInf : ref[x] + __log2f(total);
+  }
+}
+
+// Joins the parts of the key axis: one wave a row, 4 bytes a lane.
+template <int E>
+__global__ __launch_bounds__(256) void attention_join_kernel(const Attention a) {
+  const long long rows = (long long)a.q_len * a.heads * (a.seqs ? 1 : a.batch);
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  float top = -kInf;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_stats[s * rows + row].x);
+  const float from = top == -kInf ? 0.f : top;
+  float total = 0.f, o[2] = {0.f, 0.f};
+  const int d = 2 * lane;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 st = a.part_stats[s * rows + row];
+    const float f = __builtin_amdgcn_exp2f(st.x - from);
+    total += f * st.y;
+    if (d < a.dim) {
+      const float2 v = *reinterpret_cast<const float2*>(a.part + (s * rows + row) * a.dim + d);
+      o[0] += f * v.x;
+      o[1] += f * v.y;
+    }
+  }
+  const float f = total == 0.f ? 0.f : 1.f / total;
+  if (d < a.dim)
+    *reinterpret_cast<unsigned*>(a.out + row * a.dim + d) = pack2_elt<E>(o[0] * f, o[1] * f);
+  if (a.lse && lane == 0) a.lse[row] = total == 0.f ? kInf : top + __log2f(total);
+}
+
+// Sequences and tiles of a packed call. Starts that fall are taken as the largest before them, and all
+// lie within the tokens that are there. Four further sequences hold the tokens before the first and behind
+// the last start: queries that see nothing, and keys that nothing sees.
+__global__ __launch_bounds__(1024) void attention_tables_kernel(
+    const int64_t* q_starts, const int64_t* k_starts, int n, int group, int q_tokens, int k_tokens,
+    int q_rows, int k_rows, Sequence* seqs, int2* q_tiles, int2* k_tiles, int* counts) {
+  __shared__ int lds[2][16], carry[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // inclusive scan over the block of a pair, by maximum or by sum
+  auto scan = [&](int& x, int& y, bool sum) {
+    for (int d = 1; d < 64; d <<= 1) {
+      const int u = __shfl_up(x, d), v = __shfl_up(y, d);
+      if (lane >= d) {
+        x = sum ? x + u : (x > u ? x : u);
+        y = sum ? y + v : (y > v ? y : v);
+      }
+    }
+    __syncthreads();
+    if (lane == 63) lds[0][wave] = x, lds[1][wave] = y;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+      const int u = lds[0][w], v = lds[1][w];
+      x = sum ? x + u : (x > u ? x : u);
+      y = sum ? y + v : (y > v ? y : v);
+    }
+  };
+  auto held = [](int64_t s, int most) { return s < 0 ? 0 : s < most ? (int)s : most; };
+  if (tid < 4) carry[tid] = 0;
+  // the starts, made to rise
+  for (int base = 0; base <= n; base += 1024) {
+    const int i = base + tid;
+    int q = i <= n ? held(q_starts[i], q_tokens) : 0, k = i <= n ? held(k_starts[i], k_tokens) : 0;
+    __syncthreads();
+    q = q > carry[0] ? q : carry[0];
+    k = k > carry[1] ? k : carry[1];
+    scan(q, k, false);
+    __syncthreads();
+    if (tid == 1023) carry[0] = q, carry[1] = k;
+    if (i <= n) {
+      seqs[i].q0 = q;                     // [n] is overwritten below, once read
+      seqs[i].k0 = k;
+    }
+  }
+  __syncthreads();
+  __threadfence_block();
+  const int q_first = seqs[0].q0, k_first = seqs[0].k0, q_end = seqs[n].q0, k_end = seqs[n].k0;
+  __syncthreads();
+  for (int i = tid; i < n; i += 1024) {
+    const int q1 = seqs[i + 1].q0, k1 = seqs[i + 1].k0;
+    seqs[i].qn = q1 - seqs[i].q0;
+    seqs[i].kn = k1 - seqs[i].k0;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    seqs[n] = Sequence{0, q_first, 0, 0};
+    seqs[n + 1] = Sequence{q_end, q_tokens - q_end, 0, 0};
+    seqs[n + 2] = Sequence{0, 0, 0, k_first};
+    seqs[n + 3] = Sequence{0, 0, k_end, k_tokens - k_end};
+  }
+  __syncthreads();
+  __threadfence_block();
+  for (int base = 0; base < n + 4; base += 1024) {
+    const int i = base + tid;
+    int q = 0, k = 0;
+    if (i < n + 4) {
+      q = (int)(((long long)seqs[i].qn * group + q_rows - 1) / q_rows);
+      k = (seqs[i].kn + k_rows - 1) / k_rows;
+    }
+    int qe = q, ke = k;
+    scan(qe, ke, true);
+    const int qb = carry[2] + qe - q, kb = carry[3] + ke - k;
+    for (int t = 0; t < q; ++t) q_tiles[qb + t] = make_int2(i, t);
+    for (int t = 0; t < k; ++t) k_tiles[kb + t] = make_int2(i, t);
+    __syncthreads();
+    if (tid == 1023) carry[2] += qe, carry[3] += ke;
+    __syncthreads();
+  }
+  if (tid < 2) counts[tid] = carry[2 + tid];
+}
+
+template <int E, int D>
+void launch(const Attention& a, unsigned blocks, hipStream_t stream) {
+  hipLaunchKernelGGL((attention_kernel<E, D, 1>), dim3(blocks), dim3(256), 0, stream, a);
+}
+
+}  // namespace
+
+hipError_t launch_attention_tables(const Attention& a, const int64_t* q_starts, const int64_t* kv_starts,
+                                   int q_rows, int k_rows, Sequence* seqs, int2* q_tiles, int2* k_tiles,
+                                   int* counts, hipStream_t stream) {
+  hipLaunchKernelGGL(attention_tables_kernel, dim3(1), dim3(1024), 0, stream, q_starts, kv_starts, a.batch,
+                     a.group, a.q_len, a.kv_len, q_rows, k_rows, seqs, q_tiles, k_tiles, counts);
+  return hipGetLastError();
+}
+
+hipError_t launch_attention(const Attention& a, hipStream_t stream) {
+  const long long units = (long long)a.kv_heads * (a.seqs ? 1 : a.batch);
+  const long long blocks = units * a.tiles * a.splits;
+  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (blocks > 0) {
+    const bool wide = a.dim > 64;
+    if (a.dtype == DT_F16) {
+      if (wide) launch<ELT_F16, 128>(a, (unsigned)blocks, stream);
+      else launch<ELT_F16, 64>(a, (unsigned)blocks, stream);
+    } else {
+      if (wide) launch<ELT_BF16, 128>(a, (unsigned)blocks, stream);
+      else launch<ELT_BF16, 64>(a, (unsigned)blocks, stream);
+    }
+    if (a.splits > 1) {
+      const long long rows = (long long)a.q_len * a.heads * (a.seqs ? 1 : a.batch);
+      if ((rows + 3) / 4 > 0x7fffffffLL) return hipErrorInvalidValue;
+      const dim3 grid((unsigned)((rows + 3) / 4));
+      if (a.dtype == DT_F16)
+        hipLaunchKernelGGL((attention_join_kernel<ELT_F16>), grid, dim3(256), 0, stream, a);
+      else
+        hipLaunchKernelGGL((attention_join_kernel<ELT_BF16>), grid, dim3(256), 0, stream, a);
+    }
+  }
+  return hipGetLastError();
+}
+
+}  // namespace dmuon

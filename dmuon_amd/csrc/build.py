@@ -18,7 +18,8 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent.parent
 SOURCES = ["ns_gemm.hip", "gram_small.hip", "ew_kernels.hip", "adamw.hip", "clip.hip",
-           "head_gemm.hip", "head_rows.hip", "head_loss.hip", "residual_norm.hip", "abi.hip"]
+           "head_gemm.hip", "head_rows.hip", "head_loss.hip", "residual_norm.hip", "attention_fwd.hip",
+           "attention_bwd.hip", "attention.hip", "rotary_heads.hip", "embedding.hip", "abi.hip"]
 LIB_NAME = "libdmuon_amd.so"
 ARCH = "gfx950"
 

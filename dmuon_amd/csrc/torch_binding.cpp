@@ -11,6 +11,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <cmath>
 #include <optional>
 
 #include "../../include/dmuon_amd.h"
@@ -445,6 +446,8 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& y, co
 
 }  // namespace
 
+#include "torch_block.h"
+
 PYBIND11_MODULE(_dmuon_torch, m) {
   m.attr("abi_version") = DMUON_ABI_VERSION;
   m.attr("torch_version") = DMUON_TORCH;
@@ -452,4 +455,7 @@ PYBIND11_MODULE(_dmuon_torch, m) {
   m.def("linear_cross_entropy", &linear_cross_entropy, free);
   m.def("linear_distillation", &linear_distillation, free);
   m.def("residual_norm", &residual_norm, free);
+  m.def("attention", &attention, free);
+  m.def("rotary_heads", &rotary_heads, free);
+  m.def("embedding", &embedding, free);
 }

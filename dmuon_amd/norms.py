@@ -1,8 +1,9 @@
-"""The norms around a block, fused with its gate and residual scale, on the HIP kernels.
+"""The norms around a block and those of its attention's heads, on the HIP kernels.
 
-``residual_norm`` takes the residual stream and a block's output to the new stream and the next
+``rotary_heads`` norms queries and keys head by head and turns them by their positions in one pass
+(``dmuon_rotary_heads`` / ``dmuon_rotary_heads_grad``). ``residual_norm`` takes the residual stream and a block's output to the new stream and the next
 block's input in one pass over memory, and its gradients in another
-(``dmuon_residual_norm`` / ``dmuon_residual_norm_grad``). The autograd operator is native
+(``dmuon_residual_norm`` / ``dmuon_residual_norm_grad``). The autograd operators are native
 (``csrc/torch_binding.cpp``). There is no CPU path: tensors must live on the GPU.
 """
 from __future__ import annotations
@@ -38,3 +39,26 @@ def residual_norm(x: Tensor, y: Optional[Tensor], pre_weight: Tensor, *,
     """
     return _C.torch_ops().residual_norm(x, y, pre_weight, post_weight, gate, float(residual_scale),
                                         float(eps), _MAX_DIM)
+
+
+def rotary_heads(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *,
+                 q_weight: Optional[Tensor] = None, k_weight: Optional[Tensor] = None,
+                 eps: float = 1e-6, interleaved: bool = False) -> Tuple[Tensor, Tensor]:
+    """Queries ``q`` (``[..., heads, dim]``) and keys ``k`` (``[..., kv_heads, dim]``), normed head by
+    head and rotated by their positions::
+
+        z = x * rsqrt(mean(x**2) + eps) * weight           (weight None: z = x)
+        y[i], y[j] = z[i] cos t - z[j] sin t, z[j] cos t + z[i] sin t,   t = position * inv_freq[i]
+
+    with the pairs ``j = i + r / 2`` of the first ``r = 2 * len(inv_freq)`` values, or, ``interleaved``, the
+    neighbours ``2 i`` and ``2 i + 1``; values behind them are not turned. ``positions`` are integers
+    of the leading shape or of its trailing part (``[tokens]`` for a batch), ``inv_freq`` fp32 or fp64: the
+    angle is formed and reduced in 64 bits, so that far positions are as exact as near ones. ``q`` and ``k``
+    share a dtype (fp32, bf16 or fp16) that the results, which are dense, have too; the weights (``[dim]``)
+    may have it or fp32. ``dim`` is even and at most 512. Views into one product for q, k and v are read in
+    place. Arithmetic is fp32, every result is rounded once; gradients go to q, k and the weights (their
+    sums in a fixed order) and have none of their own. Dual tensors, tracers and wrapper subclasses raise.
+    Can be captured into a graph.
+    """
+    return _C.torch_ops().rotary_heads(q, k, positions, inv_freq, q_weight, k_weight, float(eps),
+                                       bool(interleaved))

@@ -72,7 +72,7 @@ extern "C" {
 const char* dmuon_last_error(void);
 
 /* ABI version (major*100 + minor): DMUON_ABI_VERSION of the header the library was built with. */
-#define DMUON_ABI_VERSION 110
+#define DMUON_ABI_VERSION 111
 int dmuon_abi_version(void);
 
 /*
@@ -550,6 +550,114 @@ int dmuon_residual_norm_grad_workspace_size(const dmuon_residual_norm_args* args
                                             int64_t* workspace_bytes);
 int dmuon_residual_norm_grad(const dmuon_residual_norm_args* args, void* workspace,
                              int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention over heads (no reference counterpart):
+ *   out[i][h] = sum_j softmax_j(scale q[i][h] . k[j][h']) v[j][h'],  h' = h / (heads / kv_heads)
+ * over the keys j that query i of its sequence sees: all of them, or, with `causal`, those up to
+ * j = i + kv tokens - q tokens (the last query sees the last key), of which a `window` > 0 leaves the
+ * last `window`. A query that sees nothing has the result 0. q, k, v, dout and the results are 16-bit words
+ * of `dtype` (DMUON_DTYPE_BF16 or _F16), heads of dim (8 .. 128, a multiple of 8) values; scores, sums
+ * and statistics are fp32, probabilities and their gradients are rounded to `dtype` between the products.
+ *   batched: q [batch][q_len][heads][dim], k and v [batch][kv_len][kv_heads][dim]; kv_lengths [batch]
+ *     (or NULL) says how many keys of each are there (held to 0 .. kv_len); what lies behind them is not read.
+ *   packed (q_starts and kv_starts [batch + 1], with batch sequences): q [q_len][heads][dim], k and v
+ *     [kv_len][kv_heads][dim], sequence b being the tokens starts[b] .. starts[b + 1] - 1 of each. Starts
+ *     are held to the tokens that are there, and one that falls to the largest before it; a token in no
+ *     sequence has the result and the gradient 0.
+ * Strides are in elements, multiples of 8, and bases 16-byte aligned; out, lse and the gradients are
+ * dense. lse [tokens][heads] (fp32, NULL where no gradient follows) keeps the log2 of each row's sum.
+ * dmuon_attention_grad: from dout, out and lse the gradients dq, dk and dv; any may be NULL. Workspaces are
+ * 256-byte aligned. Nothing depends on the order of blocks: the same arguments give the same bits.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse;
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  const int64_t* kv_lengths;
+  const int64_t* q_starts;
+  const int64_t* kv_starts;
+  int64_t batch, q_len, kv_len, heads, kv_heads, dim, window;
+  int64_t q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head;
+  int64_t do_batch, do_token, do_head;
+  float scale;
+  int causal, dtype;
+} dmuon_attention_args;
+int dmuon_attention_workspace_size(const dmuon_attention_args* args, int64_t* workspace_bytes);
+int dmuon_attention(const dmuon_attention_args* args, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+int dmuon_attention_grad_workspace_size(const dmuon_attention_args* args, int64_t* workspace_bytes);
+int dmuon_attention_grad(const dmuon_attention_args* args, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
+/*
+ * Norms of queries and keys for each head with the position rotation (no reference counterpart):
+ *   z = x rsqrt(mean(x^2) + eps) w over a head's dim values (w NULL: z = x); of its first rotary_dim
+ *   values the pairs (i, i + rotary_dim / 2), or with `interleaved` (2 i, 2 i + 1), are turned by the
+ *   angle positions[t % period] * inv_freq[i]; the rest stay.
+ * q [tokens][heads][dim] and k [tokens][kv_heads][dim] with strides in elements, results dense, all of
+ * `dtype` (DMUON_DTYPE_F32, _BF16 or _F16), dim even and 2 .. 512, any element alignment; weights [dim] with
+ * a dtype of their own; inv_freq [rotary_dim / 2] fp32, or fp64 with inv_freq_double. Angles are formed
+ * and reduced in fp64, the rest is fp32, every result rounded once. positions are 64-bit integers, of
+ * which `period` are there (a divisor of tokens).
+ * dmuon_rotary_heads_grad: from dq_out and dk_out (either may be NULL: zero) dq, dk, d_q_weight and
+ * d_k_weight, any of which may be NULL; the weights' sums have a fixed order.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  const int64_t* positions;
+  const void* inv_freq;
+  const void* q_weight;
+  const void* k_weight;
+  void* q_out;
+  void* k_out;
+  const void* dq_out;
+  const void* dk_out;
+  void* dq;
+  void* dk;
+  void* d_q_weight;
+  void* d_k_weight;
+  int64_t tokens, period, heads, kv_heads, dim, rotary_dim;
+  int64_t q_token, q_head, k_token, k_head, dq_out_token, dq_out_head, dk_out_token, dk_out_head;
+  float eps;
+  int interleaved, inv_freq_double, dtype, q_weight_dtype, k_weight_dtype;
+} dmuon_rotary_heads_args;
+int dmuon_rotary_heads(const dmuon_rotary_heads_args* args, void* stream);
+int dmuon_rotary_heads_grad_workspace_size(const dmuon_rotary_heads_args* args,
+                                           int64_t* workspace_bytes);
+int dmuon_rotary_heads_grad(const dmuon_rotary_heads_args* args, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/*
+ * Token lookup (no reference counterpart): out[t] = scale * weight[tokens[t]] for tokens_n tokens and
+ * a weight [vocab][dim] with a row pitch; a token outside 0 .. vocab - 1 gives a row of NaN. Rows are of
+ * `dtype` (DMUON_DTYPE_F32, _BF16 or _F16) at any element alignment.
+ * dmuon_embedding_grad: d_weight[v] = scale * sum of dy[t] over tokens[t] == v, for every v (dense, all of
+ * it written); tokens equal to padding_idx (negative: none) or outside the vocabulary have no share. Sums
+ * are fp32 in the order of the tokens, grouped in runs of the sorted ones: the same arguments give the same
+ * bits. The workspace is 16-byte aligned.
+ */
+typedef struct {
+  const int64_t* tokens;
+  const void* weight;
+  void* out;
+  const void* dy;
+  void* d_weight;
+  int64_t tokens_n, vocab, dim, ld_weight, ld_dy, padding_idx;
+  float scale;
+  int dtype;
+} dmuon_embedding_args;
+int dmuon_embedding(const dmuon_embedding_args* args, void* stream);
+int dmuon_embedding_grad_workspace_size(const dmuon_embedding_args* args, int64_t* workspace_bytes);
+int dmuon_embedding_grad(const dmuon_embedding_args* args, void* workspace, int64_t workspace_bytes,
+                         void* stream);
 
 #ifdef __cplusplus
 }
