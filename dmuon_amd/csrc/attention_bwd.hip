@@ -14,6 +14,7 @@ namespace dmuon {
 namespace {
 
 constexpr int kTile = 64;                 // rows or keys of a tile in LDS
+constexpr long long kPeakBlocks = 1024;
 constexpr float kInf = __builtin_inff();
 
 template <int E>
@@ -82,37 +83,52 @@ struct RowMover {
   }
 };
 
+// A block's largest value to *peak: a maximum, which no order shows in. One atomic a block: of many waves
+// at one address they took 375 us where the reads take 20.
+__device__ __forceinline__ void block_peak(float most, unsigned* peak) {
+  __shared__ float lds[4];
+  for (int o = 16; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x) return;
+  most = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+  if (most > 0.f) atomicMax(peak, __float_as_uint(most));
+}
+
 // delta of every row, and in fp16 the largest row of do. 16 lanes a row, 8 values each.
 template <int E>
 __global__ __launch_bounds__(256) void attention_delta_kernel(const Attention a, unsigned* peaks) {
   const long long rows = (long long)a.q_len * a.heads * (a.seqs ? 1 : a.batch);
-  const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
   const int at = 8 * (threadIdx.x & 15);
-  float s = 0.f, n = 0.f;
-  if (row < rows && at < a.dim) {
-    const long long token = row / a.heads, b = a.seqs ? 0 : token / a.q_len;
-    const int head = (int)(row - token * a.heads);
-    const uint16_t* d = a.dout + b * a.do_batch + (token - b * a.q_len) * a.do_token + head * a.do_head + at;
-    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(d);
-    const u32x4_t y = *reinterpret_cast<const u32x4_t*>(a.out + row * a.dim + at);
+  float most = 0.f;
+  for (long long first = (long long)blockIdx.x * 16; first < rows; first += (long long)gridDim.x * 16) {
+    const long long row = first + (threadIdx.x >> 4);
+    const bool live = row < rows;
+    float s = 0.f, n = 0.f;
+    if (live && at < a.dim) {
+      const long long token = row / a.heads, b = a.seqs ? 0 : token / a.q_len;
+      const int head = (int)(row - token * a.heads);
+      const uint16_t* d = a.dout + b * a.do_batch + (token - b * a.q_len) * a.do_token + head * a.do_head + at;
+      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(d);
+      const u32x4_t y = *reinterpret_cast<const u32x4_t*>(a.out + row * a.dim + at);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint16_t u = (uint16_t)(i & 1 ? x[i / 2] >> 16 : x[i / 2]);
-      const uint16_t w = (uint16_t)(i & 1 ? y[i / 2] >> 16 : y[i / 2]);
-      const float f = from_elt<E>(u);
-      s += f * from_elt<E>(w);
-      n += f * f;
+      for (int i = 0; i < 8; ++i) {
+        const uint16_t u = (uint16_t)(i & 1 ? x[i / 2] >> 16 : x[i / 2]);
+        const uint16_t w = (uint16_t)(i & 1 ? y[i / 2] >> 16 : y[i / 2]);
+        const float f = from_elt<E>(u);
+        s += f * from_elt<E>(w);
+        n += f * f;
+      }
+    }
+    for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
+    if (live && (threadIdx.x & 15) == 0) a.delta[row] = s;
+    if constexpr (E == ELT_F16) {
+      for (int o = 1; o < 16; o <<= 1) n += __shfl_xor(n, o);
+      // rows that see nothing, or of no numbers, do not count
+      if (live && n < kInf && a.lse[row] < kInf) most = fmaxf(most, n);
     }
   }
-  for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o), n += __shfl_xor(n, o);
-  const bool live = row < rows;
-  if (live && (threadIdx.x & 15) == 0) a.delta[row] = s;
-  if constexpr (E == ELT_F16) {
-    // a maximum, which no order shows in; rows that see nothing, or of no numbers, do not count
-    float most = live && a.lse[row] < kInf && n < kInf ? n : 0.f;
-    for (int o = 16; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
-    if ((threadIdx.x & 63) == 0 && most > 0.f) atomicMax(peaks, __float_as_uint(most));
-  }
+  if constexpr (E == ELT_F16) block_peak(most, peaks);
 }
 
 // fp16: the largest row of v among those that a query may see
@@ -141,8 +157,7 @@ __global__ __launch_bounds__(256) void attention_value_peak_kernel(const Attenti
     for (int o = 1; o < 16; o <<= 1) n += __shfl_xor(n, o);
     if (n < kInf) most = fmaxf(most, n);
   }
-  for (int o = 16; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
-  if ((threadIdx.x & 63) == 0 && most > 0.f) atomicMax(peak, __float_as_uint(most));
+  block_peak(most, peak);
 }
 
 __global__ void attention_clear_kernel(unsigned* peaks) {
@@ -158,7 +173,7 @@ void attention_keys_kernel(const Attention a) {
   __shared__ __attribute__((aligned(1024))) char lds[2 * SLOT];
   const Place p = place_of<true>(a, false);
   if (!p.live) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int j0 = p.tile * kKeyRows, j = j0 + wave * 32 + (lane & 31);
   const int rows = p.qn * a.group, before = p.kn - p.qn;
 
@@ -232,42 +247,59 @@ void attention_keys_kernel(const Attention a) {
     const bool masked = r0 < full_lo || r0 + kTile > full_hi;
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
+      // the reads' addresses are formed anew each time: held over the loop they would take the registers
+      // that the sums need
+      int ra = row_at, ta = turn_at;
+      asm volatile("" : "+v"(ra), "+v"(ta));
       f32x16_t s = {}, dp = {};
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const int at = y * 64 * D + (row_at ^ (32 * k));
-        s = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(qt + at), kf[k], s);
-        dp = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(dt + at), vf[k], dp);
-      }
+      for (int k = 0; k < KS; ++k)
+        s = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(qt + y * 64 * D + (ra ^ (32 * k))), kf[k], s);
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
-        const int r = 32 * y + result_row(i, h);
-        const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(stats + r);
-        const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(stats + kTile + r);
+        const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(stats + 32 * y + result_row(i, h));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; ++e)
           s[i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + e], a.c, kShift<E> - lse[e]));
-          dp[i + e] = s[i + e] * ((dp[i + e] - delta[e]) * sigma);
-        }
       }
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int r = r0 + 32 * y + result_row(i, h);
-          const bool seen = r >= lo && r < hi;
-          s[i] = seen ? s[i] : 0.f;
-          dp[i] = seen ? dp[i] : 0.f;
+          s[i] = r >= lo && r < hi ? s[i] : 0.f;
         }
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const bf16x8_t pf = pack8<E>(s, 8 * u), sf = pack8<E>(dp, 8 * u);
+        const bf16x8_t pf = pack8<E>(s, 8 * u);
 #pragma unroll
-        for (int b = 0; b < DB; ++b) {
-          const int at = (2 * y + u) * 32 * D;
-          dv[b] = mfma_32x32x16<E>(read_turned<D>(dt + at, turn_at ^ (64 * b)), pf, dv[b]);
-          dk[b] = mfma_32x32x16<E>(read_turned<D>(qt + at, turn_at ^ (64 * b)), sf, dk[b]);
+        for (int b = 0; b < DB; ++b)
+          dv[b] = mfma_32x32x16<E>(read_turned<D>(dt + (2 * y + u) * 32 * D, ta ^ (64 * b)), pf, dv[b]);
+      }
+      asm volatile("" : "+v"(ra), "+v"(ta));
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        dp = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(dt + y * 64 * D + (ra ^ (32 * k))), vf[k], dp);
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(stats + kTile + 32 * y + result_row(i, h));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[i + e] = s[i + e] * ((dp[i + e] - delta[e]) * sigma);
+      }
+      if (masked) {
+        // rows that do not see the key have no share, whatever their dout holds
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = r0 + 32 * y + result_row(i, h);
+          dp[i] = r >= lo && r < hi ? dp[i] : 0.f;
         }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bf16x8_t sf = pack8<E>(dp, 8 * u);
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+          dk[b] = mfma_32x32x16<E>(read_turned<D>(qt + (2 * y + u) * 32 * D, ta ^ (64 * b)), sf, dk[b]);
       }
     }
   };
@@ -295,7 +327,7 @@ void attention_queries_kernel(const Attention a) {
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
   const Place p = place_of<false>(a, a.causal);
   if (!p.live) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int r0 = p.tile * kQueryRows, rows = p.qn * a.group;
   const int r = r0 + wave * 32 + (lane & 31);
   const bool live = r < rows;
@@ -405,13 +437,14 @@ hipError_t launch_attention_grad(const Attention& a, hipStream_t stream) {
   const bool f16 = a.dtype == DT_F16;
   if (f16) {
     hipLaunchKernelGGL(attention_clear_kernel, dim3(1), dim3(64), 0, stream, peaks);
-    const long long blocks = (keys + 15) / 16 < 2048 ? (keys + 15) / 16 : 2048;
+    const long long blocks = (keys + 15) / 16 < kPeakBlocks ? (keys + 15) / 16 : kPeakBlocks;
     if (blocks > 0)
       hipLaunchKernelGGL(attention_value_peak_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a,
                          peaks + 1);
   }
   if (rows > 0) {
-    const dim3 grid((unsigned)((rows + 15) / 16));
+    const long long blocks = (rows + 15) / 16;
+    const dim3 grid((unsigned)(f16 && blocks > kPeakBlocks ? kPeakBlocks : blocks));
     if (f16) hipLaunchKernelGGL((attention_delta_kernel<ELT_F16>), grid, dim3(256), 0, stream, a, peaks);
     else hipLaunchKernelGGL((attention_delta_kernel<ELT_BF16>), grid, dim3(256), 0, stream, a, peaks);
   }

@@ -18,7 +18,7 @@ void attention_kernel(const Attention a) {
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
   const Place p = place_of<false>(a, a.causal);
   if (!p.live) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int r0 = p.tile * ROWS, rows = p.qn * a.group;
 
   // queries of this lane's rows; rows past the last one see nothing
