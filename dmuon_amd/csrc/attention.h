@@ -38,6 +38,7 @@ struct Attention {
   int causal, dtype;
   float scale, c;                         // c = scale log2(e)
   int splits;                             // parts of the key axis, joined by a second kernel
+  int few;                                // tiles of kFewRows rows, each wave alone
   float* part; float2* part_stats;        // [splits][tokens][heads][dim] sums, [..][2] (reference, sum)
   const unsigned* peaks;                  // fp16 gradients: largest |dout row|^2 and |v row|^2
 };
@@ -148,19 +149,29 @@ __device__ __forceinline__ bf16x8_t read_turned(const char* lds, int at) {
   return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// Registers from .. from + 7 of a result, rounded: one k step of the next product's operand
+template <int E>
+__device__ __forceinline__ bf16x8_t pack8(const f32x16_t& v, int from) {
+  u32x4_t w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack2_elt<E>(v[from + 2 * i], v[from + 2 * i + 1]);
+  return __builtin_bit_cast(bf16x8_t, w);
+}
+
 constexpr unsigned kNowhere = 0x80000000u;     // outside any buffer range: reads 0
 
-// Moves ROWS rows of one pitch from memory into LDS, WAVES waves together.
+// Moves ROWS rows of one pitch from memory into LDS, WAVES waves together. The swizzle repeats after four
+// instructions of a wave, so four offsets describe them all.
 template <int D, int ROWS, int WAVES>
 struct TileMover {
-  static constexpr int CPR = D / 8, RPI = 64 / CPR, N = ROWS / RPI / WAVES;
-  static_assert(N * RPI * WAVES == ROWS && N <= 4, "whole instructions");
-  unsigned off[4];                        // [N] makes clang drop the host stubs of the kernels
+  static constexpr int CPR = D / 8, RPI = 64 / CPR, N = ROWS / RPI / WAVES, PART = N < 4 ? N : 4;
+  static_assert(N * RPI * WAVES == ROWS && (N <= 4 || (WAVES == 1 && N % 4 == 0)), "whole instructions");
+  unsigned off[4];                        // [PART] makes clang drop the host stubs of the kernels
   int wave;
   __device__ __forceinline__ void init(long long pitch, int dim, int wave_, int lane) {
     wave = wave_;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < PART; ++i) {
       const int r = (wave * N + i) * RPI + lane / CPR;
       const int chunk = (lane % CPR) ^ slot_mask<D>(r);
       off[i] = chunk * 8 < dim ? (unsigned)(r * (int)pitch * 2 + chunk * 16) : kNowhere;
@@ -170,14 +181,18 @@ struct TileMover {
   __device__ __forceinline__ void issue(const uint16_t* p, long long pitch, int dim, int rows,
                                         char* lds) const {
     typedef __attribute__((address_space(3))) void* lds_ptr_t;
-    rows = rows < ROWS ? rows : ROWS;
-    const int bytes = ((rows - 1) * (int)pitch + dim) * 2;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint16_t*>(p), (short)0, bytes, 0x00020000);
+    constexpr int STEP = N > 4 ? 4 * RPI : ROWS;          // rows of a resource
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (wave * N + i) * 1024), 16,
-                                               off[i], 0, 0, 0);
+    for (int part = 0; part < N / PART; ++part) {
+      const int left = rows - part * STEP;
+      const int bytes = left > 0 ? (((left < STEP ? left : STEP) - 1) * (int)pitch + dim) * 2 : 0;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint16_t*>(p + part * STEP * pitch), (short)0, bytes, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < PART; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (wave * N + part * 4 + i) * 1024), 16,
+                                                 off[i], 0, 0, 0);
+    }
   }
 };
 
@@ -209,7 +224,8 @@ __device__ __forceinline__ Sight sight_of(const Attention& a, const Place& p, in
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-constexpr int kQueryRows = 128, kKeyRows = 128;
+// rows and keys of a block's tile; rows of one wave that works alone
+constexpr int kQueryRows = 128, kKeyRows = 128, kFewRows = 32;
 // the tables of a packed call; tiles of `rows` rows
 hipError_t launch_attention_tables(const Attention& a, const int64_t* q_starts, const int64_t* kv_starts,
                                    int q_rows, int k_rows, Sequence* seqs, int2* q_tiles, int2* k_tiles,

@@ -98,7 +98,8 @@ struct Tables {
 };
 Tables tables(Attention* r, const dmuon_attention_args& a, Carver* c) {
   Tables t;
-  r->tiles = (int)tiles_of(*r, a.q_starts != nullptr, (int64_t)r->q_len * r->group, kQueryRows);
+  r->tiles = (int)tiles_of(*r, a.q_starts != nullptr, (int64_t)r->q_len * r->group,
+                           r->few ? kFewRows : kQueryRows);
   if (!a.q_starts) return t;
   t.seqs = c->take<Sequence>(r->batch + 4);
   t.q = c->take<int2>(r->tiles);
@@ -111,15 +112,31 @@ Tables tables(Attention* r, const dmuon_attention_args& a, Carver* c) {
   return t;
 }
 
-// Few rows over many keys do not fill the card: the keys are split, in pieces of 256 or more.
+// Sequences of at most kFewRows rows a key head (packed: on average) go to waves that work alone.
+bool few_rows(const Attention& a, bool packed) {
+  const int64_t rows = (int64_t)a.q_len * a.group;
+  return packed ? rows <= (int64_t)kFewRows * a.batch : rows <= kFewRows;
+}
+
+// Few rows over many keys do not fill the card: the keys are split. Waves that work alone take pieces of 512
+// keys, or fewer where that leaves less than one wave a CU; blocks of 128 rows pieces of 256 or more, up to
+// two blocks a CU.
 int splits_of(const Attention& a, bool packed) {
   const int64_t units = (int64_t)a.kv_heads * (packed ? 1 : a.batch);
   const int64_t blocks = units * a.tiles;
   const int64_t keys = packed && a.batch ? a.kv_len / a.batch : a.kv_len;
-  if (blocks < 1 || blocks >= 512) return 1;
-  int64_t s = 1024 / blocks;
-  if (s > keys / 256) s = keys / 256;
-  return s < 1 ? 1 : s > 128 ? 128 : (int)s;
+  if (blocks < 1) return 1;
+  int64_t s;
+  if (a.few) {
+    s = (keys + 511) / 512;
+    if (s * blocks < 512) s = (512 + blocks - 1) / blocks;
+    if (s > (keys + 31) / 32) s = (keys + 31) / 32;
+  } else {
+    if (blocks >= 512) return 1;
+    s = 1024 / blocks;
+    if (s > keys / 256) s = keys / 256;
+  }
+  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
 struct Plan {
@@ -131,6 +148,7 @@ Plan plan_forward(const dmuon_attention_args& a, void* ws) {
   Plan p{describe(a), {}, 0};
   Carver c{static_cast<char*>(ws)};
   const bool packed = a.q_starts != nullptr;
+  p.a.few = few_rows(p.a, packed);
   p.t = tables(&p.a, a, &c);
   p.a.splits = splits_of(p.a, packed);
   if (p.a.splits > 1) {
@@ -161,7 +179,7 @@ int check_workspace(const char* who, int64_t need, const void* ws, int64_t bytes
 
 hipError_t fill_tables(const Plan& p, const dmuon_attention_args& a, hipStream_t s) {
   if (!a.q_starts) return hipSuccess;
-  return launch_attention_tables(p.a, a.q_starts, a.kv_starts, kQueryRows, kKeyRows, p.t.seqs, p.t.q, p.t.k,
+  return launch_attention_tables(p.a, a.q_starts, a.kv_starts, p.a.few ? kFewRows : kQueryRows, kKeyRows, p.t.seqs, p.t.q, p.t.k,
                                  p.t.counts, s);
 }
 

@@ -31,14 +31,6 @@ __device__ __forceinline__ float ds_scale(const Attention& a) {
   return __uint_as_float((unsigned)(127 + e) << 23);
 }
 
-template <int E>
-__device__ __forceinline__ bf16x8_t pack8(const f32x16_t& v, int from) {
-  u32x4_t w;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack2_elt<E>(v[from + 2 * i], v[from + 2 * i + 1]);
-  return __builtin_bit_cast(bf16x8_t, w);
-}
-
 // A row's share of a transposed result: values result_row(i, h) of each 32
 template <int E, int DB>
 __device__ __forceinline__ void store_turned(uint16_t* out, const f32x16_t* v, float f, int h, int dim) {
@@ -210,6 +202,8 @@ void attention_keys_kernel(const Attention a) {
   const int full_lo = last_lo * a.group;
   const int full_hi = last_key == j0 + kKeyRows - 1 ? first_hi * a.group : 0;
   const int n = r_hi > r_lo && j0 < p.kn ? (r_hi - r_lo + kTile - 1) / kTile : 0;
+  // from the last rows back: under a causal mask all blocks of a key head begin with the same rows then,
+  // and find them in their XCD's L2
 
   RowMover<D> mover;
   mover.init(wave, lane);
@@ -217,7 +211,7 @@ void attention_keys_kernel(const Attention a) {
   const long long row0 = p.q_row * a.heads + (long long)p.kvh * a.group;
   auto fetch = [&](int t, char* to) __attribute__((always_inline)) {
     typedef __attribute__((address_space(3))) void* lds_ptr_t;
-    const int r0 = r_lo + t * kTile;
+    const int r0 = r_lo + (n - 1 - t) * kTile;
     mover.issue(a.q + p.q_off, a.q_token, a.q_head, a.group, magic, a.dim, r0, rows, to);
     mover.issue(a.dout + p.do_off, a.do_token, a.do_head, a.group, magic, a.dim, r0, rows, to + TILE);
     if (wave < 2) {
@@ -243,7 +237,7 @@ void attention_keys_kernel(const Attention a) {
     const char* dt = qt + TILE;
     const float* stats = reinterpret_cast<const float*>(qt + 2 * TILE);
     if (t + 1 < n) fetch(t + 1, next);
-    const int r0 = r_lo + t * kTile;
+    const int r0 = r_lo + (n - 1 - t) * kTile;
     const bool masked = r0 < full_lo || r0 + kTile > full_hi;
 #pragma unroll
     for (int y = 0; y < 2; ++y) {

@@ -8,6 +8,41 @@ namespace {
 constexpr float kInf = __builtin_inff();
 constexpr int kKeys = 64;                 // keys of a tile
 
+// A lane's half of a row: the result and its statistics, or, of one part of the keys, the unfinished sums.
+template <int E, int DB>
+__device__ __forceinline__ void store_row(const Attention& a, const Place& p, bool live, int query, int head,
+                                          const f32x16_t* o, float ref, float total, int h) {
+  if (!live) return;
+  const long long row = (p.q_row + query) * a.heads + (long long)p.kvh * a.group + head;
+  if (a.splits > 1) {
+    const long long at = (long long)p.split * a.q_len * a.heads * (a.seqs ? 1 : a.batch) + row;
+    float* part = a.part + at * a.dim;
+    if (h == 0) a.part_stats[at] = make_float2(ref, total);
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int d = 32 * b + result_row(i, h);
+        if (d < a.dim)
+          *reinterpret_cast<f32x4_t*>(part + d) = f32x4_t{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]};
+      }
+    return;
+  }
+  // a row that sees nothing is 0
+  const float f = total == 0.f ? 0.f : 1.f / total;
+  uint16_t* out = a.out + row * a.dim;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = 32 * b + result_row(i, h);
+      if (d < a.dim)
+        *reinterpret_cast<u32x2_t*>(out + d) = u32x2_t{pack2_elt<E>(o[b][i] * f, o[b][i + 1] * f),
+                                                       pack2_elt<E>(o[b][i + 2] * f, o[b][i + 3] * f)};
+    }
+  if (a.lse && h == 0) a.lse[row] = total == 0.f ? kInf : ref + __log2f(total);
+}
+
 // A wave has RT x 32 rows of queries, one a lane (l % 32): S^T = K Q^T leaves each lane 16 keys of
 // every 32 for its own row, the other half of the wave's lanes the rest, and goes as it is into
 // O^T = V^T P^T.
@@ -132,13 +167,7 @@ void attention_kernel(const Attention a) {
     for (int u = 0; u < 4; ++u) {
       bf16x8_t pf[RT];
 #pragma unroll
-      for (int x = 0; x < RT; ++x) {
-        u32x4_t w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = pack2_elt<E>(s[x][u / 2][8 * (u & 1) + 2 * i], s[x][u / 2][8 * (u & 1) + 2 * i + 1]);
-        pf[x] = __builtin_bit_cast(bf16x8_t, w);
-      }
+      for (int x = 0; x < RT; ++x) pf[x] = pack8<E>(s[x][u / 2], 8 * (u & 1));
 #pragma unroll
       for (int b = 0; b < DB; ++b) {
         const bf16x8_t vf = read_turned<D>(vt + u * 32 * D, turn_at ^ (64 * b));
@@ -155,67 +184,158 @@ void attention_kernel(const Attention a) {
     step(t, lds + slot * 2 * TILE, lds + (slot ^ 1) * 2 * TILE);
   }
 #pragma unroll
-  for (int x = 0; x < RT; ++x) {
-    const float total = half_sum(sum[x]);
-    if (!row_live[x]) continue;
-    const long long token = p.q_row + query[x];
-    const long long row = token * a.heads + (long long)p.kvh * a.group + head[x];
-    if (a.splits > 1) {
-      const long long at = (long long)p.split * a.q_len * a.heads * (a.seqs ? 1 : a.batch) + row;
-      float* part = a.part + at * a.dim;
-      if (h == 0) a.part_stats[at] = make_float2(ref[x], total);
-#pragma unroll
-      for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const int d = 32 * b + result_row(i, h);
-          if (d < a.dim)
-            *reinterpret_cast<f32x4_t*>(part + d) =
-                f32x4_t{o[x][b][i], o[x][b][i + 1], o[x][b][i + 2], o[x][b][i + 3]};
-        }
-      continue;
-    }
-    // a row that sees nothing is 0
-    const float f = total == 0.f ? 0.f : 1.f / total;
-    uint16_t* out = a.out + row * a.dim;
-#pragma unroll
-    for (int b = 0; b < DB; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const int d = 32 * b + result_row(i, h);
-        if (d < a.dim)
-          *reinterpret_cast<u32x2_t*>(out + d) = u32x2_t{pack2_elt<E>(o[x][b][i] * f, o[x][b][i + 1] * f),
-                                                         pack2_elt<E>(o[x][b][i + 2] * f, o[x][b][i + 3] * f)};
-      }
-    if (a.lse && h == 0) a.lse[row] = total == 0.f ? kInf : ref[x] + __log2f(total);
-  }
+  for (int x = 0; x < RT; ++x)
+    store_row<E, DB>(a, p, row_live[x], query[x], head[x], o[x], ref[x], half_sum(sum[x]), h);
 }
 
-// Joins the parts of the key axis: one wave a row, 4 bytes a lane.
+// Few rows over many keys (single tokens over a cache): a wave for itself takes 32 rows and a part of the
+// keys, 32 at a time. Bound by reading k and v: no wave waits for another, and the next two tiles of both
+// are in flight while one is worked on (24 to 32 KB a wave, five waves a CU).
+template <int E, int D>
+__global__ __launch_bounds__(64) void attention_few_kernel(const Attention a) {
+  constexpr int KS = D / 16, DB = D / 32, KEYS = 32, TILE = KEYS * D * 2, LOADS = TILE / 1024;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
+  const Place p = place_of<false>(a, false);
+  if (!p.live) return;
+  const int lane = threadIdx.x, h = lane >> 5;
+  const int r0 = p.tile * kFewRows, rows = p.qn * a.group;
+  const int r = r0 + (lane & 31), query = r / a.group, head = r - query * a.group;
+  const bool live = r < rows;
+  const int last_row = r0 + kFewRows < rows ? r0 + kFewRows - 1 : rows - 1;
+  const Sight first = sight_of(a, p, r0 / a.group), last = sight_of(a, p, last_row / a.group);
+  const Sight see = live ? sight_of(a, p, query) : Sight{0, 0};
+  int t0 = first.lo / KEYS, t1 = (last.hi + KEYS - 1) / KEYS;
+  if (t1 < t0) t1 = t0;
+  const int each = (t1 - t0 + a.splits - 1) / a.splits;
+  t0 = t0 + p.split * each < t1 ? t0 + p.split * each : t1;
+  t1 = t0 + each < t1 ? t0 + each : t1;
+  // keys that every row sees; rows past the last one are not stored, and need no mask
+  const int full_lo = last.lo, full_hi = first.hi;
+
+  TileMover<D, KEYS, 1> mk, mv;
+  mk.init(a.k_token, a.dim, 0, lane);
+  mv.init(a.v_token, a.dim, 0, lane);
+  auto fetch_k = [&](int t, char* to) __attribute__((always_inline)) {
+    const int j0 = t * KEYS;
+    mk.issue(a.k + p.k_off + j0 * a.k_token, a.k_token, a.dim, p.kn - j0, to);
+  };
+  auto fetch_v = [&](int t, char* to) __attribute__((always_inline)) {
+    const int j0 = t * KEYS;
+    mv.issue(a.v + p.v_off + j0 * a.v_token, a.v_token, a.dim, p.kn - j0, to);
+  };
+  bf16x8_t qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int at = 16 * s + 8 * h;
+    qf[s] = bf16x8_t{};
+    if (live && at < a.dim)
+      qf[s] = *reinterpret_cast<const bf16x8_t*>(a.q + p.q_off + query * a.q_token + head * a.q_head + at);
+  }
+  const int row_at = row_form<D>(lane), turn_at = turned_form<D>(lane);
+  f32x16_t o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b) o[b] = f32x16_t{};
+  float ref = -kInf, sum = 0.f;
+  // A slot is filled again as soon as it has been read: the waits count the loads of the three tiles behind
+  // (none are missing before the last two). The slots are restrict so that the compiler adds no waits of its
+  // own; the empty asm statements keep reads and loads of one slot in their order.
+  auto step = [&](int t, const char* __restrict__ kt, const char* __restrict__ vt, char* __restrict__ k_next,
+                  char* __restrict__ v_next) __attribute__((always_inline)) {
+    const bool more = t + 2 < t1;
+    if (more) wait_vmcnt<3 * LOADS>();
+    else wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    f32x16_t s = {};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      s = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(kt + (row_at ^ (32 * k))), qf[k], s);
+    asm volatile("" : "+v"(s) : : "memory");
+    if (more) fetch_k(t + 2, k_next);
+    const int j0 = t * KEYS;
+    if (j0 < full_lo || j0 + KEYS > full_hi) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int j = j0 + result_row(i, h);
+        s[i] = j >= see.lo && j < see.hi ? s[i] : -kInf;
+      }
+    }
+    float top = -kInf;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
+    top = half_max(top) * a.c;
+    if (__ballot(top > ref + 8.f)) {
+      const float now = fmaxf(ref, top), from = now == -kInf ? 0.f : now;
+      const float f = __builtin_amdgcn_exp2f(ref - from);
+      ref = now;
+      sum *= f;
+#pragma unroll
+      for (int b = 0; b < DB; ++b) o[b] *= f;
+    }
+    const float from = ref == -kInf ? 0.f : ref;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -from));
+      sum += s[i];
+    }
+    if (more) wait_vmcnt<3 * LOADS>();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bf16x8_t pf = pack8<E>(s, 8 * u);
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+        o[b] = mfma_32x32x16<E>(read_turned<D>(vt + u * 32 * D, turn_at ^ (64 * b)), pf, o[b]);
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): every read of the slot has returned
+    asm volatile("" ::: "memory");
+    if (more) fetch_v(t + 2, v_next);
+  };
+  for (int t = t0; t < t1 && t < t0 + 2; ++t) {
+    fetch_k(t, lds + (t - t0) * 2 * TILE);
+    fetch_v(t, lds + (t - t0) * 2 * TILE + TILE);
+  }
+  for (int t = t0; t < t1; ++t) {
+    char* slot = lds + ((t - t0) & 1) * 2 * TILE;
+    step(t, slot, slot + TILE, slot, slot + TILE);
+  }
+  store_row<E, DB>(a, p, live, query, head, o, ref, half_sum(sum), h);
+}
+
+// Joins the parts of the key axis (64 at most): one wave a row, two values a lane.
 template <int E>
 __global__ __launch_bounds__(256) void attention_join_kernel(const Attention a) {
   const long long rows = (long long)a.q_len * a.heads * (a.seqs ? 1 : a.batch);
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long row = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (row >= rows) return;
-  float top = -kInf;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_stats[s * rows + row].x);
+  // part l's statistics in lane l
+  float2 st = make_float2(-kInf, 0.f);
+  if (lane < a.splits) st = a.part_stats[lane * rows + row];
+  float top = st.x;
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
   const float from = top == -kInf ? 0.f : top;
-  float total = 0.f, o[2] = {0.f, 0.f};
-  const int d = 2 * lane;
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 st = a.part_stats[s * rows + row];
-    const float f = __builtin_amdgcn_exp2f(st.x - from);
-    total += f * st.y;
-    if (d < a.dim) {
-      const float2 v = *reinterpret_cast<const float2*>(a.part + (s * rows + row) * a.dim + d);
-      o[0] += f * v.x;
-      o[1] += f * v.y;
+  const float f = __builtin_amdgcn_exp2f(st.x - from);
+  float total = f * st.y;
+  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+  float o0 = 0.f, o1 = 0.f;
+  const int d = 2 * lane < a.dim ? 2 * lane : 0;
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    float2 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int s = s0 + k < a.splits ? s0 + k : a.splits - 1;
+      v[k] = *reinterpret_cast<const float2*>(a.part + (s * rows + row) * a.dim + d);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (s0 + k) & 63));
+      o0 += s0 + k < a.splits ? g * v[k].x : 0.f;
+      o1 += s0 + k < a.splits ? g * v[k].y : 0.f;
     }
   }
-  const float f = total == 0.f ? 0.f : 1.f / total;
-  if (d < a.dim)
-    *reinterpret_cast<unsigned*>(a.out + row * a.dim + d) = pack2_elt<E>(o[0] * f, o[1] * f);
+  const float g = total == 0.f ? 0.f : 1.f / total;
+  if (2 * lane < a.dim)
+    *reinterpret_cast<unsigned*>(a.out + row * a.dim + d) = pack2_elt<E>(o0 * g, o1 * g);
   if (a.lse && lane == 0) a.lse[row] = total == 0.f ? kInf : top + __log2f(total);
 }
 
@@ -301,7 +421,8 @@ __global__ __launch_bounds__(1024) void attention_tables_kernel(
 
 template <int E, int D>
 void launch(const Attention& a, unsigned blocks, hipStream_t stream) {
-  hipLaunchKernelGGL((attention_kernel<E, D, 1>), dim3(blocks), dim3(256), 0, stream, a);
+  if (a.few) hipLaunchKernelGGL((attention_few_kernel<E, D>), dim3(blocks), dim3(64), 0, stream, a);
+  else hipLaunchKernelGGL((attention_kernel<E, D, 1>), dim3(blocks), dim3(256), 0, stream, a);
 }
 
 }  // namespace

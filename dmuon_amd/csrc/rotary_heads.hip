@@ -5,10 +5,11 @@
 // Backward, g = R^T dy:  dw = sum g xhat,  dx = r (g w - xhat mean(g w xhat)).
 //
 // Memory bound: forward reads x and writes y; backward reads x and dy and writes dx (the root mean
-// square is formed anew). A head's values are spread over 4 pairs a lane: pairs half a rotation apart need
-// no exchange between lanes, and one exchange of sums joins the lanes of a head. A block works on a few
-// tokens, whose cosines and sines it forms once for all heads: in turns, reduced in 64 bits to an eighth
-// of a turn around a multiple of a quarter, so that positions of any size keep 32 bits of accuracy.
+// square is formed anew). A lane has the same 8 pairs of every head (4, or 1, where a head has no more), so
+// that pairs half a rotation apart need no exchange, and one exchange of sums joins the lanes of a head.
+// The lanes of a group keep a token's cosines and sines in registers and walk its heads, the next one's
+// loads in flight: angles are formed once a token and part of the heads, in turns, reduced in 64 bits to an
+// eighth of a turn around a multiple of a quarter, so that positions of any size keep 32 bits of accuracy.
 #include "../../include/dmuon_amd.h"
 #include "dmuon_amd_internal.h"
 #include "mfma_tile.h"
@@ -19,24 +20,21 @@ namespace dmuon {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxDim = 512, kMaxAngles = 1024;   // angles a block holds
+constexpr int kMaxDim = 512;
 
 struct Heads {
   const void* x[2]; void* y[2]; const void* dy[2]; void* dx[2];   // queries, keys
   const void* w[2];                       // [dim] or NULL
-  void* dw[2]; float* part;               // [2][blocks][dim]
+  void* dw[2]; float* part[2];            // [parts * blocks][dim]
   long long token[2], head[2], dtoken[2], dhead[2];               // strides in elements
   const int64_t* positions; const void* inv_freq;
-  long long tokens, period, tokens_per_block;
+  long long tokens, period;
   int heads[2], dim, rotary, dtype, w_dtype[2], freq_double, interleaved;
-  int lanes;                              // of a head: a power of two
-  int at_once;                            // tokens whose angles a block holds
-  int blocks;
+  int pairs, lanes;                       // of a lane; of a head: a power of two
+  int per_part, parts[2];                 // heads that one group walks; parts of the queries', keys' heads
+  int blocks;                             // of one part
   float eps;
 };
-
-typedef u32x4_t v16_t __attribute__((aligned(2)));
-typedef u32x2_t v8_t __attribute__((aligned(2)));
 
 __device__ __forceinline__ float element(const void* p, int t, long long at) {
   if (t == DT_F32) return static_cast<const float*>(p)[at];
@@ -48,34 +46,50 @@ __device__ __forceinline__ void set_element(void* p, int t, long long at, float 
   else static_cast<uint16_t*>(p)[at] = t == DT_F16 ? to_elt<ELT_F16>(v) : to_elt<ELT_BF16>(v);
 }
 
-// Four values of type T from `p`, at any element alignment
-template <int T>
-__device__ __forceinline__ void load4(const void* p, long long at, float* v) {
-  if constexpr (T == DT_F32) {
-    typedef f32x4_t f4_t __attribute__((aligned(4)));
-    const f32x4_t x = *reinterpret_cast<const f4_t*>(static_cast<const float*>(p) + at);
+// N (4 or 8) values of type T as they lie in memory, at any element alignment
+template <int T, int N>
+struct Run {
+  static constexpr int W = T == DT_F32 ? N : N / 2;      // 32-bit words
+  unsigned w[W];
+  __device__ __forceinline__ void load(const void* p, long long at) {
+    typedef unsigned words_t __attribute__((ext_vector_type(W < 4 ? 2 : 4)));
+    typedef words_t any_t __attribute__((aligned(T == DT_F32 ? 4 : 2)));
+    constexpr int V = W < 4 ? 2 : 4;
+    const char* src = static_cast<const char*>(p) + at * (T == DT_F32 ? 4 : 2);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = x[i];
-  } else {
-    const u32x2_t x = *reinterpret_cast<const v8_t*>(static_cast<const uint16_t*>(p) + at);
+    for (int i = 0; i < W; i += V) {
+      const words_t x = *reinterpret_cast<const any_t*>(src + 4 * i);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint16_t u = (uint16_t)(i & 1 ? x[i / 2] >> 16 : x[i / 2]);
-      v[i] = T == DT_F16 ? from_elt<ELT_F16>(u) : from_elt<ELT_BF16>(u);
+      for (int k = 0; k < V; ++k) w[i + k] = x[k];
     }
   }
-}
-template <int T>
-__device__ __forceinline__ void store4(void* p, long long at, const float* v) {
-  if constexpr (T == DT_F32) {
-    typedef f32x4_t f4_t __attribute__((aligned(4)));
-    *reinterpret_cast<f4_t*>(static_cast<float*>(p) + at) = f32x4_t{v[0], v[1], v[2], v[3]};
-  } else {
-    constexpr int E = T == DT_F16 ? ELT_F16 : ELT_BF16;
-    *reinterpret_cast<v8_t*>(static_cast<uint16_t*>(p) + at) =
-        u32x2_t{pack2_elt<E>(v[0], v[1]), pack2_elt<E>(v[2], v[3])};
+  __device__ __forceinline__ void store(void* p, long long at) const {
+    typedef unsigned words_t __attribute__((ext_vector_type(W < 4 ? 2 : 4)));
+    typedef words_t any_t __attribute__((aligned(T == DT_F32 ? 4 : 2)));
+    constexpr int V = W < 4 ? 2 : 4;
+    char* dst = static_cast<char*>(p) + at * (T == DT_F32 ? 4 : 2);
+#pragma unroll
+    for (int i = 0; i < W; i += V) {
+      words_t x;
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[k] = w[i + k];
+      __builtin_nontemporal_store(x, reinterpret_cast<any_t*>(dst + 4 * i));
+    }
   }
-}
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (T == DT_F32) return __uint_as_float(w[i]);
+    const uint16_t u = (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2]);
+    return T == DT_F16 ? from_elt<ELT_F16>(u) : from_elt<ELT_BF16>(u);
+  }
+  __device__ __forceinline__ void set2(int i, float a, float b) {    // values i and i + 1
+    if constexpr (T == DT_F32) {
+      w[i] = __float_as_uint(a);
+      w[i + 1] = __float_as_uint(b);
+    } else {
+      w[i / 2] = pack2_elt<T == DT_F16 ? ELT_F16 : ELT_BF16>(a, b);
+    }
+  }
+};
 
 // Where pair p of a head lies: a rotated pair for p < rotary / 2, two neighbours behind them.
 __device__ __forceinline__ void pair_at(const Heads& a, int p, int* i, int* j) {
@@ -89,210 +103,209 @@ __device__ __forceinline__ void pair_at(const Heads& a, int p, int* i, int* j) {
   }
 }
 
-// P pairs from pair `p` on (P = 4: rotary and dim are multiples of 8): v[0 .. P) are the pairs' first
-// values, v[P .. 2P) their second
+// A lane's P pairs of a head, from pair `p` on: P = 8 (rotary and dim multiples of 16) or 4 (of 8) are two
+// runs of P values, the pairs' first and second ones or, of neighbours, one behind the other.
 template <int T, int P>
-__device__ __forceinline__ void load_pairs(const Heads& a, const void* src, long long at, int p, float* v) {
-  int i, j;
-  pair_at(a, p, &i, &j);
-  if constexpr (P == 1) {
-    v[0] = element(src, T, at + i);
-    v[1] = element(src, T, at + j);
-  } else {
-    const bool apart = j - i > 1;
-    float lo[4], hi[4];
-    load4<T>(src, at + i, lo);
-    load4<T>(src, at + (apart ? j : i + 4), hi);
+struct Pairs {
+  Run<T, P> r[2];
+  __device__ __forceinline__ void load(const void* src, long long at, int i, int j) {
+    r[0].load(src, at + i);
+    r[1].load(src, at + j);
+  }
+  __device__ __forceinline__ void get(bool apart, float* v) const {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float side = k < 2 ? lo[2 * k] : hi[2 * k - 4], next = k < 2 ? lo[2 * k + 1] : hi[2 * k - 3];
-      v[k] = apart ? lo[k] : side;
-      v[4 + k] = apart ? hi[k] : next;
+    for (int k = 0; k < P; ++k) {
+      const float lo = r[0].get(k), hi = r[1].get(k);
+      const float even = 2 * k < P ? r[0].get((2 * k) % P) : r[1].get((2 * k) % P);
+      const float odd = 2 * k < P ? r[0].get((2 * k + 1) % P) : r[1].get((2 * k + 1) % P);
+      v[k] = apart ? lo : even;
+      v[P + k] = apart ? hi : odd;
     }
   }
-}
-template <int T, int P>
-__device__ __forceinline__ void store_pairs(const Heads& a, void* dst, long long at, int p, const float* v) {
-  int i, j;
-  pair_at(a, p, &i, &j);
-  if constexpr (P == 1) {
-    set_element(dst, T, at + i, v[0]);
-    set_element(dst, T, at + j, v[1]);
-  } else {
-    const bool apart = j - i > 1;
-    float lo[4], hi[4];
+  __device__ __forceinline__ void set(bool apart, const float* v) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      lo[k] = apart ? v[k] : v[(k & 1) * 4 + k / 2];
-      hi[k] = apart ? v[4 + k] : v[(k & 1) * 4 + 2 + k / 2];
+    for (int k = 0; k < P; k += 2) {
+      // values k and k + 1 of both runs
+      r[0].set2(k, apart ? v[k] : v[k / 2], apart ? v[k + 1] : v[P + k / 2]);
+      r[1].set2(k, apart ? v[P + k] : v[(P + k) / 2], apart ? v[P + k + 1] : v[P + (P + k) / 2]);
     }
-    store4<T>(dst, at + i, lo);
-    store4<T>(dst, at + (apart ? j : i + 4), hi);
   }
-}
+  __device__ __forceinline__ void store(void* dst, long long at, int i, int j) const {
+    r[0].store(dst, at + i);
+    r[1].store(dst, at + j);
+  }
+};
+template <int T>
+struct Pairs<T, 1> {
+  float a, b;
+  __device__ __forceinline__ void load(const void* src, long long at, int i, int j) {
+    a = element(src, T, at + i);
+    b = element(src, T, at + j);
+  }
+  __device__ __forceinline__ void get(bool, float* v) const { v[0] = a, v[1] = b; }
+  __device__ __forceinline__ void set(bool, const float* v) { a = v[0], b = v[1]; }
+  __device__ __forceinline__ void store(void* dst, long long at, int i, int j) const {
+    set_element(dst, T, at + i, a);
+    set_element(dst, T, at + j, b);
+  }
+};
 
-// cos and sin of position * inv_freq
-__device__ __forceinline__ float2 turn_of(const Heads& a, long long position, int pair) {
+// cos and sin of position * inv_freq: within an eighth of a turn the Taylor polynomials are off by less
+// than 2^-29
+__device__ __forceinline__ float2 turn_of(const Heads& a, double position, int pair) {
   const double f = a.freq_double ? static_cast<const double*>(a.inv_freq)[pair]
                                  : (double)static_cast<const float*>(a.inv_freq)[pair];
-  const double turns = (double)position * f * 0.15915494309189533577;
-  const double quarters = rint(turns * 4.);
-  const float rest = (float)(turns - quarters * 0.25) * 2.f;     // in half turns, at most a quarter
-  const int k = (int)(quarters - 4. * floor(quarters * 0.25));
-  const float c = cospif(rest), s = sinpif(rest);
-  return k == 0 ? make_float2(c, s) : k == 1 ? make_float2(-s, c)
-       : k == 2 ? make_float2(-c, -s) : make_float2(s, -c);
+  const double quarters = position * f * (4. * 0.15915494309189533577);
+  const double whole = rint(quarters);
+  const float t = (float)(quarters - whole) * 1.57079632679489661923f, q = t * t;
+  const float s = t + t * q * (-1.f / 6.f + q * (1.f / 120.f + q * (-1.f / 5040.f + q * (1.f / 362880.f))));
+  const float c = 1.f + q * (-0.5f + q * (1.f / 24.f + q * (-1.f / 720.f + q * (1.f / 40320.f -
+                                                                              q * (1.f / 3628800.f)))));
+  const int k = (int)(whole - 4. * floor(whole * 0.25));
+  const float cc = k & 1 ? s : c, ss = k & 1 ? c : s;
+  return make_float2(k == 1 || k == 2 ? -cc : cc, k >= 2 ? -ss : ss);
 }
 
 // GRAD: x and dy to dx and the weights' partial sums; otherwise x to y. SLOTS: of P pairs a lane.
+// blockIdx.y is the part of the heads: the queries' parts, then the keys'.
 template <int T, int P, int SLOTS, bool GRAD>
 __global__ __launch_bounds__(kThreads) void rotary_heads_kernel(const Heads a) {
-  __shared__ float2 turn[kMaxAngles];
   __shared__ float sums[GRAD ? kThreads : 1][2 * P + 1];
   const int sub = threadIdx.x % a.lanes, group = threadIdx.x / a.lanes, groups = kThreads / a.lanes;
-  const int half = a.rotary / 2, pairs = a.dim / 2, all = a.heads[0] + a.heads[1];
+  const int half = a.rotary / 2;
+  const int z = (int)blockIdx.y >= a.parts[0], part = (int)blockIdx.y - (z ? a.parts[0] : 0);
+  const int h0 = part * a.per_part, h1 = min(h0 + a.per_part, a.heads[z]);
+  const bool norm = a.w[z] != nullptr;
   const float inv = 1.f / (float)a.dim;
-  int pair[SLOTS];
-  bool live[SLOTS];
-  float w[2][SLOTS][2 * P], dw[2][SLOTS][2 * P];
+  const void* x = a.x[z];
+  const void* dy = a.dy[z];
+  void* to = GRAD ? a.dx[z] : a.y[z];
+  int pair[SLOTS], vi[SLOTS], vj[SLOTS];
+  bool live[SLOTS], apart[SLOTS];
+  float w[SLOTS][2 * P], dw[SLOTS][2 * P];
 #pragma unroll
   for (int u = 0; u < SLOTS; ++u) {
     pair[u] = (u * a.lanes + sub) * P;
-    live[u] = pair[u] < pairs;
+    live[u] = pair[u] < a.dim / 2;
     if (!live[u]) pair[u] = 0;
+    pair_at(a, pair[u], &vi[u], &vj[u]);
+    apart[u] = vj[u] - vi[u] > 1;
+    if (P > 1 && !apart[u]) vj[u] = vi[u] + P;
 #pragma unroll
-    for (int z = 0; z < 2; ++z)
-#pragma unroll
-      for (int i = 0; i < 2 * P; ++i) {
-        int at[2];
-        pair_at(a, pair[u] + i % P, &at[0], &at[1]);
-        w[z][u][i] = a.w[z] && live[u] ? element(a.w[z], a.w_dtype[z], at[i / P]) : 1.f;
-        dw[z][u][i] = 0.f;
-      }
+    for (int i = 0; i < 2 * P; ++i) {
+      int at[2];
+      pair_at(a, pair[u] + i % P, &at[0], &at[1]);
+      w[u][i] = norm && live[u] ? element(a.w[z], a.w_dtype[z], at[i / P]) : 1.f;
+      dw[u][i] = 0.f;
+    }
   }
-  const long long begin = (long long)blockIdx.x * a.tokens_per_block;
-  const long long end = begin + a.tokens_per_block < a.tokens ? begin + a.tokens_per_block : a.tokens;
-  for (long long t0 = begin; t0 < end; t0 += a.at_once) {
-    const int n = end - t0 < a.at_once ? (int)(end - t0) : a.at_once;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n * half; i += kThreads)
-      turn[i] = turn_of(a, a.positions[a.period == a.tokens ? t0 + i / half : (t0 + i / half) % a.period],
-                        i % half);
-    __syncthreads();
-    for (int i = group; i < (n * all + groups - 1) / groups * groups; i += groups) {
-      // groups past the last head repeat it without a share of the sums
-      const bool mine = i < n * all;
-      const int it = mine ? i : n * all - 1;
-      const int t = it / all, hd = it - t * all, z = hd >= a.heads[0];
-      const int hz = z ? hd - a.heads[0] : hd;
-      const bool norm = z ? a.w[1] != nullptr : a.w[0] != nullptr;
-      const long long token = t0 + t;
-      const long long at = token * (z ? a.token[1] : a.token[0]) + hz * (z ? a.head[1] : a.head[0]);
-      const long long out = (token * (z ? a.heads[1] : a.heads[0]) + hz) * a.dim;
-      const void* src = z ? a.x[1] : a.x[0];
-      float x[SLOTS][2 * P], g[SLOTS][2 * P];
-      if constexpr (GRAD) {
-        const void* dsrc = z ? a.dy[1] : a.dy[0];
-        const long long dat = token * (z ? a.dtoken[1] : a.dtoken[0]) + hz * (z ? a.dhead[1] : a.dhead[0]);
+  for (long long token = (long long)blockIdx.x * groups + group; token < a.tokens;
+       token += (long long)gridDim.x * groups) {
+    long long at = token * a.token[z] + h0 * a.head[z], dat = token * a.dtoken[z] + h0 * a.dhead[z];
+    long long out = (token * a.heads[z] + h0) * a.dim;
+    Pairs<T, P> xr[SLOTS], gr[SLOTS];
+    auto fetch = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < SLOTS; ++u) {
-          if (dsrc) load_pairs<T, P>(a, dsrc, dat, pair[u], g[u]);
-          else
-#pragma unroll
-            for (int k = 0; k < 2 * P; ++k) g[u][k] = 0.f;
-        }
+      for (int u = 0; u < SLOTS; ++u) {
+        if (!GRAD || norm) xr[u].load(x, at, vi[u], vj[u]);
+        if (GRAD && dy) gr[u].load(dy, dat, vi[u], vj[u]);
       }
-      if (!GRAD || norm)
+    };
+    fetch();
+    float2 cs[SLOTS][P];
+    {
+      const long long slot = a.period == a.tokens ? token : token % a.period;
+      const double position = (double)a.positions[slot];
 #pragma unroll
-        for (int u = 0; u < SLOTS; ++u) load_pairs<T, P>(a, src, at, pair[u], x[u]);
-      // turns the pairs of v; back: by the opposite angle
-      auto rotate = [&](float (&v)[SLOTS][2 * P], float sign) {
+      for (int u = 0; u < SLOTS; ++u)
+#pragma unroll
+        for (int k = 0; k < P; ++k)
+          cs[u][k] = pair[u] + k < half ? turn_of(a, position, pair[u] + k) : make_float2(1.f, 0.f);
+    }
+    for (int h = h0; h < h1; ++h) {
+      float v[SLOTS][2 * P], g[SLOTS][2 * P];
+#pragma unroll
+      for (int u = 0; u < SLOTS; ++u) {
+        if (!GRAD || norm) xr[u].get(apart[u], v[u]);
+#pragma unroll
+        for (int k = 0; k < 2 * P; ++k) g[u][k] = 0.f;
+        if (GRAD && dy) gr[u].get(apart[u], g[u]);
+      }
+      at += a.head[z];
+      dat += a.dhead[z];
+      if (h + 1 < h1) fetch();
+      // turns the pairs; back: by the opposite angle
+      auto rotate = [&](float (&p)[SLOTS][2 * P], float sign) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < SLOTS; ++u)
 #pragma unroll
-          for (int k = 0; k < P; ++k)
-            if (pair[u] + k < half) {
-              const float2 cs = turn[t * half + pair[u] + k];
-              const float p = v[u][k], q = v[u][P + k], s = sign * cs.y;
-              v[u][k] = p * cs.x - q * s;
-              v[u][P + k] = q * cs.x + p * s;
-            }
+          for (int k = 0; k < P; ++k) {
+            const float i = p[u][k], j = p[u][P + k], s = sign * cs[u][k].y;
+            p[u][k] = i * cs[u][k].x - j * s;
+            p[u][P + k] = j * cs[u][k].x + i * s;
+          }
       };
       float sq = 0.f, dot = 0.f;
-      if constexpr (GRAD) {
-        rotate(g, -1.f);
-        if (norm) {
+      if constexpr (GRAD) rotate(g, -1.f);
+      if (norm) {
 #pragma unroll
-          for (int u = 0; u < SLOTS; ++u)
+        for (int u = 0; u < SLOTS; ++u)
 #pragma unroll
-            for (int k = 0; k < 2 * P; ++k)
-              if (live[u]) {
-                sq += x[u][k] * x[u][k];
-                dot += g[u][k] * (z ? w[1][u][k] : w[0][u][k]) * x[u][k];
-              }
-          for (int o = 1; o < a.lanes; o <<= 1) sq += __shfl_xor(sq, o), dot += __shfl_xor(dot, o);
-          const float r = 1.f / sqrtf(sq * inv + a.eps);
-          const float m = dot * r * inv;
+          for (int k = 0; k < 2 * P; ++k) {
+            const float e = live[u] ? v[u][k] : 0.f;
+            sq += e * e;
+            if constexpr (GRAD) dot += g[u][k] * w[u][k] * e;
+          }
+        for (int o = 1; o < a.lanes; o <<= 1) {
+          sq += __shfl_xor(sq, o);
+          if constexpr (GRAD) dot += __shfl_xor(dot, o);
+        }
+        const float r = __builtin_amdgcn_rsqf(sq * inv + a.eps);
+        const float m = dot * r * inv;
 #pragma unroll
-          for (int u = 0; u < SLOTS; ++u)
+        for (int u = 0; u < SLOTS; ++u)
 #pragma unroll
-            for (int k = 0; k < 2 * P; ++k) {
-              const float xh = x[u][k] * r;
-              const float share = mine ? g[u][k] * xh : 0.f;
-              dw[0][u][k] += z ? 0.f : share;
-              dw[1][u][k] += z ? share : 0.f;
-              g[u][k] = r * (g[u][k] * (z ? w[1][u][k] : w[0][u][k]) - xh * m);
+          for (int k = 0; k < 2 * P; ++k) {
+            v[u][k] *= r;
+            if constexpr (GRAD) {
+              dw[u][k] += g[u][k] * v[u][k];
+              g[u][k] = r * (g[u][k] * w[u][k] - v[u][k] * m);
+            } else {
+              v[u][k] *= w[u][k];
             }
-        }
-        void* dst = z ? a.dx[1] : a.dx[0];
-        if (dst && mine)
-#pragma unroll
-          for (int u = 0; u < SLOTS; ++u)
-            if (live[u]) store_pairs<T, P>(a, dst, out, pair[u], g[u]);
-      } else {
-        if (norm) {
-#pragma unroll
-          for (int u = 0; u < SLOTS; ++u)
-#pragma unroll
-            for (int k = 0; k < 2 * P; ++k)
-              if (live[u]) sq += x[u][k] * x[u][k];
-          for (int o = 1; o < a.lanes; o <<= 1) sq += __shfl_xor(sq, o);
-          const float r = 1.f / sqrtf(sq * inv + a.eps);
-#pragma unroll
-          for (int u = 0; u < SLOTS; ++u)
-#pragma unroll
-            for (int k = 0; k < 2 * P; ++k) x[u][k] = x[u][k] * r * (z ? w[1][u][k] : w[0][u][k]);
-        }
-        rotate(x, 1.f);
-        void* dst = z ? a.y[1] : a.y[0];
-        if (mine)
-#pragma unroll
-          for (int u = 0; u < SLOTS; ++u)
-            if (live[u]) store_pairs<T, P>(a, dst, out, pair[u], x[u]);
+          }
       }
+      if constexpr (!GRAD) rotate(v, 1.f);
+      if (to)
+#pragma unroll
+        for (int u = 0; u < SLOTS; ++u)
+          if (live[u]) {
+            Pairs<T, P> y;
+            y.set(apart[u], GRAD ? g[u] : v[u]);
+            y.store(to, out, vi[u], vj[u]);
+          }
+      out += a.dim;
     }
   }
   if constexpr (GRAD) {
+    if (!a.dw[z]) return;
     // the groups' shares in their order, through LDS
+    float* dst = a.part[z] + ((long long)part * gridDim.x + blockIdx.x) * a.dim;
 #pragma unroll
-    for (int z = 0; z < 2; ++z) {
-      if (!a.dw[z]) continue;
-      float* dst = a.part + ((long long)z * a.blocks + blockIdx.x) * a.dim;
+    for (int u = 0; u < SLOTS; ++u) {
+      __syncthreads();
 #pragma unroll
-      for (int u = 0; u < SLOTS; ++u) {
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 2 * P; ++k) sums[threadIdx.x][k] = dw[z][u][k];
-        __syncthreads();
-        if (group || !live[u]) continue;
-#pragma unroll
-        for (int k = 0; k < 2 * P; ++k) {
-          float total = 0.f;
-          for (int g = 0; g < groups; ++g) total += sums[g * a.lanes + sub][k];
-          int at[2];
-          pair_at(a, pair[u] + k % P, &at[0], &at[1]);
-          dst[at[k / P]] = total;
-        }
+      for (int k = 0; k < 2 * P; ++k) sums[threadIdx.x][k] = dw[u][k];
+      __syncthreads();
+      // a thread sums one value: sub's value k
+      for (int i = threadIdx.x; i < a.lanes * 2 * P; i += kThreads) {
+        const int l = i / (2 * P), k = i % (2 * P), p = (u * a.lanes + l) * P;
+        if (p >= a.dim / 2) continue;
+        float total = 0.f;
+        for (int g = 0; g < groups; ++g) total += sums[g * a.lanes + l][k];
+        int spot[2];
+        pair_at(a, p + k % P, &spot[0], &spot[1]);
+        dst[k < P ? spot[0] : spot[1]] = total;
       }
     }
   }
@@ -302,11 +315,13 @@ __global__ __launch_bounds__(kThreads) void rotary_heads_kernel(const Heads a) {
 __global__ __launch_bounds__(1024) void rotary_heads_sum_kernel(const Heads a) {
   __shared__ float lds[32][33];
   const int z = blockIdx.y, lane = threadIdx.x & 31, strand = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+  const int c = blockIdx.x * 32 + lane, rows = a.parts[z] * a.blocks;
   if (!a.dw[z]) return;
   float s = 0.f;
-  if (c < a.dim)
-    for (int k = strand; k < a.blocks; k += 32) s += a.part[((long long)z * a.blocks + k) * a.dim + c];
+  if (c < a.dim) {
+#pragma unroll 4
+    for (int k = strand; k < rows; k += 32) s += a.part[z][(long long)k * a.dim + c];
+  }
   lds[strand][lane] = s;
   __syncthreads();
   const int cc = threadIdx.x >> 5;
@@ -316,30 +331,38 @@ __global__ __launch_bounds__(1024) void rotary_heads_sum_kernel(const Heads a) {
   if (lane == 0 && oc < a.dim) set_element(a.dw[z], a.w_dtype[z], oc, s);
 }
 
-constexpr int64_t kCus = 256;
+constexpr long long kCus = 256;
 
-// Lanes, tokens and blocks of a call
+// Lanes, parts and blocks of a call
 void shape(Heads* a, bool grad) {
-  const bool four = a->rotary % 8 == 0 && a->dim % 8 == 0;
-  const int slots = four ? a->dim / 8 : a->dim / 2;
-  a->lanes = 4;
+  a->pairs = a->rotary % 16 == 0 && a->dim % 16 == 0 ? 8 : a->rotary % 8 == 0 && a->dim % 8 == 0 ? 4 : 1;
+  const int slots = a->dim / 2 / a->pairs;
+  a->lanes = 1;
   while (a->lanes < slots && a->lanes < 64) a->lanes *= 2;
-  const int half = a->rotary / 2;
-  a->at_once = half ? kThreads / half : 8;
-  if (a->at_once < 1) a->at_once = 1;
-  if (a->at_once > 16) a->at_once = 16;
-  const long long want = grad ? kCus * 4 : 0x7fffffffLL;
-  a->tokens_per_block = (a->tokens + want - 1) / want;
-  a->tokens_per_block = (a->tokens_per_block + a->at_once - 1) / a->at_once * a->at_once;
-  if (a->tokens_per_block < 1) a->tokens_per_block = 1;
-  a->blocks = (int)((a->tokens + a->tokens_per_block - 1) / a->tokens_per_block);
+  const int groups = kThreads / a->lanes;
+  const long long all = (a->tokens + groups - 1) / groups;
+  // few tokens: a group walks few heads. More than 16 a group leave too few groups, fewer form the angles too
+  // often: forward and backward over 16384 tokens of 32 + 8 heads of 128 in bf16 72 and 94 us at 16, 74 and
+  // 106 at 8, 84 and 114 at 4
+  a->per_part = 16;
+  auto blocks_at = [&](int per) {
+    return all * ((a->heads[0] + per - 1) / per + (a->heads[1] + per - 1) / per);
+  };
+  while (a->per_part > 1 && blocks_at(a->per_part) < kCus * 4) a->per_part /= 2;
+  for (int z = 0; z < 2; ++z) a->parts[z] = (a->heads[z] + a->per_part - 1) / a->per_part;
+  // the gradient's partial rows: as many blocks as their registers let run at once (of 512 it took 113 us,
+  // of 1024 98, of 768 94)
+  const long long most = grad ? (kCus * 3 + a->parts[0] + a->parts[1] - 1) / (a->parts[0] + a->parts[1])
+                              : 0x7fffffffLL;
+  a->blocks = (int)(all < most ? all : most);
 }
 
 template <int T, bool GRAD>
 void launch(const Heads& a, hipStream_t stream) {
-  const dim3 grid((unsigned)a.blocks);
-  const bool four = a.rotary % 8 == 0 && a.dim % 8 == 0;
-  if (four)
+  const dim3 grid((unsigned)a.blocks, (unsigned)(a.parts[0] + a.parts[1]));
+  if (a.pairs == 8)
+    hipLaunchKernelGGL((rotary_heads_kernel<T, 8, 1, GRAD>), grid, dim3(kThreads), 0, stream, a);
+  else if (a.pairs == 4)
     hipLaunchKernelGGL((rotary_heads_kernel<T, 4, 1, GRAD>), grid, dim3(kThreads), 0, stream, a);
   else if (a.dim <= 128)
     hipLaunchKernelGGL((rotary_heads_kernel<T, 1, 1, GRAD>), grid, dim3(kThreads), 0, stream, a);
@@ -358,6 +381,17 @@ hipError_t launch_heads(const Heads& a, hipStream_t stream) {
     hipLaunchKernelGGL(rotary_heads_sum_kernel, dim3((unsigned)((a.dim + 31) / 32), 2), dim3(1024), 0, stream,
                        a);
   return hipGetLastError();
+}
+
+// Partial rows of the weights' gradients, in bytes
+int64_t partials(Heads* h, void* ws) {
+  int64_t at = 0;
+  for (int z = 0; z < 2; ++z) {
+    if (!h->dw[z]) continue;
+    h->part[z] = ws ? static_cast<float*>(ws) + at : nullptr;
+    at += (int64_t)h->parts[z] * h->blocks * h->dim;
+  }
+  return at * 4;
 }
 
 bool float_code(int c) {
@@ -430,8 +464,8 @@ int dmuon_rotary_heads_grad_workspace_size(const dmuon_rotary_heads_args* args, 
   const char* who = "dmuon_rotary_heads_grad_workspace_size";
   if (!workspace_bytes) return fail("%s: NULL output", who);
   if (check(who, args)) return 1;
-  *workspace_bytes = args->d_q_weight || args->d_k_weight
-                         ? 8LL * describe(*args, true).blocks * args->dim : 0;
+  Heads h = describe(*args, true);
+  *workspace_bytes = partials(&h, nullptr);
   return 0;
 }
 
@@ -442,11 +476,10 @@ int dmuon_rotary_heads_grad(const dmuon_rotary_heads_args* args, void* workspace
   if ((args->d_q_weight && !args->q_weight) || (args->d_k_weight && !args->k_weight))
     return fail("%s: a gradient of an operand that is not there", who);
   Heads h = describe(*args, true);
-  const int64_t need = h.dw[0] || h.dw[1] ? 8LL * h.blocks * h.dim : 0;
+  const int64_t need = partials(&h, workspace);
   if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return fail("%s: needs a 16-byte aligned workspace of %lld bytes, got %lld", who, (long long)need,
                 (long long)workspace_bytes);
-  h.part = static_cast<float*>(workspace);
   return check_launch(launch_heads<true>(h, static_cast<hipStream_t>(stream)), who);
 }
 
