@@ -4,7 +4,7 @@
 //
 // Memory bound: forward reads and writes a row a token; backward reads a row a token and writes every
 // row of dW, most of them zeros. The gradient sorts the positions by token (stable, so that a class's rows
-// add up in their order), walks the sorted positions in runs of kRun, and joins the classes that cross
+// add up in their order), walks the sorted positions in runs of 8 or 32, and joins the classes that cross
 // from one run to the next in a second kernel: the work of a class that makes up most of the text is
 // spread like any other. Sums are fp32, rounded once.
 #include "../../include/dmuon_amd.h"
@@ -14,10 +14,15 @@
 namespace dmuon {
 namespace {
 
-constexpr int kRun = 32;                  // sorted positions of a block
+constexpr int kRun = 32;                  // sorted positions of a block, at most
+constexpr int kAhead = 8;
 constexpr int kDigit = 9, kBins = 1 << kDigit;
 constexpr int kSortTile = 1024, kSortBlocks = 64;
-constexpr int kFillRows = 32;             // rows of dW that a block clears
+constexpr int kFillRows = 32;             // rows of dW that a block of the sums clears
+constexpr long long kFillChunks = 4096;   // 16-byte chunks that a block of the sort clears
+// what the launches of one pass of the sort clear: as much as they take time (3 and 5 us) at the rate of
+// stores
+constexpr long long kFillHist = 16LL << 20, kFillScatter = 28LL << 20;
 
 struct Lookup {
   const int64_t* tokens; const void* weight; void* out;
@@ -29,6 +34,8 @@ struct Lookup {
   unsigned* key[2]; unsigned* at[2]; unsigned* hist;
   int passes, sort_blocks;
   long long sort_chunk, runs, fills;
+  int run;                                // sorted positions of a block
+  long long fill_at, fill_rows;           // rows of dW that a launch of the sort clears, behind its own work
   float* part;                            // [runs][2][dim]
 };
 
@@ -54,14 +61,16 @@ struct Vec {
       }
     }
   }
+  // past the caches
   __device__ __forceinline__ void store(void* p, long long at) const {
     if constexpr (T == DT_F32) {
-      *reinterpret_cast<f4_t*>(static_cast<float*>(p) + at) = f32x4_t{f[0], f[1], f[2], f[3]};
+      const f32x4_t x = {f[0], f[1], f[2], f[3]};
+      __builtin_nontemporal_store(x, reinterpret_cast<f4_t*>(static_cast<float*>(p) + at));
     } else {
       constexpr int E = T == DT_F16 ? ELT_F16 : ELT_BF16;
-      *reinterpret_cast<v16_t*>(static_cast<uint16_t*>(p) + at) =
-          u32x4_t{pack2_elt<E>(f[0], f[1]), pack2_elt<E>(f[2], f[3]), pack2_elt<E>(f[4], f[5]),
-                  pack2_elt<E>(f[6], f[7])};
+      const u32x4_t x = {pack2_elt<E>(f[0], f[1]), pack2_elt<E>(f[2], f[3]), pack2_elt<E>(f[4], f[5]),
+                         pack2_elt<E>(f[6], f[7])};
+      __builtin_nontemporal_store(x, reinterpret_cast<v16_t*>(static_cast<uint16_t*>(p) + at));
     }
   }
   // rows of less than V values: the first n
@@ -129,6 +138,25 @@ __global__ __launch_bounds__(256) void embedding_kernel(const Lookup a, int chun
 
 // ---- the sort: least digit first, 9 bits a pass, every block a contiguous piece -----------------
 
+// The sort leaves most of the card idle: further blocks clear rows of dW meanwhile, as 16-byte chunks of
+// one range. What a token names among them is written again by the sums.
+__device__ __forceinline__ void clear_rows(const Lookup& a, int block) {
+  const long long size = a.dtype == DT_F32 ? 4 : 2;
+  char* base = static_cast<char*>(a.dw) + a.fill_at * a.dim * size;
+  const long long bytes = a.fill_rows * a.dim * size;
+  // up to the first whole chunk, and behind the last one, in 2-byte steps
+  const long long head = (16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15, lead = head < bytes ? head : bytes;
+  const long long chunks = (bytes - lead) / 16, from = (long long)block * kFillChunks;
+  if (block == 0) {
+    for (long long i = threadIdx.x; i < lead / 2; i += blockDim.x) reinterpret_cast<uint16_t*>(base)[i] = 0;
+    for (long long i = (lead + chunks * 16) / 2 + threadIdx.x; i < bytes / 2; i += blockDim.x)
+      reinterpret_cast<uint16_t*>(base)[i] = 0;
+  }
+  const long long to = from + kFillChunks < chunks ? from + kFillChunks : chunks;
+  for (long long i = from + threadIdx.x; i < to; i += blockDim.x)
+    __builtin_nontemporal_store(u32x4_t{}, reinterpret_cast<u32x4_t*>(base + lead) + i);
+}
+
 // Pass 0 takes the tokens; those without a gradient come behind all others, as class `vocab`.
 __device__ __forceinline__ unsigned key_of(const Lookup& a, int pass, long long i) {
   if (pass) return a.key[pass & 1][i];
@@ -138,6 +166,7 @@ __device__ __forceinline__ unsigned key_of(const Lookup& a, int pass, long long 
 
 __global__ __launch_bounds__(1024) void embedding_hist_kernel(const Lookup a, int pass) {
   __shared__ unsigned bins[kBins];
+  if ((int)blockIdx.x >= a.sort_blocks) return clear_rows(a, (int)blockIdx.x - a.sort_blocks);
   for (int i = threadIdx.x; i < kBins; i += 1024) bins[i] = 0;
   __syncthreads();
   const long long begin = blockIdx.x * a.sort_chunk;
@@ -152,14 +181,20 @@ __global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Lookup a,
   __shared__ unsigned place[kBins];       // where the next of each digit goes
   __shared__ unsigned of_wave[16][kBins];
   __shared__ unsigned scan[8];
+  if ((int)blockIdx.x >= a.sort_blocks) return clear_rows(a, (int)blockIdx.x - a.sort_blocks);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // places: digits before, then this digit in the blocks before
   unsigned before = 0, total = 0;
   if (tid < kBins) {
-    for (int b = 0; b < a.sort_blocks; ++b) {
-      const unsigned h = a.hist[b * kBins + tid];
-      before += b < (int)blockIdx.x ? h : 0u;
-      total += h;
+    for (int b0 = 0; b0 < a.sort_blocks; b0 += 16) {
+      unsigned h[16];                     // loaded side by side: one after the other they took 5 us of 8
+#pragma unroll
+      for (int k = 0; k < 16; ++k) h[k] = b0 + k < a.sort_blocks ? a.hist[(b0 + k) * kBins + tid] : 0u;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        before += b0 + k < (int)blockIdx.x ? h[k] : 0u;
+        total += h[k];
+      }
     }
   }
   unsigned sum = total;
@@ -223,7 +258,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const Lookup a, int 
   const int tid = threadIdx.x;
   if (blockIdx.x >= a.runs) {
     __shared__ unsigned present;
-    const long long v0 = (blockIdx.x - a.runs) * kFillRows;
+    const long long v0 = a.fill_at + (blockIdx.x - a.runs) * kFillRows;
     const int rows = a.vocab - v0 < kFillRows ? (int)(a.vocab - v0) : kFillRows;
     if (tid == 0) present = 0;
     __syncthreads();
@@ -250,45 +285,52 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const Lookup a, int 
     }
     return;
   }
-  const long long run = blockIdx.x, i0 = run * kRun;
-  const int n = a.n - i0 < kRun ? (int)(a.n - i0) : kRun;
+  const long long run = blockIdx.x, begin = run * a.run;
+  const int n = a.n - begin < a.run ? (int)(a.n - begin) : a.run;
   // keys[0] and keys[n + 1]: the neighbours', or none
   if (tid < n + 2) {
-    const long long i = i0 + tid - 1;
+    const long long i = begin + tid - 1;
     keys[tid] = i >= 0 && i < a.n ? key[i] : 0xffffffffu;
   }
-  if (tid < n) at[tid] = a.at[a.passes & 1][i0 + tid];
+  if (tid < n) at[tid] = a.at[a.passes & 1][begin + tid];
   __syncthreads();
   for (int c = blockIdx.y * 256 + tid; c < chunks; c += gridDim.y * 256) {
     const int col = chunk_at<T>(c, a.dim);
     Vec<T> sum;
     bool whole = keys[0] != keys[1];      // the class begins in this run
-    for (int i = 0; i < n; ++i) {
-      const unsigned k = keys[i + 1];
-      if (k >= (unsigned)a.vocab) break;  // behind all classes
-      Vec<T> x;
-      load_chunk<T>(x, a.dy, at[i] * a.ld_dy, col, a.dim);
-      if (i == 0 || keys[i] != k) sum = x;
-      else
+    // kAhead rows' loads side by side (one after the other, 32 rows took 23 us)
+    for (int i0 = 0; i0 < n && keys[i0 + 1] < (unsigned)a.vocab; i0 += kAhead) {
+      Vec<T> x[kAhead];
 #pragma unroll
-        for (int e = 0; e < Vec<T>::V; ++e) sum.f[e] += x.f[e];
-      const bool more = keys[i + 2] == k;
-      if (more && i + 1 < n) continue;
-      if (whole && !more) {
+      for (int k = 0; k < kAhead; ++k)
+        load_chunk<T>(x[k], a.dy, at[i0 + k < n ? i0 + k : n - 1] * a.ld_dy, col, a.dim);
 #pragma unroll
-        for (int e = 0; e < Vec<T>::V; ++e) sum.f[e] *= a.scale;
-        store_chunk<T>(sum, a.dw, (long long)k * a.dim, col, a.dim);
-      } else {
-        // part of a class that came from the run before, or that goes on in the next one
-        float* part = a.part + (run * 2 + (whole ? 1 : 0)) * a.dim;
-        if (a.dim < Vec<T>::V) {
-          for (int e = 0; e < a.dim; ++e) part[e] = sum.f[e];
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = i0 + k;
+        const unsigned v = i < n ? keys[i + 1] : 0xffffffffu;
+        if (v >= (unsigned)a.vocab) break;               // behind all classes
+        if (i == 0 || keys[i] != v) sum = x[k];
+        else
+#pragma unroll
+          for (int e = 0; e < Vec<T>::V; ++e) sum.f[e] += x[k].f[e];
+        const bool more = keys[i + 2] == v;
+        if (more && i + 1 < n) continue;
+        if (whole && !more) {
+#pragma unroll
+          for (int e = 0; e < Vec<T>::V; ++e) sum.f[e] *= a.scale;
+          store_chunk<T>(sum, a.dw, (long long)v * a.dim, col, a.dim);
         } else {
+          // part of a class that came from the run before, or that goes on in the next one
+          float* part = a.part + (run * 2 + (whole ? 1 : 0)) * a.dim;
+          if (a.dim < Vec<T>::V) {
+            for (int e = 0; e < a.dim; ++e) part[e] = sum.f[e];
+          } else {
 #pragma unroll
-          for (int e = 0; e < Vec<T>::V; ++e) part[col + e] = sum.f[e];
+            for (int e = 0; e < Vec<T>::V; ++e) part[col + e] = sum.f[e];
+          }
         }
+        whole = true;
       }
-      whole = true;
     }
   }
 }
@@ -298,17 +340,32 @@ template <int T>
 __global__ __launch_bounds__(256) void embedding_join_kernel(const Lookup a) {
   const unsigned* key = a.key[a.passes & 1];
   const long long run = blockIdx.x;
-  const long long last = run * kRun + kRun - 1;            // there is a run behind
+  const long long last = run * a.run + a.run - 1;            // there is a run behind
   const unsigned k = key[last];
   if (k >= (unsigned)a.vocab || key[last + 1] != k) return;
-  if (key[run * kRun] == k && run > 0 && key[run * kRun - 1] == k) return;   // began before
+  if (key[run * a.run] == k && run > 0 && key[run * a.run - 1] == k) return;   // began before
+  // the runs that the class goes on in: 64 at a time, a lane each
+  const int lane = threadIdx.x & 63;
+  long long stop = run + 1;
+  for (;;) {
+    const long long r = stop + lane, end = r * a.run + a.run;
+    const bool on = r < a.runs && end < a.n && key[end - 1] == k && key[end] == k;
+    const unsigned long long all = __ballot(on);
+    if (~all) {
+      stop += __ffsll(~all);              // the first one that it does not leave counts too
+      break;
+    }
+    stop += 64;
+  }
   const int c = blockIdx.y * 256 + threadIdx.x;
   if (c >= a.dim) return;
   float s = a.part[(run * 2 + 1) * a.dim + c];
-  for (long long r = run + 1; r < a.runs; ++r) {
-    s += a.part[r * 2 * a.dim + c];
-    const long long end = r * kRun + kRun;
-    if (end >= a.n || key[end - 1] != k || key[end] != k) break;
+  for (long long r0 = run + 1; r0 < stop; r0 += 8) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = r0 + i < stop ? a.part[(r0 + i) * 2 * a.dim + c] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += x[i];
   }
   s *= a.scale;
   const long long to = (long long)k * a.dim + c;
@@ -326,8 +383,9 @@ void launch_forward(const Lookup& a, hipStream_t stream) {
 template <int T>
 void launch_sums(const Lookup& a, hipStream_t stream) {
   const int chunks = (a.dim + Vec<T>::V - 1) / Vec<T>::V;
-  hipLaunchKernelGGL((embedding_sum_kernel<T>), dim3((unsigned)(a.runs + a.fills)), dim3(256), 0, stream, a,
-                     chunks);
+  if (a.runs + a.fills > 0)
+    hipLaunchKernelGGL((embedding_sum_kernel<T>), dim3((unsigned)(a.runs + a.fills)), dim3(256), 0, stream, a,
+                       chunks);
   if (a.runs > 1)
     hipLaunchKernelGGL((embedding_join_kernel<T>), dim3((unsigned)(a.runs - 1), (unsigned)((a.dim + 255) / 256)),
                        dim3(256), 0, stream, a);
@@ -359,7 +417,9 @@ int64_t plan(Lookup* l, const dmuon_embedding_args& a, char* ws) {
   if (blocks > kSortBlocks) blocks = kSortBlocks;
   l->sort_chunk = blocks ? ((l->n + blocks - 1) / blocks + kSortTile - 1) / kSortTile * kSortTile : kSortTile;
   l->sort_blocks = (int)((l->n + l->sort_chunk - 1) / l->sort_chunk);
-  l->runs = (l->n + kRun - 1) / kRun;
+  // a few tokens: short runs, whose rows are all loaded at once (1023 tokens of 300: 22 us in runs of 32)
+  l->run = l->n <= 8192 ? kAhead : kRun;
+  l->runs = (l->n + l->run - 1) / l->run;
   l->fills = (l->vocab + kFillRows - 1) / kFillRows;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -430,11 +490,22 @@ int dmuon_embedding_grad(const dmuon_embedding_args* args, void* workspace, int6
   l.ld_dy = a.ld_dy;
   l.dw = a.d_weight;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t row = l.dim * (a.dtype == DMUON_DTYPE_F32 ? 4LL : 2LL);
+  // rows that the next launch clears; its blocks
+  auto share = [&](int64_t bytes) {
+    l.fill_rows = bytes / row < l.vocab - l.fill_at ? bytes / row : l.vocab - l.fill_at;
+    return (unsigned)(l.sort_blocks + ((l.fill_rows * row + 15) / 16 + kFillChunks - 1) / kFillChunks);
+  };
   if (l.n > 0)
     for (int p = 0; p < l.passes; ++p) {
-      hipLaunchKernelGGL(embedding_hist_kernel, dim3((unsigned)l.sort_blocks), dim3(1024), 0, s, l, p);
-      hipLaunchKernelGGL(embedding_scatter_kernel, dim3((unsigned)l.sort_blocks), dim3(1024), 0, s, l, p);
+      unsigned blocks = share(kFillHist);
+      hipLaunchKernelGGL(embedding_hist_kernel, dim3(blocks), dim3(1024), 0, s, l, p);
+      l.fill_at += l.fill_rows;
+      blocks = share(kFillScatter);
+      hipLaunchKernelGGL(embedding_scatter_kernel, dim3(blocks), dim3(1024), 0, s, l, p);
+      l.fill_at += l.fill_rows;
     }
+  l.fills = (l.vocab - l.fill_at + kFillRows - 1) / kFillRows;
   if (a.dtype == DMUON_DTYPE_F32) launch_sums<DT_F32>(l, s);
   else if (a.dtype == DMUON_DTYPE_F16) launch_sums<DT_F16>(l, s);
   else launch_sums<DT_BF16>(l, s);
