@@ -23,7 +23,7 @@ struct Attention {
   const uint16_t* q; const uint16_t* k; const uint16_t* v; const uint16_t* dout;
   uint16_t* out; uint16_t* dq; uint16_t* dk; uint16_t* dv;   // dense [tokens][heads][dim]
   float* lse;                             // [tokens][heads], log2 of the row's sum; +inf: sees nothing
-  float* delta;                           // [tokens][heads], sum of dout out
+  float* delta;                           // [tokens][heads], minus the sum of dout out
   // strides in elements
   long long q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head;
   long long do_batch, do_token, do_head;
@@ -40,7 +40,11 @@ struct Attention {
   int splits;                             // parts of the key axis, joined by a second kernel
   int few;                                // tiles of kFewRows rows, each wave alone
   float* part; float2* part_stats;        // [splits][tokens][heads][dim] sums, [..][2] (reference, sum)
-  const unsigned* peaks;                  // fp16 gradients: largest |dout row|^2 and |v row|^2
+  // gradients: tiles of keys of one (sequence, key head) (packed: of one key head), parts of their rows and
+  // [key_splits][key tokens][kv_heads][2][dim] dk and dv of each; fp16: the blocks' largest |dout row|^2 and
+  // |v row|^2
+  int key_tiles, key_splits;
+  float* peaks;
 };
 
 // Where a block works: its sequence's tokens, pointers' offsets and the tile's number
@@ -54,14 +58,14 @@ struct Place {
 // Blocks of one (sequence, key head) follow each other, on one XCD as far as there are several of them:
 // its L2 then serves the keys and values. BACK: the tiles of late queries come first, which see most.
 template <bool KEYS>
-__device__ __forceinline__ Place place_of(const Attention& a, bool back) {
+__device__ __forceinline__ Place place_of(const Attention& a, int id, int blocks, bool back) {
   Place p;
-  const int splits = KEYS ? 1 : a.splits;
-  int id = xcd_remap_contig(blockIdx.x, gridDim.x);
+  const int splits = KEYS ? a.key_splits : a.splits, tiles = KEYS ? a.key_tiles : a.tiles;
+  id = xcd_remap_contig(id, blocks);
   p.split = id % splits;
   id /= splits;
-  int t = id % a.tiles;
-  const int unit = id / a.tiles;
+  int t = id % tiles;
+  const int unit = id / tiles;
   p.kvh = unit % a.kv_heads;
   const int b = unit / a.kv_heads;
   if (a.seqs) {
@@ -82,7 +86,7 @@ __device__ __forceinline__ Place place_of(const Attention& a, bool back) {
     p.do_off = s.q0 * a.do_token;
   } else {
     p.live = true;
-    p.tile = back ? a.tiles - 1 - t : t;
+    p.tile = back ? tiles - 1 - t : t;
     p.qn = a.q_len;
     p.kn = a.kv_len;
     if (a.kv_lengths) {
@@ -226,6 +230,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 // rows and keys of a block's tile; rows of one wave that works alone
 constexpr int kQueryRows = 128, kKeyRows = 128, kFewRows = 32;
+constexpr int kPeaks = 512;                // floats in `peaks`
 // the tables of a packed call; tiles of `rows` rows
 hipError_t launch_attention_tables(const Attention& a, const int64_t* q_starts, const int64_t* kv_starts,
                                    int q_rows, int k_rows, Sequence* seqs, int2* q_tiles, int2* k_tiles,

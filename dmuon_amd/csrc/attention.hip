@@ -139,6 +139,15 @@ int splits_of(const Attention& a, bool packed) {
   return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
+// Few keys' tiles: their rows are split, to a tile of 64 at the least
+int key_splits_of(const Attention& a, bool packed) {
+  const int64_t blocks = (int64_t)a.kv_heads * (packed ? 1 : a.batch) * a.key_tiles;
+  const int64_t rows = (int64_t)a.q_len * a.group / (packed && a.batch ? a.batch : 1);
+  if (blocks < 1 || blocks >= 512) return 1;
+  const int64_t s = 512 / blocks, most = rows / 64;
+  return most < 2 || s < 2 ? 1 : (int)(s < most ? (s < 16 ? s : 16) : (most < 16 ? most : 16));
+}
+
 struct Plan {
   Attention a;
   Tables t;
@@ -164,8 +173,12 @@ Plan plan_grad(const dmuon_attention_args& a, void* ws) {
   Carver c{static_cast<char*>(ws)};
   const bool packed = a.q_starts != nullptr;
   p.t = tables(&p.a, a, &c);
-  p.a.delta = c.take<float>(a.q_len * a.heads * (packed ? 1 : a.batch));
-  p.a.peaks = c.take<unsigned>(2);
+  const int64_t batch = packed ? 1 : a.batch;
+  p.a.delta = c.take<float>(a.q_len * a.heads * batch);
+  p.a.peaks = c.take<float>(kPeaks);
+  p.a.key_tiles = (int)tiles_of(p.a, packed, p.a.kv_len, kKeyRows);
+  p.a.key_splits = key_splits_of(p.a, packed);
+  if (p.a.key_splits > 1) p.a.part = c.take<float>(p.a.key_splits * a.kv_len * a.kv_heads * batch * 2 * a.dim);
   p.bytes = c.at;
   return p;
 }

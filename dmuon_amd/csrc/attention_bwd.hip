@@ -1,8 +1,9 @@
 // The gradients of attention over heads on gfx950. With S = c q k^T, P = exp2(S log2(e) - lse) formed
 // anew and delta = sum of do o over a row:
 //   dv = P^T do,  dP = do v^T,  dS = P (dP - delta),  dq = scale dS k,  dk = scale dS^T q
-// Two kernels, one over keys (dk, dv) and one over queries (dq), each with its sums in registers: seven
-// products where one pass would do with five, but no sums over blocks, so no atomics and one order.
+// Blocks over keys (dk, dv) and blocks over queries (dq), in one launch, each with its sums in registers:
+// seven products where one pass would do with five, but no sums over blocks, so no atomics and one order.
+// Where the keys' blocks are few their rows are split, and a second kernel joins the parts in their order.
 //
 // P and dS are rounded to the operands' type between the products. In fp16 they are held times powers of
 // two: P times 2^10 (a long row's probabilities are under the type's normal range) and dS by a further one
@@ -14,17 +15,26 @@ namespace dmuon {
 namespace {
 
 constexpr int kTile = 64;                 // rows or keys of a tile in LDS
-constexpr long long kPeakBlocks = 1024;
+// fp16: blocks that look for the largest rows of do, and as many for those of v
+constexpr int kPeakBlocks = kPeaks / 2;
 constexpr float kInf = __builtin_inff();
 
 template <int E>
 constexpr float kShift = E == ELT_F16 ? 10.f : 0.f;
 
-// The power of two of dS: |dS| 2^kShift <= 2 |do| |v| 2^10 P times it stays under 2^15.
+// The power of two of dS: |dS| 2^kShift <= 2 |do| |v| 2^10 P times it stays under 2^15. Every block finds
+// the two maxima among the parts itself.
 template <int E>
 __device__ __forceinline__ float ds_scale(const Attention& a) {
   if constexpr (E != ELT_F16) return 1.f;
-  const float most = 2.f * sqrtf(__uint_as_float(a.peaks[0])) * sqrtf(__uint_as_float(a.peaks[1]));
+  __shared__ float lds[2][4];
+  float x = a.peaks[threadIdx.x], y = a.peaks[kPeakBlocks + threadIdx.x];
+  for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o)), y = fmaxf(y, __shfl_xor(y, o));
+  if ((threadIdx.x & 63) == 0) lds[0][threadIdx.x >> 6] = x, lds[1][threadIdx.x >> 6] = y;
+  __syncthreads();
+  x = fmaxf(fmaxf(lds[0][0], lds[0][1]), fmaxf(lds[0][2], lds[0][3]));
+  y = fmaxf(fmaxf(lds[1][0], lds[1][1]), fmaxf(lds[1][2], lds[1][3]));
+  const float most = 2.f * sqrtf(x) * sqrtf(y);
   if (!(most > 0.f)) return 1.f;
   int e = 5 - __builtin_amdgcn_frexp_expf(most);           // most < 2^frexp
   e = e > 60 ? 60 : e < -60 ? -60 : e;
@@ -45,7 +55,9 @@ __device__ __forceinline__ void store_turned(uint16_t* out, const f32x16_t* v, f
     }
 }
 
-// Moves 64 rows of queries (row r is query r / group of head r % group) into LDS, 4 waves together.
+// Moves a tile's rows of queries (row r is query r / group of head r % group) into LDS, 4 waves together. A
+// tile holds the rows of whole queries, up to 64 of them (more heads a key head: any 64 rows), and zeros.
+__device__ __forceinline__ int tile_rows(int group) { return group <= kTile ? kTile / group * group : kTile; }
 template <int D>
 struct RowMover {
   static constexpr int CPR = D / 8, RPI = 64 / CPR, N = kTile / RPI / 4;
@@ -55,49 +67,75 @@ struct RowMover {
     row = wave * N * RPI + lane / CPR;    // of instruction 0
     chunk = lane % CPR;
   }
-  // rows r0 .. r0 + 63 of p (the key head's first head), of which those under `end` are there
-  __device__ __forceinline__ void issue(const uint16_t* p, long long token, long long head, int group,
-                                        unsigned magic, int dim, int r0, int end, char* lds) const {
+  // offset of instruction i's row from the first one's, `rem` rows into a query
+  __device__ __forceinline__ unsigned offset(int i, int rem, long long token, long long head, int group,
+                                             int dim) const {
+    const int r = row + i * RPI, q = (rem + r) / group;
+    const int c = chunk ^ slot_mask<D>(r);
+    return c * 8 < dim ? (unsigned)(q * (int)token + (rem + r - q * group) * (int)head) * 2u + (unsigned)c * 16u
+                       : kNowhere;
+  }
+  // the rows behind p, of which `left` are there, by the offsets that `at` gives
+  template <class F>
+  __device__ __forceinline__ void issue(const uint16_t* p, int left, char* lds, F at) const {
     typedef __attribute__((address_space(3))) void* lds_ptr_t;
-    const int q0 = r0 / group, rem = r0 - q0 * group;
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint16_t*>(p + q0 * token), (short)0, 0x7fffffff, 0x00020000);
+        const_cast<uint16_t*>(p), (short)0, 0x7fffffff, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = row + i * RPI, x = rem + r;
-      const int q = (int)(group == 1 ? (unsigned)x : __umulhi((unsigned)x, magic));
-      const int c = chunk ^ slot_mask<D>(r);
-      unsigned off = (unsigned)(q * (int)token + (x - q * group) * (int)head) * 2u + (unsigned)c * 16u;
-      if (r0 + r >= end || c * 8 >= dim) off = kNowhere;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (wave * N + i) * 1024), 16, off, 0,
-                                               0, 0);
-    }
+    for (int i = 0; i < N; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (wave * N + i) * 1024), 16,
+                                               row + i * RPI < left ? at(i) : kNowhere, 0, 0, 0);
   }
 };
 
-// A block's largest value to *peak: a maximum, which no order shows in. One atomic a block: of many waves
-// at one address they took 375 us where the reads take 20.
-__device__ __forceinline__ void block_peak(float most, unsigned* peak) {
-  __shared__ float lds[4];
+// A block's largest value
+__device__ __forceinline__ void block_peak(float most, float* peak) {
+  __shared__ float lds[16];
   for (int o = 16; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = most;
   __syncthreads();
   if (threadIdx.x) return;
-  most = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
-  if (most > 0.f) atomicMax(peak, __float_as_uint(most));
+  for (int w = 1; w < (int)blockDim.x >> 6; ++w) most = fmaxf(most, lds[w]);
+  *peak = most;
 }
 
-// delta of every row, and in fp16 the largest row of do. 16 lanes a row, 8 values each.
+// What the products need besides: -delta of every row, and in fp16 the largest rows of do and v (blocks of
+// 1024 threads, kPeakBlocks for each; bf16: of 256 threads, 16 rows a block). 16 lanes a row, 8 values each.
 template <int E>
-__global__ __launch_bounds__(256) void attention_delta_kernel(const Attention a, unsigned* peaks) {
-  const long long rows = (long long)a.q_len * a.heads * (a.seqs ? 1 : a.batch);
-  const int at = 8 * (threadIdx.x & 15);
+__global__ __launch_bounds__(E == ELT_F16 ? 1024 : 256) void attention_delta_kernel(const Attention a) {
+  const int batch = a.seqs ? 1 : a.batch, at = 8 * (threadIdx.x & 15), group = threadIdx.x >> 4;
+  const int groups = blockDim.x >> 4;
   float most = 0.f;
-  for (long long first = (long long)blockIdx.x * 16; first < rows; first += (long long)gridDim.x * 16) {
-    const long long row = first + (threadIdx.x >> 4);
-    const bool live = row < rows;
+  if (E == ELT_F16 && blockIdx.x >= kPeakBlocks) {
+    // rows of v among those that a query may see
+    const long long rows = (long long)a.kv_len * a.kv_heads * batch;
+    for (long long row = (long long)(blockIdx.x - kPeakBlocks) * groups + group; row < rows;
+         row += (long long)kPeakBlocks * groups) {
+      const long long token = row / a.kv_heads, b = token / a.kv_len, j = token - b * a.kv_len;
+      const int head = (int)(row - token * a.kv_heads);
+      bool live = true;
+      if (a.kv_lengths) live = j < a.kv_lengths[b];
+      if (a.seqs) live = j >= a.seqs[a.batch + 2].kn && j < a.seqs[a.batch + 3].k0;
+      float n = 0.f;
+      if (live && at < a.dim) {
+        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(
+            a.v + b * a.v_batch + j * a.v_token + head * a.v_head + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float f = from_elt<ELT_F16>((uint16_t)(i & 1 ? x[i / 2] >> 16 : x[i / 2]));
+          n += f * f;
+        }
+      }
+      for (int o = 1; o < 16; o <<= 1) n += __shfl_xor(n, o);
+      if (n < kInf) most = fmaxf(most, n);
+    }
+    return block_peak(most, a.peaks + blockIdx.x);
+  }
+  const long long rows = (long long)a.q_len * a.heads * batch;
+  const long long step = E == ELT_F16 ? (long long)kPeakBlocks * groups : rows;
+  for (long long row = (long long)blockIdx.x * groups + group; row < rows; row += step) {
     float s = 0.f, n = 0.f;
-    if (live && at < a.dim) {
+    if (at < a.dim) {
       const long long token = row / a.heads, b = a.seqs ? 0 : token / a.q_len;
       const int head = (int)(row - token * a.heads);
       const uint16_t* d = a.dout + b * a.do_batch + (token - b * a.q_len) * a.do_token + head * a.do_head + at;
@@ -113,57 +151,27 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const Attention a,
       }
     }
     for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
-    if (live && (threadIdx.x & 15) == 0) a.delta[row] = s;
+    if ((threadIdx.x & 15) == 0) a.delta[row] = -s;
     if constexpr (E == ELT_F16) {
       for (int o = 1; o < 16; o <<= 1) n += __shfl_xor(n, o);
       // rows that see nothing, or of no numbers, do not count
-      if (live && n < kInf && a.lse[row] < kInf) most = fmaxf(most, n);
+      if (n < kInf && a.lse[row] < kInf) most = fmaxf(most, n);
     }
   }
-  if constexpr (E == ELT_F16) block_peak(most, peaks);
-}
-
-// fp16: the largest row of v among those that a query may see
-__global__ __launch_bounds__(256) void attention_value_peak_kernel(const Attention a, unsigned* peak) {
-  const int batch = a.seqs ? 1 : a.batch;
-  const long long rows = (long long)a.kv_len * a.kv_heads * batch;
-  const int at = 8 * (threadIdx.x & 15);
-  float most = 0.f;
-  for (long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); row < rows;
-       row += (long long)gridDim.x * 16) {
-    const long long token = row / a.kv_heads, b = token / a.kv_len, j = token - b * a.kv_len;
-    const int head = (int)(row - token * a.kv_heads);
-    bool live = true;
-    if (a.kv_lengths) live = j < a.kv_lengths[b];
-    if (a.seqs) live = j >= a.seqs[a.batch + 2].kn && j < a.seqs[a.batch + 3].k0;
-    float n = 0.f;
-    if (live && at < a.dim) {
-      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(
-          a.v + b * a.v_batch + j * a.v_token + head * a.v_head + at);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f = from_elt<ELT_F16>((uint16_t)(i & 1 ? x[i / 2] >> 16 : x[i / 2]));
-        n += f * f;
-      }
-    }
-    for (int o = 1; o < 16; o <<= 1) n += __shfl_xor(n, o);
-    if (n < kInf) most = fmaxf(most, n);
-  }
-  block_peak(most, peak);
-}
-
-__global__ void attention_clear_kernel(unsigned* peaks) {
-  if (threadIdx.x < 2) peaks[threadIdx.x] = 0u;
+  if constexpr (E == ELT_F16) block_peak(most, a.peaks + blockIdx.x);
 }
 
 // dk and dv of 128 keys, 32 a wave and one a lane: S = Q K^T and dP = dO V^T leave a lane 16 rows of every
 // 32 for its key, which go as they are into dV^T = dO^T P and dK^T = Q^T dS.
+template <int D>
+struct KeysLds {
+  static constexpr int TILE = kTile * D * 2, SLOT = 2 * TILE + 2 * kTile * 4;
+  static constexpr int OFFSETS = 2 * SLOT, BYTES = OFFSETS + 256 * 32 + kTile * 4;
+};
 template <int E, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void attention_keys_kernel(const Attention a) {
-  constexpr int KS = D / 16, DB = D / 32, TILE = kTile * D * 2, SLOT = 2 * TILE + 2 * kTile * 4;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * SLOT];
-  const Place p = place_of<true>(a, false);
+__device__ __forceinline__ void keys_block(const Attention& a, int id, int blocks, char* lds) {
+  constexpr int KS = D / 16, DB = D / 32, TILE = KeysLds<D>::TILE, SLOT = KeysLds<D>::SLOT;
+  const Place p = place_of<true>(a, id, blocks, false);
   if (!p.live) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int j0 = p.tile * kKeyRows, j = j0 + wave * 32 + (lane & 31);
@@ -201,30 +209,61 @@ void attention_keys_kernel(const Attention a) {
   // rows that see every key of the block need no mask
   const int full_lo = last_lo * a.group;
   const int full_hi = last_key == j0 + kKeyRows - 1 ? first_hi * a.group : 0;
-  const int n = r_hi > r_lo && j0 < p.kn ? (r_hi - r_lo + kTile - 1) / kTile : 0;
+  // tiles of whole queries; a part of them where the rows are split
+  const int tr = tile_rows(a.group);
+  int n = r_hi > r_lo && j0 < p.kn ? (r_hi - r_lo + tr - 1) / tr : 0, end = n;
+  if (a.key_splits > 1) {
+    const int each = (n + a.key_splits - 1) / a.key_splits;
+    end = n - p.split * each;
+    n = end < 0 ? 0 : end < each ? end : each;
+  }
   // from the last rows back: under a causal mask all blocks of a key head begin with the same rows then,
   // and find them in their XCD's L2
+  auto first_row = [&](int t) { return r_lo + (end - 1 - t) * tr; };
 
   RowMover<D> mover;
   mover.init(wave, lane);
-  const unsigned magic = (unsigned)(0x100000000ULL / (unsigned)a.group + 1);
+  // a lane's offsets of q and dout and of a row's statistics, kept in LDS: the sums need the registers
+  unsigned* offsets = reinterpret_cast<unsigned*>(lds + KeysLds<D>::OFFSETS) + threadIdx.x * 8;
+  unsigned* stat_at = reinterpret_cast<unsigned*>(lds + KeysLds<D>::OFFSETS + 256 * 32) + lane;
+  if (a.group <= kTile) {
+#pragma unroll
+    for (int i = 0; i < RowMover<D>::N; ++i) {
+      offsets[i] = mover.offset(i, 0, a.q_token, a.q_head, a.group, a.dim);
+      offsets[4 + i] = mover.offset(i, 0, a.do_token, a.do_head, a.group, a.dim);
+    }
+    const int q = lane / a.group;
+    if (wave == 0) *stat_at = (unsigned)(q * a.heads + lane - q * a.group) * 4u;
+  }
+  __syncthreads();
   const long long row0 = p.q_row * a.heads + (long long)p.kvh * a.group;
   auto fetch = [&](int t, char* to) __attribute__((always_inline)) {
     typedef __attribute__((address_space(3))) void* lds_ptr_t;
-    const int r0 = r_lo + (n - 1 - t) * kTile;
-    mover.issue(a.q + p.q_off, a.q_token, a.q_head, a.group, magic, a.dim, r0, rows, to);
-    mover.issue(a.dout + p.do_off, a.do_token, a.do_head, a.group, magic, a.dim, r0, rows, to + TILE);
+    const int r0 = first_row(t), q0 = r0 / a.group;
+    const int left = rows - r0 < tr ? rows - r0 : tr;
+    const uint16_t *q = a.q + p.q_off + q0 * a.q_token, *d = a.dout + p.do_off + q0 * a.do_token;
+    const float* stats = (wave == 0 ? a.lse : a.delta) + row0 + (long long)q0 * a.heads;
+    unsigned stat_off;
+    if (a.group <= kTile) {
+      const u32x4_t qo = *reinterpret_cast<const u32x4_t*>(offsets);
+      const u32x4_t dof = *reinterpret_cast<const u32x4_t*>(offsets + 4);
+      stat_off = *stat_at;
+      mover.issue(q, left, to, [&](int i) { return qo[i]; });
+      mover.issue(d, left, to + TILE, [&](int i) { return dof[i]; });
+    } else {
+      const int rem = r0 - q0 * a.group;
+      mover.issue(q, left, to, [&](int i) { return mover.offset(i, rem, a.q_token, a.q_head, a.group, a.dim); });
+      mover.issue(d, left, to + TILE,
+                  [&](int i) { return mover.offset(i, rem, a.do_token, a.do_head, a.group, a.dim); });
+      const int over = (rem + lane) / a.group;
+      stat_off = (unsigned)(over * a.heads + rem + lane - over * a.group) * 4u;
+    }
     if (wave < 2) {
-      // lse (wave 0) and delta (wave 1) of the rows
-      const int q0 = r0 / a.group, x = r0 - q0 * a.group + lane;
-      const int q = (int)(a.group == 1 ? (unsigned)x : __umulhi((unsigned)x, magic));
-      const float* src = (wave == 0 ? a.lse : a.delta) + row0 + (long long)q0 * a.heads;
+      // lse (wave 0) and -delta (wave 1) of the rows
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<float*>(src), (short)0, 0x7fffffff, 0x00020000);
-      unsigned off = (unsigned)(q * a.heads + (x - q * a.group)) * 4u;
-      if (r0 + lane >= rows) off = kNowhere;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(to + 2 * TILE + wave * kTile * 4), 4, off, 0,
-                                               0, 0);
+          const_cast<float*>(stats), (short)0, 0x7fffffff, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(to + 2 * TILE + wave * kTile * 4), 4,
+                                               lane < left ? stat_off : kNowhere, 0, 0, 0);
     }
   };
   const int row_at = row_form<D>(lane), turn_at = turned_form<D>(lane);
@@ -237,7 +276,7 @@ void attention_keys_kernel(const Attention a) {
     const char* dt = qt + TILE;
     const float* stats = reinterpret_cast<const float*>(qt + 2 * TILE);
     if (t + 1 < n) fetch(t + 1, next);
-    const int r0 = r_lo + (n - 1 - t) * kTile;
+    const int r0 = first_row(t);
     const bool masked = r0 < full_lo || r0 + kTile > full_hi;
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
@@ -245,7 +284,7 @@ void attention_keys_kernel(const Attention a) {
       // that the sums need
       int ra = row_at, ta = turn_at;
       asm volatile("" : "+v"(ra), "+v"(ta));
-      f32x16_t s = {}, dp = {};
+      f32x16_t s = {}, dp;
 #pragma unroll
       for (int k = 0; k < KS; ++k)
         s = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(qt + y * 64 * D + (ra ^ (32 * k))), kf[k], s);
@@ -271,15 +310,18 @@ void attention_keys_kernel(const Attention a) {
           dv[b] = mfma_32x32x16<E>(read_turned<D>(dt + (2 * y + u) * 32 * D, ta ^ (64 * b)), pf, dv[b]);
       }
       asm volatile("" : "+v"(ra), "+v"(ta));
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-        dp = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(dt + y * 64 * D + (ra ^ (32 * k))), vf[k], dp);
+      // dP - delta: the product begins at -delta. Rows that are not there are zeros throughout.
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(stats + kTile + 32 * y + result_row(i, h));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dp[i + e] = s[i + e] * ((dp[i + e] - delta[e]) * sigma);
+        for (int e = 0; e < 4; ++e) dp[i + e] = delta[e];
       }
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        dp = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(dt + y * 64 * D + (ra ^ (32 * k))), vf[k], dp);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dp[i] = s[i] * (E == ELT_F16 ? dp[i] * sigma : dp[i]);
       if (masked) {
         // rows that do not see the key have no share, whatever their dout holds
 #pragma unroll
@@ -305,21 +347,59 @@ void attention_keys_kernel(const Attention a) {
   }
   // keys past a sequence's own, up to the tensor's, have no gradient
   const int most = a.seqs ? p.kn : a.kv_len;
-  if (j < most) {
-    const long long at = ((p.k_row + j) * a.kv_heads + p.kvh) * a.dim;
-    constexpr float down = E == ELT_F16 ? 1.f / 1024.f : 1.f;
-    if (a.dk) store_turned<E, DB>(a.dk + at, dk, a.scale * down / sigma, h, a.dim);
-    if (a.dv) store_turned<E, DB>(a.dv + at, dv, down, h, a.dim);
+  if (j >= most) return;
+  const long long key = (p.k_row + j) * a.kv_heads + p.kvh;
+  constexpr float down = E == ELT_F16 ? 1.f / 1024.f : 1.f;
+  const float fk = a.scale * down / sigma;
+  if (a.key_splits > 1) {
+    const long long keys = (long long)a.kv_len * a.kv_heads * (a.seqs ? 1 : a.batch);
+    float* part = a.part + (p.split * keys + key) * 2 * a.dim;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int d = 32 * b + result_row(i, h);
+        if (d >= a.dim) continue;
+        *reinterpret_cast<f32x4_t*>(part + d) =
+            f32x4_t{dk[b][i] * fk, dk[b][i + 1] * fk, dk[b][i + 2] * fk, dk[b][i + 3] * fk};
+        *reinterpret_cast<f32x4_t*>(part + a.dim + d) =
+            f32x4_t{dv[b][i] * down, dv[b][i + 1] * down, dv[b][i + 2] * down, dv[b][i + 3] * down};
+      }
+    return;
+  }
+  if (a.dk) store_turned<E, DB>(a.dk + key * a.dim, dk, fk, h, a.dim);
+  if (a.dv) store_turned<E, DB>(a.dv + key * a.dim, dv, down, h, a.dim);
+}
+
+// Joins the parts of the keys' gradients in their order: 16 lanes a key, 8 values of dk and dv each.
+template <int E>
+__global__ __launch_bounds__(256) void attention_keys_join_kernel(const Attention a) {
+  const long long keys = (long long)a.kv_len * a.kv_heads * (a.seqs ? 1 : a.batch);
+  const long long key = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int at = 8 * (threadIdx.x & 15);
+  if (key >= keys || at >= a.dim) return;
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    uint16_t* out = z ? a.dv : a.dk;
+    if (!out) continue;
+    f32x4_t lo = {}, hi = {};
+#pragma unroll 4
+    for (int s = 0; s < a.key_splits; ++s) {
+      const float* part = a.part + ((s * keys + key) * 2 + z) * a.dim + at;
+      lo += *reinterpret_cast<const f32x4_t*>(part);
+      hi += *reinterpret_cast<const f32x4_t*>(part + 4);
+    }
+    *reinterpret_cast<u32x4_t*>(out + key * a.dim + at) =
+        u32x4_t{pack2_elt<E>(lo[0], lo[1]), pack2_elt<E>(lo[2], lo[3]), pack2_elt<E>(hi[0], hi[1]),
+                pack2_elt<E>(hi[2], hi[3])};
   }
 }
 
 // dq of 128 rows, 32 a wave and one a lane: S^T = K Q^T and dP^T = V dO^T, dQ^T = K^T dS^T.
 template <int E, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void attention_queries_kernel(const Attention a) {
+__device__ __forceinline__ void queries_block(const Attention& a, int id, int blocks, char* lds) {
   constexpr int KS = D / 16, DB = D / 32, TILE = kTile * D * 2;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
-  const Place p = place_of<false>(a, a.causal);
+  const Place p = place_of<false>(a, id, blocks, a.causal);
   if (!p.live) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int r0 = p.tile * kQueryRows, rows = p.qn * a.group;
@@ -337,7 +417,7 @@ void attention_queries_kernel(const Attention a) {
       df[s] = *reinterpret_cast<const bf16x8_t*>(a.dout + p.do_off + query * a.do_token + head * a.do_head + at);
     }
   }
-  const float lse = live ? a.lse[row] : kInf, delta = live ? a.delta[row] : 0.f;
+  const float lse = live ? a.lse[row] : kInf, minus_delta = live ? a.delta[row] : 0.f;
   const Sight see = live ? sight_of(a, p, query) : Sight{0, 0};
   const int last_row = r0 + kQueryRows < rows ? r0 + kQueryRows - 1 : rows - 1;
   const Sight first = sight_of(a, p, r0 / a.group), last = sight_of(a, p, last_row / a.group);
@@ -374,7 +454,7 @@ void attention_queries_kernel(const Attention a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         dp[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kShift<E> - lse)) *
-                ((dp[i] - delta) * sigma);
+                (E == ELT_F16 ? (dp[i] + minus_delta) * sigma : dp[i] + minus_delta);
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -402,20 +482,23 @@ void attention_queries_kernel(const Attention a) {
   if (live) store_turned<E, DB>(a.dq + row * a.dim, dq, a.scale * down / sigma, h, a.dim);
 }
 
+// The keys' blocks come first: they take longer.
 template <int E, int D>
-void launch_main(Attention a, unsigned* peaks, hipStream_t stream) {
-  const long long units = (long long)a.kv_heads * (a.seqs ? 1 : a.batch);
-  (void)peaks;
-  if (a.dk || a.dv) {
-    Attention k = a;
-    k.tiles = a.seqs ? a.kv_len / kKeyRows + a.batch + 4 : (a.kv_len + kKeyRows - 1) / kKeyRows;
-    if (units * k.tiles > 0)
-      hipLaunchKernelGGL((attention_keys_kernel<E, D>), dim3((unsigned)(units * k.tiles)), dim3(256), 0,
-                         stream, k);
-  }
-  if (a.dq && units * a.tiles > 0)
-    hipLaunchKernelGGL((attention_queries_kernel<E, D>), dim3((unsigned)(units * a.tiles)), dim3(256), 0,
-                       stream, a);
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void attention_grad_kernel(const Attention a, int key_blocks, int query_blocks) {
+  __shared__ __attribute__((aligned(1024))) char lds[KeysLds<D>::BYTES];
+  // a multiple of 8 blocks keeps each XCD's blocks on it
+  const int from = (key_blocks + 7) / 8 * 8, id = blockIdx.x;
+  if (id < key_blocks) keys_block<E, D>(a, id, key_blocks, lds);
+  else if (id >= from) queries_block<E, D>(a, id - from, query_blocks, lds);
+}
+
+template <int E, int D>
+void launch_main(const Attention& a, long long key_blocks, long long query_blocks, hipStream_t stream) {
+  const long long blocks = (key_blocks + 7) / 8 * 8 + query_blocks;
+  if (blocks > 0)
+    hipLaunchKernelGGL((attention_grad_kernel<E, D>), dim3((unsigned)blocks), dim3(256), 0, stream, a,
+                       (int)key_blocks, (int)query_blocks);
 }
 
 }  // namespace
@@ -424,31 +507,27 @@ hipError_t launch_attention_grad(const Attention& a, hipStream_t stream) {
   const long long batch = a.seqs ? 1 : a.batch;
   const long long rows = (long long)a.q_len * a.heads * batch, keys = (long long)a.kv_len * a.kv_heads * batch;
   const long long units = (long long)a.kv_heads * batch;
-  const long long most = units * ((long long)a.kv_len / kKeyRows + a.batch + 4);
-  if (rows / 16 > 0x7ffffff0LL || most > 0x7fffffffLL || units * a.tiles > 0x7fffffffLL)
+  const long long key_blocks = a.dk || a.dv ? units * a.key_tiles * a.key_splits : 0;
+  const long long query_blocks = a.dq ? units * a.tiles : 0;
+  if (rows / 16 > 0x7ffffff0LL || keys / 16 > 0x7ffffff0LL || key_blocks + query_blocks > 0x7ffffff0LL)
     return hipErrorInvalidValue;
-  unsigned* peaks = const_cast<unsigned*>(a.peaks);
-  const bool f16 = a.dtype == DT_F16;
+  const bool f16 = a.dtype == DT_F16, wide = a.dim > 64;
+  if (f16)
+    hipLaunchKernelGGL((attention_delta_kernel<ELT_F16>), dim3(2 * kPeakBlocks), dim3(1024), 0, stream, a);
+  else if (rows > 0)
+    hipLaunchKernelGGL((attention_delta_kernel<ELT_BF16>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0,
+                       stream, a);
   if (f16) {
-    hipLaunchKernelGGL(attention_clear_kernel, dim3(1), dim3(64), 0, stream, peaks);
-    const long long blocks = (keys + 15) / 16 < kPeakBlocks ? (keys + 15) / 16 : kPeakBlocks;
-    if (blocks > 0)
-      hipLaunchKernelGGL(attention_value_peak_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a,
-                         peaks + 1);
-  }
-  if (rows > 0) {
-    const long long blocks = (rows + 15) / 16;
-    const dim3 grid((unsigned)(f16 && blocks > kPeakBlocks ? kPeakBlocks : blocks));
-    if (f16) hipLaunchKernelGGL((attention_delta_kernel<ELT_F16>), grid, dim3(256), 0, stream, a, peaks);
-    else hipLaunchKernelGGL((attention_delta_kernel<ELT_BF16>), grid, dim3(256), 0, stream, a, peaks);
-  }
-  const bool wide = a.dim > 64;
-  if (f16) {
-    if (wide) launch_main<ELT_F16, 128>(a, peaks, stream);
-    else launch_main<ELT_F16, 64>(a, peaks, stream);
+    if (wide) launch_main<ELT_F16, 128>(a, key_blocks, query_blocks, stream);
+    else launch_main<ELT_F16, 64>(a, key_blocks, query_blocks, stream);
   } else {
-    if (wide) launch_main<ELT_BF16, 128>(a, peaks, stream);
-    else launch_main<ELT_BF16, 64>(a, peaks, stream);
+    if (wide) launch_main<ELT_BF16, 128>(a, key_blocks, query_blocks, stream);
+    else launch_main<ELT_BF16, 64>(a, key_blocks, query_blocks, stream);
+  }
+  if (key_blocks > 0 && a.key_splits > 1) {
+    const dim3 grid((unsigned)((keys + 15) / 16));
+    if (f16) hipLaunchKernelGGL((attention_keys_join_kernel<ELT_F16>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attention_keys_join_kernel<ELT_BF16>), grid, dim3(256), 0, stream, a);
   }
   return hipGetLastError();
 }

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2
 void attention_kernel(const Attention a) {
   constexpr int ROWS = 128 * RT, KS = D / 16, DB = D / 32, TILE = kKeys * D * 2;
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
-  const Place p = place_of<false>(a, a.causal);
+  const Place p = place_of<false>(a, blockIdx.x, gridDim.x, a.causal);
   if (!p.live) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int r0 = p.tile * ROWS, rows = p.qn * a.group;
@@ -195,7 +195,7 @@ template <int E, int D>
 __global__ __launch_bounds__(64) void attention_few_kernel(const Attention a) {
   constexpr int KS = D / 16, DB = D / 32, KEYS = 32, TILE = KEYS * D * 2, LOADS = TILE / 1024;
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
-  const Place p = place_of<false>(a, false);
+  const Place p = place_of<false>(a, blockIdx.x, gridDim.x, false);
   if (!p.live) return;
   const int lane = threadIdx.x, h = lane >> 5;
   const int r0 = p.tile * kFewRows, rows = p.qn * a.group;

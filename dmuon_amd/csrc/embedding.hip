@@ -17,7 +17,7 @@ namespace {
 constexpr int kRun = 32;                  // sorted positions of a block, at most
 constexpr int kAhead = 8;
 constexpr int kDigit = 9, kBins = 1 << kDigit;
-constexpr int kSortTile = 1024, kSortBlocks = 64;
+constexpr int kSortTile = 1024, kSortBlocks = 64, kSortAlone = 2048;
 constexpr int kFillRows = 32;             // rows of dW that a block of the sums clears
 constexpr long long kFillChunks = 4096;   // 16-byte chunks that a block of the sort clears
 // what the launches of one pass of the sort clear: as much as they take time (3 and 5 us) at the rate of
@@ -98,34 +98,35 @@ struct Vec {
 };
 
 // Chunk c of a row: the last one of a row that is no multiple of V begins earlier, over values that the
-// one before holds too, and gives them the same result.
-template <int T>
+// one before holds too, and gives them the same result. Rows of less than V values are SHORT: known to the
+// compiler, since a branch at each load would have one wait for the other.
+template <int T, bool SHORT>
 __device__ __forceinline__ int chunk_at(int c, int dim) {
   constexpr int V = Vec<T>::V;
-  return dim < V ? 0 : c * V + V <= dim ? c * V : dim - V;
+  return SHORT ? 0 : c * V + V <= dim ? c * V : dim - V;
 }
-template <int T>
+template <int T, bool SHORT>
 __device__ __forceinline__ void load_chunk(Vec<T>& v, const void* p, long long row, int at, int dim) {
-  if (dim < Vec<T>::V) v.load_n(p, row, dim);
+  if constexpr (SHORT) v.load_n(p, row, dim);
   else v.load(p, row + at);
 }
-template <int T>
+template <int T, bool SHORT>
 __device__ __forceinline__ void store_chunk(const Vec<T>& v, void* p, long long row, int at, int dim) {
-  if (dim < Vec<T>::V) v.store_n(p, row, dim);
+  if constexpr (SHORT) v.store_n(p, row, dim);
   else v.store(p, row + at);
 }
 
 // One chunk a thread, `lanes` threads a row
-template <int T>
+template <int T, bool SHORT>
 __global__ __launch_bounds__(256) void embedding_kernel(const Lookup a, int chunks) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
   const long long t = id / chunks;
   if (t >= a.n) return;
-  const int at = chunk_at<T>((int)(id - t * chunks), a.dim);
+  const int at = chunk_at<T, SHORT>((int)(id - t * chunks), a.dim);
   const long long v = a.tokens[t];
   Vec<T> x;
   if (v >= 0 && v < a.vocab) {
-    load_chunk<T>(x, a.weight, v * a.ld, at, a.dim);
+    load_chunk<T, SHORT>(x, a.weight, v * a.ld, at, a.dim);
 #pragma unroll
     for (int i = 0; i < Vec<T>::V; ++i) x.f[i] *= a.scale;
   } else {
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(256) void embedding_kernel(const Lookup a, int chun
 #pragma unroll
     for (int i = 0; i < Vec<T>::V; ++i) x.f[i] = __builtin_nanf("");
   }
-  store_chunk<T>(x, a.out, t * a.dim, at, a.dim);
+  store_chunk<T, SHORT>(x, a.out, t * a.dim, at, a.dim);
 }
 
 // ---- the sort: least digit first, 9 bits a pass, every block a contiguous piece -----------------
@@ -177,15 +178,23 @@ __global__ __launch_bounds__(1024) void embedding_hist_kernel(const Lookup a, in
   for (int i = threadIdx.x; i < kBins; i += 1024) a.hist[blockIdx.x * kBins + i] = bins[i];
 }
 
-__global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Lookup a, int pass) {
+__device__ __forceinline__ void scatter(const Lookup& a, int pass, bool alone) {
   __shared__ unsigned place[kBins];       // where the next of each digit goes
   __shared__ unsigned of_wave[16][kBins];
   __shared__ unsigned scan[8];
-  if ((int)blockIdx.x >= a.sort_blocks) return clear_rows(a, (int)blockIdx.x - a.sort_blocks);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // places: digits before, then this digit in the blocks before
   unsigned before = 0, total = 0;
-  if (tid < kBins) {
+  if (alone) {
+    // the only block counts its digits itself
+    if (tid < kBins) place[tid] = 0;
+    __syncthreads();
+    for (long long i = tid; i < a.n; i += 1024)
+      atomicAdd(&place[key_of(a, pass, i) >> (pass * kDigit) & (kBins - 1)], 1u);
+    __syncthreads();
+    if (tid < kBins) total = place[tid];
+    __syncthreads();
+  } else if (tid < kBins) {
     for (int b0 = 0; b0 < a.sort_blocks; b0 += 16) {
       unsigned h[16];                     // loaded side by side: one after the other they took 5 us of 8
 #pragma unroll
@@ -231,6 +240,7 @@ __global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Lookup a,
     __syncthreads();
     if (tid < kBins) {
       unsigned p = place[tid];
+#pragma unroll
       for (int w = 0; w < 16; ++w) {
         const unsigned c = of_wave[w][tid];
         of_wave[w][tid] = p;
@@ -247,11 +257,26 @@ __global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Lookup a,
   }
 }
 
+__global__ __launch_bounds__(1024) void embedding_scatter_kernel(const Lookup a, int pass) {
+  if ((int)blockIdx.x >= a.sort_blocks) return clear_rows(a, (int)blockIdx.x - a.sort_blocks);
+  scatter(a, pass, false);
+}
+
+// All passes of a few tokens in one block (1023 tokens: 7 us for the four launches' 15)
+__global__ __launch_bounds__(1024) void embedding_sort_kernel(const Lookup a) {
+  if (blockIdx.x) return clear_rows(a, (int)blockIdx.x - 1);
+  for (int pass = 0; pass < a.passes; ++pass) {
+    scatter(a, pass, true);
+    __threadfence_block();
+    __syncthreads();
+  }
+}
+
 // ---- sums over the sorted positions -------------------------------------------------------------
 
 // A block: one run of sorted positions for 256 chunks of columns, or, behind the runs, the rows of dW
 // that no token names.
-template <int T>
+template <int T, bool SHORT>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(const Lookup a, int chunks) {
   __shared__ unsigned keys[kRun + 2], at[kRun];
   const unsigned* key = a.key[a.passes & 1];
@@ -281,7 +306,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const Lookup a, int 
     for (int r = 0; r < rows; ++r) {
       if (held >> r & 1u) continue;
       for (int c = tid; c < chunks; c += 256)
-        store_chunk<T>(zero, a.dw, (v0 + r) * a.dim, chunk_at<T>(c, a.dim), a.dim);
+        store_chunk<T, SHORT>(zero, a.dw, (v0 + r) * a.dim, chunk_at<T, SHORT>(c, a.dim), a.dim);
     }
     return;
   }
@@ -295,7 +320,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const Lookup a, int 
   if (tid < n) at[tid] = a.at[a.passes & 1][begin + tid];
   __syncthreads();
   for (int c = blockIdx.y * 256 + tid; c < chunks; c += gridDim.y * 256) {
-    const int col = chunk_at<T>(c, a.dim);
+    const int col = chunk_at<T, SHORT>(c, a.dim);
     Vec<T> sum;
     bool whole = keys[0] != keys[1];      // the class begins in this run
     // kAhead rows' loads side by side (one after the other, 32 rows took 23 us)
@@ -303,7 +328,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const Lookup a, int 
       Vec<T> x[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
-        load_chunk<T>(x[k], a.dy, at[i0 + k < n ? i0 + k : n - 1] * a.ld_dy, col, a.dim);
+        load_chunk<T, SHORT>(x[k], a.dy, at[i0 + k < n ? i0 + k : n - 1] * a.ld_dy, col, a.dim);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int i = i0 + k;
@@ -318,11 +343,11 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const Lookup a, int 
         if (whole && !more) {
 #pragma unroll
           for (int e = 0; e < Vec<T>::V; ++e) sum.f[e] *= a.scale;
-          store_chunk<T>(sum, a.dw, (long long)v * a.dim, col, a.dim);
+          store_chunk<T, SHORT>(sum, a.dw, (long long)v * a.dim, col, a.dim);
         } else {
           // part of a class that came from the run before, or that goes on in the next one
           float* part = a.part + (run * 2 + (whole ? 1 : 0)) * a.dim;
-          if (a.dim < Vec<T>::V) {
+          if constexpr (SHORT) {
             for (int e = 0; e < a.dim; ++e) part[e] = sum.f[e];
           } else {
 #pragma unroll
@@ -376,16 +401,21 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const Lookup a) {
 template <int T>
 void launch_forward(const Lookup& a, hipStream_t stream) {
   const int chunks = (a.dim + Vec<T>::V - 1) / Vec<T>::V;
-  hipLaunchKernelGGL((embedding_kernel<T>), dim3((unsigned)((a.n * chunks + 255) / 256)), dim3(256), 0, stream,
-                     a, chunks);
+  const dim3 grid((unsigned)((a.n * chunks + 255) / 256));
+  if (a.dim < Vec<T>::V)
+    hipLaunchKernelGGL((embedding_kernel<T, true>), grid, dim3(256), 0, stream, a, chunks);
+  else
+    hipLaunchKernelGGL((embedding_kernel<T, false>), grid, dim3(256), 0, stream, a, chunks);
 }
 
 template <int T>
 void launch_sums(const Lookup& a, hipStream_t stream) {
   const int chunks = (a.dim + Vec<T>::V - 1) / Vec<T>::V;
-  if (a.runs + a.fills > 0)
-    hipLaunchKernelGGL((embedding_sum_kernel<T>), dim3((unsigned)(a.runs + a.fills)), dim3(256), 0, stream, a,
-                       chunks);
+  const dim3 grid((unsigned)(a.runs + a.fills));
+  if (a.runs + a.fills > 0 && a.dim < Vec<T>::V)
+    hipLaunchKernelGGL((embedding_sum_kernel<T, true>), grid, dim3(256), 0, stream, a, chunks);
+  else if (a.runs + a.fills > 0)
+    hipLaunchKernelGGL((embedding_sum_kernel<T, false>), grid, dim3(256), 0, stream, a, chunks);
   if (a.runs > 1)
     hipLaunchKernelGGL((embedding_join_kernel<T>), dim3((unsigned)(a.runs - 1), (unsigned)((a.dim + 255) / 256)),
                        dim3(256), 0, stream, a);
@@ -413,7 +443,7 @@ int64_t plan(Lookup* l, const dmuon_embedding_args& a, char* ws) {
   l->padding = a.padding_idx;
   l->passes = 1;
   while (l->passes * kDigit < 32 && (a.vocab >> (l->passes * kDigit))) ++l->passes;
-  long long blocks = (l->n + kSortTile - 1) / kSortTile;
+  long long blocks = l->n <= kSortAlone ? (l->n > 0) : (l->n + kSortTile - 1) / kSortTile;
   if (blocks > kSortBlocks) blocks = kSortBlocks;
   l->sort_chunk = blocks ? ((l->n + blocks - 1) / blocks + kSortTile - 1) / kSortTile * kSortTile : kSortTile;
   l->sort_blocks = (int)((l->n + l->sort_chunk - 1) / l->sort_chunk);
@@ -496,7 +526,11 @@ int dmuon_embedding_grad(const dmuon_embedding_args* args, void* workspace, int6
     l.fill_rows = bytes / row < l.vocab - l.fill_at ? bytes / row : l.vocab - l.fill_at;
     return (unsigned)(l.sort_blocks + ((l.fill_rows * row + 15) / 16 + kFillChunks - 1) / kFillChunks);
   };
-  if (l.n > 0)
+  if (l.sort_blocks == 1) {
+    const unsigned blocks = share(kFillHist + kFillScatter);
+    hipLaunchKernelGGL(embedding_sort_kernel, dim3(blocks), dim3(1024), 0, s, l);
+    l.fill_at += l.fill_rows;
+  } else if (l.n > 0) {
     for (int p = 0; p < l.passes; ++p) {
       unsigned blocks = share(kFillHist);
       hipLaunchKernelGGL(embedding_hist_kernel, dim3(blocks), dim3(1024), 0, s, l, p);
@@ -505,6 +539,7 @@ int dmuon_embedding_grad(const dmuon_embedding_args* args, void* workspace, int6
       hipLaunchKernelGGL(embedding_scatter_kernel, dim3(blocks), dim3(1024), 0, s, l, p);
       l.fill_at += l.fill_rows;
     }
+  }
   l.fills = (l.vocab - l.fill_at + kFillRows - 1) / kFillRows;
   if (a.dtype == DMUON_DTYPE_F32) launch_sums<DT_F32>(l, s);
   else if (a.dtype == DMUON_DTYPE_F16) launch_sums<DT_F16>(l, s);
