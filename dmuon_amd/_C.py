@@ -75,7 +75,7 @@ c_np = ctypes.POINTER(ResidualNormArgs)
 class AttentionArgs(ctypes.Structure):
     """``dmuon_attention_args``: one call of attention over heads."""
 
-    _fields_ = [(k, c_vp) for k in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv",
+    _fields_ = [(k, c_vp) for k in ("q", "k", "v", "out", "rest", "lse", "dout", "dq", "dk", "dv",
                                     "kv_lengths", "q_starts", "kv_starts")] + \
         [(k, c_i64) for k in ("batch", "q_len", "kv_len", "heads", "kv_heads", "dim", "window",
                               "q_batch", "q_token", "q_head", "k_batch", "k_token", "k_head",

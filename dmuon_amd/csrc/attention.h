@@ -22,6 +22,7 @@ struct Sequence {
 struct Attention {
   const uint16_t* q; const uint16_t* k; const uint16_t* v; const uint16_t* dout;
   uint16_t* out; uint16_t* dq; uint16_t* dk; uint16_t* dv;   // dense [tokens][heads][dim]
+  uint16_t* rest;                         // what out's rounding left, rounded itself, or NULL
   float* lse;                             // [tokens][heads], log2 of the row's sum; +inf: sees nothing
   float* delta;                           // [tokens][heads], minus the sum of dout out
   // strides in elements

@@ -54,6 +54,7 @@ Attention describe(const dmuon_attention_args& a) {
   r.v = static_cast<const uint16_t*>(a.v);
   r.out = static_cast<uint16_t*>(a.out);
   r.lse = a.lse;
+  r.rest = static_cast<uint16_t*>(a.rest);
   r.q_batch = a.q_batch; r.q_token = a.q_token; r.q_head = a.q_head;
   r.k_batch = a.k_batch; r.k_token = a.k_token; r.k_head = a.k_head;
   r.v_batch = a.v_batch; r.v_token = a.v_token; r.v_head = a.v_head;
@@ -217,7 +218,8 @@ int dmuon_attention(const dmuon_attention_args* args, void* workspace, int64_t w
   const Plan p = plan_forward(*args, workspace);
   if (check_workspace(who, p.bytes, workspace, workspace_bytes)) return 1;
   if (args->q_len == 0 || (!args->q_starts && args->batch == 0)) return 0;
-  if (!args->out || !aligned(args->out)) return fail("%s: out is NULL or not 16-byte aligned", who);
+  if (!args->out || !aligned(args->out) || !aligned(args->rest))
+    return fail("%s: out is NULL, or out or rest not 16-byte aligned", who);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (int rc = check_launch(fill_tables(p, *args, s), who)) return rc;
   return check_launch(launch_attention(p.a, s), who);
@@ -238,8 +240,8 @@ int dmuon_attention_grad(const dmuon_attention_args* args, void* workspace, int6
   const dmuon_attention_args& a = *args;
   const bool rows = a.q_len > 0 && (a.q_starts || a.batch > 0);
   if (rows && (!a.out || !a.lse || !a.dout)) return fail("%s: out, lse or dout is NULL", who);
-  if (!aligned(a.out) || !aligned(a.dout) || !aligned(a.dq) || !aligned(a.dk) || !aligned(a.dv))
-    return fail("%s: out, dout and the gradients must be 16-byte aligned", who);
+  if (!aligned(a.out) || !aligned(a.rest) || !aligned(a.dout) || !aligned(a.dq) || !aligned(a.dk) || !aligned(a.dv))
+    return fail("%s: out, rest, dout and the gradients must be 16-byte aligned", who);
   for (int64_t s : {a.do_batch, a.do_token, a.do_head})
     if (s < 0 || s % 8) return fail("%s: strides must be multiples of 8 values", who);
   if (65 * a.do_token + a.heads / a.kv_heads * a.do_head >= kMost)

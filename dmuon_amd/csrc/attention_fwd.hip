@@ -8,6 +8,12 @@ namespace {
 constexpr float kInf = __builtin_inff();
 constexpr int kKeys = 64;                 // keys of a tile
 
+// What is left of two values behind their rounding
+template <int E>
+__device__ __forceinline__ unsigned rest2(unsigned w, float lo, float hi) {
+  return pack2_elt<E>(lo - from_elt<E>((uint16_t)w), hi - from_elt<E>((uint16_t)(w >> 16)));
+}
+
 // A lane's half of a row: the result and its statistics, or, of one part of the keys, the unfinished sums.
 template <int E, int DB>
 __device__ __forceinline__ void store_row(const Attention& a, const Place& p, bool live, int query, int head,
@@ -30,15 +36,19 @@ __device__ __forceinline__ void store_row(const Attention& a, const Place& p, bo
   }
   // a row that sees nothing is 0
   const float f = total == 0.f ? 0.f : 1.f / total;
-  uint16_t* out = a.out + row * a.dim;
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       const int d = 32 * b + result_row(i, h);
-      if (d < a.dim)
-        *reinterpret_cast<u32x2_t*>(out + d) = u32x2_t{pack2_elt<E>(o[b][i] * f, o[b][i + 1] * f),
-                                                       pack2_elt<E>(o[b][i + 2] * f, o[b][i + 3] * f)};
+      if (d >= a.dim) continue;
+      const u32x2_t w = {pack2_elt<E>(o[b][i] * f, o[b][i + 1] * f),
+                         pack2_elt<E>(o[b][i + 2] * f, o[b][i + 3] * f)};
+      *reinterpret_cast<u32x2_t*>(a.out + row * a.dim + d) = w;
+      if (a.rest)
+        *reinterpret_cast<u32x2_t*>(a.rest + row * a.dim + d) =
+            u32x2_t{rest2<E>(w[0], o[b][i] * f, o[b][i + 1] * f),
+                    rest2<E>(w[1], o[b][i + 2] * f, o[b][i + 3] * f)};
     }
   if (a.lse && h == 0) a.lse[row] = total == 0.f ? kInf : ref + __log2f(total);
 }
@@ -334,8 +344,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Attention a) 
     }
   }
   const float g = total == 0.f ? 0.f : 1.f / total;
-  if (2 * lane < a.dim)
-    *reinterpret_cast<unsigned*>(a.out + row * a.dim + d) = pack2_elt<E>(o0 * g, o1 * g);
+  if (2 * lane < a.dim) {
+    const unsigned w = pack2_elt<E>(o0 * g, o1 * g);
+    *reinterpret_cast<unsigned*>(a.out + row * a.dim + d) = w;
+    if (a.rest) *reinterpret_cast<unsigned*>(a.rest + row * a.dim + d) = rest2<E>(w, o0 * g, o1 * g);
+  }
   if (a.lse && lane == 0) a.lse[row] = total == 0.f ? kInf : top + __log2f(total);
 }
 

@@ -65,7 +65,7 @@ struct AttentionCall {
   }
 
   Tensor forward(const HeadsView& q, const HeadsView& k, const HeadsView& v, const Tensor& lengths,
-                 const Tensor& q_starts, const Tensor& kv_starts, Tensor* lse) const {
+                 const Tensor& q_starts, const Tensor& kv_starts, Tensor* lse, Tensor* rest) const {
     const c10::DeviceGuard guard(q.t.device());
     auto a = describe(q, k, v, lengths, q_starts, kv_starts);
     Tensor out = at::empty(q.t.sizes(), q.t.options());
@@ -73,6 +73,8 @@ struct AttentionCall {
     if (lse) {
       *lse = at::empty(q.t.sizes().slice(0, q.t.dim() - 1), q.t.options().dtype(at::kFloat));
       a.lse = static_cast<float*>(ptr(*lse));
+      *rest = at::empty(q.t.sizes(), q.t.options());
+      a.rest = ptr(*rest);
     }
     int64_t need = 0;
     call(dmuon_attention_workspace_size(&a, &need));
@@ -87,17 +89,17 @@ struct Attend : torch::autograd::Function<Attend> {
                         const OptTensor& lengths, const OptTensor& q_starts, const OptTensor& kv_starts,
                         const AttentionCall& c) {
     const HeadsView qv(q, false, c.group), kv(k, true, c.group), vv(v, true, c.group);
-    Tensor lse;
+    Tensor lse, rest;
     const Tensor n = lengths.value_or(Tensor()), qs = q_starts.value_or(Tensor()),
                  ks = kv_starts.value_or(Tensor());
-    const Tensor out = c.forward(qv, kv, vv, n, qs, ks, &lse);
+    const Tensor out = c.forward(qv, kv, vv, n, qs, ks, &lse, &rest);
     ctx->saved_data["causal"] = c.causal;
     ctx->saved_data["packed"] = c.packed;
     ctx->saved_data["window"] = c.window;
     ctx->saved_data["batch"] = c.batch;
     ctx->saved_data["group"] = c.group;
     ctx->saved_data["scale"] = c.scale;
-    ctx->save_for_backward({qv.t, kv.t, vv.t, out, lse, n, qs, ks});
+    ctx->save_for_backward({qv.t, kv.t, vv.t, out, lse, n, qs, ks, rest});
     return out;
   }
 
@@ -116,6 +118,7 @@ struct Attend : torch::autograd::Function<Attend> {
     const HeadsView d(grads[0], false, c.group);
     auto a = c.describe(q, k, v, s[5], s[6], s[7]);
     a.out = ptr(s[3]);
+    a.rest = ptr(s[8]);
     a.lse = static_cast<float*>(ptr(s[4]));
     a.dout = ptr(d.t);
     a.do_batch = d.batch;
@@ -196,7 +199,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, bool causal,
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return Attend::apply(q, k, v, n, qs, ks, c);
   const HeadsView qv(q, false, c.group), kv(k, true, c.group), vv(v, true, c.group);
-  return c.forward(qv, kv, vv, n.value_or(Tensor()), qs.value_or(Tensor()), ks.value_or(Tensor()), nullptr);
+  return c.forward(qv, kv, vv, n.value_or(Tensor()), qs.value_or(Tensor()), ks.value_or(Tensor()), nullptr, nullptr);
 }
 
 // ---- the heads' norms and rotation --------------------------------------------------------------

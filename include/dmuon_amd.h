@@ -566,8 +566,9 @@ int dmuon_residual_norm_grad(const dmuon_residual_norm_args* args, void* workspa
  *     are held to the tokens that are there, and one that falls to the largest before it; a token in no
  *     sequence has the result and the gradient 0.
  * Strides are in elements, multiples of 8, and bases 16-byte aligned; out, lse and the gradients are
- * dense. lse [tokens][heads] (fp32, NULL where no gradient follows) keeps the log2 of each row's sum.
- * dmuon_attention_grad: from dout, out and lse the gradients dq, dk and dv; any may be NULL. Workspaces are
+ * dense. lse [tokens][heads] (fp32, NULL where no gradient follows) keeps the log2 of each row's sum, and
+ * rest (as out, or NULL) what out's rounding left, with which the gradients are more exact.
+ * dmuon_attention_grad: from dout, out, rest and lse the gradients dq, dk and dv; any may be NULL. Workspaces are
  * 256-byte aligned. Nothing depends on the order of blocks: the same arguments give the same bits.
  */
 typedef struct {
@@ -575,6 +576,7 @@ typedef struct {
   const void* k;
   const void* v;
   void* out;
+  void* rest;
   float* lse;
   const void* dout;
   void* dq;

@@ -432,7 +432,7 @@ def test_c_entry_refusals_without_gpu():
 
     from dmuon_amd import _C
     lib, need = _C.lib(), ctypes.c_int64()
-    good = dict(q=4096, k=4096, v=4096, out=4096, lse=4096, dout=4096, dq=4096, dk=4096, dv=4096,
+    good = dict(q=4096, k=4096, v=4096, out=4096, rest=4096, lse=4096, dout=4096, dq=4096, dk=4096, dv=4096,
                 batch=2, q_len=40, kv_len=50, heads=4, kv_heads=2, dim=64, q_batch=40 * 256, q_token=256,
                 q_head=64, k_batch=50 * 128, k_token=128, k_head=64, v_batch=50 * 128, v_token=128,
                 v_head=64, do_batch=40 * 256, do_token=256, do_head=64, scale=0.125, causal=1, dtype=1)
@@ -474,6 +474,7 @@ def test_c_entry_refusals_without_gpu():
     says(lib.dmuon_attention_grad(args(), 4097, 1 << 40, None), "aligned")
     says(grad(args(lse=None)), "lse")
     says(grad(args(dq=4104)), "aligned")
+    says(grad(args(rest=4104)), "aligned")
     says(grad(args(do_head=4)), "multiples of 8")
     says(grad(args(do_token=1 << 25)), "span")
 
