@@ -165,6 +165,10 @@ __device__ __forceinline__ bf16x8_t pack8(const f32x16_t& v, int from) {
 
 constexpr unsigned kNowhere = 0x80000000u;     // outside any buffer range: reads 0
 
+// Loads of a wave that works alone are of use to no other: not temporal (the loads' second policy bit).
+// 48 x 1 token over up to 8192 keys: 181 -> 165 us.
+constexpr int kPastCaches = 2;
+
 // Moves ROWS rows of one pitch from memory into LDS, WAVES waves together. The swizzle repeats after four
 // instructions of a wave, so four offsets describe them all.
 template <int D, int ROWS, int WAVES>
@@ -196,7 +200,7 @@ struct TileMover {
 #pragma unroll
       for (int i = 0; i < PART; ++i)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(lds + (wave * N + part * 4 + i) * 1024), 16,
-                                                 off[i], 0, 0, 0);
+                                                 off[i], 0, 0, WAVES == 1 ? kPastCaches : 0);
     }
   }
 };

@@ -119,8 +119,9 @@ bool few_rows(const Attention& a, bool packed) {
   return packed ? rows <= (int64_t)kFewRows * a.batch : rows <= kFewRows;
 }
 
-// Few rows over many keys do not fill the card: the keys are split. Waves that work alone take pieces of 512
-// keys, or fewer where that leaves less than one wave a CU; blocks of 128 rows pieces of 256 or more, up to
+// Few rows over many keys do not fill the card: the keys are split. Waves that work alone take pieces of 1024
+// keys (48 x 8 x 8192 keys: 157 us, of 512 165, of 256 173), or fewer where that leaves less than two waves a
+// CU; blocks of 128 rows pieces of 256 or more, up to
 // two blocks a CU.
 int splits_of(const Attention& a, bool packed) {
   const int64_t units = (int64_t)a.kv_heads * (packed ? 1 : a.batch);
@@ -129,7 +130,7 @@ int splits_of(const Attention& a, bool packed) {
   if (blocks < 1) return 1;
   int64_t s;
   if (a.few) {
-    s = (keys + 511) / 512;
+    s = (keys + 1023) / 1024;
     if (s * blocks < 512) s = (512 + blocks - 1) / blocks;
     if (s > (keys + 31) / 32) s = (keys + 31) / 32;
   } else {

@@ -53,42 +53,35 @@ __device__ __forceinline__ void store_row(const Attention& a, const Place& p, bo
   if (a.lse && h == 0) a.lse[row] = total == 0.f ? kInf : ref + __log2f(total);
 }
 
-// A wave has RT x 32 rows of queries, one a lane (l % 32): S^T = K Q^T leaves each lane 16 keys of
+// A block has 128 rows of queries, 32 a wave and one a lane (l % 32): S^T = K Q^T leaves each lane 16 keys of
 // every 32 for its own row, the other half of the wave's lanes the rest, and goes as it is into
 // O^T = V^T P^T.
-template <int E, int D, int RT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1, RT == 1 ? 2 : 1)))
+// Waves of a SIMD: two of dim 128 by their registers, four of dim 64 (68 -> 63 us at 8191 x 16 heads in a
+// window of 1024).
+template <int E, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2, D == 64 ? 4 : 2)))
 void attention_kernel(const Attention a) {
-  constexpr int ROWS = 128 * RT, KS = D / 16, DB = D / 32, TILE = kKeys * D * 2;
+  constexpr int KS = D / 16, DB = D / 32, TILE = kKeys * D * 2;
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
   const Place p = place_of<false>(a, blockIdx.x, gridDim.x, a.causal);
   if (!p.live) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const int r0 = p.tile * ROWS, rows = p.qn * a.group;
+  const int r0 = p.tile * kQueryRows, rows = p.qn * a.group;
 
-  // queries of this lane's rows; rows past the last one see nothing
-  bf16x8_t qf[RT][KS];
-  int query[RT], head[RT];
-  bool row_live[RT];
+  // this lane's row; rows past the last one see nothing
+  const int r = r0 + wave * 32 + (lane & 31), query = r / a.group, head = r - query * a.group;
+  const bool live = r < rows;
+  bf16x8_t qf[KS];
 #pragma unroll
-  for (int x = 0; x < RT; ++x) {
-    const int r = r0 + (wave * RT + x) * 32 + (lane & 31);
-    row_live[x] = r < rows;
-    query[x] = r / a.group;
-    head[x] = r - query[x] * a.group;
-    const uint16_t* src = a.q + p.q_off + query[x] * a.q_token + head[x] * a.q_head;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int at = 16 * s + 8 * h;
-      qf[x][s] = bf16x8_t{};
-      if (row_live[x] && at < a.dim) qf[x][s] = *reinterpret_cast<const bf16x8_t*>(src + at);
-    }
+  for (int s = 0; s < KS; ++s) {
+    const int at = 16 * s + 8 * h;
+    qf[s] = bf16x8_t{};
+    if (live && at < a.dim)
+      qf[s] = *reinterpret_cast<const bf16x8_t*>(a.q + p.q_off + query * a.q_token + head * a.q_head + at);
   }
-  Sight see[RT];
-#pragma unroll
-  for (int x = 0; x < RT; ++x) see[x] = row_live[x] ? sight_of(a, p, query[x]) : Sight{0, 0};
+  const Sight see = live ? sight_of(a, p, query) : Sight{0, 0};
   // the block's tiles: what its first and last row see
-  const int last_row = r0 + ROWS < rows ? r0 + ROWS - 1 : rows - 1;
+  const int last_row = r0 + kQueryRows < rows ? r0 + kQueryRows - 1 : rows - 1;
   const Sight first = sight_of(a, p, r0 / a.group), last = sight_of(a, p, last_row / a.group);
   int t0 = first.lo / kKeys, t1 = (last.hi + kKeys - 1) / kKeys;
   if (t1 < t0) t1 = t0;
@@ -98,7 +91,7 @@ void attention_kernel(const Attention a) {
     t1 = t0 + each < t1 ? t0 + each : t1;
   }
   // keys that every row sees need no mask
-  const int full_lo = last.lo, full_hi = last_row == r0 + ROWS - 1 ? first.hi : 0;
+  const int full_lo = last.lo, full_hi = last_row == r0 + kQueryRows - 1 ? first.hi : 0;
 
   TileMover<D, kKeys, 4> mk, mv;
   mk.init(a.k_token, a.dim, wave, lane);
@@ -110,80 +103,70 @@ void attention_kernel(const Attention a) {
   };
   const int row_at = row_form<D>(lane), turn_at = turned_form<D>(lane);
 
-  f32x16_t o[RT][DB];
-  float ref[RT], sum[RT];
+  f32x16_t o[DB];
 #pragma unroll
-  for (int x = 0; x < RT; ++x) {
-#pragma unroll
-    for (int b = 0; b < DB; ++b) o[x][b] = f32x16_t{};
-    ref[x] = -kInf;
-    sum[x] = 0.f;
-  }
+  for (int b = 0; b < DB; ++b) o[b] = f32x16_t{};
+  float ref = -kInf, sum = 0.f;
   // the slots' pointers are restrict: the compiler need not wait for loads into `next` before reads of `kt`
   auto step = [&](int t, const char* __restrict__ kt, char* __restrict__ next) __attribute__((always_inline)) {
     const char* vt = kt + TILE;
     if (t + 1 < t1) fetch(t + 1, next);
-    f32x16_t s[RT][2];
-#pragma unroll
-    for (int x = 0; x < RT; ++x) s[x][0] = s[x][1] = f32x16_t{};
+    f32x16_t s[2] = {};
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kt + b * 64 * D + (row_at ^ (32 * k)));
+      for (int b = 0; b < 2; ++b)
+        s[b] = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(kt + b * 64 * D + (row_at ^ (32 * k))), qf[k],
+                                s[b]);
+    // six reads ahead of the products (read and used in pairs, 2 x 8192 tokens took 1070 us where these
+    // take 1040)
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
-        for (int x = 0; x < RT; ++x) s[x][b] = mfma_32x32x16<E>(kf, qf[x][k], s[x][b]);
-      }
+    for (int i = 0; i < KS - 3; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
     const int j0 = t * kKeys;
     if (j0 < full_lo || j0 + kKeys > full_hi) {
-#pragma unroll
-      for (int x = 0; x < RT; ++x)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = j0 + 32 * b + result_row(i, h);
-            s[x][b][i] = j >= see[x].lo && j < see[x].hi ? s[x][b][i] : -kInf;
-          }
-    }
-#pragma unroll
-    for (int x = 0; x < RT; ++x) {
-      float top = -kInf;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][b][i]);
-      top = half_max(top) * a.c;
-      // the reference follows the maximum only when that has grown by 2^8: any reference gives the same
-      // quotient, and sums and 16-bit probabilities have room for 256
-      if (__ballot(top > ref[x] + 8.f)) {
-        const float now = fmaxf(ref[x], top), from = now == -kInf ? 0.f : now;
-        const float f = __builtin_amdgcn_exp2f(ref[x] - from);
-        ref[x] = now;
-        sum[x] *= f;
-#pragma unroll
-        for (int b = 0; b < DB; ++b) o[x][b] *= f;
-      }
-      const float from = ref[x] == -kInf ? 0.f : ref[x];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s[x][b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][b][i], a.c, -from));
-          sum[x] += s[x][b][i];
+          const int j = j0 + 32 * b + result_row(i, h);
+          s[b][i] = j >= see.lo && j < see.hi ? s[b][i] : -kInf;
         }
     }
+    float top = -kInf;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top = half_max(top) * a.c;
+    // the reference follows the maximum only when that has grown by 2^8: any reference gives the same
+    // quotient, and sums and 16-bit probabilities have room for 256
+    if (__ballot(top > ref + 8.f)) {
+      const float now = fmaxf(ref, top), from = now == -kInf ? 0.f : now;
+      const float f = __builtin_amdgcn_exp2f(ref - from);
+      ref = now;
+      sum *= f;
+#pragma unroll
+      for (int b = 0; b < DB; ++b) o[b] *= f;
+    }
+    const float from = ref == -kInf ? 0.f : ref;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], a.c, -from));
+        sum += s[b][i];
+      }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      bf16x8_t pf[RT];
+      const bf16x8_t pf = pack8<E>(s[u / 2], 8 * (u & 1));
 #pragma unroll
-      for (int x = 0; x < RT; ++x) pf[x] = pack8<E>(s[x][u / 2], 8 * (u & 1));
-#pragma unroll
-      for (int b = 0; b < DB; ++b) {
-        const bf16x8_t vf = read_turned<D>(vt + u * 32 * D, turn_at ^ (64 * b));
-#pragma unroll
-        for (int x = 0; x < RT; ++x) o[x][b] = mfma_32x32x16<E>(vf, pf[x], o[x][b]);
-      }
+      for (int b = 0; b < DB; ++b)
+        o[b] = mfma_32x32x16<E>(read_turned<D>(vt + u * 32 * D, turn_at ^ (64 * b)), pf, o[b]);
     }
   };
   if (t0 < t1) fetch(t0, lds);
@@ -193,9 +176,7 @@ void attention_kernel(const Attention a) {
     const int slot = (t - t0) & 1;
     step(t, lds + slot * 2 * TILE, lds + (slot ^ 1) * 2 * TILE);
   }
-#pragma unroll
-  for (int x = 0; x < RT; ++x)
-    store_row<E, DB>(a, p, row_live[x], query[x], head[x], o[x], ref[x], half_sum(sum[x]), h);
+  store_row<E, DB>(a, p, live, query, head, o, ref, half_sum(sum), h);
 }
 
 // Few rows over many keys (single tokens over a cache): a wave for itself takes 32 rows and a part of the
@@ -435,7 +416,7 @@ __global__ __launch_bounds__(1024) void attention_tables_kernel(
 template <int E, int D>
 void launch(const Attention& a, unsigned blocks, hipStream_t stream) {
   if (a.few) hipLaunchKernelGGL((attention_few_kernel<E, D>), dim3(blocks), dim3(64), 0, stream, a);
-  else hipLaunchKernelGGL((attention_kernel<E, D, 1>), dim3(blocks), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((attention_kernel<E, D>), dim3(blocks), dim3(256), 0, stream, a);
 }
 
 }  // namespace
