@@ -349,6 +349,7 @@ void shape(Heads* a, bool grad) {
     return all * ((a->heads[0] + per - 1) / per + (a->heads[1] + per - 1) / per);
   };
   while (a->per_part > 1 && blocks_at(a->per_part) < kCus * 4) a->per_part /= 2;
+  while ((a->heads[0] + a->heads[1]) / a->per_part > 32768) a->per_part *= 2;    // a grid's second extent
   for (int z = 0; z < 2; ++z) a->parts[z] = (a->heads[z] + a->per_part - 1) / a->per_part;
   // the gradient's partial rows: as many blocks as their registers let run at once (of 512 it took 113 us,
   // of 1024 98, of 768 94)

@@ -126,7 +126,8 @@ SHAPES = [  # batch, tokens, keys, heads, key heads, dim, causal, window
     (1, 257, 65, 2, 1, 128, True, None), (1, 300, 300, 8, 2, 64, True, 37), (1, 64, 1000, 2, 2, 96, False, None),
     (1, 5, 2100, 8, 1, 128, True, None), (3, 70, 70, 2, 1, 16, True, 1), (1, 128, 128, 1, 1, 128, False, None),
     (1, 200, 450, 5, 1, 120, True, 64), (1, 1, 3000, 12, 2, 56, True, 500), (2, 64, 64, 7, 7, 64, True, 1000),
-    (1, 500, 1, 3, 3, 32, True, None), (1, 129, 640, 4, 2, 128, True, 128), (1, 700, 700, 2, 2, 128, True, None),
+    (1, 500, 1, 3, 3, 32, True, None), (2, 40, 40, 71, 1, 64, True, None), (1, 70, 90, 130, 1, 128, True, 33),
+    (1, 150, 150, 96, 1, 24, False, None), (2, 1, 400, 64, 1, 64, True, None), (3, 300, 40, 33, 3, 64, True, None), (1, 129, 640, 4, 2, 128, True, 128), (1, 700, 700, 2, 2, 128, True, None),
 ]
 
 
@@ -339,6 +340,21 @@ def test_same_bits_every_time_on_any_stream_and_in_a_graph(gpu):
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(want, held))
+
+
+@pytest.mark.gpu
+def test_calls_at_once(gpu):
+    """Calls on two streams, with nothing between them: each has its own workspace."""
+    sets = [_make(gpu, (1, 300, 8, 64), (1, 2000, 2, 64), torch.float16, 40 + i) for i in range(6)]
+    want = [_grads(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for i, s in enumerate(sets):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(_grads(*s))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 @pytest.mark.gpu

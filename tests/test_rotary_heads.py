@@ -110,7 +110,7 @@ def _check(v, positions, inv_freq, outs, interleaved=False):
     ((1,), 1, 1, 2, 2), ((1,), 32, 8, 128, 128), ((), 3, 2, 64, 32), ((7,), 5, 1, 72, 36), ((3, 50), 4, 2, 128, 64),
     ((2, 3, 33), 1, 1, 96, 96), ((130,), 3, 3, 20, 6), ((65,), 2, 1, 130, 130), ((40,), 2, 2, 256, 128),
     ((19,), 1, 2, 512, 512), ((21,), 1, 1, 510, 10), ((900,), 6, 2, 64, 64), ((5,), 40, 8, 80, 80),
-    ((11,), 2, 1, 40, 16)])
+    ((11,), 2, 1, 40, 16), ((2,), 71, 1, 64, 64)])
 def test_sizes_and_types(gpu, lead, h, hk, d, r, dt, wt, interleaved):
     _check(*_make(gpu, lead, h, hk, d, r, dt, wt), interleaved)
 
@@ -175,6 +175,11 @@ def test_strides_and_alignment(gpu, kind):
         y = _call(leaves, p, f)
         return [t.detach() for t in y] + list(torch.autograd.grad(y, list(leaves.values()), o))
     assert all(torch.equal(a, b) for a, b in zip(run(v, outs), run(w, douts)))
+
+
+@pytest.mark.gpu
+def test_as_many_heads_as_there_may_be(gpu):
+    _check(*_make(gpu, (1,), 65536, 40000, 8, 8, torch.float32, torch.float32, seed=11))
 
 
 @pytest.mark.gpu
