@@ -104,30 +104,28 @@ __device__ __forceinline__ void pair_at(const Heads& a, int p, int* i, int* j) {
 }
 
 // A lane's P pairs of a head, from pair `p` on: P = 8 (rotary and dim multiples of 16) or 4 (of 8) are two
-// runs of P values, the pairs' first and second ones or, of neighbours, one behind the other.
-template <int T, int P>
+// runs of P values, the pairs' first and second ones or, SIDE by side, one run behind the other. (Values that
+// are not rotated may pair as they lie.)
+template <int T, int P, bool SIDE>
 struct Pairs {
   Run<T, P> r[2];
   __device__ __forceinline__ void load(const void* src, long long at, int i, int j) {
     r[0].load(src, at + i);
     r[1].load(src, at + j);
   }
-  __device__ __forceinline__ void get(bool apart, float* v) const {
-#pragma unroll
-    for (int k = 0; k < P; ++k) {
-      const float lo = r[0].get(k), hi = r[1].get(k);
-      const float even = 2 * k < P ? r[0].get((2 * k) % P) : r[1].get((2 * k) % P);
-      const float odd = 2 * k < P ? r[0].get((2 * k + 1) % P) : r[1].get((2 * k + 1) % P);
-      v[k] = apart ? lo : even;
-      v[P + k] = apart ? hi : odd;
-    }
+  // where value k of both runs stands among the pairs' first ones, then their second ones
+  static __device__ __forceinline__ constexpr int place(int run, int k) {
+    return SIDE ? ((run * P + k) & 1) * P + (run * P + k) / 2 : run * P + k;
   }
-  __device__ __forceinline__ void set(bool apart, const float* v) {
+  __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[place(0, k)] = r[0].get(k), v[place(1, k)] = r[1].get(k);
+  }
+  __device__ __forceinline__ void set(const float* v) {
 #pragma unroll
     for (int k = 0; k < P; k += 2) {
-      // values k and k + 1 of both runs
-      r[0].set2(k, apart ? v[k] : v[k / 2], apart ? v[k + 1] : v[P + k / 2]);
-      r[1].set2(k, apart ? v[P + k] : v[(P + k) / 2], apart ? v[P + k + 1] : v[P + (P + k) / 2]);
+      r[0].set2(k, v[place(0, k)], v[place(0, k + 1)]);
+      r[1].set2(k, v[place(1, k)], v[place(1, k + 1)]);
     }
   }
   __device__ __forceinline__ void store(void* dst, long long at, int i, int j) const {
@@ -135,20 +133,28 @@ struct Pairs {
     r[1].store(dst, at + j);
   }
 };
-template <int T>
-struct Pairs<T, 1> {
+template <int T, bool SIDE>
+struct Pairs<T, 1, SIDE> {
   float a, b;
   __device__ __forceinline__ void load(const void* src, long long at, int i, int j) {
     a = element(src, T, at + i);
     b = element(src, T, at + j);
   }
-  __device__ __forceinline__ void get(bool, float* v) const { v[0] = a, v[1] = b; }
-  __device__ __forceinline__ void set(bool, const float* v) { a = v[0], b = v[1]; }
+  __device__ __forceinline__ void get(float* v) const { v[0] = a, v[1] = b; }
+  __device__ __forceinline__ void set(const float* v) { a = v[0], b = v[1]; }
   __device__ __forceinline__ void store(void* dst, long long at, int i, int j) const {
     set_element(dst, T, at + i, a);
     set_element(dst, T, at + j, b);
   }
 };
+
+// The place in its head of a lane's value k (the pairs' first values, then their second), whose runs begin
+// at i and j
+template <int P, bool SIDE>
+__device__ __forceinline__ int value_at(int i, int j, int k) {
+  if (P > 1 && SIDE) return i + 2 * (k % P) + k / P;
+  return k < P ? i + k : j + k - P;
+}
 
 // cos and sin of position * inv_freq: within an eighth of a turn the Taylor polynomials are off by less
 // than 2^-29
@@ -168,8 +174,11 @@ __device__ __forceinline__ float2 turn_of(const Heads& a, double position, int p
 
 // GRAD: x and dy to dx and the weights' partial sums; otherwise x to y. SLOTS: of P pairs a lane.
 // blockIdx.y is the part of the heads: the queries' parts, then the keys'.
-template <int T, int P, int SLOTS, bool GRAD>
+// SIDE: rotated pairs are neighbours (of P = 1: either, by their places).
+template <int T, int P, int SLOTS, bool SIDE, bool GRAD>
 __global__ __launch_bounds__(kThreads) void rotary_heads_kernel(const Heads a) {
+  // heads whose loads are in flight: forward 79 us of one, 75 of two (16384 tokens of 32 + 8 heads of 128)
+  constexpr int AHEAD = GRAD ? 1 : 2;
   __shared__ float sums[GRAD ? kThreads : 1][2 * P + 1];
   const int sub = threadIdx.x % a.lanes, group = threadIdx.x / a.lanes, groups = kThreads / a.lanes;
   const int half = a.rotary / 2;
@@ -181,7 +190,7 @@ __global__ __launch_bounds__(kThreads) void rotary_heads_kernel(const Heads a) {
   const void* dy = a.dy[z];
   void* to = GRAD ? a.dx[z] : a.y[z];
   int pair[SLOTS], vi[SLOTS], vj[SLOTS];
-  bool live[SLOTS], apart[SLOTS];
+  bool live[SLOTS];
   float w[SLOTS][2 * P], dw[SLOTS][2 * P];
 #pragma unroll
   for (int u = 0; u < SLOTS; ++u) {
@@ -189,13 +198,10 @@ __global__ __launch_bounds__(kThreads) void rotary_heads_kernel(const Heads a) {
     live[u] = pair[u] < a.dim / 2;
     if (!live[u]) pair[u] = 0;
     pair_at(a, pair[u], &vi[u], &vj[u]);
-    apart[u] = vj[u] - vi[u] > 1;
-    if (P > 1 && !apart[u]) vj[u] = vi[u] + P;
+    if (P > 1 && vj[u] == vi[u] + 1) vj[u] = vi[u] + P;
 #pragma unroll
     for (int i = 0; i < 2 * P; ++i) {
-      int at[2];
-      pair_at(a, pair[u] + i % P, &at[0], &at[1]);
-      w[u][i] = norm && live[u] ? element(a.w[z], a.w_dtype[z], at[i / P]) : 1.f;
+      w[u][i] = norm && live[u] ? element(a.w[z], a.w_dtype[z], value_at<P, SIDE>(vi[u], vj[u], i)) : 1.f;
       dw[u][i] = 0.f;
     }
   }
@@ -203,15 +209,20 @@ __global__ __launch_bounds__(kThreads) void rotary_heads_kernel(const Heads a) {
        token += (long long)gridDim.x * groups) {
     long long at = token * a.token[z] + h0 * a.head[z], dat = token * a.dtoken[z] + h0 * a.dhead[z];
     long long out = (token * a.heads[z] + h0) * a.dim;
-    Pairs<T, P> xr[SLOTS], gr[SLOTS];
-    auto fetch = [&]() __attribute__((always_inline)) {
+    // AHEAD heads' loads are in flight
+    Pairs<T, P, SIDE> xr[AHEAD][SLOTS], gr[AHEAD][SLOTS];
+    auto fetch = [&](int ring) __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < SLOTS; ++u) {
-        if (!GRAD || norm) xr[u].load(x, at, vi[u], vj[u]);
-        if (GRAD && dy) gr[u].load(dy, dat, vi[u], vj[u]);
+        if (!GRAD || norm) xr[ring][u].load(x, at, vi[u], vj[u]);
+        if (GRAD && dy) gr[ring][u].load(dy, dat, vi[u], vj[u]);
       }
+      at += a.head[z];
+      dat += a.dhead[z];
     };
-    fetch();
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (h0 + k < h1) fetch(k);
     float2 cs[SLOTS][P];
     {
       const long long slot = a.period == a.tokens ? token : token % a.period;
@@ -222,18 +233,20 @@ __global__ __launch_bounds__(kThreads) void rotary_heads_kernel(const Heads a) {
         for (int k = 0; k < P; ++k)
           cs[u][k] = pair[u] + k < half ? turn_of(a, position, pair[u] + k) : make_float2(1.f, 0.f);
     }
-    for (int h = h0; h < h1; ++h) {
+    for (int first = h0; first < h1; first += AHEAD)
+#pragma unroll
+    for (int ring = 0; ring < AHEAD; ++ring) {
+      const int h = first + ring;
+      if (h >= h1) break;
       float v[SLOTS][2 * P], g[SLOTS][2 * P];
 #pragma unroll
       for (int u = 0; u < SLOTS; ++u) {
-        if (!GRAD || norm) xr[u].get(apart[u], v[u]);
+        if (!GRAD || norm) xr[ring][u].get(v[u]);
 #pragma unroll
         for (int k = 0; k < 2 * P; ++k) g[u][k] = 0.f;
-        if (GRAD && dy) gr[u].get(apart[u], g[u]);
+        if (GRAD && dy) gr[ring][u].get(g[u]);
       }
-      at += a.head[z];
-      dat += a.dhead[z];
-      if (h + 1 < h1) fetch();
+      if (h + AHEAD < h1) fetch(ring);
       // turns the pairs; back: by the opposite angle
       auto rotate = [&](float (&p)[SLOTS][2 * P], float sign) __attribute__((always_inline)) {
 #pragma unroll
@@ -280,8 +293,8 @@ __global__ __launch_bounds__(kThreads) void rotary_heads_kernel(const Heads a) {
 #pragma unroll
         for (int u = 0; u < SLOTS; ++u)
           if (live[u]) {
-            Pairs<T, P> y;
-            y.set(apart[u], GRAD ? g[u] : v[u]);
+            Pairs<T, P, SIDE> y;
+            y.set(GRAD ? g[u] : v[u]);
             y.store(to, out, vi[u], vj[u]);
           }
       out += a.dim;
@@ -303,9 +316,10 @@ __global__ __launch_bounds__(kThreads) void rotary_heads_kernel(const Heads a) {
         if (p >= a.dim / 2) continue;
         float total = 0.f;
         for (int g = 0; g < groups; ++g) total += sums[g * a.lanes + l][k];
-        int spot[2];
-        pair_at(a, p + k % P, &spot[0], &spot[1]);
-        dst[k < P ? spot[0] : spot[1]] = total;
+        int vi0, vj0;
+        pair_at(a, p, &vi0, &vj0);
+        if (P > 1 && vj0 == vi0 + 1) vj0 = vi0 + P;
+        dst[value_at<P, SIDE>(vi0, vj0, k)] = total;
       }
     }
   }
@@ -361,14 +375,15 @@ void shape(Heads* a, bool grad) {
 template <int T, bool GRAD>
 void launch(const Heads& a, hipStream_t stream) {
   const dim3 grid((unsigned)a.blocks, (unsigned)(a.parts[0] + a.parts[1]));
-  if (a.pairs == 8)
-    hipLaunchKernelGGL((rotary_heads_kernel<T, 8, 1, GRAD>), grid, dim3(kThreads), 0, stream, a);
-  else if (a.pairs == 4)
-    hipLaunchKernelGGL((rotary_heads_kernel<T, 4, 1, GRAD>), grid, dim3(kThreads), 0, stream, a);
-  else if (a.dim <= 128)
-    hipLaunchKernelGGL((rotary_heads_kernel<T, 1, 1, GRAD>), grid, dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((rotary_heads_kernel<T, 1, 4, GRAD>), grid, dim3(kThreads), 0, stream, a);
+#define DMUON_RH(P, SLOTS, SIDE) \
+  hipLaunchKernelGGL((rotary_heads_kernel<T, P, SLOTS, SIDE, GRAD>), grid, dim3(kThreads), 0, stream, a)
+  if (a.pairs == 8 && a.interleaved) DMUON_RH(8, 1, true);
+  else if (a.pairs == 8) DMUON_RH(8, 1, false);
+  else if (a.pairs == 4 && a.interleaved) DMUON_RH(4, 1, true);
+  else if (a.pairs == 4) DMUON_RH(4, 1, false);
+  else if (a.dim <= 128) DMUON_RH(1, 1, false);
+  else DMUON_RH(1, 4, false);
+#undef DMUON_RH
 }
 
 template <bool GRAD>
