@@ -5,6 +5,11 @@
 // seven products where one pass would do with five, but no sums over blocks, so no atomics and one order.
 // Where the keys' blocks are few their rows are split, and a second kernel joins the parts in their order.
 //
+// Bound like the forward pass: 2 x 8192 causal tokens, 32/8 heads of 128, bf16 3.5 ms (1.1 PFLOP/s of the seven
+// products, 0.78 of five); 16384 packed tokens in 23 documents 0.64 ms; 8191 tokens of 16 heads of 64 in a
+// window of 1024 in fp16 170 us. The key blocks' sums (dk and dv of 32 keys a wave) and operands take 192 of
+// 256 registers; a third of what they read from LDS is turned on the way (transposing reads).
+//
 // P and dS are rounded to the operands' type between the products. In fp16 they are held times powers of
 // two: P times 2^10 (a long row's probabilities are under the type's normal range) and dS by a further one
 // that the largest rows of do and v set, so that it neither over- nor underflows with a loss scale or a

@@ -7,6 +7,11 @@
 // add up in their order), walks the sorted positions in runs of 8 or 32, and joins the classes that cross
 // from one run to the next in a second kernel: the work of a class that makes up most of the text is
 // spread like any other. Sums are fp32, rounded once.
+//
+// 16384 tokens of 128256 x 4096 in bf16: lookup 32 us (8.4 TB/s, some of it from the caches), sort 21 (which
+// clears 88 MB of the gradient meanwhile), sums 185 (6.2), joining 9. 1023 tokens of 5003 x 300 in fp16: 3, 8, 5
+// and 3.5. One block sorting 16384 tokens under the clearing of dW took as long in all (radix of 9 bits 96 us, of
+// 4 bits in LDS 38).
 #include "../../include/dmuon_amd.h"
 #include "dmuon_amd_internal.h"
 #include "mfma_tile.h"

@@ -10,6 +10,9 @@
 // The lanes of a group keep a token's cosines and sines in registers and walk its heads, the next one's
 // loads in flight: angles are formed once a token and part of the heads, in turns, reduced in 64 bits to an
 // eighth of a turn around a multiple of a quarter, so that positions of any size keep 32 bits of accuracy.
+//
+// 16384 tokens of 32 + 8 heads of 128 in bf16, read from rows of 48 heads: forward 73 us (4.6 TB/s), backward
+// 94 (5.3) and 4 of joining the weights' gradients; 1777 x 6 heads of 72 in fp32, pairs side by side 6 and 11.
 #include "../../include/dmuon_amd.h"
 #include "dmuon_amd_internal.h"
 #include "mfma_tile.h"
