@@ -348,8 +348,7 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
   };
   if (n > 0) fetch(0, lds);
   for (int t = 0; t < n; ++t) {
-    wait_vmcnt<0>();
-    bare_barrier();
+    slice_barrier<0>();                   // this tile has landed, the slot filled next has been read
     step(t, lds + (t & 1) * SLOT, lds + ((t & 1) ^ 1) * SLOT);
   }
   // keys past a sequence's own, up to the tensor's, have no gradient
@@ -480,8 +479,7 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
   };
   if (t0 < t1) fetch(t0, lds);
   for (int t = t0; t < t1; ++t) {
-    wait_vmcnt<0>();
-    bare_barrier();
+    slice_barrier<0>();                   // this tile has landed, the slot filled next has been read
     const int slot = (t - t0) & 1;
     step(t, lds + slot * 2 * TILE, lds + (slot ^ 1) * 2 * TILE);
   }

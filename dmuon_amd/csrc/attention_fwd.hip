@@ -183,8 +183,7 @@ void attention_kernel(const Attention a) {
   };
   if (t0 < t1) fetch(t0, lds);
   for (int t = t0; t < t1; ++t) {
-    wait_vmcnt<0>();
-    bare_barrier();
+    slice_barrier<0>();                   // this tile has landed, the slot filled next has been read
     const int slot = (t - t0) & 1;
     step(t, lds + slot * 2 * TILE, lds + (slot ^ 1) * 2 * TILE);
   }
