@@ -20,7 +20,7 @@ namespace dmuon {
 namespace {
 
 constexpr int kTile = 64;                 // rows or keys of a tile in LDS
-// fp16: blocks that look for the largest rows of do, and as many for those of v
+// fp16: at most so many blocks look for the largest rows of do, and as many for those of v
 constexpr int kPeakBlocks = kPeaks / 2;
 constexpr float kInf = __builtin_inff();
 
@@ -28,23 +28,28 @@ template <int E>
 constexpr float kShift = E == ELT_F16 ? 10.f : 0.f;
 
 // The power of two of dS: |dS| 2^kShift <= 2 |do| |v| 2^10 P times it stays under 2^15. Every block finds
-// the two maxima among the parts itself.
+// the two maxima among the parts itself. Returns its exponent.
 template <int E>
-__device__ __forceinline__ float ds_scale(const Attention& a) {
-  if constexpr (E != ELT_F16) return 1.f;
+__device__ __forceinline__ int ds_exponent(const Attention& a) {
+  if constexpr (E != ELT_F16) return 0;
   __shared__ float lds[2][4];
-  float x = a.peaks[threadIdx.x], y = a.peaks[kPeakBlocks + threadIdx.x];
+  float x = 0.f, y = 0.f;
+  for (int i = threadIdx.x; i < a.do_peaks + a.v_peaks; i += 256) {
+    const float peak = a.peaks[i];
+    if (i < a.do_peaks) x = fmaxf(x, peak);
+    else y = fmaxf(y, peak);
+  }
   for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o)), y = fmaxf(y, __shfl_xor(y, o));
   if ((threadIdx.x & 63) == 0) lds[0][threadIdx.x >> 6] = x, lds[1][threadIdx.x >> 6] = y;
   __syncthreads();
   x = fmaxf(fmaxf(lds[0][0], lds[0][1]), fmaxf(lds[0][2], lds[0][3]));
   y = fmaxf(fmaxf(lds[1][0], lds[1][1]), fmaxf(lds[1][2], lds[1][3]));
   const float most = 2.f * sqrtf(x) * sqrtf(y);
-  if (!(most > 0.f)) return 1.f;
-  int e = 5 - __builtin_amdgcn_frexp_expf(most);           // most < 2^frexp
-  e = e > 60 ? 60 : e < -60 ? -60 : e;
-  return __uint_as_float((unsigned)(127 + e) << 23);
+  if (!(most > 0.f)) return 0;
+  const int e = 5 - __builtin_amdgcn_frexp_expf(most);     // most < 2^frexp
+  return e > 60 ? 60 : e < -60 ? -60 : e;
 }
+__device__ __forceinline__ float power(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
 
 // A row's share of a transposed result: values result_row(i, h) of each 32
 template <int E, int DB>
@@ -96,7 +101,7 @@ struct RowMover {
 // A block's largest value
 __device__ __forceinline__ void block_peak(float most, float* peak) {
   __shared__ float lds[16];
-  for (int o = 16; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = most;
   __syncthreads();
   if (threadIdx.x) return;
@@ -105,18 +110,19 @@ __device__ __forceinline__ void block_peak(float most, float* peak) {
 }
 
 // What the products need besides: -delta of every row (of out and what its rounding left: all of a row's dS
-// share delta's error, which took dq's from 1.4 to 1.5 to 1.6 times its own rounding), and in fp16 the largest rows of do and v (blocks of
-// 1024 threads, kPeakBlocks for each; bf16: of 256 threads, 16 rows a block). 16 lanes a row, 8 values each.
-template <int E>
+// share delta's error, which took dq's from 1.4 to 1.5 to 1.6 times its own rounding), and in fp16 the largest
+// rows of do and v (blocks of 1024 threads, kPeakBlocks for each; bf16: of 256 threads, a row a group). L lanes
+// a row, 8 values each. Reading do, out and rest at 6.3 TB/s: 64 us for 2 x 8192 tokens of 32 heads of 128.
+template <int E, int L>
 __global__ __launch_bounds__(E == ELT_F16 ? 1024 : 256) void attention_delta_kernel(const Attention a) {
-  const int batch = a.seqs ? 1 : a.batch, at = 8 * (threadIdx.x & 15), group = threadIdx.x >> 4;
-  const int groups = blockDim.x >> 4;
+  const int batch = a.seqs ? 1 : a.batch, at = 8 * (threadIdx.x % L), group = threadIdx.x / L;
+  const int groups = blockDim.x / L;
   float most = 0.f;
-  if (E == ELT_F16 && blockIdx.x >= kPeakBlocks) {
+  if (E == ELT_F16 && (int)blockIdx.x >= a.do_peaks) {
     // rows of v among those that a query may see
     const long long rows = (long long)a.kv_len * a.kv_heads * batch;
-    for (long long row = (long long)(blockIdx.x - kPeakBlocks) * groups + group; row < rows;
-         row += (long long)kPeakBlocks * groups) {
+    for (long long row = (long long)((int)blockIdx.x - a.do_peaks) * groups + group; row < rows;
+         row += (long long)a.v_peaks * groups) {
       const long long token = row / a.kv_heads, b = token / a.kv_len, j = token - b * a.kv_len;
       const int head = (int)(row - token * a.kv_heads);
       bool live = true;
@@ -132,13 +138,13 @@ __global__ __launch_bounds__(E == ELT_F16 ? 1024 : 256) void attention_delta_ker
           n += f * f;
         }
       }
-      for (int o = 1; o < 16; o <<= 1) n += __shfl_xor(n, o);
+      for (int o = 1; o < L; o <<= 1) n += __shfl_xor(n, o);
       if (n < kInf) most = fmaxf(most, n);
     }
     return block_peak(most, a.peaks + blockIdx.x);
   }
   const long long rows = (long long)a.q_len * a.heads * batch;
-  const long long step = E == ELT_F16 ? (long long)kPeakBlocks * groups : rows;
+  const long long step = E == ELT_F16 ? (long long)a.do_peaks * groups : rows;
   for (long long row = (long long)blockIdx.x * groups + group; row < rows; row += step) {
     float s = 0.f, n = 0.f;
     if (at < a.dim) {
@@ -157,10 +163,10 @@ __global__ __launch_bounds__(E == ELT_F16 ? 1024 : 256) void attention_delta_ker
         n += f * f;
       }
     }
-    for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
-    if ((threadIdx.x & 15) == 0) a.delta[row] = -s;
+    for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o);
+    if (threadIdx.x % L == 0) a.delta[row] = -s;
     if constexpr (E == ELT_F16) {
-      for (int o = 1; o < 16; o <<= 1) n += __shfl_xor(n, o);
+      for (int o = 1; o < L; o <<= 1) n += __shfl_xor(n, o);
       // rows that see nothing, or of no numbers, do not count
       if (n < kInf && a.lse[row] < kInf) most = fmaxf(most, n);
     }
@@ -274,7 +280,7 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
     }
   };
   const int row_at = row_form<D>(lane), turn_at = turned_form<D>(lane);
-  const float sigma = ds_scale<E>(a);
+  const float sigma = power(ds_exponent<E>(a));
   f32x16_t dk[DB], dv[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b) dk[b] = dv[b] = f32x16_t{};
@@ -439,7 +445,9 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
     mv.issue(a.v + p.v_off + j0 * a.v_token, a.v_token, a.dim, p.kn - j0, to + TILE);
   };
   const int row_at = row_form<D>(lane), turn_at = turned_form<D>(lane);
-  const float sigma = ds_scale<E>(a);
+  // dS needs P times both powers of two, which the exponent takes in
+  const int up = ds_exponent<E>(a);
+  const float from = lse - (kShift<E> + (float)up);
   f32x16_t dq[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b) dq[b] = f32x16_t{};
@@ -459,8 +467,7 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        dp[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kShift<E> - lse)) *
-                (E == ELT_F16 ? (dp[i] + minus_delta) * sigma : dp[i] + minus_delta);
+        dp[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -from)) * (dp[i] + minus_delta);
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -484,7 +491,7 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
     step(t, lds + slot * 2 * TILE, lds + (slot ^ 1) * 2 * TILE);
   }
   constexpr float down = E == ELT_F16 ? 1.f / 1024.f : 1.f;
-  if (live) store_turned<E, DB>(a.dq + row * a.dim, dq, a.scale * down / sigma, h, a.dim);
+  if (live) store_turned<E, DB>(a.dq + row * a.dim, dq, a.scale * down * power(-up), h, a.dim);
 }
 
 // The keys' blocks come first: they take longer. Waves of a SIMD: two of dim 128 by their registers, three of
@@ -509,7 +516,7 @@ void launch_main(const Attention& a, long long key_blocks, long long query_block
 
 }  // namespace
 
-hipError_t launch_attention_grad(const Attention& a, hipStream_t stream) {
+hipError_t launch_attention_grad(Attention a, hipStream_t stream) {
   const long long batch = a.seqs ? 1 : a.batch;
   const long long rows = (long long)a.q_len * a.heads * batch, keys = (long long)a.kv_len * a.kv_heads * batch;
   const long long units = (long long)a.kv_heads * batch;
@@ -518,11 +525,22 @@ hipError_t launch_attention_grad(const Attention& a, hipStream_t stream) {
   if (rows / 16 > 0x7ffffff0LL || keys / 16 > 0x7ffffff0LL || key_blocks + query_blocks > 0x7ffffff0LL)
     return hipErrorInvalidValue;
   const bool f16 = a.dtype == DT_F16, wide = a.dim > 64;
-  if (f16)
-    hipLaunchKernelGGL((attention_delta_kernel<ELT_F16>), dim3(2 * kPeakBlocks), dim3(1024), 0, stream, a);
-  else if (rows > 0)
-    hipLaunchKernelGGL((attention_delta_kernel<ELT_BF16>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0,
-                       stream, a);
+  if (f16) {
+    const long long each = wide ? 64 : 128;                // rows of a block
+    a.do_peaks = (int)((rows + each - 1) / each < kPeakBlocks ? (rows + each - 1) / each : kPeakBlocks);
+    a.v_peaks = (int)((keys + each - 1) / each < kPeakBlocks ? (keys + each - 1) / each : kPeakBlocks);
+  }
+  const unsigned blocks = f16 ? a.do_peaks + a.v_peaks
+                              : (unsigned)(wide ? (rows + 15) / 16 : (rows + 31) / 32);
+#define DMUON_DELTA(E, L) \
+  hipLaunchKernelGGL((attention_delta_kernel<E, L>), dim3(blocks), dim3(f16 ? 1024 : 256), 0, stream, a)
+  if (blocks > 0) {
+    if (f16 && wide) DMUON_DELTA(ELT_F16, 16);
+    else if (f16) DMUON_DELTA(ELT_F16, 8);
+    else if (wide) DMUON_DELTA(ELT_BF16, 16);
+    else DMUON_DELTA(ELT_BF16, 8);
+  }
+#undef DMUON_DELTA
   if (f16) {
     if (wide) launch_main<ELT_F16, 128>(a, key_blocks, query_blocks, stream);
     else launch_main<ELT_F16, 64>(a, key_blocks, query_blocks, stream);
