@@ -154,6 +154,19 @@ __device__ __forceinline__ bf16x8_t read_turned(const char* lds, int at) {
   return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// A result's 32 rows (keys, or queries' rows) from `at` on, of which those under `end` or from `begin` on stay and
+// the others become `off`: a comparison with a constant and a selection a value.
+__device__ __forceinline__ void cut_end(f32x16_t& s, int at, int end, int h, float off) {
+  const int stay = end - at - 4 * h;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = result_row(i, 0) < stay ? s[i] : off;
+}
+__device__ __forceinline__ void cut_begin(f32x16_t& s, int at, int begin, int h, float off) {
+  const int stay = begin - at - 4 * h;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = result_row(i, 0) >= stay ? s[i] : off;
+}
+
 // Registers from .. from + 7 of a result, rounded: one k step of the next product's operand
 template <int E>
 __device__ __forceinline__ bf16x8_t pack8(const f32x16_t& v, int from) {

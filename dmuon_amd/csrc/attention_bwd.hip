@@ -290,7 +290,7 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
     const float* stats = reinterpret_cast<const float*>(qt + 2 * TILE);
     if (t + 1 < n) fetch(t + 1, next);
     const int r0 = first_row(t);
-    const bool masked = r0 < full_lo || r0 + kTile > full_hi;
+    const bool early = r0 < full_lo, late = r0 + kTile > full_hi;
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
       // the reads' addresses are formed anew each time: held over the loop they would take the registers
@@ -308,13 +308,8 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
         for (int e = 0; e < 4; ++e)
           s[i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + e], a.c, kShift<E> - lse[e]));
       }
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = r0 + 32 * y + result_row(i, h);
-          s[i] = r >= lo && r < hi ? s[i] : 0.f;
-        }
-      }
+      if (early) cut_begin(s, r0 + 32 * y, lo, h, 0.f);
+      if (late) cut_end(s, r0 + 32 * y, hi, h, 0.f);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const bf16x8_t pf = pack8<E>(s, 8 * u);
@@ -335,14 +330,9 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
         dp = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(dt + y * 64 * D + (ra ^ (32 * k))), vf[k], dp);
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] = s[i] * (E == ELT_F16 ? dp[i] * sigma : dp[i]);
-      if (masked) {
-        // rows that do not see the key have no share, whatever their dout holds
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = r0 + 32 * y + result_row(i, h);
-          dp[i] = r >= lo && r < hi ? dp[i] : 0.f;
-        }
-      }
+      // rows that do not see the key have no share, whatever their dout holds
+      if (early) cut_begin(dp, r0 + 32 * y, lo, h, 0.f);
+      if (late) cut_end(dp, r0 + 32 * y, hi, h, 0.f);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const bf16x8_t sf = pack8<E>(dp, 8 * u);
@@ -455,7 +445,6 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
     const char* vt = kt + TILE;
     if (t + 1 < t1) fetch(t + 1, next);
     const int j0 = t * kTile;
-    const bool masked = j0 < full_lo || j0 + kTile > full_hi;
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
       f32x16_t s = {}, dp = {};
@@ -468,13 +457,8 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         dp[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -from)) * (dp[i] + minus_delta);
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = j0 + 32 * y + result_row(i, h);
-          dp[i] = j >= see.lo && j < see.hi ? dp[i] : 0.f;
-        }
-      }
+      if (j0 + kTile > full_hi) cut_end(dp, j0 + 32 * y, see.hi, h, 0.f);
+      if (j0 < full_lo) cut_begin(dp, j0 + 32 * y, see.lo, h, 0.f);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const bf16x8_t sf = pack8<E>(dp, 8 * u);

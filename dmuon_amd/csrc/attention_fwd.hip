@@ -140,14 +140,13 @@ void attention_kernel(const Attention a) {
     }
     __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
     const int j0 = t * kKeys;
-    if (j0 < full_lo || j0 + kKeys > full_hi) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = j0 + 32 * b + result_row(i, h);
-          s[b][i] = j >= see.lo && j < see.hi ? s[b][i] : -kInf;
-        }
+    if (j0 + kKeys > full_hi) {
+      cut_end(s[0], j0, see.hi, h, -kInf);
+      cut_end(s[1], j0 + 32, see.hi, h, -kInf);
+    }
+    if (j0 < full_lo) {
+      cut_begin(s[0], j0, see.lo, h, -kInf);
+      cut_begin(s[1], j0 + 32, see.lo, h, -kInf);
     }
     float top = -kInf;
 #pragma unroll
@@ -254,13 +253,8 @@ __global__ __launch_bounds__(64) void attention_few_kernel(const Attention a) {
     asm volatile("" : "+v"(s) : : "memory");
     if (more) fetch_k(t + 2, k_next);
     const int j0 = t * KEYS;
-    if (j0 < full_lo || j0 + KEYS > full_hi) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int j = j0 + result_row(i, h);
-        s[i] = j >= see.lo && j < see.hi ? s[i] : -kInf;
-      }
-    }
+    if (j0 + KEYS > full_hi) cut_end(s, j0, see.hi, h, -kInf);
+    if (j0 < full_lo) cut_begin(s, j0, see.lo, h, -kInf);
     float top = -kInf;
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
