@@ -244,6 +244,13 @@ __device__ __forceinline__ Sight sight_of(const Attention& a, const Place& p, in
   return s;
 }
 
+// What any of the 32 rows from `first` on sees: a wave passes over the other tiles of its block.
+__device__ __forceinline__ Sight wave_sight(const Attention& a, const Place& p, int first, int rows) {
+  if (first >= rows) return Sight{0, 0};
+  const int last = first + 31 < rows ? first + 31 : rows - 1;
+  return Sight{sight_of(a, p, first / a.group).lo, sight_of(a, p, last / a.group).hi};
+}
+
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // rows and keys of a block's tile; rows of one wave that works alone

@@ -222,6 +222,16 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
   // rows that see every key of the block need no mask
   const int full_lo = last_lo * a.group;
   const int full_hi = last_key == j0 + kKeyRows - 1 ? first_hi * a.group : 0;
+  // rows that see any of this wave's keys: it passes over the other tiles
+  const int j_first = j0 + wave * 32, j_last = j_first + 31 < p.kn ? j_first + 31 : p.kn - 1;
+  int mine_lo = 0, mine_hi = 0;
+  if (j_first < p.kn) {
+    int unused;
+    rows_of(j_first, &mine_lo, &unused);
+    rows_of(j_last, &unused, &mine_hi);
+    mine_lo *= a.group;
+    mine_hi = mine_hi > 0 ? mine_hi * a.group : 0;
+  }
   // tiles of whole queries; a part of them where the rows are split
   const int tr = tile_rows(a.group);
   int n = r_hi > r_lo && j0 < p.kn ? (r_hi - r_lo + tr - 1) / tr : 0, end = n;
@@ -290,6 +300,7 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
     const float* stats = reinterpret_cast<const float*>(qt + 2 * TILE);
     if (t + 1 < n) fetch(t + 1, next);
     const int r0 = first_row(t);
+    if (r0 >= mine_hi || r0 + kTile <= mine_lo) return;
     const bool early = r0 < full_lo, late = r0 + kTile > full_hi;
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
@@ -425,6 +436,7 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
   const Sight first = sight_of(a, p, r0 / a.group), last = sight_of(a, p, last_row / a.group);
   const int t0 = first.lo / kTile, t1 = (last.hi + kTile - 1) / kTile;
   const int full_lo = last.lo, full_hi = last_row == r0 + kQueryRows - 1 ? first.hi : 0;
+  const Sight mine = wave_sight(a, p, r0 + wave * 32, rows);
 
   TileMover<D, kTile, 4> mk, mv;
   mk.init(a.k_token, a.dim, wave, lane);
@@ -445,6 +457,7 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
     const char* vt = kt + TILE;
     if (t + 1 < t1) fetch(t + 1, next);
     const int j0 = t * kTile;
+    if (j0 >= mine.hi || j0 + kTile <= mine.lo) return;
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
       f32x16_t s = {}, dp = {};

@@ -102,6 +102,7 @@ void attention_kernel(const Attention a) {
     t0 = t0 + p.split * each < t1 ? t0 + p.split * each : t1;
     t1 = t0 + each < t1 ? t0 + each : t1;
   }
+  const Sight mine = wave_sight(a, p, r0 + wave * 32, rows);
   // keys that every row sees need no mask
   const int full_lo = last.lo, full_hi = last_row == r0 + kQueryRows - 1 ? first.hi : 0;
 
@@ -123,6 +124,8 @@ void attention_kernel(const Attention a) {
   auto step = [&](int t, const char* __restrict__ kt, char* __restrict__ next) __attribute__((always_inline)) {
     const char* vt = kt + TILE;
     if (t + 1 < t1) fetch(t + 1, next);
+    const int j0 = t * kKeys;
+    if (j0 >= mine.hi || j0 + kKeys <= mine.lo) return;
     f32x16_t s[2] = {};
 #pragma unroll
     for (int k = 0; k < KS; ++k)
@@ -139,7 +142,6 @@ void attention_kernel(const Attention a) {
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
-    const int j0 = t * kKeys;
     if (j0 + kKeys > full_hi) {
       cut_end(s[0], j0, see.hi, h, -kInf);
       cut_end(s[1], j0 + 32, see.hi, h, -kInf);
