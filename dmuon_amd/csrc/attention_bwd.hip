@@ -6,8 +6,8 @@
 // Where the keys' blocks are few their rows are split, and a second kernel joins the parts in their order.
 //
 // Bound like the forward pass: 2 x 8192 causal tokens, 32/8 heads of 128, bf16 3.5 ms (1.1 PFLOP/s of the seven
-// products, 0.78 of five); 16384 packed tokens in 23 documents 0.64 ms; 8191 tokens of 16 heads of 64 in a
-// window of 1024 in fp16 170 us. The key blocks' sums (dk and dv of 32 keys a wave) and operands take 192 of
+// products, 0.78 of five); 16384 packed tokens in 23 documents 0.62 ms; 8191 tokens of 16 heads of 64 in a
+// window of 1024 in fp16 160 us. The key blocks' sums (dk and dv of 32 keys a wave) and operands take 192 of
 // 256 registers; a third of what they read from LDS is turned on the way (transposing reads).
 //
 // P and dS are rounded to the operands' type between the products. In fp16 they are held times powers of

@@ -7,8 +7,8 @@
 //
 // 4 dim operations a pair of a query and a key on the matrix pipe, some five on the vector one. At dim 128
 // bound by the matrix pipe under the board's power limit (busy 56% of the cycles at 1.8 of 2.4 GHz): 2 x 8192
-// causal tokens, 32/8 heads, bf16 1.04 ms (1.06 PFLOP/s); 2047 tokens over 32768 keys 1.04 ms (1.02). At dim 64
-// by the vector pipe: 8191 tokens of 16 heads in a window of 1024 in fp16 63 us (0.52). Single tokens by
+// causal tokens, 32/8 heads, bf16 1.04 ms (1.06 PFLOP/s); 2047 tokens over 32768 keys 1.02 ms (1.04). At dim 64
+// by the vector pipe: 8191 tokens of 16 heads in a window of 1024 in fp16 57 us (0.57). Single tokens by
 // reading the cache: 48 x 1 over up to 8192 keys 157 us (6.5 TB/s). A tile of 64 keys lies in LDS twice, one
 // copy read while the other is loaded; keys go through LDS since all waves read them, queries stay in
 // registers. 64 rows a wave (half the reads, one wave a SIMD) took 1.44 ms.
