@@ -358,6 +358,53 @@ def test_calls_at_once(gpu):
 
 
 @pytest.mark.gpu
+def test_a_cache_that_grows_under_a_graph(gpu):
+    """One captured call of a decoding loop: the token, the cache and its lengths change between replays."""
+    b, room, h, hk, d = 3, 200, 8, 2, 64
+    q, k, v, _ = _make(gpu, (b, 1, h, d), (b, room, hk, d), torch.bfloat16, 50)
+    lengths = torch.tensor([0, 63, 199], device=gpu)
+    with torch.no_grad():
+        dmuon.attention(q, k, v, kv_lengths=lengths)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = dmuon.attention(q, k, v, kv_lengths=lengths)
+        for step in range(4):
+            q.copy_(_make(gpu, (b, 1, h, d), (b, 1, hk, d), torch.bfloat16, 60 + step)[0])
+            lengths += 1
+            graph.replay()
+            torch.cuda.synchronize()
+            n = lengths.clamp(max=room).tolist()
+            _check([held], [((i,), (i, slice(0, m))) for i, m in enumerate(n)], q, k, v, None, True, None)
+            assert torch.equal(held, dmuon.attention(q, k, v, kv_lengths=lengths))
+
+
+@pytest.mark.gpu
+def test_a_kept_graph_gives_its_gradients_again(gpu):
+    q, k, v, do = _make(gpu, (1, 90, 4, 64), (1, 90, 2, 64), torch.float16, 51)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = dmuon.attention(*leaves)
+    first = torch.autograd.grad(out, leaves, do, retain_graph=True)
+    # a sum's gradient is one value seen everywhere
+    torch.autograd.grad(out.sum(), leaves, retain_graph=True)
+    again = torch.autograd.grad(out, leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    ones = _grads(q, k, v, torch.ones_like(do))
+    seen = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    total = torch.autograd.grad(dmuon.attention(*seen).sum(), seen)
+    assert all(torch.equal(a, b) for a, b in zip(total, ones[1:]))
+
+
+@pytest.mark.gpu
+def test_one_tensor_in_all_places(gpu):
+    x, _, _, do = _make(gpu, (1, 70, 2, 64), (1, 70, 2, 64), torch.bfloat16, 52)
+    one = x.clone().requires_grad_(True)
+    (got,) = torch.autograd.grad(dmuon.attention(one, one, one), one, do)
+    parts = _grads(x, x, x, do)[1:]
+    assert torch.equal(got, parts[0] + parts[1] + parts[2]) or \
+        torch.equal(got, parts[2] + parts[1] + parts[0]) or torch.equal(got, parts[0] + parts[2] + parts[1])
+
+
+@pytest.mark.gpu
 def test_operands_written_to_in_between_are_refused(gpu):
     q, k, v, do = _make(gpu, (1, 10, 2, 64), (1, 10, 2, 64), torch.bfloat16)
     for i in range(3):

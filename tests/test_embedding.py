@@ -201,6 +201,32 @@ def test_tokens_written_to_in_between_and_second_gradients_are_refused(gpu):
         y.backward(dy)
 
 
+class _Wrapped(torch.Tensor):
+    """A tensor that holds another and has no memory itself, as distributed tensors do."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype,
+                                                   device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        out = func(*(t.inner if isinstance(t, _Wrapped) else t for t in args), **(kwargs or {}))
+        return _Wrapped(out) if isinstance(out, torch.Tensor) else out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 1])
+def test_tensors_without_memory_are_refused(gpu, which):
+    ops = list(_make(gpu, 20, 30, 64, torch.float32)[:2])
+    ops[which] = _Wrapped(ops[which])
+    with pytest.raises(RuntimeError, match="memory"):
+        dmuon.embedding(*ops)
+
+
 def _refuse(match, *args, kind=ValueError, **kw):
     with pytest.raises(kind, match=match):
         dmuon.embedding(*args, **kw)

@@ -283,6 +283,47 @@ def test_no_second_gradient(gpu):
         torch.autograd.grad(_call(v, p, f)[0], v["q"], outs[0], create_graph=True)
 
 
+class _Wrapped(torch.Tensor):
+    """A tensor that holds another and has no memory itself, as distributed tensors do."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype,
+                                                   device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        out = func(*(t.inner if isinstance(t, _Wrapped) else t for t in args), **(kwargs or {}))
+        return _Wrapped(out) if isinstance(out, torch.Tensor) else out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["q", "k", "q_weight", "k_weight", "positions", "inv_freq"])
+def test_tensors_without_memory_are_refused(gpu, which):
+    v, p, f, _ = _make(gpu, (5,), 2, 1, 64, 48, torch.float32, torch.float32)
+    v.update(positions=p, inv_freq=f)
+    v[which] = _Wrapped(v[which])
+    with pytest.raises(RuntimeError, match="memory"):
+        _call(v, v["positions"], v["inv_freq"])
+
+
+@pytest.mark.gpu
+def test_operands_written_to_in_between_are_refused(gpu):
+    v, p, f, outs = _make(gpu, (5,), 2, 1, 64, 48, torch.float32, torch.float32)
+    for which in ("q", "q_weight", "positions"):
+        leaves = {k: t.clone().requires_grad_(True) for k, t in v.items()}
+        held = {k: t * 1 for k, t in leaves.items()}
+        spots = p.clone()
+        y = _call(held, spots, f)
+        with torch.no_grad():
+            (spots if which == "positions" else held[which]).mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.backward(y, outs)
+
+
 def _refuse(match, *args, kind=ValueError, **kw):
     with pytest.raises(kind, match=match):
         dmuon.rotary_heads(*args, **kw)
