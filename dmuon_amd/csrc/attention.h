@@ -42,10 +42,8 @@ struct Attention {
   int few;                                // tiles of kFewRows rows, each wave alone
   float* part; float2* part_stats;        // [splits][tokens][heads][dim] sums, [..][2] (reference, sum)
   // gradients: tiles of keys of one (sequence, key head) (packed: of one key head), parts of their rows and
-  // [key_splits][key tokens][kv_heads][2][dim] dk and dv of each; fp16: do_peaks blocks' largest |dout row|^2
-  // and v_peaks blocks' largest |v row|^2
-  int key_tiles, key_splits, do_peaks, v_peaks;
-  float* peaks;
+  // [key_splits][key tokens][kv_heads][2][dim] dk and dv of each
+  int key_tiles, key_splits;
 };
 
 // Where a block works: its sequence's tokens, pointers' offsets and the tile's number
@@ -255,12 +253,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 // rows and keys of a block's tile; rows of one wave that works alone
 constexpr int kQueryRows = 128, kKeyRows = 128, kFewRows = 32;
-constexpr int kPeaks = 1024;              // floats in `peaks`
 // the tables of a packed call; tiles of `rows` rows
 hipError_t launch_attention_tables(const Attention& a, const int64_t* q_starts, const int64_t* kv_starts,
                                    int q_rows, int k_rows, Sequence* seqs, int2* q_tiles, int2* k_tiles,
                                    int* counts, hipStream_t stream);
 hipError_t launch_attention(const Attention& a, hipStream_t stream);
-hipError_t launch_attention_grad(Attention a, hipStream_t stream);
+hipError_t launch_attention_grad(const Attention& a, hipStream_t stream);
 
 }  // namespace dmuon

@@ -177,7 +177,6 @@ Plan plan_grad(const dmuon_attention_args& a, void* ws) {
   p.t = tables(&p.a, a, &c);
   const int64_t batch = packed ? 1 : a.batch;
   p.a.delta = c.take<float>(a.q_len * a.heads * batch);
-  p.a.peaks = c.take<float>(kPeaks);
   p.a.key_tiles = (int)tiles_of(p.a, packed, p.a.kv_len, kKeyRows);
   p.a.key_splits = key_splits_of(p.a, packed);
   if (p.a.key_splits > 1) p.a.part = c.take<float>(p.a.key_splits * a.kv_len * a.kv_heads * batch * 2 * a.dim);

@@ -11,43 +11,35 @@
 // 256 registers; a third of what they read from LDS is turned on the way (transposing reads).
 //
 // P and dS are rounded to the operands' type between the products. In fp16 they are held times powers of
-// two: P times 2^10 (a long row's probabilities are under the type's normal range) and dS by a further one
-// that the largest rows of do and v set, so that it neither over- nor underflows with a loss scale or a
-// row's length.
+// two: P times 2^10 (a long row's probabilities are under the type's normal range) and dS by one that follows
+// the largest dS so far of a row (blocks over queries) or of a key (blocks over keys), so that it neither over-
+// nor underflows with a loss scale, a row's length or what other rows and sequences hold.
 #include "attention.h"
 
 namespace dmuon {
 namespace {
 
 constexpr int kTile = 64;                 // rows or keys of a tile in LDS
-// fp16: at most so many blocks look for the largest rows of do, and as many for those of v
-constexpr int kPeakBlocks = kPeaks / 2;
 constexpr float kInf = __builtin_inff();
 
 template <int E>
 constexpr float kShift = E == ELT_F16 ? 10.f : 0.f;
 
-// The power of two of dS: |dS| 2^kShift <= 2 |do| |v| 2^10 P times it stays under 2^15. Every block finds
-// the two maxima among the parts itself. Returns its exponent.
-template <int E>
-__device__ __forceinline__ int ds_exponent(const Attention& a) {
-  if constexpr (E != ELT_F16) return 0;
-  __shared__ float lds[2][4];
-  float x = 0.f, y = 0.f;
-  for (int i = threadIdx.x; i < a.do_peaks + a.v_peaks; i += 256) {
-    const float peak = a.peaks[i];
-    if (i < a.do_peaks) x = fmaxf(x, peak);
-    else y = fmaxf(y, peak);
-  }
-  for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o)), y = fmaxf(y, __shfl_xor(y, o));
-  if ((threadIdx.x & 63) == 0) lds[0][threadIdx.x >> 6] = x, lds[1][threadIdx.x >> 6] = y;
-  __syncthreads();
-  x = fmaxf(fmaxf(lds[0][0], lds[0][1]), fmaxf(lds[0][2], lds[0][3]));
-  y = fmaxf(fmaxf(lds[1][0], lds[1][1]), fmaxf(lds[1][2], lds[1][3]));
-  const float most = 2.f * sqrtf(x) * sqrtf(y);
-  if (!(most > 0.f)) return 0;
-  const int e = 5 - __builtin_amdgcn_frexp_expf(most);     // most < 2^frexp
-  return e > 60 ? 60 : e < -60 ? -60 : e;
+// fp16's dS is held times 2^60 until its largest magnitude reaches 2^15; then, and whenever it does so again,
+// times the power that brings it to 2^13 .. 2^14. That costs one maximum of the values at hand, and the sums
+// are multiplied (exactly) where the power falls. 2^-38 of the largest is then the least error that is not
+// relative; dS under 2^-47 in all of a row is lost to fp16's results anyway. In fp32 dS 2^70 < 2^112.
+constexpr float kFull = 32768.f;
+constexpr int kFirstPower = 60;
+// The exponent that a row's (key's) powers change by, 0 where `v`, this lane's 16 of its 32 values, has room
+__device__ __forceinline__ int power_step(const f32x16_t& v, bool* any) {
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i]));
+  most = half_max(most);
+  *any = __ballot(most >= kFull) != 0;
+  // most < 2^frexp; infinities stay what they are
+  return most >= kFull && most < kInf ? 14 - __builtin_amdgcn_frexp_expf(most) : 0;
 }
 __device__ __forceinline__ float power(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
 
@@ -98,80 +90,32 @@ struct RowMover {
   }
 };
 
-// A block's largest value
-__device__ __forceinline__ void block_peak(float most, float* peak) {
-  __shared__ float lds[16];
-  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = most;
-  __syncthreads();
-  if (threadIdx.x) return;
-  for (int w = 1; w < (int)blockDim.x >> 6; ++w) most = fmaxf(most, lds[w]);
-  *peak = most;
-}
-
 // What the products need besides: -delta of every row (of out and what its rounding left: all of a row's dS
-// share delta's error, which took dq's from 1.4 to 1.5 to 1.6 times its own rounding), and in fp16 the largest
-// rows of do and v (blocks of 1024 threads, kPeakBlocks for each; bf16: of 256 threads, a row a group). L lanes
-// a row, 8 values each. Reading do, out and rest at 6.3 TB/s: 64 us for 2 x 8192 tokens of 32 heads of 128.
+// share delta's error, which took dq's from 1.4 to 1.5 to 1.6 times its own rounding). L lanes a row, 8 values
+// each. Reading do, out and rest at 6.3 TB/s: 64 us for 2 x 8192 tokens of 32 heads of 128.
 template <int E, int L>
-__global__ __launch_bounds__(E == ELT_F16 ? 1024 : 256) void attention_delta_kernel(const Attention a) {
-  const int batch = a.seqs ? 1 : a.batch, at = 8 * (threadIdx.x % L), group = threadIdx.x / L;
-  const int groups = blockDim.x / L;
-  float most = 0.f;
-  if (E == ELT_F16 && (int)blockIdx.x >= a.do_peaks) {
-    // rows of v among those that a query may see
-    const long long rows = (long long)a.kv_len * a.kv_heads * batch;
-    for (long long row = (long long)((int)blockIdx.x - a.do_peaks) * groups + group; row < rows;
-         row += (long long)a.v_peaks * groups) {
-      const long long token = row / a.kv_heads, b = token / a.kv_len, j = token - b * a.kv_len;
-      const int head = (int)(row - token * a.kv_heads);
-      bool live = true;
-      if (a.kv_lengths) live = j < a.kv_lengths[b];
-      if (a.seqs) live = j >= a.seqs[a.batch + 2].kn && j < a.seqs[a.batch + 3].k0;
-      float n = 0.f;
-      if (live && at < a.dim) {
-        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(
-            a.v + b * a.v_batch + j * a.v_token + head * a.v_head + at);
+__global__ __launch_bounds__(256) void attention_delta_kernel(const Attention a) {
+  const int at = 8 * (threadIdx.x % L);
+  const long long rows = (long long)a.q_len * a.heads * (a.seqs ? 1 : a.batch);
+  const long long row = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+  if (row >= rows) return;
+  float s = 0.f;
+  if (at < a.dim) {
+    const long long token = row / a.heads, b = a.seqs ? 0 : token / a.q_len;
+    const int head = (int)(row - token * a.heads);
+    const uint16_t* d = a.dout + b * a.do_batch + (token - b * a.q_len) * a.do_token + head * a.do_head + at;
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(d);
+    const u32x4_t y = *reinterpret_cast<const u32x4_t*>(a.out + row * a.dim + at);
+    u32x4_t z = {};
+    if (a.rest) z = *reinterpret_cast<const u32x4_t*>(a.rest + row * a.dim + at);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float f = from_elt<ELT_F16>((uint16_t)(i & 1 ? x[i / 2] >> 16 : x[i / 2]));
-          n += f * f;
-        }
-      }
-      for (int o = 1; o < L; o <<= 1) n += __shfl_xor(n, o);
-      if (n < kInf) most = fmaxf(most, n);
-    }
-    return block_peak(most, a.peaks + blockIdx.x);
-  }
-  const long long rows = (long long)a.q_len * a.heads * batch;
-  const long long step = E == ELT_F16 ? (long long)a.do_peaks * groups : rows;
-  for (long long row = (long long)blockIdx.x * groups + group; row < rows; row += step) {
-    float s = 0.f, n = 0.f;
-    if (at < a.dim) {
-      const long long token = row / a.heads, b = a.seqs ? 0 : token / a.q_len;
-      const int head = (int)(row - token * a.heads);
-      const uint16_t* d = a.dout + b * a.do_batch + (token - b * a.q_len) * a.do_token + head * a.do_head + at;
-      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(d);
-      const u32x4_t y = *reinterpret_cast<const u32x4_t*>(a.out + row * a.dim + at);
-      u32x4_t z = {};
-      if (a.rest) z = *reinterpret_cast<const u32x4_t*>(a.rest + row * a.dim + at);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        auto value = [&](const u32x4_t& w) { return from_elt<E>((uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2])); };
-        const float f = value(x);
-        s += f * (value(y) + value(z));
-        n += f * f;
-      }
-    }
-    for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o);
-    if (threadIdx.x % L == 0) a.delta[row] = -s;
-    if constexpr (E == ELT_F16) {
-      for (int o = 1; o < L; o <<= 1) n += __shfl_xor(n, o);
-      // rows that see nothing, or of no numbers, do not count
-      if (n < kInf && a.lse[row] < kInf) most = fmaxf(most, n);
+    for (int i = 0; i < 8; ++i) {
+      auto value = [&](const u32x4_t& w) { return from_elt<E>((uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2])); };
+      s += value(x) * (value(y) + value(z));
     }
   }
-  if constexpr (E == ELT_F16) block_peak(most, a.peaks + blockIdx.x);
+  for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o);
+  if (threadIdx.x % L == 0) a.delta[row] = -s;
 }
 
 // dk and dv of 128 keys, 32 a wave and one a lane: S = Q K^T and dP = dO V^T leave a lane 16 rows of every
@@ -290,7 +234,7 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
     }
   };
   const int row_at = row_form<D>(lane), turn_at = turned_form<D>(lane);
-  const float sigma = power(ds_exponent<E>(a));
+  float sigma = E == ELT_F16 ? power(kFirstPower) : 1.f;
   f32x16_t dk[DB], dv[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b) dk[b] = dv[b] = f32x16_t{};
@@ -344,6 +288,17 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
       // rows that do not see the key have no share, whatever their dout holds
       if (early) cut_begin(dp, r0 + 32 * y, lo, h, 0.f);
       if (late) cut_end(dp, r0 + 32 * y, hi, h, 0.f);
+      if constexpr (E == ELT_F16) {
+        bool any;
+        const int by = power_step(dp, &any);
+        if (any) {
+          const float f = power(by);
+          sigma *= f;
+          dp *= f;
+#pragma unroll
+          for (int b = 0; b < DB; ++b) dk[b] *= f;
+        }
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const bf16x8_t sf = pack8<E>(dp, 8 * u);
@@ -447,9 +402,9 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
     mv.issue(a.v + p.v_off + j0 * a.v_token, a.v_token, a.dim, p.kn - j0, to + TILE);
   };
   const int row_at = row_form<D>(lane), turn_at = turned_form<D>(lane);
-  // dS needs P times both powers of two, which the exponent takes in
-  const int up = ds_exponent<E>(a);
-  const float from = lse - (kShift<E> + (float)up);
+  // the exponent takes in dS's power of two
+  int up = E == ELT_F16 ? kFirstPower : 0;
+  float from = lse - (float)up;
   f32x16_t dq[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b) dq[b] = f32x16_t{};
@@ -472,6 +427,18 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
         dp[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -from)) * (dp[i] + minus_delta);
       if (j0 + kTile > full_hi) cut_end(dp, j0 + 32 * y, see.hi, h, 0.f);
       if (j0 < full_lo) cut_begin(dp, j0 + 32 * y, see.lo, h, 0.f);
+      if constexpr (E == ELT_F16) {
+        bool any;
+        const int by = power_step(dp, &any);
+        if (any) {
+          const float f = power(by);
+          up += by;
+          from = lse - (float)up;
+          dp *= f;
+#pragma unroll
+          for (int b = 0; b < DB; ++b) dq[b] *= f;
+        }
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const bf16x8_t sf = pack8<E>(dp, 8 * u);
@@ -487,8 +454,7 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
     const int slot = (t - t0) & 1;
     step(t, lds + slot * 2 * TILE, lds + (slot ^ 1) * 2 * TILE);
   }
-  constexpr float down = E == ELT_F16 ? 1.f / 1024.f : 1.f;
-  if (live) store_turned<E, DB>(a.dq + row * a.dim, dq, a.scale * down * power(-up), h, a.dim);
+  if (live) store_turned<E, DB>(a.dq + row * a.dim, dq, a.scale * power(-up), h, a.dim);
 }
 
 // The keys' blocks come first: they take longer. Waves of a SIMD: two of dim 128 by their registers, three of
@@ -513,7 +479,7 @@ void launch_main(const Attention& a, long long key_blocks, long long query_block
 
 }  // namespace
 
-hipError_t launch_attention_grad(Attention a, hipStream_t stream) {
+hipError_t launch_attention_grad(const Attention& a, hipStream_t stream) {
   const long long batch = a.seqs ? 1 : a.batch;
   const long long rows = (long long)a.q_len * a.heads * batch, keys = (long long)a.kv_len * a.kv_heads * batch;
   const long long units = (long long)a.kv_heads * batch;
@@ -522,15 +488,9 @@ hipError_t launch_attention_grad(Attention a, hipStream_t stream) {
   if (rows / 16 > 0x7ffffff0LL || keys / 16 > 0x7ffffff0LL || key_blocks + query_blocks > 0x7ffffff0LL)
     return hipErrorInvalidValue;
   const bool f16 = a.dtype == DT_F16, wide = a.dim > 64;
-  if (f16) {
-    const long long each = wide ? 64 : 128;                // rows of a block
-    a.do_peaks = (int)((rows + each - 1) / each < kPeakBlocks ? (rows + each - 1) / each : kPeakBlocks);
-    a.v_peaks = (int)((keys + each - 1) / each < kPeakBlocks ? (keys + each - 1) / each : kPeakBlocks);
-  }
-  const unsigned blocks = f16 ? a.do_peaks + a.v_peaks
-                              : (unsigned)(wide ? (rows + 15) / 16 : (rows + 31) / 32);
+  const unsigned blocks = (unsigned)(wide ? (rows + 15) / 16 : (rows + 31) / 32);
 #define DMUON_DELTA(E, L) \
-  hipLaunchKernelGGL((attention_delta_kernel<E, L>), dim3(blocks), dim3(f16 ? 1024 : 256), 0, stream, a)
+  hipLaunchKernelGGL((attention_delta_kernel<E, L>), dim3(blocks), dim3(256), 0, stream, a)
   if (blocks > 0) {
     if (f16 && wide) DMUON_DELTA(ELT_F16, 16);
     else if (f16) DMUON_DELTA(ELT_F16, 8);

@@ -557,3 +557,71 @@ def test_tangents_and_tracers_are_refused(dev):
         torch.jit.trace(lambda *x: dmuon.attention(*x), tuple(v), check_trace=False)
     with pytest.raises(RuntimeError, match="tracer"):
         make_fx(lambda *x: dmuon.attention(*x))(*v)
+
+
+def _own_peaks(q, k, v, do, causal):
+    """[tokens, heads, dim] of one sequence as many heads as key heads in fp16, where dS is held times a power
+    of two of its own for each row (dq) and each key (dk): (dq, dk) and their bounds. A row's (a key's) dS is at
+    most ``2 |do| max|v|`` over what it has to do with, and is held with an absolute error of at most 2^-38 of
+    its largest one (2^-25 under the normal range, where the largest has reached 2^13)."""
+    d, scale, u = q.shape[-1], q.shape[-1] ** -0.5, U[torch.float16]
+    want, bound = ([], []), ([], [])
+    for h in range(q.shape[1]):
+        x = [t[:, h].double() for t in (q, k, v, do)]
+        (_, dq, dk, _), (_, bq, bk, _) = _one_head(*x, scale, causal, None, 0.0)
+        seen = torch.ones(q.shape[0], k.shape[0], dtype=torch.bool, device=q.device)
+        if causal:
+            seen = seen.tril(k.shape[0] - q.shape[0])
+        most = seen * (2 * x[3].norm(dim=1)[:, None] * x[2].norm(dim=1).max())
+        bq = bq + scale * 2.0 ** -38 * (most.amax(1, keepdim=True) * (seen.double() @ x[1].abs()))
+        bk = bk + scale * 2.0 ** -38 * (most.amax(0)[:, None] * (seen.double().t() @ x[0].abs()))
+        for pair, add in ((want, (dq, dk)), (bound, (bq, bk))):
+            for to, t in zip(pair, add):
+                to.append(t)
+    return tuple(tuple(torch.stack(t, 1) for t in pair) for pair in (want, bound))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("packed", [True, False])
+def test_gradients_of_one_sequence_do_not_depend_on_another(gpu, packed, d):
+    """fp16 gradients 2^24 apart, as of losses that are averaged over documents of very different lengths."""
+    n, dt = 200, torch.float16
+    q, k, v, do = _make(gpu, (2, n, 2, d), (2, n, 2, d), dt, 70)
+    do[0] *= 4096
+    do[1] *= 2.0 ** -12
+    kw = {}
+    if packed:
+        q, k, v, do = (t.flatten(0, 1) for t in (q, k, v, do))
+        kw = {"q_starts": torch.tensor([0, n, 2 * n], device=gpu)}
+        kw["kv_starts"] = kw["q_starts"]
+    halves = lambda t: t.reshape(2, n, 2, d)
+    got = [halves(t) for t in _grads(q, k, v, do, **kw)]
+    for i in range(2):
+        want, bound = _own_peaks(*(halves(t)[i] for t in (q, k, v, do)), True)
+        for name, g, w, b in zip(("dq", "dk"), got[1:], want, bound):
+            _within(f"{name} of sequence {i}", g[i], w, b, dt)
+    # the first one's values and gradients are nothing to the second one
+    first = slice(0, n) if packed else 0
+    other_v, other_do = v.clone(), do.clone()
+    other_v[first] *= 16
+    other_do[first] = 0
+    again = [halves(t) for t in _grads(q, k, other_v, other_do, **kw)]
+    assert all(torch.equal(a[1], b[1]) for a, b in zip(got, again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("which", ["early", "late", "every_other", "rising"])
+def test_gradients_of_rows_of_very_different_sizes(gpu, which, d):
+    """A row's dq and the dk of keys that only small rows see keep their own accuracy in fp16."""
+    n, dt = 330, torch.float16
+    q, k, v, do = _make(gpu, (1, n, 2, d), (1, n, 2, d), dt, 71)
+    at = torch.arange(n, device=gpu)
+    small = {"early": at < n // 2, "late": at >= n // 2, "every_other": at % 2 == 1}.get(which)
+    size = torch.where(small, 2.0 ** -12, 4096.0) if small is not None else 2.0 ** (-12 + 24 * at / n).floor()
+    do *= size[None, :, None, None].to(dt)
+    got = _grads(q, k, v, do)
+    want, bound = _own_peaks(q[0], k[0], v[0], do[0], True)
+    for name, g, w, b in zip(("dq", "dk"), got[1:], want, bound):
+        _within(name, g[0], w, b, dt)
