@@ -18,6 +18,8 @@ namespace dmuon {
 namespace {
 
 constexpr float kInf = __builtin_inff();
+// A row's reference where all it sees has the score -infinity; only a row that sees nothing keeps -infinity itself
+constexpr float kLeast = -3.402823466e38f;
 constexpr int kKeys = 64;                 // keys of a tile
 
 // What is left of two values behind their rounding
@@ -46,8 +48,8 @@ __device__ __forceinline__ void store_row(const Attention& a, const Place& p, bo
       }
     return;
   }
-  // a row that sees nothing is 0
-  const float f = total == 0.f ? 0.f : 1.f / total;
+  // a row that sees nothing is 0; one that sees scores of -infinity alone is 0 / 0
+  const float f = ref == -kInf ? 0.f : 1.f / total;
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
@@ -62,7 +64,7 @@ __device__ __forceinline__ void store_row(const Attention& a, const Place& p, bo
             u32x2_t{rest2<E>(w[0], o[b][i] * f, o[b][i + 1] * f),
                     rest2<E>(w[1], o[b][i + 2] * f, o[b][i + 3] * f)};
     }
-  if (a.lse && h == 0) a.lse[row] = total == 0.f ? kInf : ref + __log2f(total);
+  if (a.lse && h == 0) a.lse[row] = ref == -kInf ? kInf : ref + __log2f(total);
 }
 
 // A block has 128 rows of queries, 32 a wave and one a lane (l % 32): S^T = K Q^T leaves each lane 16 keys of
@@ -188,6 +190,7 @@ void attention_kernel(const Attention a) {
     const int slot = (t - t0) & 1;
     step(t, lds + slot * 2 * TILE, lds + (slot ^ 1) * 2 * TILE);
   }
+  if (see.hi > see.lo) ref = fmaxf(ref, kLeast);
   store_row<E, DB>(a, p, live, query, head, o, ref, half_sum(sum), h);
 }
 
@@ -296,6 +299,7 @@ __global__ __launch_bounds__(64) void attention_few_kernel(const Attention a) {
     char* slot = lds + ((t - t0) & 1) * 2 * TILE;
     step(t, slot, slot + TILE, slot, slot + TILE);
   }
+  if (see.hi > see.lo) ref = fmaxf(ref, kLeast);
   store_row<E, DB>(a, p, live, query, head, o, ref, half_sum(sum), h);
 }
 
@@ -331,13 +335,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Attention a) 
       o1 += s0 + k < a.splits ? g * v[k].y : 0.f;
     }
   }
-  const float g = total == 0.f ? 0.f : 1.f / total;
+  const float g = top == -kInf ? 0.f : 1.f / total;
   if (2 * lane < a.dim) {
     const unsigned w = pack2_elt<E>(o0 * g, o1 * g);
     *reinterpret_cast<unsigned*>(a.out + row * a.dim + d) = w;
     if (a.rest) *reinterpret_cast<unsigned*>(a.rest + row * a.dim + d) = rest2<E>(w, o0 * g, o1 * g);
   }
-  if (a.lse && lane == 0) a.lse[row] = total == 0.f ? kInf : top + __log2f(total);
+  if (a.lse && lane == 0) a.lse[row] = top == -kInf ? kInf : top + __log2f(total);
 }
 
 // Sequences and tiles of a packed call. Starts that fall are taken as the largest before them, and all

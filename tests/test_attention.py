@@ -625,3 +625,48 @@ def test_gradients_of_rows_of_very_different_sizes(gpu, which, d):
     want, bound = _own_peaks(q[0], k[0], v[0], do[0], True)
     for name, g, w, b in zip(("dq", "dk"), got[1:], want, bound):
         _within(name, g[0], w, b, dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("sq,sk,h,hk,d", [(1, 40, 2, 1, 64), (1, 5000, 8, 2, 128), (100, 300, 2, 2, 128),
+                                          (100, 5000, 4, 1, 64), (70, 70, 1, 1, 72)])
+def test_scores_of_minus_infinity(gpu, sq, sk, h, hk, d, dt):
+    """A key whose score is minus infinity has no share; a row that sees only such keys has no numbers, as
+    the formula has it, and is not one that sees nothing."""
+    q, k, v, do = _make(gpu, (1, sq, h, d), (1, sk, hk, d), dt, 72)
+    q[..., 0] = -q[..., 0].abs() - 1
+    k[..., 0] = float("inf")
+    got = _grads(q, k, v, do, causal=False)
+    for name, t in zip(("out", "dq", "dk", "dv"), got):
+        assert bool(torch.isnan(t).all()), name
+    # one key of numbers among them takes the whole row, wherever it stands
+    for one in (0, sk // 2, sk - 1):
+        single = k.clone()
+        single[:, one, :, 0] = 1
+        with torch.no_grad():
+            out = dmuon.attention(q, single, v, causal=False)
+        assert torch.equal(out, v[:, one, None].repeat_interleave(h // hk, 2).expand_as(out))
+
+
+@pytest.mark.gpu
+def test_rows_of_minus_infinity_beside_others(gpu):
+    """Under a causal mask, lengths and starts: rows that see nothing are 0 and have no gradient, rows that
+    see only minus infinities are no numbers, the others are as without those keys."""
+    d, dt = 64, torch.bfloat16
+    q, k, v, do = _make(gpu, (3, 50, 2, d), (3, 40, 2, d), dt, 73)
+    q[..., 0] = -q[..., 0].abs() - 1
+    k[:, :8, :, 0] = float("inf")
+    lengths = torch.tensor([40, 0, 40], device=gpu)
+    # query i sees the keys up to i - 10; those of the second sequence see none
+    got = _grads(q, k, v, do, kv_lengths=lengths)
+    for b in (0, 2):
+        out, dv = got[0][b], got[3][b]
+        assert not bool(out[:10].any()) and bool(torch.isnan(out[10:18]).all())
+        assert bool(torch.isfinite(out[18:]).all())
+        assert bool(torch.isnan(dv[:8]).all()) and bool(torch.isfinite(dv[8:]).all())
+        assert not bool(got[1][b][:10, :, 1:].any())           # (a key's infinity may reach rows near its own)
+        want = _one_head(q[b, 18:, 0].double(), k[b, 8:, 0].double(), v[b, 8:, 0].double(), None, d ** -0.5, True,
+                         None, None)
+        _within("out", out[18:, 0], want[0][0], want[1][0], dt)
+    assert all(not bool(t[1].any()) for t in got)
