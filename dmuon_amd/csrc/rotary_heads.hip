@@ -8,8 +8,8 @@
 // square is formed anew). A lane has the same 8 pairs of every head (4, or 1, where a head has no more), so
 // that pairs half a rotation apart need no exchange, and one exchange of sums joins the lanes of a head.
 // The lanes of a group keep a token's cosines and sines in registers and walk its heads, the next one's
-// loads in flight: angles are formed once a token and part of the heads, in turns, reduced in 64 bits to an
-// eighth of a turn around a multiple of a quarter, so that positions of any size keep 32 bits of accuracy.
+// loads in flight: angles are formed once a token and part of the heads, in turns, as sums of two fp64 values
+// reduced to an eighth of a turn around a multiple of a quarter: all 64-bit positions are as exact as near ones.
 //
 // 16384 tokens of 32 + 8 heads of 128 in bf16, read from rows of 48 heads: forward 73 us (4.6 TB/s), backward
 // 94 (5.3) and 4 of joining the weights' gradients; 1777 x 6 heads of 72 in fp32, pairs side by side 6 and 11.
@@ -159,17 +159,36 @@ __device__ __forceinline__ int value_at(int i, int j, int k) {
   return k < P ? i + k : j + k - P;
 }
 
-// cos and sin of position * inv_freq: within an eighth of a turn the Taylor polynomials are off by less
-// than 2^-29
-__device__ __forceinline__ float2 turn_of(const Heads& a, double position, int pair) {
+// The position in two parts that fp64 holds: position = hi + lo, hi a multiple of 2^32
+struct Position {
+  double hi, lo;
+};
+__device__ __forceinline__ Position position_of(int64_t p) {
+  return {(double)(p >> 32) * 4294967296., (double)(unsigned)p};
+}
+
+// cos and sin of position * inv_freq. In quarters of a turn the angle is position f 2 / pi, formed as sums of
+// two: f 2 / pi = fh + fl to 2^-105 of it, and the products of both parts of the position with fh as their
+// rounded values, of which whole turns are dropped without an error, and the rest of those. What is rounded is
+// under 2^12 quarters then: angles of 64-bit positions and frequencies up to 1 (products up to 2^63) are
+// within 2^-40, ones under 2^31 within 2^-50. Within an eighth of a turn the Taylor polynomials are off by less
+// than 2^-29. No contraction: a product that is rounded in one place must be the same in the other.
+__device__ __forceinline__ float2 turn_of(const Heads& a, const Position& position, int pair) {
+#pragma clang fp contract(off)
+  constexpr double kTwoByPi = 0x1.45f306dc9c883p-1, kTwoByPiRest = -0x1.6b01ec5417056p-55;
   const double f = a.freq_double ? static_cast<const double*>(a.inv_freq)[pair]
                                  : (double)static_cast<const float*>(a.inv_freq)[pair];
-  const double quarters = position * f * (4. * 0.15915494309189533577);
-  const double whole = rint(quarters);
-  const float t = (float)(quarters - whole) * 1.57079632679489661923f, q = t * t;
-  const float s = t + t * q * (-1.f / 6.f + q * (1.f / 120.f + q * (-1.f / 5040.f + q * (1.f / 362880.f))));
-  const float c = 1.f + q * (-0.5f + q * (1.f / 24.f + q * (-1.f / 720.f + q * (1.f / 40320.f -
-                                                                              q * (1.f / 3628800.f)))));
+  const double fh = f * kTwoByPi;
+  const double fl = __builtin_fma(f, kTwoByPiRest, __builtin_fma(f, kTwoByPi, -fh));
+  const double p = position.hi * fh, q = position.lo * fh;
+  const double rest = __builtin_fma(position.hi, fh, -p) + __builtin_fma(position.lo, fh, -q) +
+                      (position.hi + position.lo) * fl;
+  const double near = (p - 4. * rint(p * 0.25)) + (q - 4. * rint(q * 0.25));
+  const double whole = rint(near + rest);
+  const float t = (float)((near - whole) + rest) * 1.57079632679489661923f, z = t * t;
+  const float s = t + t * z * (-1.f / 6.f + z * (1.f / 120.f + z * (-1.f / 5040.f + z * (1.f / 362880.f))));
+  const float c = 1.f + z * (-0.5f + z * (1.f / 24.f + z * (-1.f / 720.f + z * (1.f / 40320.f -
+                                                                              z * (1.f / 3628800.f)))));
   const int k = (int)(whole - 4. * floor(whole * 0.25));
   const float cc = k & 1 ? s : c, ss = k & 1 ? c : s;
   return make_float2(k == 1 || k == 2 ? -cc : cc, k >= 2 ? -ss : ss);
@@ -229,7 +248,7 @@ __global__ __launch_bounds__(kThreads) void rotary_heads_kernel(const Heads a) {
     float2 cs[SLOTS][P];
     {
       const long long slot = a.period == a.tokens ? token : token % a.period;
-      const double position = (double)a.positions[slot];
+      const Position position = position_of(a.positions[slot]);
 #pragma unroll
       for (int u = 0; u < SLOTS; ++u)
 #pragma unroll

@@ -53,7 +53,8 @@ def rotary_heads(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, *,
     with the pairs ``j = i + r / 2`` of the first ``r = 2 * len(inv_freq)`` values, or, ``interleaved``, the
     neighbours ``2 i`` and ``2 i + 1``; values behind them are not turned. ``positions`` are integers
     of the leading shape or of its trailing part (``[tokens]`` for a batch), ``inv_freq`` fp32 or fp64: the
-    angle is formed and reduced in 64 bits, so that far positions are as exact as near ones. ``q`` and ``k``
+    angle is formed and reduced in twice 64 bits, so that far positions (all of 64 bits, with frequencies up
+    to 1) are as exact as near ones. ``q`` and ``k``
     share a dtype (fp32, bf16 or fp16) that the results, which are dense, have too; the weights (``[dim]``)
     may have it or fp32. ``dim`` is even and at most 512. Views into one product for q, k and v are read in
     place. Arithmetic is fp32, every result is rounded once; gradients go to q, k and the weights (their

@@ -606,7 +606,7 @@ int dmuon_attention_grad(const dmuon_attention_args* args, void* workspace, int6
  * q [tokens][heads][dim] and k [tokens][kv_heads][dim] with strides in elements, results dense, all of
  * `dtype` (DMUON_DTYPE_F32, _BF16 or _F16), dim even and 2 .. 512, any element alignment; weights [dim] with
  * a dtype of their own; inv_freq [rotary_dim / 2] fp32, or fp64 with inv_freq_double. Angles are formed
- * and reduced in fp64, the rest is fp32, every result rounded once. positions are 64-bit integers, of
+ * and reduced in pairs of fp64 values, the rest is fp32, every result rounded once. positions are 64-bit integers, of
  * which `period` are there (a divisor of tokens).
  * dmuon_rotary_heads_grad: from dq_out and dk_out (either may be NULL: zero) dq, dk, d_q_weight and
  * d_k_weight, any of which may be NULL; the weights' sums have a fixed order.

@@ -409,3 +409,49 @@ def test_tangents_and_tracers_are_refused(dev):
         torch.jit.trace(call, tuple(v), check_trace=False)
     with pytest.raises(RuntimeError, match="tracer"):
         make_fx(call)(*v)
+
+
+def _turns(positions, inv_freq):
+    """cos and sin of the exact products, in 64 bits: whole numbers reduced by 2 pi to 300 bits (Machin)."""
+    from fractions import Fraction
+    bits = 300
+
+    def arctan_of_inverse(n):
+        total, term, k = 0, (1 << bits) // n, 0
+        while term:
+            total += (-term if k & 1 else term) // (2 * k + 1)
+            term //= n * n
+            k += 1
+        return total
+    turn = 8 * (4 * arctan_of_inverse(5) - arctan_of_inverse(239))         # 2 pi, times 2^bits
+    angles = []
+    for p in positions.tolist():
+        for f in inv_freq.double().tolist():
+            exact = Fraction(f) * p * (1 << bits)
+            rest = (exact.numerator // exact.denominator) % turn
+            angles.append((rest - turn if 2 * rest > turn else rest) / (1 << bits))
+    angle = torch.tensor(angles, dtype=torch.float64).view(len(positions), -1).to(positions.device)
+    return angle.cos(), angle.sin()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("freq", [torch.float32, torch.float64])
+@pytest.mark.parametrize("far", [0, 2 ** 28, 2 ** 31, -2 ** 33, 2 ** 40, 2 ** 53 + 1, -2 ** 57 - 3, 2 ** 63 - 500, -2 ** 63])
+def test_positions_of_any_size_with_any_frequencies(gpu, far, freq):
+    """Angles of whole 64-bit positions and frequencies that are no powers of two, as exact as near ones:
+    the bounds of near positions hold."""
+    d, n = 64, 40
+    gen = torch.Generator(device=gpu).manual_seed(20)
+    q, k, dq, dk = (torch.randn(n, h, d, device=gpu, generator=gen) for h in (2, 1, 2, 1))
+    positions = torch.arange(n, device=gpu) * 7 + far
+    inv_freq = (10000.0 ** (-torch.arange(d // 2, device=gpu, dtype=torch.float64) * 2 / d)).to(freq)
+    inv_freq[-3:] = torch.tensor([1.7, 0.0, -0.31], device=gpu)
+    cos, sin = (t[:, None] for t in _turns(positions, inv_freq))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k)]
+    got = dmuon.rotary_heads(*leaves, positions, inv_freq)
+    grads = torch.autograd.grad(got, leaves, (dq, dk))
+    rel = 2.0 ** -24 * (d / 16 + 24)
+    for x, y, sign in ((q, got[0], 1), (k, got[1], 1), (dq, grads[0], -1), (dk, grads[1], -1)):
+        a, b = x.double().chunk(2, -1)
+        want = torch.cat((a * cos - sign * b * sin, b * cos + sign * a * sin), -1)
+        _within(f"{far}", y.detach(), want, torch.float32, rel * (a.abs() + b.abs()).repeat(1, 1, 2))
