@@ -244,9 +244,9 @@ __global__ __launch_bounds__(64) void attention_few_kernel(const Attention a) {
   float ref = -kInf, sum = 0.f;
   // A slot is filled again as soon as it has been read: the waits count the loads of the three tiles behind
   // (none are missing before the last two). The slots are restrict so that the compiler adds no waits of its
-  // own; the empty asm statements keep reads and loads of one slot in their order.
-  auto step = [&](int t, const char* __restrict__ kt, const char* __restrict__ vt, char* __restrict__ k_next,
-                  char* __restrict__ v_next) __attribute__((always_inline)) {
+  // own, each read and filled through its one pointer; the empty asm statements keep reads and loads of one slot
+  // in their order.
+  auto step = [&](int t, char* __restrict__ kt, char* __restrict__ vt) __attribute__((always_inline)) {
     const bool more = t + 2 < t1;
     if (more) wait_vmcnt<3 * LOADS>();
     else wait_vmcnt<0>();
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(64) void attention_few_kernel(const Attention a) {
     for (int k = 0; k < KS; ++k)
       s = mfma_32x32x16<E>(*reinterpret_cast<const bf16x8_t*>(kt + (row_at ^ (32 * k))), qf[k], s);
     asm volatile("" : "+v"(s) : : "memory");
-    if (more) fetch_k(t + 2, k_next);
+    if (more) fetch_k(t + 2, kt);
     const int j0 = t * KEYS;
     if (j0 + KEYS > full_hi) cut_end(s, j0, see.hi, h, -kInf);
     if (j0 < full_lo) cut_begin(s, j0, see.lo, h, -kInf);
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(64) void attention_few_kernel(const Attention a) {
     }
     __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): every read of the slot has returned
     asm volatile("" ::: "memory");
-    if (more) fetch_v(t + 2, v_next);
+    if (more) fetch_v(t + 2, vt);
   };
   for (int t = t0; t < t1 && t < t0 + 2; ++t) {
     fetch_k(t, lds + (t - t0) * 2 * TILE);
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(64) void attention_few_kernel(const Attention a) {
   }
   for (int t = t0; t < t1; ++t) {
     char* slot = lds + ((t - t0) & 1) * 2 * TILE;
-    step(t, slot, slot + TILE, slot, slot + TILE);
+    step(t, slot, slot + TILE);
   }
   if (see.hi > see.lo) ref = fmaxf(ref, kLeast);
   store_row<E, DB>(a, p, live, query, head, o, ref, half_sum(sum), h);

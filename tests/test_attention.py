@@ -670,3 +670,17 @@ def test_rows_of_minus_infinity_beside_others(gpu):
                          None, None)
         _within("out", out[18:, 0], want[0][0], want[1][0], dt)
     assert all(not bool(t[1].any()) for t in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 40)])
+def test_waves_of_none_to_several_tiles(gpu, dt, d):
+    """Single tokens whose waves have no, one, two and more tiles of keys, whole ones and ends."""
+    lens = [0, 1, 31, 32, 33, 64, 65, 96, 1000, 1024, 1025, 2047, 2048, 2080, 3071, 4000]
+    b = len(lens)
+    for sk in (4000, 40000):              # few and many keys a wave
+        q, k, v, _ = _make(gpu, (b, 1, 4, d), (b, sk, 2, d), dt, 76)
+        lengths = torch.tensor(lens, device=gpu) * (sk // 4000)
+        with torch.no_grad():
+            got = dmuon.attention(q, k, v, kv_lengths=lengths)
+        _check([got], [((i,), (i, slice(0, int(n)))) for i, n in enumerate(lengths)], q, k, v, None, True, None)
