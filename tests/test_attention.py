@@ -684,3 +684,30 @@ def test_waves_of_none_to_several_tiles(gpu, dt, d):
         with torch.no_grad():
             got = dmuon.attention(q, k, v, kv_lengths=lengths)
         _check([got], [((i,), (i, slice(0, int(n)))) for i, n in enumerate(lengths)], q, k, v, None, True, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("sq,sk,h,hk", [(700, 700, 2, 2), (8, 512, 4, 1), (2, 4096, 8, 1), (60, 3000, 4, 1)])
+def test_gradients_take_in_what_the_rounding_of_the_result_left(gpu, sq, sk, h, hk, dt):
+    """delta = sum do o stands in every dS of a row. Keys and values with a large common part make its error
+    show: the exact dS of a row add up to 0, so the keys' common part c drops out of dq, where an error e of
+    delta stays as scale e c. With o rounded, its values of 8 .. 16 are off by up to half a step, of even
+    spread: e of sqrt(d) half / sqrt(3) on average, for dout of size 1. What else there is: P in o is
+    rounded, by up to u of each term, which moves a row's values together by 8 u sqrt(sum P^2 / 3), e by sqrt(d)
+    times that, for rows of some hundred keys a twentieth of the former; dS is rounded, u of terms that
+    are as small as P |v - o|, and dq itself. A quarter holds all of these."""
+    d, common = 128, 4.0
+    q, k, v, do = _make(gpu, (1, sq, h, d), (1, sk, hk, d), dt, 75)
+    q, k, v = (0.25 * q.float()).to(dt), (common + 0.3 * k.float()).to(dt), (10 + 0.5 * v.float()).to(dt)
+    dq = _grads(q, k, v, do)[1][0].double()
+    rows = slice(0, sq) if sq + 400 < sk else slice(400, sq)          # rows that see some hundred keys
+    errors = []
+    for i in range(h):
+        at = i * hk // h
+        want = _one_head(q[0, :, i].double(), k[0, :, at].double(), v[0, :, at].double(), do[0, :, i].double(),
+                         d ** -0.5, True, None, None)[0][1]
+        errors.append((dq[:, i] - want)[rows])
+    rms = float(torch.stack(errors).pow(2).mean().sqrt())
+    half = 8 * U[dt]                      # half a step of values of 8 .. 16
+    assert rms <= 0.25 * d ** -0.5 * common * d ** 0.5 * half / 3 ** 0.5, rms
