@@ -184,7 +184,8 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
     end = n - p.split * each;
     n = end < 0 ? 0 : end < each ? end : each;
   }
-  // from the last rows back: under a causal mask all blocks of a key head begin with the same rows then,
+  // (rows that see nothing stand before r_lo, in no tile: no key's sums meet what they hold.)
+  // From the last rows back: under a causal mask all blocks of a key head begin with the same rows then,
   // and find them in their XCD's L2
   auto first_row = [&](int t) { return r_lo + (end - 1 - t) * tr; };
 

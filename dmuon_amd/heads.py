@@ -36,8 +36,10 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, window: O
     Scores, sums and statistics are fp32; the probabilities, and in the gradient theirs, are rounded to
     the operands' type between the products. A value or key of no number (infinity or NaN) reaches every row
     that sees it, and may reach rows near those, whose mask hides it. (A key whose score is minus infinity has
-    no share in a row; a row that sees only such keys is NaN, as the formula has it.) The same call gives the
-    same bits. The gradient has no gradient of its own. Can be captured into a graph.
+    no share in a row; a row that sees only such keys is NaN, as the formula has it.) In the gradient a query
+    or a gradient of no number likewise reaches the keys that its row sees, and may reach keys near those; of
+    rows that see nothing they are not read. The same call gives the same bits. The gradient has no gradient
+    of its own. Can be captured into a graph.
     """
     return _C.torch_ops().attention(
         q, k, v, bool(causal), None if window is None else int(window),

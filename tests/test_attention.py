@@ -711,3 +711,30 @@ def test_gradients_take_in_what_the_rounding_of_the_result_left(gpu, sq, sk, h, 
     rms = float(torch.stack(errors).pow(2).mean().sqrt())
     half = 8 * U[dt]                      # half a step of values of 8 .. 16
     assert rms <= 0.25 * d ** -0.5 * common * d ** 0.5 * half / 3 ** 0.5, rms
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_gradients_of_rows_that_see_nothing_are_not_read(gpu, dt, bad):
+    """Queries before the first key, of an empty cache and outside of the sequences: whatever their gradient
+    and they themselves hold."""
+    q, k, v, do = _make(gpu, (2, 90, 6, 64), (2, 40, 2, 64), dt, 74)
+    lengths = torch.tensor([40, 0], device=gpu)
+    # sequence 0: queries under 50; sequence 1: all
+    blind = torch.ones(2, 90, dtype=torch.bool, device=gpu)
+    blind[0, 50:] = False
+    for window in (None, 30):
+        want = _grads(q, k, v, do.masked_fill(blind[..., None, None], 0), kv_lengths=lengths, window=window)
+        no_q, no_do = (t.masked_fill(blind[..., None, None], bad) for t in (q, do))
+        got = _grads(no_q, k, v, no_do, kv_lengths=lengths, window=window)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    starts, kstarts = torch.tensor([30, 90, 150], device=gpu), torch.tensor([5, 25, 75], device=gpu)
+    flat = [t.flatten(0, 1) for t in (q, k, v, do)]
+    at = torch.arange(180, device=gpu)
+    # sequence 0: 60 queries of 20 keys; sequence 1: 60 of 50
+    blind = ((at < 70) | ((at >= 90) & (at < 100)) | (at >= 150))[:, None, None]
+    kw = {"q_starts": starts, "kv_starts": kstarts}
+    want = _grads(*flat[:3], flat[3].masked_fill(blind, 0), **kw)
+    got = _grads(flat[0].masked_fill(blind, bad), *flat[1:3], flat[3].masked_fill(blind, bad), **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
