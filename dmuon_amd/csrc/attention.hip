@@ -2,8 +2,6 @@
 #include "../../include/dmuon_amd.h"
 #include "attention.h"
 
-#include <math.h>
-
 namespace dmuon {
 namespace {
 
@@ -25,7 +23,9 @@ int check(const char* who, const dmuon_attention_args* a) {
                 (long long)a->heads, (long long)a->kv_heads);
   if (a->q_len * (a->heads / a->kv_heads) > kMost)
     return fail("%s: q_len times the heads of a key head must be at most 2^30", who);
-  if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return fail("%s: scale must be positive and finite", who);
+  // a normal fp32 number, and one times log2(e)
+  if (!(a->scale >= 0x1p-126f && a->scale < 0x1p127f))
+    return fail("%s: scale must be 2^-126 .. 2^127", who);
   if (a->window < 0 || (a->window > 0 && !a->causal))
     return fail("%s: a window must be positive, and needs causal", who);
   if ((a->q_starts == nullptr) != (a->kv_starts == nullptr))

@@ -557,8 +557,9 @@ int dmuon_residual_norm_grad(const dmuon_residual_norm_args* args, void* workspa
  * over the keys j that query i of its sequence sees: all of them, or, with `causal`, those up to
  * j = i + kv tokens - q tokens (the last query sees the last key), of which a `window` > 0 leaves the
  * last `window`. A query that sees nothing has the result 0. q, k, v, dout and the results are 16-bit words
- * of `dtype` (DMUON_DTYPE_BF16 or _F16), heads of dim (8 .. 128, a multiple of 8) values; scores, sums
- * and statistics are fp32, probabilities and their gradients are rounded to `dtype` between the products.
+ * of `dtype` (DMUON_DTYPE_BF16 or _F16), heads of dim (8 .. 128, a multiple of 8) values, scale
+ * 2^-126 or more and under 2^127; scores, sums and statistics are fp32, probabilities and their gradients are
+ * rounded to `dtype` between the products.
  *   batched: q [batch][q_len][heads][dim], k and v [batch][kv_len][kv_heads][dim]; kv_lengths [batch]
  *     (or NULL) says how many keys of each are there (held to 0 .. kv_len); what lies behind them is not read.
  *   packed (q_starts and kv_starts [batch + 1], with batch sequences): q [q_len][heads][dim], k and v

@@ -738,3 +738,21 @@ def test_gradients_of_rows_that_see_nothing_are_not_read(gpu, dt, bad):
     want = _grads(*flat[:3], flat[3].masked_fill(blind, 0), **kw)
     got = _grads(flat[0].masked_fill(blind, bad), *flat[1:3], flat[3].masked_fill(blind, bad), **kw)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_c_entry_refuses_scales_that_leave_fp32():
+    """The kernels multiply scores by scale log2(e) in fp32."""
+    import ctypes
+
+    from dmuon_amd import _C
+    lib, need = _C.lib(), ctypes.c_int64()
+    good = dict(q=4096, k=4096, v=4096, batch=1, q_len=4, kv_len=4, heads=1, kv_heads=1, dim=64, q_batch=256,
+                q_token=64, q_head=64, k_batch=256, k_token=64, k_head=64, v_batch=256, v_token=64, v_head=64,
+                causal=1, dtype=1)
+
+    def size(scale):
+        return lib.dmuon_attention_workspace_size(ctypes.byref(_C.AttentionArgs(**good, scale=scale)),
+                                                  ctypes.byref(need))
+    assert size(2.0 ** -126) == 0 and size(2.0 ** 126) == 0
+    for bad in (2.0 ** -127, 3e38, float("inf")):
+        assert size(bad) != 0 and "scale" in lib.dmuon_last_error().decode()
