@@ -461,6 +461,9 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale,
                         weight.size(1) <= (1 << 20), who,
                     ": weight must be [vocab, dim] with dim up to 2^20, got ", weight.sizes());
   TORCH_CHECK_VALUE(code(weight.scalar_type()) >= 0, who, ": unsupported dtype ", weight.scalar_type());
+  // the kernels multiply by it in fp32
+  TORCH_CHECK_VALUE(scale == 0. || (std::abs(scale) >= 0x1p-126 && std::abs(scale) <= 0x1.fffffep127), who,
+                    ": scale must be 0 or within fp32, got ", scale);
   EmbeddingCall c;
   c.scale = scale;
   if (padding_idx.has_value()) {

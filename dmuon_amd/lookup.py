@@ -16,7 +16,8 @@ from . import _C
 def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0,
               padding_idx: Optional[int] = None) -> Tensor:
     """``scale * weight[tokens]``: a row of ``weight`` ``[vocab, dim]`` (fp32, bf16 or fp16, rows of any
-    pitch) for every token (integers of any shape), in ``weight``'s dtype.
+    pitch) for every token (integers of any shape), in ``weight``'s dtype. ``scale`` is 0 or a normal fp32
+    number.
 
     The gradient of ``weight`` is dense and of its dtype; sums are fp32 in a fixed order, rounded once.
     Tokens equal to ``padding_idx`` (which may count from the vocabulary's end) have no share in it. A token

@@ -290,3 +290,12 @@ def test_tangents_and_tracers_are_refused(dev):
         torch.jit.trace(lambda x: dmuon.embedding(t, x), (w,), check_trace=False)
     with pytest.raises(RuntimeError, match="tracer"):
         make_fx(lambda x: dmuon.embedding(t, x))(w)
+
+
+def test_scales_that_leave_fp32_are_refused():
+    """The kernels multiply in fp32: a scale that it holds as infinity or not in full would give other rows."""
+    t, w = torch.zeros(3, dtype=torch.long), torch.ones(5, 8)
+    for bad in (1e39, -1e39, 1e-39, float("inf"), float("nan")):
+        _refuse("scale must", t, w, scale=bad)
+    for good in (0.0, -2.0, 1e38, 2.0 ** -126):
+        _refuse("GPU", t, w, scale=good, kind=RuntimeError)
