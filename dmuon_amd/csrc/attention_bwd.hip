@@ -31,13 +31,15 @@ constexpr float kShift = E == ELT_F16 ? 10.f : 0.f;
 // relative; dS under 2^-47 in all of a row is lost to fp16's results anyway. In fp32 dS 2^70 < 2^112.
 constexpr float kFull = 32768.f;
 constexpr int kFirstPower = 60;
-// The exponent that a row's (key's) powers change by, 0 where `v`, this lane's 16 of its 32 values, has room
-__device__ __forceinline__ int power_step(const f32x16_t& v, bool* any) {
+// A lane's 16 of a row's (key's) 32 values: the largest, and what the power changes by for both lanes'
+__device__ __forceinline__ float largest(const f32x16_t& v) {
   float most = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i]));
+  for (int i = 0; i < 16; i += 2) most = fmaxf(fmaxf(fabsf(v[i]), fabsf(v[i + 1])), most);
+  return most;
+}
+__device__ __forceinline__ int power_step(float most) {
   most = half_max(most);
-  *any = __ballot(most >= kFull) != 0;
   // most < 2^frexp; infinities stay what they are
   return most >= kFull && most < kInf ? 14 - __builtin_amdgcn_frexp_expf(most) : 0;
 }
@@ -290,10 +292,9 @@ __device__ __forceinline__ void keys_block(const Attention& a, int id, int block
       if (early) cut_begin(dp, r0 + 32 * y, lo, h, 0.f);
       if (late) cut_end(dp, r0 + 32 * y, hi, h, 0.f);
       if constexpr (E == ELT_F16) {
-        bool any;
-        const int by = power_step(dp, &any);
-        if (any) {
-          const float f = power(by);
+        const float most = largest(dp);
+        if (__ballot(most >= kFull)) {
+          const float f = power(power_step(most));
           sigma *= f;
           dp *= f;
 #pragma unroll
@@ -429,9 +430,9 @@ __device__ __forceinline__ void queries_block(const Attention& a, int id, int bl
       if (j0 + kTile > full_hi) cut_end(dp, j0 + 32 * y, see.hi, h, 0.f);
       if (j0 < full_lo) cut_begin(dp, j0 + 32 * y, see.lo, h, 0.f);
       if constexpr (E == ELT_F16) {
-        bool any;
-        const int by = power_step(dp, &any);
-        if (any) {
+        const float most = largest(dp);
+        if (__ballot(most >= kFull)) {
+          const int by = power_step(most);
           const float f = power(by);
           up += by;
           from = lse - (float)up;
