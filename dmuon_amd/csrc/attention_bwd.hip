@@ -5,9 +5,10 @@
 // seven products where one pass would do with five, but no sums over blocks, so no atomics and one order.
 // Where the keys' blocks are few their rows are split, and a second kernel joins the parts in their order.
 //
-// Bound like the forward pass: 2 x 8192 causal tokens, 32/8 heads of 128, bf16 3.5 ms (1.1 PFLOP/s of the seven
-// products, 0.78 of five); 16384 packed tokens in 23 documents 0.62 ms; 8191 tokens of 16 heads of 64 in a
-// window of 1024 in fp16 160 us. The key blocks' sums (dk and dv of 32 keys a wave) and operands take 192 of
+// Bound like the forward pass, by two pipes that hardly overlap: 2 x 8192 causal tokens, 32/8 heads of 128, bf16
+// 3.6 ms (1.07 PFLOP/s of the seven products, 0.76 of five; matrix pipe busy 54% of the cycles, vector pipe 39,
+// both at once 15); 16384 packed tokens in 23 documents 0.62 ms; 8191 tokens of 16 heads of 64 in a window of
+// 1024 in fp16 172 us (33%, 58, 15). The key blocks' sums (dk and dv of 32 keys a wave) and operands take 192 of
 // 256 registers; a third of what they read from LDS is turned on the way (transposing reads).
 //
 // P and dS are rounded to the operands' type between the products. In fp16 they are held times powers of
@@ -28,7 +29,9 @@ constexpr float kShift = E == ELT_F16 ? 10.f : 0.f;
 // fp16's dS is held times 2^60 until its largest magnitude reaches 2^15; then, and whenever it does so again,
 // times the power that brings it to 2^13 .. 2^14. That costs one maximum of the values at hand, and the sums
 // are multiplied (exactly) where the power falls. 2^-38 of the largest is then the least error that is not
-// relative; dS under 2^-47 in all of a row is lost to fp16's results anyway. In fp32 dS 2^70 < 2^112.
+// relative; dS under 2^-47 in all of a row is lost to fp16's results anyway. In fp32 dS 2^70 < 2^112. One power
+// for the whole call took no maximum (2 x 4096 tokens of 32/8 heads with gradients 894 us at dim 64 and 1418 at
+// 128, this 933 and 1435), but lost the rows that are 2^20 under the call's largest.
 constexpr float kFull = 32768.f;
 constexpr int kFirstPower = 60;
 // A lane's 16 of a row's (key's) 32 values: the largest, and what the power changes by for both lanes'
@@ -94,7 +97,7 @@ struct RowMover {
 
 // What the products need besides: -delta of every row (of out and what its rounding left: all of a row's dS
 // share delta's error, which took dq's from 1.4 to 1.5 to 1.6 times its own rounding). L lanes a row, 8 values
-// each. Reading do, out and rest at 6.3 TB/s: 64 us for 2 x 8192 tokens of 32 heads of 128.
+// each. Reading do, out and rest at 6.3 TB/s: 64 us for 2 x 8192 tokens of 32 heads of 128, 9 for 8191 of 16 of 64.
 template <int E, int L>
 __global__ __launch_bounds__(256) void attention_delta_kernel(const Attention a) {
   const int at = 8 * (threadIdx.x % L);

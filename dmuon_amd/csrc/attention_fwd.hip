@@ -5,13 +5,17 @@
 // Scores, sums and statistics are fp32. p is rounded to the operands' type before it meets v, as the matrix
 // instruction takes it (2^-9 of each term on average, against the result's own rounding of as much).
 //
-// 4 dim operations a pair of a query and a key on the matrix pipe, some five on the vector one. At dim 128
-// bound by the matrix pipe under the board's power limit (busy 56% of the cycles at 1.8 of 2.4 GHz): 2 x 8192
-// causal tokens, 32/8 heads, bf16 1.04 ms (1.06 PFLOP/s); 2047 tokens over 32768 keys 1.02 ms (1.04). At dim 64
-// by the vector pipe: 8191 tokens of 16 heads in a window of 1024 in fp16 57 us (0.57). Single tokens by
-// reading the cache: 48 x 1 over up to 8192 keys 157 us (6.5 TB/s). A tile of 64 keys lies in LDS twice, one
+// 4 dim operations a pair of a query and a key on the matrix pipe, some five on the vector one. A wave has all
+// of a tile's scores before their softmax and that before P v, so that only the SIMD's other waves can overlap
+// the two pipes, and they hardly do. Dim 128: 2 x 8192 causal tokens, 32/8 heads, bf16 1.07 ms (1.03 PFLOP/s, at
+// 1.8 of 2.4 GHz under the board's power limit), of whose cycles the matrix pipe is busy 54%, the vector pipe 49
+// and both at once 20; 2047 tokens over 32768 keys 1.01 ms (1.05). Dim 64: 8191 tokens of 16 heads in a window
+// of 1024 in fp16 57 us (0.57), matrix pipe 25%, vector pipe 46, both 13. Single tokens are bound by
+// reading the cache: 48 x 1 over up to 8192 keys 155 us (6.6 TB/s). A tile of 64 keys lies in LDS twice, one
 // copy read while the other is loaded; keys go through LDS since all waves read them, queries stay in
-// registers. 64 rows a wave (half the reads, one wave a SIMD) took 1.44 ms.
+// registers. 64 rows a wave (half the reads, one wave a SIMD) took 1.44 ms where 32 took 1.04. Heads are padded
+// with zeros to 64 or 128 values, which the products do not leave out: 2 x 4096 tokens of 32/8 heads in bf16
+// take 181 us at dim 64, 237 at 80, 244 at 96, 264 at 128, and as long at 32 as at 64.
 #include "attention.h"
 
 namespace dmuon {
@@ -346,7 +350,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Attention a) 
 
 // Sequences and tiles of a packed call. Starts that fall are taken as the largest before them, and all
 // lie within the tokens that are there. Four further sequences hold the tokens before the first and behind
-// the last start: queries that see nothing, and keys that nothing sees.
+// the last start: queries that see nothing, and keys that nothing sees. One block; a sequence's tiles are written
+// by one thread (23 documents of 16384 tokens: 8 us).
 __global__ __launch_bounds__(1024) void attention_tables_kernel(
     const int64_t* q_starts, const int64_t* k_starts, int n, int group, int q_tokens, int k_tokens,
     int q_rows, int k_rows, Sequence* seqs, int2* q_tiles, int2* k_tiles, int* counts) {

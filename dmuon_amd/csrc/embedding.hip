@@ -5,8 +5,9 @@
 // Memory bound: forward reads and writes a row a token; backward reads a row a token and writes every
 // row of dW, most of them zeros. The gradient sorts the positions by token (stable, so that a class's rows
 // add up in their order), walks the sorted positions in runs of 8 or 32, and joins the classes that cross
-// from one run to the next in a second kernel: the work of a class that makes up most of the text is
-// spread like any other. Sums are fp32, rounded once.
+// from one run to the next in a second kernel: the sums of a class that makes up most of the text are
+// spread like any other's, the join adds its runs one after the other (131072 tokens of 128256 x 4096 in bf16,
+// lookup and gradient: 844 us, with half of them one class 967, all of them 1065). Sums are fp32, rounded once.
 //
 // 16384 tokens of 128256 x 4096 in bf16: lookup 32 us (8.4 TB/s, some of it from the caches), sort 21 (which
 // clears 88 MB of the gradient meanwhile), sums 185 (6.2), joining 9. 1023 tokens of 5003 x 300 in fp16: 3, 8, 5

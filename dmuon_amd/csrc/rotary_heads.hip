@@ -12,7 +12,10 @@
 // reduced to an eighth of a turn around a multiple of a quarter: all 64-bit positions are as exact as near ones.
 //
 // 16384 tokens of 32 + 8 heads of 128 in bf16, read from rows of 48 heads: forward 73 us (4.6 TB/s), backward
-// 94 (5.3) and 4 of joining the weights' gradients; 1777 x 6 heads of 72 in fp32, pairs side by side 6 and 11.
+// 94 (5.3) and 4 of joining the weights' gradients; 1777 x 6 heads of 72 in fp32, pairs side by side 7 and 11.
+// One token 6.9, of which the angles' chain of fp64 instructions is one. In fp32, 16384 tokens of 40 heads of 128 as
+// dense rows 192 (3.5 TB/s) and 196 (5.1). Rotated widths or heads that are no multiple of 8 go value by value:
+// heads of 80 in bf16 with 80 rotated 60 and 70 us, with 20 rotated 92 and 366.
 #include "../../include/dmuon_amd.h"
 #include "dmuon_amd_internal.h"
 #include "mfma_tile.h"

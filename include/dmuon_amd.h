@@ -62,7 +62,7 @@ extern "C" {
 
 #define DMUON_DTYPE_F32 0
 #define DMUON_DTYPE_BF16 1
-#define DMUON_DTYPE_F16 2 /* 16-bit product operands only (dmuon_syrk, dmuon_ns_gemm*) */
+#define DMUON_DTYPE_F16 2 /* in the optimizer 16-bit product operands only (dmuon_syrk, dmuon_ns_gemm*) */
 
 /* Newton-Schulz device algorithms (the `backend` argument below). */
 #define DMUON_NS_DIRECT 0 /* X <- a X + (b A + c A A^T) X, A = X X^T, every step */
